@@ -1,4 +1,5 @@
-"""Loader of libspiky_lut.so, the HIP kernels behind the C ABI in include/spiky_lut.h.
+"""Loader of libspiky_lut.so, the HIP kernels behind the C ABI in include/spiky_lut.h
+and include/spiky_lm.h.
 
 The library is built in-tree (``python -m spiky_amd.build``).  There is no
 fallback: if the library is missing or fails to load, every device entry point
@@ -21,6 +22,7 @@ _lib = None
 _u32 = ctypes.c_uint32
 _u64 = ctypes.c_uint64
 _i32 = ctypes.c_int
+_i64 = ctypes.c_int64
 _f32 = ctypes.c_float
 _f64 = ctypes.c_double
 _vp = ctypes.c_void_p
@@ -70,9 +72,55 @@ _OPTIONAL_SIGNATURES = {
 }
 
 
+# include/spiky_lm.h
+F32, BF16, F16 = 0, 1, 2
+NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
+
+
+class LmResidualArgs(ctypes.Structure):
+    """spiky_lm_residual_args"""
+    _fields_ = [("rows", _u64), ("cols", _u64), ("res_dtype", _i32), ("act_dtype", _i32), ("post_norm", _i32),
+                ("pre_norm", _i32), ("par_f32", _i32), ("gate_f32", _i32), ("residual", _vp), ("branch", _vp),
+                ("residual_stride", _i64), ("branch_stride", _i64), ("post_weight", _vp), ("post_bias", _vp),
+                ("pre_weight", _vp), ("pre_bias", _vp), ("gate", _vp), ("gate_rows", _u64), ("post_eps", _f64),
+                ("pre_eps", _f64), ("residual_scale", _f64), ("branch_scale", _f64), ("dropout_p", _f64),
+                ("seed", _u64), ("offset", _u64), ("rng", _vp), ("stats", _vp)]
+
+
+class LmResidualGrads(ctypes.Structure):
+    """spiky_lm_residual_grads"""
+    _fields_ = [("d_out", _vp), ("d_normed", _vp), ("d_out_stride", _i64), ("d_normed_stride", _i64),
+                ("d_residual", _vp), ("d_branch", _vp), ("d_post_weight", _vp), ("d_post_bias", _vp),
+                ("d_pre_weight", _vp), ("d_pre_bias", _vp), ("d_gate", _vp), ("workspace", _vp),
+                ("workspace_bytes", _u64)]
+
+
+class LmLogitsArgs(ctypes.Structure):
+    """spiky_lm_logits_args"""
+    _fields_ = [("rows", _u64), ("vocab", _u64), ("logits", _vp), ("out", _vp), ("logits_stride", _i64),
+                ("out_stride", _i64), ("dtype", _i32), ("out_dtype", _i32), ("tokens", _vp), ("tokens_stride", _i64),
+                ("history", _u64), ("tokens_i64", _i32), ("lengths_i64", _i32), ("lengths", _vp),
+                ("prompt_lengths", _vp), ("repetition", _f32), ("presence", _f32), ("frequency", _f32),
+                ("temperature", _f32), ("repetition_rows", _vp), ("presence_rows", _vp), ("frequency_rows", _vp),
+                ("temperature_rows", _vp), ("bias", _vp), ("bias_stride", _i64), ("bias_dtype", _i32),
+                ("bias_ids", _vp), ("bias_values", _vp), ("bias_ids_stride", _i64), ("bias_values_stride", _i64),
+                ("n_bias", _u64), ("bias_ids_i64", _i32), ("mask", _vp), ("mask_stride", _i64), ("mask_bits", _i32)]
+
+
+_LM_SIGNATURES = {
+    "spiky_lm_last_error": ([], ctypes.c_char_p),
+    "spiky_lm_dropout": ([_vp, _i64, _vp, _u64, _u64, _i32, _f64, _u64, _u64, _vp, _vp], _i32),
+    "spiky_lm_residual_norm": ([ctypes.POINTER(LmResidualArgs), _vp, _vp, _vp], _i32),
+    "spiky_lm_residual_norm_workspace": ([ctypes.POINTER(LmResidualArgs), ctypes.POINTER(LmResidualGrads)], _u64),
+    "spiky_lm_residual_norm_backward": (
+        [ctypes.POINTER(LmResidualArgs), ctypes.POINTER(LmResidualGrads), _vp], _i32),
+    "spiky_lm_process_logits": ([ctypes.POINTER(LmLogitsArgs), _vp], _i32),
+}
+
+
 def exported_symbols():
     """Names of every C-ABI entry point this module binds."""
-    return list(_SIGNATURES) + list(_OPTIONAL_SIGNATURES)
+    return list(_SIGNATURES) + list(_OPTIONAL_SIGNATURES) + list(_LM_SIGNATURES)
 
 
 def lib():
@@ -88,7 +136,7 @@ def lib():
                 f"spiky_amd native library not found at {LIB_PATH}; build it with "
                 "`python -m spiky_amd.build` (hipcc, gfx950)")
         L = ctypes.CDLL(LIB_PATH)
-        for name, (args, res) in _SIGNATURES.items():
+        for name, (args, res) in [*_SIGNATURES.items(), *_LM_SIGNATURES.items()]:
             fn = getattr(L, name)
             fn.argtypes = args
             fn.restype = res
@@ -106,6 +154,16 @@ def check(status):
     if status == SPIKY_OK:
         return
     msg = lib().spiky_lut_last_error().decode("utf-8", "replace")
+    if status == SPIKY_VALUE_ERROR:
+        raise ValueError(msg)
+    raise RuntimeError(msg)
+
+
+def check_lm(status):
+    """check() for the entry points of include/spiky_lm.h, which keep their own last error."""
+    if status == SPIKY_OK:
+        return
+    msg = lib().spiky_lm_last_error().decode("utf-8", "replace")
     if status == SPIKY_VALUE_ERROR:
         raise ValueError(msg)
     raise RuntimeError(msg)

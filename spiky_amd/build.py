@@ -11,7 +11,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libspiky_lut.so")
 SOURCES = ["lut_fc.hip", "lut_tm.hip", "lut_seq.hip", "lut_sparse.hip", "lut_densify.hip", "lut_product.hip", "lut_seq_sparse.hip",
-           "lut_builder.hip", "lut_capi.hip"]
+           "lut_builder.hip", "lut_capi.hip", "lm/lm_dropout.hip", "lm/lm_residual.hip", "lm/lm_logits.hip",
+           "lm/lm_capi.hip"]
 ARCH = os.environ.get("SPIKY_OFFLOAD_ARCH", "gfx950")
 
 HIPCC_FLAGS = [
@@ -43,7 +44,7 @@ def build(verbose=False):
         path = os.path.join(CSRC, src)
         if not os.path.exists(path):
             continue
-        obj = os.path.join(HERE, "_build", src.replace(".hip", ".o"))
+        obj = os.path.join(HERE, "_build", os.path.basename(src).replace(".hip", ".o"))
         cmd = [hipcc, *HIPCC_FLAGS, "-c", path, "-o", obj]
         if verbose:
             print(" ".join(cmd), flush=True)

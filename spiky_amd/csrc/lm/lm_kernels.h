@@ -1,0 +1,146 @@
+// lm_kernels.h -- what the language-model operators' kernels share (gfx950):
+// element types, rows in 16-byte pieces, the dropout generator, row sums.
+//
+// Internal to libspiky_lut.so; the public C ABI is include/spiky_lm.h.
+#pragma once
+
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include "../../../include/spiky_lm.h"
+
+namespace spiky {
+namespace lm {
+
+constexpr uint32_t kCUs = 256;
+
+// ---- elements --------------------------------------------------------------
+struct bf16 {
+    uint16_t bits;
+};
+typedef _Float16 f16;
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(bf16 x) { return __uint_as_float((uint32_t)x.bits << 16); }
+__device__ __forceinline__ float to_f32(f16 x) { return (float)x; }
+
+template <typename T>
+__device__ __forceinline__ T from_f32(float x);
+template <>
+__device__ __forceinline__ float from_f32<float>(float x) {
+    return x;
+}
+// Round to nearest, ties to even (the compiler's conversion, v_cvt_pk_bf16_f32).
+template <>
+__device__ __forceinline__ bf16 from_f32<bf16>(float x) {
+    const __bf16 b = (__bf16)x;
+    bf16 r;
+    __builtin_memcpy(&r, &b, 2);
+    return r;
+}
+template <>
+__device__ __forceinline__ f16 from_f32<f16>(float x) {
+    return (f16)x;
+}
+
+// N elements from p, of which the first n exist; the others read as 0.  A whole
+// piece is one load of its full width at any alignment of the element type
+// (the target's unaligned access mode); a row's last piece goes by element.
+template <typename T, int N>
+__device__ __forceinline__ void load(float (&v)[N], const T *p, int n) {
+    T t[N];
+    if (n >= N) {
+        __builtin_memcpy(t, p, sizeof(t));
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = to_f32(t[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = i < n ? to_f32(p[i]) : 0.f;
+    }
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void store(T *p, const float (&v)[N], int n) {
+    T t[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) t[i] = from_f32<T>(v[i]);
+    if (n >= N) {
+        __builtin_memcpy(p, t, sizeof(t));
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            if (i < n) p[i] = t[i];
+    }
+}
+
+// ---- dropout ---------------------------------------------------------------
+// The kept elements of a tensor are a function of (seed, offset, row, column)
+// alone: 7 rounds of Philox4x32 (Salmon, Moraes, Dror, Shaw, "Parallel random
+// numbers: as easy as 1, 2, 3", 2011) give four 32-bit words for four columns.
+// Seven rounds are the fewest the authors find to pass BigCrush; a round is two
+// 32 x 32 -> 64 products at a quarter of the VALU rate, and ten of them take
+// longer than the copy of a 2-byte element.
+struct Dropper {
+    uint32_t threshold;  // kept: word >= threshold
+    float scale;         // 1 / (1 - p); 0: nothing is kept
+    uint32_t k0, k1, o0, o1;
+};
+
+struct DropArgs {
+    uint32_t threshold;
+    float scale;
+    uint64_t seed, offset;
+    const int64_t *rng;
+};
+
+__device__ __forceinline__ Dropper dropper(const DropArgs &a) {
+    const uint64_t seed = a.rng ? (uint64_t)a.rng[0] : a.seed;
+    const uint64_t offset = a.rng ? (uint64_t)a.rng[1] : a.offset;
+    return {a.threshold,    a.scale, (uint32_t)seed, (uint32_t)(seed >> 32), (uint32_t)offset,
+            (uint32_t)(offset >> 32)};
+}
+
+__device__ __forceinline__ void drop4(float *v, const Dropper &d, uint32_t row, uint32_t group) {
+    uint32_t c0 = group, c1 = row, c2 = d.o0, c3 = d.o1, k0 = d.k0, k1 = d.k1;
+#pragma unroll
+    for (int i = 0; i < 7; i++) {
+        const uint64_t p0 = (uint64_t)c0 * 0xD2511F53u, p1 = (uint64_t)c2 * 0xCD9E8D57u;
+        c0 = (uint32_t)(p1 >> 32) ^ c1 ^ k0;
+        c1 = (uint32_t)p1;
+        c2 = (uint32_t)(p0 >> 32) ^ c3 ^ k1;
+        c3 = (uint32_t)p0;
+        k0 += 0x9E3779B9u;
+        k1 += 0xBB67AE85u;
+    }
+    const bool any = d.scale != 0.f;
+    v[0] = any && c0 >= d.threshold ? v[0] * d.scale : 0.f;
+    v[1] = any && c1 >= d.threshold ? v[1] * d.scale : 0.f;
+    v[2] = any && c2 >= d.threshold ? v[2] * d.scale : 0.f;
+    v[3] = any && c3 >= d.threshold ? v[3] * d.scale : 0.f;
+}
+
+// The same for the N columns from col, a multiple of 4.
+template <int N>
+__device__ __forceinline__ void drop(float (&v)[N], const Dropper &d, uint32_t row, uint64_t col) {
+    static_assert(N % 4 == 0, "whole groups");
+#pragma unroll
+    for (int i = 0; i < N; i += 4) drop4(v + i, d, row, (uint32_t)(col / 4) + i / 4);
+}
+
+// ---- launchers -------------------------------------------------------------
+hipError_t launch_dropout(const void *x, int64_t x_stride, void *y, uint64_t rows, uint64_t cols,
+                          int dtype, const DropArgs &drop, hipStream_t st);
+
+hipError_t launch_residual_norm(const spiky_lm_residual_args &a, const DropArgs &drop, void *out,
+                                void *normed, hipStream_t st);
+uint64_t residual_norm_workspace(const spiky_lm_residual_args &a, const spiky_lm_residual_grads &g);
+hipError_t launch_residual_norm_backward(const spiky_lm_residual_args &a, const DropArgs &drop,
+                                         const spiky_lm_residual_grads &g, hipStream_t st);
+
+hipError_t launch_process_logits(const spiky_lm_logits_args &a, hipStream_t st);
+
+}  // namespace lm
+}  // namespace spiky

@@ -1,0 +1,4 @@
+"""Operators around the LUT blocks of a language model: dropout, the residual join, logits."""
+from .dropout import CounterDropout, counter_dropout  # noqa: F401
+from .logits import process_logits  # noqa: F401
+from .residual import ResidualNorm, residual_norm  # noqa: F401

@@ -1,0 +1,82 @@
+"""Dropout whose mask is a function of a counter and is never stored."""
+import torch
+
+from .. import _native
+from .common import as_rows, check_probability, dtype_code, generator_state, on_device, require_device, stream_of
+
+
+def _apply(x, p, seed, offset, rng):
+    x, stride = as_rows(x)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    cols = x.shape[-1] if x.dim() else 1
+    rows = x.numel() // cols if cols else 0
+    with on_device(x.device):
+        _native.check_lm(_native.lib().spiky_lm_dropout(
+            x.data_ptr(), stride, y.data_ptr(), rows, cols, dtype_code(x, "x"), p, seed, offset,
+            None if rng is None else rng.data_ptr(), stream_of(x.device)))
+    return y
+
+
+class _CounterDropoutFN(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, p, seed, offset, rng):
+        ctx.how = (p, seed, offset)
+        ctx.save_for_backward(*(() if rng is None else (rng,)))
+        return _apply(x, p, seed, offset, rng)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        p, seed, offset = ctx.how
+        rng = ctx.saved_tensors[0] if ctx.saved_tensors else None
+        return _apply(dy, p, seed, offset, rng), None, None, None, None
+
+
+def counter_dropout(x, p, seed, offset=0):
+    """x / (1 - p) where an element is kept, 0 where it is dropped (infinities and NaN too).
+
+    Whether the element at row r, column c of x, seen as rows of its last dimension, is kept is a
+    function of (seed, offset, r, c): word c % 4 of Philox4x32-7 under key `seed` and counter
+    (c // 4, r, offset), kept from floor(p * 2**32 + 1/2) on.  So the same call gives the same
+    mask, for any type, stride or size of launch, and the backward pass makes it again.  Use
+    another offset for each call of a step.
+
+    x: float32, bfloat16 or float16 on a HIP device, any shape.  seed, offset: whole numbers of
+    64 bits, or seed an int64 device tensor of [seed, offset], read when the kernels run (for
+    graphs whose replays advance it in place, after the backward pass)."""
+    require_device(x, "x")
+    dtype_code(x, "x")
+    check_probability(p)
+    seed, offset, rng = generator_state(seed, offset, x.device)
+    if x.requires_grad and torch.is_grad_enabled():
+        return _CounterDropoutFN.apply(x, float(p), seed, offset, rng)
+    return _apply(x, float(p), seed, offset, rng)
+
+
+class CounterDropout(torch.nn.Module):
+    """nn.Dropout over counter_dropout: call number n of a module in training uses offset n.
+
+    Modules of one model take different seeds.  The calls' number is part of the state dict, so a
+    resumed run goes on with masks that it has not used."""
+
+    def __init__(self, p=0.5, seed=0):
+        super().__init__()
+        check_probability(p)
+        self.p = float(p)
+        self.seed = int(seed)
+        self.calls = 0
+
+    def get_extra_state(self):
+        return {"seed": self.seed, "calls": self.calls}
+
+    def set_extra_state(self, state):
+        self.seed, self.calls = int(state["seed"]), int(state["calls"])
+
+    def forward(self, x):
+        if not self.training or self.p == 0.0:
+            return x
+        self.calls += 1
+        return counter_dropout(x, self.p, self.seed, self.calls)
+
+    def extra_repr(self):
+        return f"p={self.p}, seed={self.seed}"
