@@ -308,6 +308,321 @@ __global__ __launch_bounds__(1024) void k_join_wide(Join<TZ, TA> j) {
 }
 
 // ---- backward --------------------------------------------------------------
+// The words of N elements as they were loaded, so that a load may be in flight
+// while the values of the row before are worked on.
+template <typename T, int N>
+struct Raw {
+    uint32_t w[N * sizeof(T) / 4];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (uint32_t i = 0; i < N * sizeof(T) / 4; i++) w[i] = 0;
+    }
+    // n of them exist, the others are 0.
+    __device__ __forceinline__ void load(const T *p, int n) {
+        if (n >= N) {
+            __builtin_memcpy(w, p, sizeof(w));
+            return;
+        }
+        clear();
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            if (i >= n) continue;
+            if (sizeof(T) == 4) {
+                __builtin_memcpy(&w[i], p + i, 4);
+            } else {
+                uint16_t h;
+                __builtin_memcpy(&h, p + i, 2);
+                w[i / 2] |= (uint32_t)h << (16 * (i % 2));
+            }
+        }
+    }
+    __device__ __forceinline__ float operator[](int i) const {
+        T t;
+        if (sizeof(T) == 4) {
+            __builtin_memcpy(&t, &w[i], sizeof(T));
+        } else {
+            const uint16_t h = (uint16_t)(w[i / 2] >> (16 * (i % 2)));
+            __builtin_memcpy(&t, &h, 2);
+        }
+        return to_f32(t);
+    }
+};
+
+// Sums of K values over the `waves` waves of a row (TPR > 64) or its TPR lanes,
+// in every lane.  The waves' sums go through LDS, two buffers in turn: a buffer
+// is written again only after the barrier of the call in between, which its
+// readers have passed.  Lane i reads the sums of wave i % 16.
+template <int TPR, int K>
+__device__ __forceinline__ void row_sums(float (&x)[K], float4 (*lds)[(K + 3) / 4][16], uint32_t &turn,
+                                         uint32_t waves) {
+#pragma unroll
+    for (int k = 0; k < K; k++) x[k] = lanes_sum<(TPR < 64 ? TPR : 64)>(x[k]);
+    if constexpr (TPR > 64) {
+        constexpr int H = (K + 3) / 4;
+        float v[4 * H];
+#pragma unroll
+        for (int k = 0; k < 4 * H; k++) v[k] = k < K ? x[k < K ? k : 0] : 0.f;
+        if ((threadIdx.x & 63) == 0)
+#pragma unroll
+            for (int h = 0; h < H; h++)
+                lds[turn][h][threadIdx.x / 64] = make_float4(v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]);
+        __syncthreads();
+        const uint32_t wave = threadIdx.x & 15;
+#pragma unroll
+        for (int h = 0; h < H; h++) {
+            const float4 f = wave < waves ? lds[turn][h][wave] : make_float4(0.f, 0.f, 0.f, 0.f);
+            v[4 * h] = f.x, v[4 * h + 1] = f.y, v[4 * h + 2] = f.z, v[4 * h + 3] = f.w;
+        }
+#pragma unroll
+        for (int k = 0; k < K; k++) x[k] = lanes_sum<16>(v[k]);
+        turn ^= 1;
+    }
+}
+
+// The rows [row, end) of chunk number `chunk`.
+template <typename J>
+__device__ __forceinline__ void chunk_rows(const J &j, uint32_t chunk, uint32_t &row, uint32_t &end) {
+    if (j.chunks_per_span) {
+        const uint32_t first = chunk / j.chunks_per_span * j.span;
+        const uint64_t from = (uint64_t)(chunk % j.chunks_per_span) * j.chunk;
+        row = first + (uint32_t)min(from, (uint64_t)j.span);
+        end = first + (uint32_t)min(from + j.chunk, (uint64_t)j.span);
+    } else {
+        const uint64_t from = (uint64_t)chunk * j.chunk;
+        row = (uint32_t)min(from, (uint64_t)j.rows);
+        end = (uint32_t)min(from + j.chunk, (uint64_t)j.rows);
+    }
+}
+
+// Rows of up to 1024 * N * P columns: a workgroup walks the rows of its chunk (a
+// slot of TPR lanes its share of them), a thread always with the same columns,
+// so parameters and column sums stay in registers and every input crosses HBM
+// once.  q is linear in the sums of the pre norm, so those of the post norm
+// follow from sums that need none of them, and a row has one reduction: with
+// c = keep / (1 - p) beta g w1 and e = dz + r2 t,
+//   sum dn n1 = sum c n1 e - r2 (mean t sum c n1 + mean(t n2) sum c n1 n2)
+// and alike without n1.  The next row's loads are issued before the reduction,
+// into the registers that this row's left.  FULL: with layer norms or biases.
+template <typename TZ, typename TA, int N, int P, int TPR, bool FULL>
+__global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_join_back(Join<TZ, TA> j) {
+    constexpr int kSlots = TPR <= 64 ? 256 / TPR : 1, W = N * P, K = FULL ? 8 : 3;
+    __shared__ float4 red[TPR > 64 ? 2 : 1][(K + 3) / 4][16];
+    __shared__ float joint[kSlots > 1 ? kSlots : 1][kSlots > 1 ? TPR * W : 1];
+    const uint32_t threads = TPR <= 64 ? TPR : blockDim.x, waves = blockDim.x / 64;
+    const uint32_t lane = TPR <= 64 ? threadIdx.x % TPR : threadIdx.x;
+    uint32_t row, end, turn = 0;
+    chunk_rows(j, blockIdx.x, row, end);
+    if (kSlots > 1) {
+        uint32_t share = (end - row + kSlots - 1) / kSlots;
+        if (!j.chunks_per_span) share = (share + j.span - 1) / j.span * j.span;  // whole spans
+        row += min(end - row, threadIdx.x / TPR * share);
+        end = row + min(end - row, share);
+    }
+    if (TPR == 64) row = __builtin_amdgcn_readfirstlane(row), end = __builtin_amdgcn_readfirstlane(end);
+    const Dropper dr = dropper(j.drop);
+    const bool row_gates = j.g && j.gate_rows == 1;
+    uint32_t gate_row = j.g ? row / j.gate_rows : 0, in_gate = j.g ? row - gate_row * j.gate_rows : 0;
+
+    uint64_t col[P];
+    int n[P];
+    float w1[P][N], w2[P][N], b1[FULL ? P : 1][N], g[P][N];
+    float acc_w1[P][N], acc_w2[P][N], acc_g[P][N], acc_b1[FULL ? P : 1][N], acc_b2[FULL ? P : 1][N];
+    Raw<TZ, N> z_raw[P], dz_raw[P];
+    Raw<TA, N> a_raw[P], dh_raw[P];
+    Raw<float, N> g_raw[P];  // half of the words where the gate is of a shorter type
+    float4 st = {0.f, 1.f, 0.f, 1.f};
+
+    auto gate_words = [&](int p, uint32_t at_row) {
+        const uint64_t at = (uint64_t)at_row * j.cols + col[p];
+        if (sizeof(TA) == 4 || j.gate_f32) {
+            g_raw[p].load(static_cast<const float *>(j.g) + at, n[p]);
+        } else {
+            Raw<TA, N> half;
+            half.load(static_cast<const TA *>(j.g) + at, n[p]);
+            __builtin_memcpy(g_raw[p].w, half.w, sizeof(half.w));
+        }
+    };
+    auto gate_values = [&](int p) {
+        if (sizeof(TA) == 4 || j.gate_f32) {
+#pragma unroll
+            for (int i = 0; i < N; i++) g[p][i] = g_raw[p][i];
+        } else {
+            Raw<TA, N> half;
+            __builtin_memcpy(half.w, g_raw[p].w, sizeof(half.w));
+#pragma unroll
+            for (int i = 0; i < N; i++) g[p][i] = half[i];
+        }
+    };
+    auto fetch = [&](uint32_t r) {
+        st = j.stats[r];
+#pragma unroll
+        for (int p = 0; p < P; p++) {
+            if (j.dz) dz_raw[p].load(j.dz + (int64_t)r * j.dz_stride + col[p], n[p]);
+            if (j.a) a_raw[p].load(j.a + (int64_t)r * j.a_stride + col[p], n[p]);
+            if (j.dh) {
+                z_raw[p].load(j.r + (int64_t)r * j.r_stride + col[p], n[p]);
+                dh_raw[p].load(j.dh + (int64_t)r * j.dh_stride + col[p], n[p]);
+            }
+            if (row_gates) gate_words(p, r);
+        }
+    };
+#pragma unroll
+    for (int p = 0; p < P; p++) {
+        col[p] = (uint64_t)(p * threads + lane) * N;
+        n[p] = piece_size(j.cols, col[p], N);
+        z_raw[p].clear(), dz_raw[p].clear(), a_raw[p].clear(), dh_raw[p].clear(), g_raw[p].clear();
+    }
+    if (row < end) fetch(row);
+#pragma unroll
+    for (int p = 0; p < P; p++) {
+        // columns past the row's end have weights of 0, so they add nothing to any sum
+        if (j.w1) param<TA>(w1[p], j.w1, j.par_f32, col[p], n[p]);
+        if (j.w2) param<TA>(w2[p], j.w2, j.par_f32, col[p], n[p]);
+        if (FULL && j.b1) param<TA>(b1[p], j.b1, j.par_f32, col[p], n[p]);
+        if (j.g && !row_gates && row < end) gate_words(p, gate_row), gate_values(p);
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            if (!j.w1) w1[p][i] = i < n[p] ? 1.f : 0.f;
+            if (!j.w2) w2[p][i] = 1.f;
+            if (FULL && !j.b1) b1[FULL ? p : 0][i] = 0.f;
+            if (!j.g) g[p][i] = 1.f;
+            acc_w1[p][i] = acc_w2[p][i] = acc_g[p][i] = 0.f;
+            if (FULL) acc_b1[FULL ? p : 0][i] = acc_b2[FULL ? p : 0][i] = 0.f;
+        }
+    }
+    const float alpha = j.a ? j.alpha : 1.f;
+
+    for (; row < end; row++) {
+        float n1[P][N], n2[P][N], e[P][N], keep[P][N];
+        float s[K];
+#pragma unroll
+        for (int k = 0; k < K; k++) s[k] = 0.f;
+        const float r1 = st.y, r2 = j.dh ? st.w : 0.f;
+#pragma unroll
+        for (int p = 0; p < P; p++) {
+            if (row_gates) gate_values(p);
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                keep[p][i] = 1.f;
+                n1[p][i] = (a_raw[p][i] - st.x) * st.y;
+            }
+            if (j.drops) drop(keep[p], dr, row, col[p]);
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                float v = n1[p][i] * w1[p][i];
+                if (FULL) v += b1[FULL ? p : 0][i];
+                const bool kept = keep[p][i] != 0.f;
+                v = kept ? v * keep[p][i] : 0.f;  // a dropped element is 0 whatever it holds
+                float z = z_raw[p][i];
+                if (j.a) z = alpha * z + j.beta * (g[p][i] * v);
+                n2[p][i] = j.dh ? (z - st.z) * r2 : 0.f;
+                const float dh = dh_raw[p][i], t = dh * w2[p][i];
+                e[p][i] = dz_raw[p][i] + r2 * t;
+                acc_w2[p][i] += dh * n2[p][i];
+                const float c = keep[p][i] * (j.beta * g[p][i]) * w1[p][i];
+                const float ce = kept ? c * e[p][i] : 0.f, cn = c * n1[p][i];
+                s[0] += t * n2[p][i];
+                s[1] += ce * n1[p][i];
+                s[2] += cn * n2[p][i];
+                if constexpr (FULL) {
+                    acc_b2[p][i] += dh;
+                    s[3] += t;
+                    s[4] += ce;
+                    s[5] += c;
+                    s[6] += c * n2[p][i];
+                    s[7] += cn;
+                }
+            }
+        }
+        if (row + 1 < end) fetch(row + 1);
+        row_sums<TPR, K>(s, red, turn, waves);
+        // means over the row
+        float mean_t = 0.f, mean_tn, mean_dn = 0.f, mean_dnn = 0.f;
+        mean_tn = s[0] * j.inv_cols;
+        if (FULL && j.pre == SPIKY_NORM_LAYER) mean_t = s[FULL ? 3 : 0] * j.inv_cols;
+        if (j.post != SPIKY_NORM_NONE) {
+            mean_dnn = s[1] - r2 * (mean_tn * s[2]);
+            if constexpr (FULL) {
+                mean_dnn -= r2 * (mean_t * s[7]);
+                if (j.post == SPIKY_NORM_LAYER)
+                    mean_dn = (s[4] - r2 * (mean_t * s[5] + mean_tn * s[6])) * j.inv_cols;
+            }
+            mean_dnn *= j.inv_cols;
+        }
+        const bool gate_ends = j.dgate && in_gate + 1 == j.gate_rows;
+#pragma unroll
+        for (int p = 0; p < P; p++) {
+            const uint64_t at = (uint64_t)row * j.cols + col[p];
+            float out[N], da[N];
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const float q = e[p][i] - r2 * (mean_t + n2[p][i] * mean_tn);
+                out[i] = alpha * q;
+                const bool kept = keep[p][i] != 0.f;
+                float v = n1[p][i] * w1[p][i];
+                if (FULL) v += b1[FULL ? p : 0][i];
+                v = kept ? v * keep[p][i] : 0.f;
+                acc_g[p][i] += j.beta * (v * q);
+                const float dv = kept ? j.beta * (g[p][i] * q) * keep[p][i] : 0.f;
+                acc_w1[p][i] += dv * n1[p][i];
+                if (FULL) acc_b1[FULL ? p : 0][i] += dv;
+                da[i] = dv;
+                if (j.post != SPIKY_NORM_NONE) da[i] = r1 * (dv * w1[p][i] - mean_dn - n1[p][i] * mean_dnn);
+            }
+            if (j.dr) store(j.dr + at, out, n[p]);
+            if (j.da) store(j.da + at, da, n[p]);
+            if (gate_ends) {
+                const uint64_t to = (uint64_t)gate_row * j.cols + col[p];
+                if (sizeof(TA) == 4 || j.gate_f32)
+                    store(static_cast<float *>(j.dgate) + to, acc_g[p], n[p]);
+                else
+                    store(static_cast<TA *>(j.dgate) + to, acc_g[p], n[p]);
+#pragma unroll
+                for (int i = 0; i < N; i++) acc_g[p][i] = 0.f;
+            }
+        }
+        if (j.g && ++in_gate == j.gate_rows) {
+            in_gate = 0;
+            gate_row++;
+            if (!row_gates && row + 1 < end)
+#pragma unroll
+                for (int p = 0; p < P; p++) gate_words(p, gate_row), gate_values(p);
+        }
+    }
+
+    auto column_sums = [&](float *part, float (&acc)[P][N]) {
+        if (!part) return;
+        part += (uint64_t)blockIdx.x * j.cols;
+        if constexpr (kSlots == 1) {
+#pragma unroll
+            for (int p = 0; p < P; p++) store(part + col[p], acc[p], n[p]);
+        } else {
+            __syncthreads();
+#pragma unroll
+            for (int p = 0; p < P; p++)
+#pragma unroll
+                for (int i = 0; i < N; i++) joint[threadIdx.x / TPR][(p * TPR + lane) * N + i] = acc[p][i];
+            __syncthreads();
+            for (uint32_t c = threadIdx.x; c < TPR * W && c < j.cols; c += 256) {
+                float sum = 0.f;
+#pragma unroll
+                for (int k = 0; k < kSlots; k++) sum += joint[k][c];
+                part[c] = sum;
+            }
+        }
+    };
+    column_sums(j.part[0], acc_w1);
+    column_sums(j.part[2], acc_w2);
+    column_sums(j.part[4], acc_g);
+    if constexpr (FULL) {
+        column_sums(j.part[1], acc_b1);
+        column_sums(j.part[3], acc_b2);
+    }
+}
+
+// Wider rows take two passes over the inputs: the sums over each row, then
+// columns.
+//
 // What a piece of N columns of one row holds on the way back.
 template <typename TZ, typename TA, int N>
 struct Piece {
@@ -450,16 +765,7 @@ __global__ __launch_bounds__(64) void k_join_back_cols(Join<TZ, TA> j) {
     const int n = piece_size(j.cols, col, N);
     if (n == 0) return;
     uint32_t row, end;
-    if (j.chunks_per_span) {
-        const uint32_t first = blockIdx.y / j.chunks_per_span * j.span;
-        const uint64_t from = (uint64_t)(blockIdx.y % j.chunks_per_span) * j.chunk;
-        row = first + (uint32_t)from;
-        end = first + (uint32_t)min(from + j.chunk, (uint64_t)j.span);
-    } else {
-        const uint64_t from = (uint64_t)blockIdx.y * j.chunk;
-        row = (uint32_t)from;
-        end = (uint32_t)min(from + j.chunk, (uint64_t)j.rows);
-    }
+    chunk_rows(j, blockIdx.y, row, end);
     const Dropper dr = dropper(j.drop);
     float acc[5][N];
 #pragma unroll
@@ -532,22 +838,27 @@ struct Sums {
     uint32_t count[5], groups[5];
 };
 
+// A workgroup takes 32 columns, its thread (k, c) every 32nd row from k on.
 template <typename TA>
-__global__ __launch_bounds__(256) void k_join_sums(Sums s, uint64_t cols) {
-    __shared__ float lds[4][64];
+__global__ __launch_bounds__(1024) void k_join_sums(Sums s, uint64_t cols) {
+    __shared__ float lds[32][33];
     const int k = blockIdx.z;
     if (!s.part[k] || blockIdx.y >= s.groups[k]) return;
-    const uint64_t col = (uint64_t)blockIdx.x * 64 + (threadIdx.x & 63);
-    const uint32_t wave = threadIdx.x / 64, count = s.count[k];
+    const uint32_t c = threadIdx.x & 31, first = threadIdx.x / 32, count = s.count[k];
+    const uint64_t col = (uint64_t)blockIdx.x * 32 + c;
     const float *p = s.part[k] + (uint64_t)blockIdx.y * count * cols + col;
     float sum = 0.f;
     if (col < cols)
-        for (uint32_t c = wave; c < count; c += 4) sum += p[(uint64_t)c * cols];
-    lds[wave][threadIdx.x & 63] = sum;
+#pragma unroll 8
+        for (uint32_t r = first; r < count; r += 32) sum += p[(uint64_t)r * cols];
+    lds[first][c] = sum;
     __syncthreads();
-    if (wave != 0 || col >= cols) return;
-    sum = (lds[0][threadIdx.x] + lds[1][threadIdx.x]) + (lds[2][threadIdx.x] + lds[3][threadIdx.x]);
-    const uint64_t at = (uint64_t)blockIdx.y * cols + col;
+    // row `first` of the transposed sums: its 32 lanes hold one column's
+    sum = lds[c][first];
+    sum = lanes_sum<32>(sum);
+    const uint64_t to = (uint64_t)blockIdx.x * 32 + first;
+    if (c != 0 || to >= cols) return;
+    const uint64_t at = (uint64_t)blockIdx.y * cols + to;
     if (s.f32[k])
         static_cast<float *>(s.out[k])[at] = sum;
     else
@@ -576,7 +887,7 @@ Join<TZ, TA> view(const spiky_lm_residual_args &a, const DropArgs &drop) {
     j.alpha = (float)a.residual_scale;
     j.beta = (float)a.branch_scale;
     j.inv_cols = (float)(1.0 / (double)a.cols);
-    j.drops = a.dropout_p > 0.0;
+    j.drops = a.branch && a.dropout_p > 0.0;
     j.drop = drop;
     j.rows = (uint32_t)a.rows;
     j.gate_rows = a.gate ? (uint32_t)a.gate_rows : (uint32_t)a.rows;
@@ -627,17 +938,26 @@ hipError_t forward(const spiky_lm_residual_args &a, const DropArgs &drop, void *
 
 // How the rows are cut into chunks, and the workspace's regions.
 struct Plan {
+    uint32_t tpr;  // lanes of a row in k_join_back, 1024 for all rows of more than 64; 0: the passes for wider rows
     uint32_t chunk, chunks, span, chunks_per_span;
     bool part[5];
     uint64_t row_sums, parts[5], bytes;
 };
 
+// Columns of a thread of k_join_back.
+constexpr uint64_t kBackCols = 8;
+
 Plan plan(const spiky_lm_residual_args &a, const spiky_lm_residual_grads &g) {
-    constexpr uint32_t kChunks = 512;
     Plan p = {};
+    const uint64_t threads = (a.cols + kBackCols - 1) / kBackCols;
+    p.tpr = threads <= 16 ? 16 : threads <= 32 ? 32 : threads <= 64 ? 64 : threads <= 1024 ? 1024 : 0;
     const uint64_t span = a.gate && g.d_gate ? a.gate_rows : a.rows;
-    uint64_t chunk = (a.rows + kChunks - 1) / kChunks;
-    if (chunk < 8) chunk = 8;
+    // two workgroups to a CU; one, where that leaves each fewer than two rounds of rows
+    const uint64_t slots = p.tpr && p.tpr <= 64 ? 256 / p.tpr : 1;
+    const uint64_t most = a.rows >= 4 * kCUs * slots ? 2 * kCUs : kCUs;
+    uint64_t chunk = (a.rows + most - 1) / most;
+    if (chunk < slots) chunk = slots;
+    if (!p.tpr && chunk < 8) chunk = 8;
     if (span >= chunk) {
         p.chunks_per_span = (uint32_t)((span + chunk - 1) / chunk);
         chunk = (span + p.chunks_per_span - 1) / p.chunks_per_span;
@@ -654,13 +974,32 @@ Plan plan(const spiky_lm_residual_args &a, const spiky_lm_residual_grads &g) {
     p.part[3] = g.d_pre_bias != nullptr;
     p.part[4] = g.d_gate != nullptr && p.chunks_per_span > 0;
     p.row_sums = 0;
-    uint64_t at = (a.rows * sizeof(float4) + 255) & ~255ull;
+    uint64_t at = p.tpr ? 0 : (a.rows * sizeof(float4) + 255) & ~255ull;
     for (int k = 0; k < 5; k++) {
         p.parts[k] = at;
         if (p.part[k]) at += ((uint64_t)p.chunks * a.cols * sizeof(float) + 255) & ~255ull;
     }
     p.bytes = at;
     return p;
+}
+
+template <typename TZ, typename TA, bool FULL>
+void run_back(const Join<TZ, TA> &j, const Plan &p, hipStream_t st) {
+    constexpr int N = sizeof(TA) == 4 ? 4 : 8, P = kBackCols / N;
+    const dim3 grid(p.chunks);
+    const uint32_t threads = (uint32_t)((j.cols + kBackCols - 1) / kBackCols + 63) & ~63u;
+    if (p.tpr == 16)
+        k_join_back<TZ, TA, N, P, 16, FULL><<<grid, dim3(256), 0, st>>>(j);
+    else if (p.tpr == 32)
+        k_join_back<TZ, TA, N, P, 32, FULL><<<grid, dim3(256), 0, st>>>(j);
+    else if (p.tpr == 64)
+        k_join_back<TZ, TA, N, P, 64, FULL><<<grid, dim3(256), 0, st>>>(j);
+    else if (threads <= 256)
+        k_join_back<TZ, TA, N, P, 256, FULL><<<grid, dim3(threads), 0, st>>>(j);
+    else if (threads <= 512)
+        k_join_back<TZ, TA, N, P, 512, FULL><<<grid, dim3(threads), 0, st>>>(j);
+    else
+        k_join_back<TZ, TA, N, P, 1024, FULL><<<grid, dim3(threads), 0, st>>>(j);
 }
 
 template <typename TZ, typename TA>
@@ -682,13 +1021,21 @@ hipError_t backward(const spiky_lm_residual_args &a, const DropArgs &drop, const
     j.chunk = p.chunk;
     j.span = p.span;
     j.chunks_per_span = p.chunks_per_span;
-    hipError_t err = over_rows(j, 1, 256, [&](dim3 grid, dim3 block) {
-        k_join_back_rows<TZ, TA, N, 256><<<grid, block, 0, st>>>(j);
-    });
-    if (err != hipSuccess) return err;
-    const uint64_t tiles = (a.cols + 64 * N - 1) / (64 * N);
-    // fewer than 2048 chunks, in y
-    k_join_back_cols<TZ, TA, N><<<dim3((uint32_t)tiles, p.chunks), dim3(64), 0, st>>>(j);
+    hipError_t err;
+    if (p.tpr) {
+        if (a.post_norm == SPIKY_NORM_LAYER || a.pre_norm == SPIKY_NORM_LAYER || a.post_bias || a.pre_bias)
+            run_back<TZ, TA, true>(j, p, st);
+        else
+            run_back<TZ, TA, false>(j, p, st);
+    } else {
+        err = over_rows(j, 1, 256, [&](dim3 grid, dim3 block) {
+            k_join_back_rows<TZ, TA, N, 256><<<grid, block, 0, st>>>(j);
+        });
+        if (err != hipSuccess) return err;
+        const uint64_t tiles = (a.cols + 64 * N - 1) / (64 * N);
+        // fewer than 2048 chunks, in y
+        k_join_back_cols<TZ, TA, N><<<dim3((uint32_t)tiles, p.chunks), dim3(64), 0, st>>>(j);
+    }
     err = hipGetLastError();
     if (err != hipSuccess) return err;
     Sums s = {};
@@ -703,7 +1050,7 @@ hipError_t backward(const spiky_lm_residual_args &a, const DropArgs &drop, const
         if (s.part[k] && s.groups[k] > groups) groups = s.groups[k];
     }
     if (groups == 0) return hipSuccess;
-    k_join_sums<TA><<<dim3((uint32_t)((a.cols + 63) / 64), groups, 5), dim3(256), 0, st>>>(s, a.cols);
+    k_join_sums<TA><<<dim3((uint32_t)((a.cols + 31) / 32), groups, 5), dim3(1024), 0, st>>>(s, a.cols);
     return hipGetLastError();
 }
 
