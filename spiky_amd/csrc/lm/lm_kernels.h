@@ -76,6 +76,46 @@ __device__ __forceinline__ void store(T *p, const float (&v)[N], int n) {
     }
 }
 
+// The words of N elements as they were loaded, so that a load may be in flight
+// while the values of the row before are worked on.
+template <typename T, int N>
+struct Raw {
+    uint32_t w[N * sizeof(T) / 4];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (uint32_t i = 0; i < N * sizeof(T) / 4; i++) w[i] = 0;
+    }
+    // n of them exist, the others are 0.
+    __device__ __forceinline__ void load(const T *p, int n) {
+        if (n >= N) {
+            __builtin_memcpy(w, p, sizeof(w));
+            return;
+        }
+        clear();
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            if (i >= n) continue;
+            if (sizeof(T) == 4) {
+                __builtin_memcpy(&w[i], p + i, 4);
+            } else {
+                uint16_t h;
+                __builtin_memcpy(&h, p + i, 2);
+                w[i / 2] |= (uint32_t)h << (16 * (i % 2));
+            }
+        }
+    }
+    __device__ __forceinline__ float operator[](int i) const {
+        T t;
+        if (sizeof(T) == 4) {
+            __builtin_memcpy(&t, &w[i], sizeof(T));
+        } else {
+            const uint16_t h = (uint16_t)(w[i / 2] >> (16 * (i % 2)));
+            __builtin_memcpy(&t, &h, 2);
+        }
+        return to_f32(t);
+    }
+};
+
 // ---- dropout ---------------------------------------------------------------
 // The kept elements of a tensor are a function of (seed, offset, row, column)
 // alone: 7 rounds of Philox4x32 (Salmon, Moraes, Dror, Shaw, "Parallel random

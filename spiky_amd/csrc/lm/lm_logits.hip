@@ -7,159 +7,315 @@ namespace spiky {
 namespace lm {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr uint32_t kThreads = 256;
 constexpr uint32_t kSeen = 0x80000000u;    // among the prompt's tokens
 constexpr uint32_t kBiased = 0x40000000u;  // among the bias ids
 constexpr uint32_t kCount = 0x3fffffffu;   // times among the tokens after the prompt
-constexpr uint32_t kList = 256;            // bias entries of a chunk held in LDS
 
-__device__ __forceinline__ int64_t id_at(const void *p, bool i64, uint64_t i) {
-    return i64 ? static_cast<const int64_t *>(p)[i] : static_cast<const int32_t *>(p)[i];
-}
-
-__device__ __forceinline__ uint64_t length_at(const void *p, bool i64, uint32_t row, uint64_t most) {
+__device__ __forceinline__ uint32_t length_at(const void *p, bool i64, uint32_t row, uint32_t most) {
     if (!p) return most;
-    const int64_t n = id_at(p, i64, row);
-    return n < 0 ? 0 : (uint64_t)n < most ? (uint64_t)n : most;
+    const int64_t n = i64 ? static_cast<const int64_t *>(p)[row] : static_cast<const int32_t *>(p)[row];
+    return n < 0 ? 0 : n < (int64_t)most ? (uint32_t)n : most;
 }
 
-// One workgroup to a chunk of a row's vocabulary.  The chunk's counts of the
-// row's tokens, and which entries have sparse biases, are words in LDS, so the
-// logits are read and written once and no count is kept in memory.
-template <typename TI, typename TO, int N>
-__global__ __launch_bounds__(kThreads) void k_logits(spiky_lm_logits_args a, uint32_t chunk) {
-    extern __shared__ uint32_t words[];  // [chunk], where there are tokens or bias ids
-    __shared__ uint32_t list_id[kList];
-    __shared__ float list_value[kList];
-    __shared__ uint32_t listed;
-    const uint32_t tid = threadIdx.x, row = blockIdx.y;
-    const uint64_t base = (uint64_t)blockIdx.x * chunk;
-    const uint32_t size = (uint32_t)min((uint64_t)chunk, a.vocab - base);
-    const bool marks = a.tokens || a.bias_ids;
-    if (marks) {
-        for (uint32_t i = tid; i < size; i += kThreads) words[i] = 0;
-        __syncthreads();
-        if (a.tokens) {
-            const uint64_t len = length_at(a.lengths, a.lengths_i64, row, a.history);
-            const uint64_t prompt = a.prompt_lengths ? length_at(a.prompt_lengths, a.lengths_i64, row, len) : 0;
-            const uint64_t first = (uint64_t)row * a.tokens_stride;
-            for (uint64_t i = tid; i < len; i += kThreads) {
-                const uint64_t o = (uint64_t)id_at(a.tokens, a.tokens_i64, first + i) - base;
-                if (o >= size) continue;
-                if (i < prompt)
-                    atomicOr(&words[o], kSeen);
-                else
-                    atomicAdd(&words[o], 1u);
-            }
+// An element `at` elements past a pointer that is the same for all lanes: one
+// 32-bit offset a lane.
+template <typename T>
+__device__ __forceinline__ T *past(T *p, uint32_t at) {
+    using C = std::conditional_t<std::is_const_v<T>, const char, char>;
+    return reinterpret_cast<T *>(reinterpret_cast<C *>(p) + at * (uint32_t)sizeof(T));
+}
+
+// The tokens a thread holds at a time: numbers at + thread, at + thread + kThreads, ...
+template <typename T>
+struct Tokens {
+    static constexpr uint32_t kAhead = 64 / sizeof(T);
+    T id[kAhead];
+
+    // Those past `end` are -1.
+    __device__ __forceinline__ void load(const T *tokens, uint32_t at, uint32_t end) {
+#pragma unroll
+        for (uint32_t k = 0; k < kAhead; k++) {
+            const uint32_t i = at + k * kThreads + threadIdx.x;
+            id[k] = (T)-1;
+            if (i < end) id[k] = tokens[i];
         }
-        // the chunk's sparse biases in their order, by the first wave
-        if (a.bias_ids && tid < 64) {
-            const uint64_t first = (uint64_t)row * a.bias_ids_stride, firstv = (uint64_t)row * a.bias_values_stride;
-            uint32_t count = 0;
-            for (uint64_t k0 = 0; k0 < a.n_bias; k0 += 64) {
-                const uint64_t k = k0 + tid;
-                const uint64_t o = k < a.n_bias ? (uint64_t)id_at(a.bias_ids, a.bias_ids_i64, first + k) - base : size;
-                const bool in = o < size;
-                const uint64_t all = __ballot(in);
-                const uint32_t at = count + __popcll(all & ((1ull << tid) - 1));
-                if (in) {
-                    atomicOr(&words[o], kBiased);
-                    if (at < kList) {
-                        list_id[at] = (uint32_t)o;
-                        list_value[at] = a.bias_values[firstv + k];
-                    }
-                }
-                count += __popcll(all);
-            }
-            if (tid == 0) listed = count;
-        }
-        __syncthreads();
     }
+    // Adds those before len to the words of the chunk's entries.
+    __device__ __forceinline__ void count(uint32_t at, uint32_t len, uint32_t prompt, uint32_t base, uint32_t size,
+                                          uint32_t *words) const {
+#pragma unroll
+        for (uint32_t k = 0; k < kAhead; k++) {
+            if (at + k * kThreads >= len) break;
+            const uint32_t i = at + k * kThreads + threadIdx.x;
+            // base < 2^31, so a negative token stays past any chunk
+            const uint32_t o = (uint32_t)id[k] - base;
+            bool there = o < size && i < len;
+            if (sizeof(T) == 8) there = there && (uint32_t)((uint64_t)id[k] >> 32) == 0;
+            if (!there) continue;
+            if (i < prompt)
+                atomicOr(&words[o], kSeen);
+            else
+                atomicAdd(&words[o], 1u);
+        }
+    }
+};
+
+// Bias id number k of the row, or -1, and its value.
+__device__ __forceinline__ int64_t bias_id(const spiky_lm_logits_args &a, uint32_t row, uint64_t k) {
+    const uint64_t at = (uint64_t)row * a.bias_ids_stride + k;
+    if (k >= a.n_bias) return -1;
+    return a.bias_ids_i64 ? static_cast<const int64_t *>(a.bias_ids)[at] : static_cast<const int32_t *>(a.bias_ids)[at];
+}
+
+__device__ __forceinline__ float bias_value(const spiky_lm_logits_args &a, uint32_t row, uint64_t k) {
+    return k < a.n_bias ? a.bias_values[(uint64_t)row * a.bias_values_stride + k] : 0.f;
+}
+
+// The sums of the row's sparse biases for the chunk's entries: sums[slots[o]] for
+// an entry o that is flagged.  The ids go by kThreads (id and value: a thread's
+// first): those in the chunk are listed in their order, and the first of each
+// entry adds up the others, so repeated ids are added in their order whatever the
+// threads do.
+__device__ __forceinline__ void add_sparse(const spiky_lm_logits_args &a, uint32_t row, uint32_t base, uint32_t size,
+                                           int64_t id, float value, uint32_t *words, uint16_t *slots, float *sums) {
+    __shared__ uint32_t list_id[kThreads];
+    __shared__ float list_value[kThreads];
+    __shared__ uint32_t wave_count[2][kThreads / 64], taken;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid / 64;
+    if (tid == 0) taken = 0;
+    uint32_t turn = 0;
+    for (uint64_t k0 = 0; k0 < a.n_bias; k0 += kThreads, turn ^= 1) {
+        if (k0) id = bias_id(a, row, k0 + tid), value = bias_value(a, row, k0 + tid);
+        const uint64_t o = (uint64_t)id - base;
+        const bool there = o < size;
+        const uint64_t all = __ballot(there);
+        if (lane == 0) wave_count[turn][wave] = __popcll(all);
+        __syncthreads();
+        uint32_t at = __popcll(all & ((1ull << lane) - 1)), listed = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < kThreads / 64; w++) {
+            if (w < wave) at += wave_count[turn][w];
+            listed += wave_count[turn][w];
+        }
+        if (listed == 0) continue;
+        if (there) {
+            list_id[at] = (uint32_t)o;
+            list_value[at] = value;
+        }
+        __syncthreads();
+        if (tid < listed) {
+            const uint32_t mine = list_id[tid];
+            bool leads = true;
+            float sum = 0.f;
+            for (uint32_t j = 0; j < listed; j++) {
+                if (list_id[j] != mine) continue;
+                leads = leads && j >= tid;
+                sum += list_value[j];
+            }
+            if (leads) {
+                if (words[mine] & kBiased) {  // by a round before
+                    sums[slots[mine]] += sum;
+                } else {
+                    const uint32_t slot = atomicAdd(&taken, 1u);
+                    slots[mine] = (uint16_t)slot;
+                    sums[slot] = sum;
+                    atomicOr(&words[mine], kBiased);
+                }
+            }
+        }
+        __syncthreads();  // the list is written again
+    }
+}
+
+// A workgroup takes a chunk of up to kThreads * P * N entries of a row.  Counts
+// of the row's tokens in the chunk, and which entries have sparse biases, are
+// words in LDS, so the logits are read and written once and no count is kept in
+// memory.  Loads are issued in the order in which they are waited for: tokens,
+// logits, bias, mask.
+template <typename TI, typename TO, int N, int P>
+__global__ __launch_bounds__(kThreads) void k_logits(spiky_lm_logits_args a) {
+    constexpr uint32_t kChunk = kThreads * P * N;
+    // words where there are tokens or bias ids; slots and as many sums as may be needed where there are bias ids
+    extern __shared__ uint4 space[];
+    uint32_t *const words = reinterpret_cast<uint32_t *>(space);
+    uint16_t *const slots = reinterpret_cast<uint16_t *>(words + kChunk);
+    float *const sums = reinterpret_cast<float *>(slots + kChunk);
+    const uint32_t tid = threadIdx.x, row = blockIdx.y, base = blockIdx.x * kChunk;
+    const uint32_t size = min(kChunk, (uint32_t)a.vocab - base);
+    const bool marks = a.tokens || a.bias_ids;
+    const TI *in = static_cast<const TI *>(a.logits) + (int64_t)row * a.logits_stride + base;
+    TO *out = static_cast<TO *>(a.out) + (int64_t)row * a.out_stride + base;
+    const uint64_t bias_at = (uint64_t)row * a.bias_stride + base;
+
+    const uint32_t history = (uint32_t)a.history;
+    const uint64_t first = (uint64_t)row * a.tokens_stride;
+    Tokens<int32_t> short_ids;
+    Tokens<int64_t> long_ids;
+    if (a.tokens) {
+        if (a.tokens_i64)
+            long_ids.load(static_cast<const int64_t *>(a.tokens) + first, 0, history);
+        else
+            short_ids.load(static_cast<const int32_t *>(a.tokens) + first, 0, history);
+    }
+    int64_t sparse_id = -1;
+    float sparse_value = 0.f;
+    if (a.bias_ids) sparse_id = bias_id(a, row, tid), sparse_value = bias_value(a, row, tid);
     const float rho = a.repetition_rows ? a.repetition_rows[row] : a.repetition;
     const float phi = a.frequency_rows ? a.frequency_rows[row] : a.frequency;
     const float pi = a.presence_rows ? a.presence_rows[row] : a.presence;
     const float heat = a.temperature_rows ? a.temperature_rows[row] : a.temperature;
-    const float less = 1.f / rho, cool = heat > 0.f ? 1.f / heat : 1.f;
-    const TI *in = static_cast<const TI *>(a.logits) + (int64_t)row * a.logits_stride + base;
-    TO *out = static_cast<TO *>(a.out) + (int64_t)row * a.out_stride + base;
-    for (uint32_t o = tid * N; o < size; o += kThreads * N) {
-        const int n = size - o < N ? (int)(size - o) : N;
-        float x[N], b[N];
-        load(x, in + o, n);
+
+    struct Piece {
+        Raw<TI, N> x;
+        Raw<float, N> bias;                // half of the words where it is of a shorter type
+        uint32_t allowed[(N + 3) / 4];     // a byte an entry, or the byte that holds the piece's bits
+    };
+    auto load = [&](Piece &q, uint32_t o, int n) {
+        q.x.load(past(in, o), n);
         if (a.bias) {
-            const uint64_t at = (uint64_t)row * a.bias_stride + base + o;
-            if (a.bias_dtype == SPIKY_F32)
-                load(b, static_cast<const float *>(a.bias) + at, n);
-            else if (a.bias_dtype == SPIKY_BF16)
-                load(b, static_cast<const bf16 *>(a.bias) + at, n);
-            else
-                load(b, static_cast<const f16 *>(a.bias) + at, n);
+            if (a.bias_dtype == SPIKY_F32) {
+                q.bias.load(past(static_cast<const float *>(a.bias) + bias_at, o), n);
+            } else {
+                Raw<bf16, N> half;
+                half.load(past(static_cast<const bf16 *>(a.bias) + bias_at, o), n);
+                __builtin_memcpy(q.bias.w, half.w, sizeof(half.w));
+            }
+        }
+        if (!a.mask) return;
+        if (a.mask_bits) {
+            // chunks start at multiples of 32 entries, so a piece's bits lie in one byte
+            const uint32_t *m = static_cast<const uint32_t *>(a.mask) + (int64_t)row * a.mask_stride;
+            q.allowed[0] = *past(reinterpret_cast<const uint8_t *>(m) + base / 8, o / 8);
+        } else {
+            const uint8_t *m = past(static_cast<const uint8_t *>(a.mask) + (int64_t)row * a.mask_stride + base, o);
+            if (n >= N) {
+                __builtin_memcpy(q.allowed, m, N);
+            } else {
 #pragma unroll
-            for (int i = 0; i < N; i++) x[i] += b[i];
+                for (int i = 0; i < N; i++) {
+                    if (i % 4 == 0) q.allowed[i / 4] = 0;
+                    if (i < n) q.allowed[i / 4] |= (uint32_t)m[i] << (8 * (i % 4));
+                }
+            }
+        }
+    };
+    // Products with reciprocals; a reciprocal past the largest number is not one.
+    const float less = 1.f / rho, cool = heat > 0.f ? 1.f / heat : 1.f;
+    const bool divide_heat = heat > 0.f && __builtin_isinf(cool), divide_rho = __builtin_isinf(less);
+    auto finish = [&](const Piece &q, uint32_t o, int n) {
+        float x[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) x[i] = q.x[i];
+        if (a.bias) {
+            if (a.bias_dtype == SPIKY_F32) {
+#pragma unroll
+                for (int i = 0; i < N; i++) x[i] += q.bias[i];
+            } else {
+                Raw<bf16, N> b;
+                Raw<f16, N> f;
+                __builtin_memcpy(b.w, q.bias.w, sizeof(b.w));
+                __builtin_memcpy(f.w, q.bias.w, sizeof(f.w));
+#pragma unroll
+                for (int i = 0; i < N; i++) x[i] += a.bias_dtype == SPIKY_BF16 ? b[i] : f[i];
+            }
         }
         if (marks) {
+            uint32_t w[N], any = 0;
 #pragma unroll
-            for (int i = 0; i < N; i++) {
-                const uint32_t w = i < n ? words[o + i] : 0;
-                if (w & kBiased) {
-                    float s = 0.f;
-                    if (listed <= kList) {
-                        for (uint32_t k = 0; k < listed; k++)
-                            if (list_id[k] == o + i) s += list_value[k];
-                    } else {
-                        const uint64_t first = (uint64_t)row * a.bias_ids_stride;
-                        for (uint64_t k = 0; k < a.n_bias; k++)
-                            if ((uint64_t)id_at(a.bias_ids, a.bias_ids_i64, first + k) == base + o + i)
-                                s += a.bias_values[(uint64_t)row * a.bias_values_stride + k];
-                    }
-                    x[i] += s;
+            for (int i = 0; i < N; i += 4) {
+                const uint4 four = space[o / 4 + i / 4];
+                w[i] = four.x, w[i + 1] = four.y, w[i + 2] = four.z, w[i + 3] = four.w;
+                any |= four.x | four.y | four.z | four.w;
+            }
+            if (any & kBiased) {
+#pragma unroll
+                for (int i = 0; i < N; i++)
+                    if (w[i] & kBiased) x[i] += sums[slots[o + i]];
+            }
+            if (any & (kSeen | kCount)) {
+#pragma unroll
+                for (int i = 0; i < N; i++) {
+                    float y = x[i] * (x[i] > 0.f ? less : rho);
+                    if (divide_rho && x[i] > 0.f) y = x[i] / rho;
+                    x[i] = w[i] & (kSeen | kCount) ? y : x[i];
+                    const uint32_t times = w[i] & kCount;
+                    x[i] = times ? x[i] - (phi * (float)times + pi) : x[i];
                 }
-                const uint32_t times = w & kCount;
-                if (w & (kSeen | kCount)) x[i] = x[i] > 0.f ? x[i] * less : x[i] * rho;
-                if (times) x[i] -= phi * (float)times + pi;
             }
         }
+        if (divide_heat) {
 #pragma unroll
-        for (int i = 0; i < N; i++) x[i] *= cool;
+            for (int i = 0; i < N; i++) x[i] /= heat;
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i++) x[i] *= cool;
+        }
         if (a.mask) {
             if (a.mask_bits) {
-                // the piece's bits lie in one or two words
-                const uint32_t *m = static_cast<const uint32_t *>(a.mask) + (int64_t)row * a.mask_stride;
-                const uint64_t v = base + o;
-                const uint32_t shift = (uint32_t)(v & 31);
-                uint64_t bits = m[v / 32];
-                if (shift + n > 32) bits |= (uint64_t)m[v / 32 + 1] << 32;
-                bits >>= shift;
+                const uint32_t bits = q.allowed[0] >> (o % 8);
 #pragma unroll
-                for (int i = 0; i < N; i++)
-                    if (!(bits >> i & 1)) x[i] = -__builtin_inff();
+                for (int i = 0; i < N; i++) x[i] = bits >> i & 1 ? x[i] : -__builtin_inff();
             } else {
-                const uint8_t *m = static_cast<const uint8_t *>(a.mask) + (int64_t)row * a.mask_stride + base + o;
-                uint8_t allowed[N];
-                if (n >= N) {
-                    __builtin_memcpy(allowed, m, N);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < N; i++) allowed[i] = i < n ? m[i] : 0;
-                }
 #pragma unroll
                 for (int i = 0; i < N; i++)
-                    if (!allowed[i]) x[i] = -__builtin_inff();
+                    x[i] = q.allowed[i / 4] >> (8 * (i % 4)) & 0xff ? x[i] : -__builtin_inff();
             }
         }
-        store(out + o, x, n);
+        store(past(out, o), x, n);
+    };
+
+    const bool whole = size == kChunk;
+    Piece piece[P];
+    if (whole)
+#pragma unroll
+        for (int p = 0; p < P; p++) load(piece[p], (p * kThreads + tid) * N, N);
+    if (marks) {
+        for (uint32_t i = tid; i < kChunk / 4; i += kThreads) space[i] = make_uint4(0, 0, 0, 0);
+        __syncthreads();
+        if (a.tokens) {
+            const uint32_t len = length_at(a.lengths, a.lengths_i64, row, history);
+            const uint32_t prompt = a.prompt_lengths ? length_at(a.prompt_lengths, a.lengths_i64, row, len) : 0;
+            auto count_all = [&](auto &ids, auto *tokens) {
+                uint32_t at = 0;
+                while (true) {
+                    ids.count(at, len, prompt, base, size, words);
+                    at += ids.kAhead * kThreads;
+                    if (at >= len) break;
+                    ids.load(tokens + first, at, len);
+                }
+            };
+            if (a.tokens_i64)
+                count_all(long_ids, static_cast<const int64_t *>(a.tokens));
+            else
+                count_all(short_ids, static_cast<const int32_t *>(a.tokens));
+        }
+        if (a.bias_ids) add_sparse(a, row, base, size, sparse_id, sparse_value, words, slots, sums);
+        __syncthreads();
+    }
+    if (whole) {
+#pragma unroll
+        for (int p = 0; p < P; p++) finish(piece[p], (p * kThreads + tid) * N, N);
+    } else {
+#pragma unroll 1
+        for (uint32_t o = tid * N; o < size; o += kThreads * N) {
+            const int n = size - o < N ? (int)(size - o) : N;
+            load(piece[0], o, n);
+            finish(piece[0], o, n);
+        }
     }
 }
 
 template <typename TI, typename TO>
 hipError_t launch(const spiky_lm_logits_args &a, hipStream_t st) {
-    constexpr int N = 8;
     // enough workgroups for the chip, but no more than a row's history is worth reading for
-    uint64_t chunk = 8192;
-    while (chunk > 2048 && (a.vocab + chunk - 1) / chunk * a.rows < 2 * kCUs) chunk /= 2;
+    constexpr int N = sizeof(TO) == 4 ? 4 : 8, kMost = 16 / N;
+    // enough workgroups for the chip, but no more than a row's history is worth reading for
+    uint64_t chunk = kThreads * 16;
+    while (chunk > kThreads * N && (a.vocab + chunk - 1) / chunk * a.rows < 2 * kCUs) chunk /= 2;
     const uint64_t chunks = (a.vocab + chunk - 1) / chunk;
-    if (chunks > 0xffffffffull / kThreads) return hipErrorInvalidValue;
-    const size_t lds = a.tokens || a.bias_ids ? chunk * sizeof(uint32_t) : 0;
+    size_t lds = a.tokens || a.bias_ids ? chunk * sizeof(uint32_t) : 0;
+    if (a.bias_ids) lds += chunk * sizeof(uint16_t) + (a.n_bias < chunk ? a.n_bias : chunk) * sizeof(float);
     // 65535 rows a launch, in y
     for (uint64_t row0 = 0; row0 < a.rows; row0 += 65535) {
         const uint32_t n = (uint32_t)(a.rows - row0 < 65535 ? a.rows - row0 : 65535);
@@ -181,7 +337,13 @@ hipError_t launch(const spiky_lm_logits_args &a, hipStream_t st) {
         skip(part.bias_ids, a.bias_ids_stride * (a.bias_ids_i64 ? 8 : 4));
         skip(part.bias_values, a.bias_values_stride * 4);
         skip(part.mask, a.mask_stride * (a.mask_bits ? 4 : 1));
-        k_logits<TI, TO, N><<<dim3((uint32_t)chunks, n), dim3(kThreads), lds, st>>>(part, (uint32_t)chunk);
+        const dim3 grid((uint32_t)chunks, n);
+        if (chunk == kThreads * 16)
+            k_logits<TI, TO, N, kMost><<<grid, dim3(kThreads), lds, st>>>(part);
+        else if (chunk == kThreads * 8)
+            k_logits<TI, TO, N, kMost / 2><<<grid, dim3(kThreads), lds, st>>>(part);
+        else
+            k_logits<TI, TO, N, 1><<<grid, dim3(kThreads), lds, st>>>(part);
         const hipError_t err = hipGetLastError();
         if (err != hipSuccess) return err;
     }

@@ -308,46 +308,6 @@ __global__ __launch_bounds__(1024) void k_join_wide(Join<TZ, TA> j) {
 }
 
 // ---- backward --------------------------------------------------------------
-// The words of N elements as they were loaded, so that a load may be in flight
-// while the values of the row before are worked on.
-template <typename T, int N>
-struct Raw {
-    uint32_t w[N * sizeof(T) / 4];
-    __device__ __forceinline__ void clear() {
-#pragma unroll
-        for (uint32_t i = 0; i < N * sizeof(T) / 4; i++) w[i] = 0;
-    }
-    // n of them exist, the others are 0.
-    __device__ __forceinline__ void load(const T *p, int n) {
-        if (n >= N) {
-            __builtin_memcpy(w, p, sizeof(w));
-            return;
-        }
-        clear();
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            if (i >= n) continue;
-            if (sizeof(T) == 4) {
-                __builtin_memcpy(&w[i], p + i, 4);
-            } else {
-                uint16_t h;
-                __builtin_memcpy(&h, p + i, 2);
-                w[i / 2] |= (uint32_t)h << (16 * (i % 2));
-            }
-        }
-    }
-    __device__ __forceinline__ float operator[](int i) const {
-        T t;
-        if (sizeof(T) == 4) {
-            __builtin_memcpy(&t, &w[i], sizeof(T));
-        } else {
-            const uint16_t h = (uint16_t)(w[i / 2] >> (16 * (i % 2)));
-            __builtin_memcpy(&t, &h, 2);
-        }
-        return to_f32(t);
-    }
-};
-
 // Sums of K values over the `waves` waves of a row (TPR > 64) or its TPR lanes,
 // in every lane.  The waves' sums go through LDS, two buffers in turn: a buffer
 // is written again only after the barrier of the call in between, which its
