@@ -18,6 +18,7 @@ SPIKY_RUNTIME_ERROR = 2
 
 _lock = threading.Lock()
 _lib = None
+_lm = None
 
 _u32 = ctypes.c_uint32
 _u64 = ctypes.c_uint64
@@ -147,6 +148,21 @@ def lib():
                 fn.restype = res
         _lib = L
     return _lib
+
+
+def lm():
+    """The torch binding of include/spiky_lm.h (csrc/lm/lm_torch.cpp); raises if it is absent."""
+    global _lm
+    if _lm is None:
+        lib()
+        import torch  # noqa: F401  (its libraries are the binding's)
+        try:
+            from . import _lm_torch
+        except ImportError as e:
+            raise RuntimeError("spiky_amd's torch binding _lm_torch.so is missing or does not load; build it with "
+                               f"`python -m spiky_amd.build`: {e}") from e
+        _lm = _lm_torch
+    return _lm
 
 
 def check(status):

@@ -3,9 +3,11 @@
 Run as ``python -m spiky_amd.build`` or through ``__graft_entry__.build()``.
 The library lands next to this file so that it travels with the source tree.
 """
+import importlib.util
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -28,6 +30,11 @@ HIPCC_FLAGS = [
 ]
 
 
+# The operators on torch tensors: host code, which calls the library.
+BINDING = os.path.join(HERE, "_lm_torch.so")
+BINDING_SOURCE = os.path.join("lm", "lm_torch.cpp")
+
+
 def _hipcc():
     for cand in (os.environ.get("HIPCC"), "/opt/rocm/bin/hipcc", "hipcc"):
         if cand and (os.path.sep not in cand or os.path.exists(cand)):
@@ -35,8 +42,25 @@ def _hipcc():
     raise RuntimeError("hipcc not found")
 
 
+def build_binding(verbose=False):
+    """Compile the torch binding against the library, which must be there."""
+    torch = os.path.dirname(importlib.util.find_spec("torch").origin)
+    tmp = BINDING + ".tmp"
+    include = [os.path.join(torch, "include"), os.path.join(torch, "include", "torch", "csrc", "api", "include"),
+               "/opt/rocm/include", sysconfig.get_paths()["include"]]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__",
+           "-DUSE_ROCM", *(f for i in include for f in ("-isystem", i)), os.path.join(CSRC, BINDING_SOURCE), "-o", tmp,
+           "-L" + os.path.join(torch, "lib"), "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python", "-L" + HERE,
+           "-l:" + os.path.basename(LIB), "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.check_call(cmd)
+    os.replace(tmp, BINDING)
+    return BINDING
+
+
 def build(verbose=False):
-    """Compile every source to an object, then link the shared library."""
+    """Compile every source to an object, link the shared library, then build the torch binding."""
     hipcc = _hipcc()
     objs = []
     os.makedirs(os.path.join(HERE, "_build"), exist_ok=True)
@@ -56,6 +80,7 @@ def build(verbose=False):
         print(" ".join(cmd), flush=True)
     subprocess.check_call(cmd)
     os.replace(tmp, LIB)
+    build_binding(verbose)
     return LIB
 
 

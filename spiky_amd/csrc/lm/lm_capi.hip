@@ -125,8 +125,8 @@ int spiky_lm_residual_norm_backward(const spiky_lm_residual_args *args, const sp
                 "a gradient of no input");
         if (args->rows == 0 || args->cols == 0) return;
         require(args->stats != nullptr, "the backward pass needs the forward's stats");
-        require(grads->workspace && grads->workspace_bytes >= spiky::lm::residual_norm_workspace(*args, *grads),
-                "residual_norm workspace too small");
+        const uint64_t need = spiky::lm::residual_norm_workspace(*args, *grads);
+        require(grads->workspace_bytes >= need && (grads->workspace || need == 0), "residual_norm workspace too small");
         check_launch(spiky::lm::launch_residual_norm_backward(*args, d, *grads, as_stream(stream)),
                      "residual_norm_backward");
     });

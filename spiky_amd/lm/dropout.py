@@ -2,34 +2,7 @@
 import torch
 
 from .. import _native
-from .common import as_rows, check_probability, dtype_code, generator_state, on_device, require_device, stream_of
-
-
-def _apply(x, p, seed, offset, rng):
-    x, stride = as_rows(x)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    cols = x.shape[-1] if x.dim() else 1
-    rows = x.numel() // cols if cols else 0
-    with on_device(x.device):
-        _native.check_lm(_native.lib().spiky_lm_dropout(
-            x.data_ptr(), stride, y.data_ptr(), rows, cols, dtype_code(x, "x"), p, seed, offset,
-            None if rng is None else rng.data_ptr(), stream_of(x.device)))
-    return y
-
-
-class _CounterDropoutFN(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, p, seed, offset, rng):
-        ctx.how = (p, seed, offset)
-        ctx.save_for_backward(*(() if rng is None else (rng,)))
-        return _apply(x, p, seed, offset, rng)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        p, seed, offset = ctx.how
-        rng = ctx.saved_tensors[0] if ctx.saved_tensors else None
-        return _apply(dy, p, seed, offset, rng), None, None, None, None
+from .common import check_probability
 
 
 def counter_dropout(x, p, seed, offset=0):
@@ -44,13 +17,7 @@ def counter_dropout(x, p, seed, offset=0):
     x: float32, bfloat16 or float16 on a HIP device, any shape.  seed, offset: whole numbers of
     64 bits, or seed an int64 device tensor of [seed, offset], read when the kernels run (for
     graphs whose replays advance it in place, after the backward pass)."""
-    require_device(x, "x")
-    dtype_code(x, "x")
-    check_probability(p)
-    seed, offset, rng = generator_state(seed, offset, x.device)
-    if x.requires_grad and torch.is_grad_enabled():
-        return _CounterDropoutFN.apply(x, float(p), seed, offset, rng)
-    return _apply(x, float(p), seed, offset, rng)
+    return _native.lm().dropout(x, p, seed, offset)
 
 
 class CounterDropout(torch.nn.Module):

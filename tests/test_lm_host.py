@@ -7,7 +7,6 @@ import pytest
 import torch
 
 from spiky_amd import CounterDropout, ResidualNorm, _native, counter_dropout, process_logits, residual_norm
-from spiky_amd.lm import common
 import lm_plain
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -69,8 +68,11 @@ def test_modules_check_their_arguments():
 
 
 def test_gate_rows():
-    from spiky_amd.lm.residual import _gate_rows
     shape = torch.Size((2, 3, 5, 4))
+
+    def _gate_rows(gate, shape):
+        return _native.lm().rows_of_gate(gate, torch.zeros(shape))
+
     assert _gate_rows(torch.zeros(4), shape)[1] == 30
     assert _gate_rows(torch.zeros(2, 1, 1, 4), shape)[1] == 15
     assert _gate_rows(torch.zeros(2, 3, 1, 4), shape)[1] == 5
@@ -87,12 +89,12 @@ def test_rows_of_a_tensor():
     base = torch.arange(4 * 6 * 8).reshape(4, 6, 8)
     for t, step in ((base, 8), (base[:, 1], 48), (base[:, 2:4], None), (base[::2, :1], 96), (base[..., 1:3], 8),
                     (base[..., ::2], None), (base.transpose(0, 1), None), (base[0, 0].expand(5, 8), 0), (base[:1, :1], 8)):
-        rows, stride = common.as_rows(t)
+        rows, stride = _native.lm().rows_of_tensor(t)
         flat = rows.as_strided((t.numel() // t.shape[-1], t.shape[-1]), (stride, 1))
         assert torch.equal(flat, t.reshape(-1, t.shape[-1]))
         if step is not None:
             assert rows is t and stride == step
-    assert common.as_rows(torch.tensor(3.0))[1] == 1
+    assert _native.lm().rows_of_tensor(torch.tensor(3.0))[1] == 1
 
 
 def refuse(status, message):
