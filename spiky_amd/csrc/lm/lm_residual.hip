@@ -354,20 +354,193 @@ __device__ __forceinline__ void chunk_rows(const J &j, uint32_t chunk, uint32_t 
     }
 }
 
+// The column sums of a backward pass, numbered as Join::part.
+enum { kSumW1, kSumB1, kSumW2, kSumB2, kSumG };
+
+// What a thread has of one piece of N columns on the way back: parameters, the
+// loads of the next row, and what the row's sums are awaited with.  FULL: with
+// layer norms or biases.
+template <typename TZ, typename TA, int N, bool FULL>
+struct Piece {
+    static constexpr int K = FULL ? 8 : 3;
+    uint64_t col;
+    int n;
+    float w1[N], w2[N], b1[FULL ? N : 1], g[N];
+    Raw<TZ, N> z_raw, dz_raw;
+    Raw<TA, N> a_raw, dh_raw;
+    Raw<float, N> g_raw;  // half of the words where the gate is of a shorter type
+    float n1[N], n2[N], e[N], keep[N];
+
+    template <typename J>
+    __device__ __forceinline__ void place(const J &j, uint64_t column) {
+        col = column;
+        n = piece_size(j.cols, col, N);
+        z_raw.clear(), dz_raw.clear(), a_raw.clear(), dh_raw.clear(), g_raw.clear();
+    }
+    // Columns past the row's end have weights of 0, so they add nothing to any sum.
+    template <typename J>
+    __device__ __forceinline__ void parameters(const J &j) {
+        if (j.w1) param<TA>(w1, j.w1, j.par_f32, col, n);
+        if (j.w2) param<TA>(w2, j.w2, j.par_f32, col, n);
+        if constexpr (FULL)
+            if (j.b1) param<TA>(b1, j.b1, j.par_f32, col, n);
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            if (!j.w1) w1[i] = i < n ? 1.f : 0.f;
+            if (!j.w2) w2[i] = 1.f;
+            if (FULL && !j.b1) b1[FULL ? i : 0] = 0.f;
+            if (!j.g) g[i] = 1.f;
+        }
+    }
+    template <typename J>
+    __device__ __forceinline__ void load_gate(const J &j, uint32_t gate_row) {
+        const uint64_t at = (uint64_t)gate_row * j.cols + col;
+        if (sizeof(TA) == 4 || j.gate_f32) {
+            g_raw.load(static_cast<const float *>(j.g) + at, n);
+        } else {
+            Raw<TA, N> half;
+            half.load(static_cast<const TA *>(j.g) + at, n);
+            __builtin_memcpy(g_raw.w, half.w, sizeof(half.w));
+        }
+    }
+    template <typename J>
+    __device__ __forceinline__ void take_gate(const J &j) {
+        if (sizeof(TA) == 4 || j.gate_f32) {
+#pragma unroll
+            for (int i = 0; i < N; i++) g[i] = g_raw[i];
+        } else {
+            Raw<TA, N> half;
+            __builtin_memcpy(half.w, g_raw.w, sizeof(half.w));
+#pragma unroll
+            for (int i = 0; i < N; i++) g[i] = half[i];
+        }
+    }
+    template <typename J>
+    __device__ __forceinline__ void fetch(const J &j, uint32_t row, bool row_gates) {
+        if (j.dz) dz_raw.load(j.dz + (int64_t)row * j.dz_stride + col, n);
+        if (j.a) a_raw.load(j.a + (int64_t)row * j.a_stride + col, n);
+        if (j.dh) {
+            z_raw.load(j.r + (int64_t)row * j.r_stride + col, n);
+            dh_raw.load(j.dh + (int64_t)row * j.dh_stride + col, n);
+        }
+        if (row_gates) load_gate(j, row);
+    }
+    // v of the forward pass, and then d: a dropped element is 0 whatever it holds.
+    __device__ __forceinline__ float dropped(int i) const {
+        float v = n1[i] * w1[i];
+        if (FULL) v += b1[FULL ? i : 0];
+        return keep[i] != 0.f ? v * keep[i] : 0.f;
+    }
+    // The row's values from its loads, and the piece's share of the row's sums s;
+    // add(k, v) adds v to the column sums k.
+    template <typename J, typename F>
+    __device__ __forceinline__ void consume(const J &j, const Dropper &dr, const float4 &st, uint32_t row,
+                                            float (&s)[K], F &&add) {
+        const float r2 = j.dh ? st.w : 0.f;
+        float dw2[N], db2[FULL ? N : 1];
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            keep[i] = 1.f;
+            n1[i] = (a_raw[i] - st.x) * st.y;
+        }
+        if (j.drops) drop(keep, dr, row, col);
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            float z = z_raw[i];
+            if (j.a) z = j.alpha * z + j.beta * (g[i] * dropped(i));
+            n2[i] = j.dh ? (z - st.z) * r2 : 0.f;
+            const float dh = dh_raw[i], t = dh * w2[i];
+            e[i] = dz_raw[i] + r2 * t;
+            dw2[i] = dh * n2[i];
+            const float c = keep[i] * (j.beta * g[i]) * w1[i];
+            const float ce = keep[i] != 0.f ? c * e[i] : 0.f, cn = c * n1[i];
+            s[0] += t * n2[i];
+            s[1] += ce * n1[i];
+            s[2] += cn * n2[i];
+            if constexpr (FULL) {
+                db2[i] = dh;
+                s[3] += t;
+                s[4] += ce;
+                s[5] += c;
+                s[6] += c * n2[i];
+                s[7] += cn;
+            }
+        }
+        if (j.part[kSumW2]) add(kSumW2, dw2);
+        if constexpr (FULL)
+            if (j.part[kSumB2]) add(kSumB2, db2);
+    }
+    // The row's gradients, from its means (mean t, mean t n2, mean dn, mean dn n1).
+    template <typename J, typename F>
+    __device__ __forceinline__ void finish(const J &j, const float4 &st, const float4 &m, uint32_t row, F &&add) {
+        const float r2 = j.dh ? st.w : 0.f, alpha = j.a ? j.alpha : 1.f;
+        const uint64_t at = (uint64_t)row * j.cols + col;
+        float out[N], da[N], dg[N], dw1[N], db1[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const float q = e[i] - r2 * (m.x + n2[i] * m.y);
+            out[i] = alpha * q;
+            dg[i] = j.beta * (dropped(i) * q);
+            db1[i] = keep[i] != 0.f ? j.beta * (g[i] * q) * keep[i] : 0.f;
+            dw1[i] = db1[i] * n1[i];
+            da[i] = db1[i];
+            if (j.post != SPIKY_NORM_NONE) da[i] = st.y * (db1[i] * w1[i] - m.z - n1[i] * m.w);
+        }
+        if (j.dr) store(j.dr + at, out, n);
+        if (j.da) store(j.da + at, da, n);
+        if (j.dgate && j.gate_rows == 1)
+            store_gate(j, row, dg);
+        else if (j.dgate || j.part[kSumG])
+            add(kSumG, dg);
+        if (j.part[kSumW1]) add(kSumW1, dw1);
+        if constexpr (FULL)
+            if (j.part[kSumB1]) add(kSumB1, db1);
+    }
+    template <typename J>
+    __device__ __forceinline__ void store_gate(const J &j, uint32_t gate_row, const float (&dg)[N]) const {
+        const uint64_t to = (uint64_t)gate_row * j.cols + col;
+        if (sizeof(TA) == 4 || j.gate_f32)
+            store(static_cast<float *>(j.dgate) + to, dg, n);
+        else
+            store(static_cast<TA *>(j.dgate) + to, dg, n);
+    }
+};
+
+// A row's means from its sums.  q is linear in the sums of the pre norm, so those
+// of the post norm follow from sums that need none of them, and a row has one
+// reduction: with c = keep / (1 - p) beta g w1 and e = dz + r2 t,
+//   sum dn n1 = sum c n1 e - r2 (mean t sum c n1 + mean(t n2) sum c n1 n2)
+// and alike without n1.
+template <bool FULL, typename J, int K>
+__device__ __forceinline__ float4 row_means(const J &j, const float4 &st, const float (&s)[K]) {
+    const float r2 = j.dh ? st.w : 0.f;
+    float4 m = {0.f, s[0] * j.inv_cols, 0.f, 0.f};
+    if (FULL && j.pre == SPIKY_NORM_LAYER) m.x = s[FULL ? 3 : 0] * j.inv_cols;
+    if (j.post != SPIKY_NORM_NONE) {
+        m.w = s[1] - r2 * (m.y * s[2]);
+        if constexpr (FULL) {
+            m.w -= r2 * (m.x * s[7]);
+            if (j.post == SPIKY_NORM_LAYER) m.z = (s[4] - r2 * (m.x * s[5] + m.y * s[6])) * j.inv_cols;
+        }
+        m.w *= j.inv_cols;
+    }
+    return m;
+}
+
 // Rows of up to 1024 * N * P columns: a workgroup walks the rows of its chunk (a
 // slot of TPR lanes its share of them), a thread always with the same columns,
-// so parameters and column sums stay in registers and every input crosses HBM
-// once.  q is linear in the sums of the pre norm, so those of the post norm
-// follow from sums that need none of them, and a row has one reduction: with
-// c = keep / (1 - p) beta g w1 and e = dz + r2 t,
-//   sum dn n1 = sum c n1 e - r2 (mean t sum c n1 + mean(t n2) sum c n1 n2)
-// and alike without n1.  The next row's loads are issued before the reduction,
-// into the registers that this row's left.  FULL: with layer norms or biases.
+// so every input crosses HBM once.  Parameters stay in registers; column sums are
+// in LDS, each thread's its own, which costs a read and a write of LDS a row and
+// frees the registers that more waves need.  The next row's loads are issued
+// before the reduction, into the registers that this row's left.
 template <typename TZ, typename TA, int N, int P, int TPR, bool FULL>
 __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_join_back(Join<TZ, TA> j) {
-    constexpr int kSlots = TPR <= 64 ? 256 / TPR : 1, W = N * P, K = FULL ? 8 : 3;
+    constexpr int kThreads = TPR <= 64 ? 256 : TPR, kSlots = TPR <= 64 ? 256 / TPR : 1;
+    constexpr int W = N * P, K = FULL ? 8 : 3, kQuads = W / 4;
     __shared__ float4 red[TPR > 64 ? 2 : 1][(K + 3) / 4][16];
-    __shared__ float joint[kSlots > 1 ? kSlots : 1][kSlots > 1 ? TPR * W : 1];
+    // sums of w1, w2, g and, FULL, b1; those of b2 stay in registers, where 1024 threads have no LDS for them
+    constexpr int kInLds = FULL ? 4 : 3;
+    __shared__ float4 acc[kInLds][kQuads][kThreads];
     const uint32_t threads = TPR <= 64 ? TPR : blockDim.x, waves = blockDim.x / 64;
     const uint32_t lane = TPR <= 64 ? threadIdx.x % TPR : threadIdx.x;
     uint32_t row, end, turn = 0;
@@ -383,410 +556,206 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_join_back(Join<TZ, TA
     const bool row_gates = j.g && j.gate_rows == 1;
     uint32_t gate_row = j.g ? row / j.gate_rows : 0, in_gate = j.g ? row - gate_row * j.gate_rows : 0;
 
-    uint64_t col[P];
-    int n[P];
-    float w1[P][N], w2[P][N], b1[FULL ? P : 1][N], g[P][N];
-    float acc_w1[P][N], acc_w2[P][N], acc_g[P][N], acc_b1[FULL ? P : 1][N], acc_b2[FULL ? P : 1][N];
-    Raw<TZ, N> z_raw[P], dz_raw[P];
-    Raw<TA, N> a_raw[P], dh_raw[P];
-    Raw<float, N> g_raw[P];  // half of the words where the gate is of a shorter type
+    auto slot_of = [](int k) { return k == kSumW1 ? 0 : k == kSumW2 ? 1 : k == kSumG ? 2 : 3; };
+    float acc_b2[P][N];
+    Piece<TZ, TA, N, FULL> x[P];
     float4 st = {0.f, 1.f, 0.f, 1.f};
-
-    auto gate_words = [&](int p, uint32_t at_row) {
-        const uint64_t at = (uint64_t)at_row * j.cols + col[p];
-        if (sizeof(TA) == 4 || j.gate_f32) {
-            g_raw[p].load(static_cast<const float *>(j.g) + at, n[p]);
-        } else {
-            Raw<TA, N> half;
-            half.load(static_cast<const TA *>(j.g) + at, n[p]);
-            __builtin_memcpy(g_raw[p].w, half.w, sizeof(half.w));
-        }
-    };
-    auto gate_values = [&](int p) {
-        if (sizeof(TA) == 4 || j.gate_f32) {
-#pragma unroll
-            for (int i = 0; i < N; i++) g[p][i] = g_raw[p][i];
-        } else {
-            Raw<TA, N> half;
-            __builtin_memcpy(half.w, g_raw[p].w, sizeof(half.w));
-#pragma unroll
-            for (int i = 0; i < N; i++) g[p][i] = half[i];
-        }
-    };
-    auto fetch = [&](uint32_t r) {
-        st = j.stats[r];
-#pragma unroll
-        for (int p = 0; p < P; p++) {
-            if (j.dz) dz_raw[p].load(j.dz + (int64_t)r * j.dz_stride + col[p], n[p]);
-            if (j.a) a_raw[p].load(j.a + (int64_t)r * j.a_stride + col[p], n[p]);
-            if (j.dh) {
-                z_raw[p].load(j.r + (int64_t)r * j.r_stride + col[p], n[p]);
-                dh_raw[p].load(j.dh + (int64_t)r * j.dh_stride + col[p], n[p]);
-            }
-            if (row_gates) gate_words(p, r);
-        }
-    };
 #pragma unroll
     for (int p = 0; p < P; p++) {
-        col[p] = (uint64_t)(p * threads + lane) * N;
-        n[p] = piece_size(j.cols, col[p], N);
-        z_raw[p].clear(), dz_raw[p].clear(), a_raw[p].clear(), dh_raw[p].clear(), g_raw[p].clear();
+        x[p].place(j, (uint64_t)(p * threads + lane) * N);
+        if (row < end) x[p].fetch(j, row, row_gates);
     }
-    if (row < end) fetch(row);
+    if (row < end) st = j.stats[row];
+#pragma unroll
+    for (int k = 0; k < kInLds; k++)
+#pragma unroll
+        for (int q = 0; q < kQuads; q++) acc[k][q][threadIdx.x] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int p = 0; p < P; p++) {
-        // columns past the row's end have weights of 0, so they add nothing to any sum
-        if (j.w1) param<TA>(w1[p], j.w1, j.par_f32, col[p], n[p]);
-        if (j.w2) param<TA>(w2[p], j.w2, j.par_f32, col[p], n[p]);
-        if (FULL && j.b1) param<TA>(b1[p], j.b1, j.par_f32, col[p], n[p]);
-        if (j.g && !row_gates && row < end) gate_words(p, gate_row), gate_values(p);
+        x[p].parameters(j);
+        if (j.g && !row_gates && row < end) x[p].load_gate(j, gate_row), x[p].take_gate(j);
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-            if (!j.w1) w1[p][i] = i < n[p] ? 1.f : 0.f;
-            if (!j.w2) w2[p][i] = 1.f;
-            if (FULL && !j.b1) b1[FULL ? p : 0][i] = 0.f;
-            if (!j.g) g[p][i] = 1.f;
-            acc_w1[p][i] = acc_w2[p][i] = acc_g[p][i] = 0.f;
-            if (FULL) acc_b1[FULL ? p : 0][i] = acc_b2[FULL ? p : 0][i] = 0.f;
-        }
+        for (int i = 0; i < N; i++) acc_b2[p][i] = 0.f;
     }
-    const float alpha = j.a ? j.alpha : 1.f;
 
     for (; row < end; row++) {
-        float n1[P][N], n2[P][N], e[P][N], keep[P][N];
         float s[K];
 #pragma unroll
         for (int k = 0; k < K; k++) s[k] = 0.f;
-        const float r1 = st.y, r2 = j.dh ? st.w : 0.f;
+        const float4 now = st;
+        auto adds_to = [&](int p) {
+            return [&acc_b2, slot_of, p](int k, const float (&v)[N]) {
+                if (FULL && k == kSumB2) {
 #pragma unroll
-        for (int p = 0; p < P; p++) {
-            if (row_gates) gate_values(p);
-#pragma unroll
-            for (int i = 0; i < N; i++) {
-                keep[p][i] = 1.f;
-                n1[p][i] = (a_raw[p][i] - st.x) * st.y;
-            }
-            if (j.drops) drop(keep[p], dr, row, col[p]);
-#pragma unroll
-            for (int i = 0; i < N; i++) {
-                float v = n1[p][i] * w1[p][i];
-                if (FULL) v += b1[FULL ? p : 0][i];
-                const bool kept = keep[p][i] != 0.f;
-                v = kept ? v * keep[p][i] : 0.f;  // a dropped element is 0 whatever it holds
-                float z = z_raw[p][i];
-                if (j.a) z = alpha * z + j.beta * (g[p][i] * v);
-                n2[p][i] = j.dh ? (z - st.z) * r2 : 0.f;
-                const float dh = dh_raw[p][i], t = dh * w2[p][i];
-                e[p][i] = dz_raw[p][i] + r2 * t;
-                acc_w2[p][i] += dh * n2[p][i];
-                const float c = keep[p][i] * (j.beta * g[p][i]) * w1[p][i];
-                const float ce = kept ? c * e[p][i] : 0.f, cn = c * n1[p][i];
-                s[0] += t * n2[p][i];
-                s[1] += ce * n1[p][i];
-                s[2] += cn * n2[p][i];
-                if constexpr (FULL) {
-                    acc_b2[p][i] += dh;
-                    s[3] += t;
-                    s[4] += ce;
-                    s[5] += c;
-                    s[6] += c * n2[p][i];
-                    s[7] += cn;
+                    for (int i = 0; i < N; i++) acc_b2[p][i] += v[i];
+                    return;
                 }
-            }
-        }
-        if (row + 1 < end) fetch(row + 1);
-        row_sums<TPR, K>(s, red, turn, waves);
-        // means over the row
-        float mean_t = 0.f, mean_tn, mean_dn = 0.f, mean_dnn = 0.f;
-        mean_tn = s[0] * j.inv_cols;
-        if (FULL && j.pre == SPIKY_NORM_LAYER) mean_t = s[FULL ? 3 : 0] * j.inv_cols;
-        if (j.post != SPIKY_NORM_NONE) {
-            mean_dnn = s[1] - r2 * (mean_tn * s[2]);
-            if constexpr (FULL) {
-                mean_dnn -= r2 * (mean_t * s[7]);
-                if (j.post == SPIKY_NORM_LAYER)
-                    mean_dn = (s[4] - r2 * (mean_t * s[5] + mean_tn * s[6])) * j.inv_cols;
-            }
-            mean_dnn *= j.inv_cols;
-        }
-        const bool gate_ends = j.dgate && in_gate + 1 == j.gate_rows;
+#pragma unroll
+                for (int i = 0; i < N; i += 4) {
+                    float4 &f = acc[slot_of(k)][(p * N + i) / 4][threadIdx.x];
+                    float4 t = f;
+                    t.x += v[i], t.y += v[i + 1], t.z += v[i + 2], t.w += v[i + 3];
+                    f = t;
+                }
+            };
+        };
 #pragma unroll
         for (int p = 0; p < P; p++) {
-            const uint64_t at = (uint64_t)row * j.cols + col[p];
-            float out[N], da[N];
-#pragma unroll
-            for (int i = 0; i < N; i++) {
-                const float q = e[p][i] - r2 * (mean_t + n2[p][i] * mean_tn);
-                out[i] = alpha * q;
-                const bool kept = keep[p][i] != 0.f;
-                float v = n1[p][i] * w1[p][i];
-                if (FULL) v += b1[FULL ? p : 0][i];
-                v = kept ? v * keep[p][i] : 0.f;
-                acc_g[p][i] += j.beta * (v * q);
-                const float dv = kept ? j.beta * (g[p][i] * q) * keep[p][i] : 0.f;
-                acc_w1[p][i] += dv * n1[p][i];
-                if (FULL) acc_b1[FULL ? p : 0][i] += dv;
-                da[i] = dv;
-                if (j.post != SPIKY_NORM_NONE) da[i] = r1 * (dv * w1[p][i] - mean_dn - n1[p][i] * mean_dnn);
-            }
-            if (j.dr) store(j.dr + at, out, n[p]);
-            if (j.da) store(j.da + at, da, n[p]);
-            if (gate_ends) {
-                const uint64_t to = (uint64_t)gate_row * j.cols + col[p];
-                if (sizeof(TA) == 4 || j.gate_f32)
-                    store(static_cast<float *>(j.dgate) + to, acc_g[p], n[p]);
-                else
-                    store(static_cast<TA *>(j.dgate) + to, acc_g[p], n[p]);
-#pragma unroll
-                for (int i = 0; i < N; i++) acc_g[p][i] = 0.f;
-            }
+            if (row_gates) x[p].take_gate(j);
+            x[p].consume(j, dr, now, row, s, adds_to(p));
         }
-        if (j.g && ++in_gate == j.gate_rows) {
+        if (row + 1 < end) {
+            st = j.stats[row + 1];
+#pragma unroll
+            for (int p = 0; p < P; p++) x[p].fetch(j, row + 1, row_gates);
+        }
+        row_sums<TPR, K>(s, red, turn, waves);
+        const float4 m = row_means<FULL>(j, now, s);
+#pragma unroll
+        for (int p = 0; p < P; p++) x[p].finish(j, now, m, row, adds_to(p));
+        if (j.g && !row_gates && ++in_gate == j.gate_rows) {
+            // the rows of a gate end here, and with them its sum, where no other chunk has some of them
+#pragma unroll
+            for (int p = 0; p < P; p++) {
+                if (j.dgate) {
+                    float dg[N];
+#pragma unroll
+                    for (int i = 0; i < N; i += 4) {
+                        float4 &f = acc[2][(p * N + i) / 4][threadIdx.x];
+                        dg[i] = f.x, dg[i + 1] = f.y, dg[i + 2] = f.z, dg[i + 3] = f.w;
+                        f = make_float4(0.f, 0.f, 0.f, 0.f);
+                    }
+                    x[p].store_gate(j, gate_row, dg);
+                }
+                if (row + 1 < end) x[p].load_gate(j, gate_row + 1), x[p].take_gate(j);
+            }
             in_gate = 0;
             gate_row++;
-            if (!row_gates && row + 1 < end)
-#pragma unroll
-                for (int p = 0; p < P; p++) gate_words(p, gate_row), gate_values(p);
         }
     }
 
-    auto column_sums = [&](float *part, float (&acc)[P][N]) {
-        if (!part) return;
-        part += (uint64_t)blockIdx.x * j.cols;
+    auto write_sums = [&](int k, const float4 (*sums)[kThreads]) {
+        float *part = j.part[k] + (uint64_t)blockIdx.x * j.cols;
         if constexpr (kSlots == 1) {
 #pragma unroll
-            for (int p = 0; p < P; p++) store(part + col[p], acc[p], n[p]);
+            for (int p = 0; p < P; p++) {
+                float v[N];
+#pragma unroll
+                for (int i = 0; i < N; i += 4) {
+                    const float4 f = sums[(p * N + i) / 4][threadIdx.x];
+                    v[i] = f.x, v[i + 1] = f.y, v[i + 2] = f.z, v[i + 3] = f.w;
+                }
+                store(part + x[p].col, v, x[p].n);
+            }
         } else {
-            __syncthreads();
+            // columns 4 q' .. + 3 of the row: quad q of lane l of every slot
+            for (uint32_t c = threadIdx.x * 4; c < (uint32_t)TPR * W && c < j.cols; c += 1024) {
+                const uint32_t piece = c / N, q = piece / TPR * (N / 4) + c % N / 4, l = piece % TPR;
+                float v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int p = 0; p < P; p++)
-#pragma unroll
-                for (int i = 0; i < N; i++) joint[threadIdx.x / TPR][(p * TPR + lane) * N + i] = acc[p][i];
-            __syncthreads();
-            for (uint32_t c = threadIdx.x; c < TPR * W && c < j.cols; c += 256) {
-                float sum = 0.f;
-#pragma unroll
-                for (int k = 0; k < kSlots; k++) sum += joint[k][c];
-                part[c] = sum;
+                for (int slot = 0; slot < kSlots; slot++) {
+                    const float4 f = sums[q][slot * TPR + l];
+                    v[0] += f.x, v[1] += f.y, v[2] += f.z, v[3] += f.w;
+                }
+                store(part + c, v, piece_size(j.cols, c, 4));
             }
         }
     };
-    column_sums(j.part[0], acc_w1);
-    column_sums(j.part[2], acc_w2);
-    column_sums(j.part[4], acc_g);
+    if (kSlots > 1) __syncthreads();
+    if (j.part[kSumW1]) write_sums(kSumW1, acc[0]);
+    if (j.part[kSumW2]) write_sums(kSumW2, acc[1]);
+    if (j.part[kSumG]) write_sums(kSumG, acc[2]);
     if constexpr (FULL) {
-        column_sums(j.part[1], acc_b1);
-        column_sums(j.part[3], acc_b2);
+        if (j.part[kSumB1]) write_sums(kSumB1, acc[3]);
+        if (j.part[kSumB2]) {
+            if (kSlots > 1) __syncthreads();
+#pragma unroll
+            for (int p = 0; p < P; p++)
+#pragma unroll
+                for (int i = 0; i < N; i += 4)
+                    acc[0][(p * N + i) / 4][threadIdx.x] =
+                        make_float4(acc_b2[p][i], acc_b2[p][i + 1], acc_b2[p][i + 2], acc_b2[p][i + 3]);
+            if (kSlots > 1) __syncthreads();
+            write_sums(kSumB2, acc[0]);
+        }
     }
 }
 
-// Wider rows take two passes over the inputs: the sums over each row, then
-// columns.
-//
-// What a piece of N columns of one row holds on the way back.
-template <typename TZ, typename TA, int N>
-struct Piece {
-    float dz[N], dh[N], n2[N], t[N];  // t = dh w2
-    float n1[N], d[N], g[N], keep[N];
-
-    // Everything that does not depend on sums over the row.
-    template <typename J>
-    __device__ __forceinline__ void read(const J &j, const Dropper &dr, const float4 &st, uint32_t row,
-                                         uint32_t gate_row, uint64_t col, int n) {
-        if (j.dz)
-            load(dz, j.dz + (int64_t)row * j.dz_stride + col, n);
-        else
-#pragma unroll
-            for (int i = 0; i < N; i++) dz[i] = 0.f;
-        if (j.a) {
-            load(n1, j.a + (int64_t)row * j.a_stride + col, n);
-#pragma unroll
-            for (int i = 0; i < N; i++) {
-                n1[i] = (n1[i] - st.x) * st.y;
-                d[i] = n1[i];
-                keep[i] = 1.f;
-            }
-            if (j.w1) {
-                float w[N];
-                param<TA>(w, j.w1, j.par_f32, col, n);
-#pragma unroll
-                for (int i = 0; i < N; i++) d[i] *= w[i];
-            }
-            if (j.b1) {
-                float b[N];
-                param<TA>(b, j.b1, j.par_f32, col, n);
-#pragma unroll
-                for (int i = 0; i < N; i++) d[i] += b[i];
-            }
-            if (j.drops) {
-                drop(keep, dr, row, col);
-                // a dropped element is 0 whatever it holds
-#pragma unroll
-                for (int i = 0; i < N; i++) d[i] = keep[i] != 0.f ? d[i] * keep[i] : 0.f;
-            }
-            gate_of<TA>(g, j, gate_row, col, n);
-        }
-        if (j.dh) {
-            float z[N], w[N];
-            load(dh, j.dh + (int64_t)row * j.dh_stride + col, n);
-            load(z, j.r + (int64_t)row * j.r_stride + col, n);
-            if (j.a)
-#pragma unroll
-                for (int i = 0; i < N; i++) z[i] = j.alpha * z[i] + j.beta * (g[i] * d[i]);
-            if (j.w2) param<TA>(w, j.w2, j.par_f32, col, n);
-#pragma unroll
-            for (int i = 0; i < N; i++) {
-                n2[i] = i < n ? (z[i] - st.z) * st.w : 0.f;
-                t[i] = j.w2 ? dh[i] * w[i] : dh[i];
-            }
-        }
-    }
-
-    // q in place of dz.
-    template <typename J>
-    __device__ __forceinline__ void through_pre(const J &j, const float4 &st, float mean_t, float mean_tn) {
-        if (!j.dh) return;
-#pragma unroll
-        for (int i = 0; i < N; i++) dz[i] += st.w * (t[i] - mean_t - n2[i] * mean_tn);
-    }
-
-    // dv, from q.
-    template <typename J>
-    __device__ __forceinline__ void through_gate(const J &j, float (&dv)[N]) const {
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            const float x = j.beta * (g[i] * dz[i]);
-            dv[i] = !j.drops ? x : keep[i] != 0.f ? x * keep[i] : 0.f;
-        }
-    }
-};
-
-// The sums over each row, and dr.
-template <typename TZ, typename TA, int N, int WG>
+// Wider rows take two passes over the inputs: the means of each row, then columns.
+template <typename TZ, typename TA, int N, int WG, bool FULL>
 __global__ __launch_bounds__(WG) void k_join_back_rows(Join<TZ, TA> j) {
-    __shared__ float red[2][2][16];
-    RowSum<WG, 2> row_sum{red};
+    constexpr int K = FULL ? 8 : 3;
+    __shared__ float4 red[2][(K + 3) / 4][16];
     const uint32_t row = j.row0 + blockIdx.x;
     const Dropper dr = dropper(j.drop);
-    const uint32_t gate_row = j.g ? row / j.gate_rows : 0;
     const float4 st = j.stats[row];
-    float4 sums = {0.f, 0.f, 0.f, 0.f};
-    Piece<TZ, TA, N> x;
-    if (j.dh) {
-        float s[2] = {0.f, 0.f};
-        for (uint64_t col = (uint64_t)threadIdx.x * N; col < j.cols; col += WG * N) {
-            x.read(j, dr, st, row, gate_row, col, piece_size(j.cols, col, N));
+    float s[K];
 #pragma unroll
-            for (int i = 0; i < N; i++) {
-                s[0] += x.t[i];
-                s[1] += x.t[i] * x.n2[i];
-            }
-        }
-        row_sum(s);
-        sums.x = j.pre == SPIKY_NORM_LAYER ? s[0] * j.inv_cols : 0.f;
-        sums.y = s[1] * j.inv_cols;
-    }
-    float s[2] = {0.f, 0.f};
+    for (int k = 0; k < K; k++) s[k] = 0.f;
     for (uint64_t col = (uint64_t)threadIdx.x * N; col < j.cols; col += WG * N) {
-        const int n = piece_size(j.cols, col, N);
-        x.read(j, dr, st, row, gate_row, col, n);
-        x.through_pre(j, st, sums.x, sums.y);
-        if (j.dr) {
-            float d[N];
-            const float alpha = j.a ? j.alpha : 1.f;
-#pragma unroll
-            for (int i = 0; i < N; i++) d[i] = alpha * x.dz[i];
-            store(j.dr + (uint64_t)row * j.cols + col, d, n);
-        }
-        if (j.a && j.post != SPIKY_NORM_NONE) {
-            float dv[N], w[N];
-            x.through_gate(j, dv);
-            if (j.w1) param<TA>(w, j.w1, j.par_f32, col, n);
-#pragma unroll
-            for (int i = 0; i < N; i++) {
-                const float dn = i < n ? (j.w1 ? dv[i] * w[i] : dv[i]) : 0.f;
-                s[0] += dn;
-                s[1] += dn * x.n1[i];
-            }
-        }
+        Piece<TZ, TA, N, FULL> x;
+        x.place(j, col);
+        x.fetch(j, row, false);
+        x.parameters(j);
+        if (j.g) x.load_gate(j, row / j.gate_rows), x.take_gate(j);
+        x.consume(j, dr, st, row, s, [](int, auto &) {});
     }
-    if (j.a && j.post != SPIKY_NORM_NONE) {
-        row_sum(s);
-        sums.z = j.post == SPIKY_NORM_LAYER ? s[0] * j.inv_cols : 0.f;
-        sums.w = s[1] * j.inv_cols;
-    }
-    if (threadIdx.x == 0) j.row_sums[row] = sums;
+    uint32_t turn = 0;
+    row_sums<WG, K>(s, red, turn, WG / 64);
+    if (threadIdx.x == 0) j.row_sums[row] = row_means<FULL>(j, st, s);
 }
 
-// da, and the sums over the rows of a chunk for N columns a thread.
-template <typename TZ, typename TA, int N>
+// The gradients, and the sums over the rows of a chunk for N columns a thread.
+template <typename TZ, typename TA, int N, bool FULL>
 __global__ __launch_bounds__(64) void k_join_back_cols(Join<TZ, TA> j) {
-    const uint64_t col = ((uint64_t)blockIdx.x * 64 + threadIdx.x) * N;
-    const int n = piece_size(j.cols, col, N);
-    if (n == 0) return;
+    constexpr int K = FULL ? 8 : 3;
+    Piece<TZ, TA, N, FULL> x;
+    x.place(j, ((uint64_t)blockIdx.x * 64 + threadIdx.x) * N);
+    if (x.n == 0) return;
     uint32_t row, end;
     chunk_rows(j, blockIdx.y, row, end);
+    if (row >= end) return;
     const Dropper dr = dropper(j.drop);
-    float acc[5][N];
+    const bool row_gates = j.g && j.gate_rows == 1;
+    uint32_t gate_row = j.g ? row / j.gate_rows : 0, in_gate = j.g ? row - gate_row * j.gate_rows : 0;
+    float acc[5][N], s[K];
 #pragma unroll
     for (int k = 0; k < 5; k++)
 #pragma unroll
         for (int i = 0; i < N; i++) acc[k][i] = 0.f;
-    Piece<TZ, TA, N> x;
+    x.fetch(j, row, row_gates);
+    float4 st = j.stats[row], m = j.row_sums[row];
+    x.parameters(j);
+    if (j.g && !row_gates) x.load_gate(j, gate_row), x.take_gate(j);
+    auto add = [&](int k, const float (&v)[N]) {
+#pragma unroll
+        for (int i = 0; i < N; i++) acc[k][i] += v[i];
+    };
     for (; row < end; row++) {
-        const uint32_t gate_row = j.g ? row / j.gate_rows : 0;
-        const float4 st = j.stats[row], sums = j.row_sums[row];
-        x.read(j, dr, st, row, gate_row, col, n);
-        if (j.dh) {
+        const float4 now = st, means = m;
 #pragma unroll
-            for (int i = 0; i < N; i++) {
-                acc[2][i] += x.dh[i] * x.n2[i];
-                acc[3][i] += x.dh[i];
-            }
+        for (int k = 0; k < K; k++) s[k] = 0.f;
+        if (row_gates) x.take_gate(j);
+        x.consume(j, dr, now, row, s, add);
+        if (row + 1 < end) {
+            st = j.stats[row + 1], m = j.row_sums[row + 1];
+            x.fetch(j, row + 1, row_gates);
         }
-        if (!j.a) continue;
-        x.through_pre(j, st, sums.x, sums.y);
-        float dv[N];
-        x.through_gate(j, dv);
-        if (j.dgate || j.part[4]) {
-            float dg[N];
+        x.finish(j, now, means, row, add);
+        if (j.g && !row_gates && ++in_gate == j.gate_rows) {
+            if (j.dgate) {
+                x.store_gate(j, gate_row, acc[kSumG]);
 #pragma unroll
-            for (int i = 0; i < N; i++) {
-                dg[i] = j.beta * (x.d[i] * x.dz[i]);
-                acc[4][i] += dg[i];
+                for (int i = 0; i < N; i++) acc[kSumG][i] = 0.f;
             }
-            // the rows of a gate end here: its sum is whole, or the gate has one row for each
-            if (j.dgate && (row + 1) % j.gate_rows == 0) {
-                const uint64_t at = (uint64_t)gate_row * j.cols + col;
-                if (j.gate_f32)
-                    store(static_cast<float *>(j.dgate) + at, acc[4], n);
-                else
-                    store(static_cast<TA *>(j.dgate) + at, acc[4], n);
-#pragma unroll
-                for (int i = 0; i < N; i++) acc[4][i] = 0.f;
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            acc[0][i] += dv[i] * x.n1[i];
-            acc[1][i] += dv[i];
-        }
-        if (j.da) {
-            if (j.post != SPIKY_NORM_NONE) {
-                float w[N];
-                if (j.w1) param<TA>(w, j.w1, j.par_f32, col, n);
-#pragma unroll
-                for (int i = 0; i < N; i++) {
-                    const float dn = j.w1 ? dv[i] * w[i] : dv[i];
-                    dv[i] = st.y * (dn - sums.z - x.n1[i] * sums.w);
-                }
-            }
-            store(j.da + (uint64_t)row * j.cols + col, dv, n);
+            if (row + 1 < end) x.load_gate(j, gate_row + 1), x.take_gate(j);
+            in_gate = 0;
+            gate_row++;
         }
     }
 #pragma unroll
     for (int k = 0; k < 5; k++)
-        if (j.part[k]) store(j.part[k] + (uint64_t)blockIdx.y * j.cols + col, acc[k], n);
+        if (j.part[k]) store(j.part[k] + (uint64_t)blockIdx.y * j.cols + x.col, acc[k], x.n);
 }
 
 // Column sums of the chunks' rows, in one order: out[g][c] = the sum of the
@@ -906,18 +875,27 @@ struct Plan {
 
 // Columns of a thread of k_join_back.
 constexpr uint64_t kBackCols = 8;
+constexpr uint64_t kLeast = 4;
 
 Plan plan(const spiky_lm_residual_args &a, const spiky_lm_residual_grads &g) {
     Plan p = {};
     const uint64_t threads = (a.cols + kBackCols - 1) / kBackCols;
     p.tpr = threads <= 16 ? 16 : threads <= 32 ? 32 : threads <= 64 ? 64 : threads <= 1024 ? 1024 : 0;
     const uint64_t span = a.gate && g.d_gate ? a.gate_rows : a.rows;
-    // two workgroups to a CU; one, where that leaves each fewer than two rounds of rows
     const uint64_t slots = p.tpr && p.tpr <= 64 ? 256 / p.tpr : 1;
-    const uint64_t most = a.rows >= 4 * kCUs * slots ? 2 * kCUs : kCUs;
-    uint64_t chunk = (a.rows + most - 1) / most;
-    if (chunk < slots) chunk = slots;
-    if (!p.tpr && chunk < 8) chunk = 8;
+    const uint64_t waves = p.tpr && p.tpr <= 64 ? 4 : (threads + 63) / 64;
+    uint64_t chunk;
+    if (p.tpr) {
+        // 16 waves to a CU, where each has kLeast rows of its own
+        const uint64_t most = kCUs * (waves > 8 ? 1 : 16 / waves);
+        chunk = (a.rows + most - 1) / most;
+        const uint64_t one_each = (a.rows + kCUs - 1) / kCUs, least = kLeast * slots;
+        if (chunk < least) chunk = one_each < least ? one_each : least;
+        if (chunk < slots) chunk = slots;
+    } else {
+        chunk = (a.rows + 2 * kCUs - 1) / (2 * kCUs);
+        if (chunk < 8) chunk = 8;
+    }
     if (span >= chunk) {
         p.chunks_per_span = (uint32_t)((span + chunk - 1) / chunk);
         chunk = (span + p.chunks_per_span - 1) / p.chunks_per_span;
@@ -944,8 +922,18 @@ Plan plan(const spiky_lm_residual_args &a, const spiky_lm_residual_grads &g) {
 }
 
 template <typename TZ, typename TA, bool FULL>
-void run_back(const Join<TZ, TA> &j, const Plan &p, hipStream_t st) {
+hipError_t run_back(Join<TZ, TA> &j, const Plan &p, hipStream_t st) {
     constexpr int N = sizeof(TA) == 4 ? 4 : 8, P = kBackCols / N;
+    if (!p.tpr) {
+        const hipError_t err = over_rows(j, 1, 512, [&](dim3 grid, dim3 block) {
+            k_join_back_rows<TZ, TA, N, 512, FULL><<<grid, block, 0, st>>>(j);
+        });
+        if (err != hipSuccess) return err;
+        const uint64_t tiles = (j.cols + 64 * N - 1) / (64 * N);
+        // fewer than 2048 chunks, in y
+        k_join_back_cols<TZ, TA, N, FULL><<<dim3((uint32_t)tiles, p.chunks), dim3(64), 0, st>>>(j);
+        return hipGetLastError();
+    }
     const dim3 grid(p.chunks);
     const uint32_t threads = (uint32_t)((j.cols + kBackCols - 1) / kBackCols + 63) & ~63u;
     if (p.tpr == 16)
@@ -954,18 +942,20 @@ void run_back(const Join<TZ, TA> &j, const Plan &p, hipStream_t st) {
         k_join_back<TZ, TA, N, P, 32, FULL><<<grid, dim3(256), 0, st>>>(j);
     else if (p.tpr == 64)
         k_join_back<TZ, TA, N, P, 64, FULL><<<grid, dim3(256), 0, st>>>(j);
+    else if (threads <= 128)
+        k_join_back<TZ, TA, N, P, 128, FULL><<<grid, dim3(threads), 0, st>>>(j);
     else if (threads <= 256)
         k_join_back<TZ, TA, N, P, 256, FULL><<<grid, dim3(threads), 0, st>>>(j);
     else if (threads <= 512)
         k_join_back<TZ, TA, N, P, 512, FULL><<<grid, dim3(threads), 0, st>>>(j);
     else
         k_join_back<TZ, TA, N, P, 1024, FULL><<<grid, dim3(threads), 0, st>>>(j);
+    return hipGetLastError();
 }
 
 template <typename TZ, typename TA>
 hipError_t backward(const spiky_lm_residual_args &a, const DropArgs &drop, const spiky_lm_residual_grads &g,
                     hipStream_t st) {
-    constexpr int N = sizeof(TA) == 4 ? 4 : 8;
     const Plan p = plan(a, g);
     Join<TZ, TA> j = view<TZ, TA>(a, drop);
     char *ws = static_cast<char *>(g.workspace);
@@ -981,22 +971,8 @@ hipError_t backward(const spiky_lm_residual_args &a, const DropArgs &drop, const
     j.chunk = p.chunk;
     j.span = p.span;
     j.chunks_per_span = p.chunks_per_span;
-    hipError_t err;
-    if (p.tpr) {
-        if (a.post_norm == SPIKY_NORM_LAYER || a.pre_norm == SPIKY_NORM_LAYER || a.post_bias || a.pre_bias)
-            run_back<TZ, TA, true>(j, p, st);
-        else
-            run_back<TZ, TA, false>(j, p, st);
-    } else {
-        err = over_rows(j, 1, 256, [&](dim3 grid, dim3 block) {
-            k_join_back_rows<TZ, TA, N, 256><<<grid, block, 0, st>>>(j);
-        });
-        if (err != hipSuccess) return err;
-        const uint64_t tiles = (a.cols + 64 * N - 1) / (64 * N);
-        // fewer than 2048 chunks, in y
-        k_join_back_cols<TZ, TA, N><<<dim3((uint32_t)tiles, p.chunks), dim3(64), 0, st>>>(j);
-    }
-    err = hipGetLastError();
+    const bool full = a.post_norm == SPIKY_NORM_LAYER || a.pre_norm == SPIKY_NORM_LAYER || a.post_bias || a.pre_bias;
+    hipError_t err = full ? run_back<TZ, TA, true>(j, p, st) : run_back<TZ, TA, false>(j, p, st);
     if (err != hipSuccess) return err;
     Sums s = {};
     void *outs[5] = {g.d_post_weight, g.d_post_bias, g.d_pre_weight, g.d_pre_bias, g.d_gate};
