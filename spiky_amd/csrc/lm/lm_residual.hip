@@ -143,38 +143,132 @@ __device__ __forceinline__ void gate_of(float (&g)[N], const J &j, uint32_t gate
     }
 }
 
+// Sums of K values over the `waves` waves of a row (TPR > 64) or its TPR lanes,
+// in every lane.  The waves' sums go through LDS, two buffers in turn: a buffer
+// is written again only after the barrier of the call in between, which its
+// readers have passed.  Lane i reads the sums of wave i % 16.
+template <int TPR, int K>
+__device__ __forceinline__ void row_sums(float (&x)[K], float4 (*lds)[(K + 3) / 4][16], uint32_t &turn,
+                                         uint32_t waves) {
+#pragma unroll
+    for (int k = 0; k < K; k++) x[k] = lanes_sum<(TPR < 64 ? TPR : 64)>(x[k]);
+    if constexpr (TPR > 64) {
+        constexpr int H = (K + 3) / 4;
+        float v[4 * H];
+#pragma unroll
+        for (int k = 0; k < 4 * H; k++) v[k] = k < K ? x[k < K ? k : 0] : 0.f;
+        if ((threadIdx.x & 63) == 0)
+#pragma unroll
+            for (int h = 0; h < H; h++)
+                lds[turn][h][threadIdx.x / 64] = make_float4(v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]);
+        __syncthreads();
+        const uint32_t wave = threadIdx.x & 15;
+#pragma unroll
+        for (int h = 0; h < H; h++) {
+            const float4 f = wave < waves ? lds[turn][h][wave] : make_float4(0.f, 0.f, 0.f, 0.f);
+            v[4 * h] = f.x, v[4 * h + 1] = f.y, v[4 * h + 2] = f.z, v[4 * h + 3] = f.w;
+        }
+#pragma unroll
+        for (int k = 0; k < K; k++) x[k] = lanes_sum<16>(v[k]);
+        turn ^= 1;
+    }
+}
+
 // ---- forward ---------------------------------------------------------------
-// A row in the registers of TPR threads, P pieces of N columns each: every
-// input is read once, the sums of both norms run over registers.
-template <typename TZ, typename TA, int N, int P, int TPR>
-__global__ __launch_bounds__(TPR < 256 && TPR <= 64 ? 256 : TPR) void k_join(Join<TZ, TA> j) {
-    constexpr int kRows = TPR <= 64 ? 256 / TPR : 1;
-    __shared__ float red[TPR > 64 ? 2 : 1][1][16];
-    RowSum<TPR, 1> row_sum{red};
-    const uint32_t lane = threadIdx.x % TPR;
-    const uint32_t row = j.row0 + blockIdx.x * kRows + threadIdx.x / TPR;
-    if (TPR <= 64 && row >= j.rows) return;
-    float z[P][N], v[P][N];
+// N values of a parameter or gate row: its words as loaded (half of them where it
+// is of a shorter type than float), and their values.
+template <typename TA, int N>
+__device__ __forceinline__ void words_of(Raw<float, N> &raw, const void *p, bool f32, uint64_t at, int n) {
+    if (sizeof(TA) == 4 || f32) {
+        raw.load(static_cast<const float *>(p) + at, n);
+    } else {
+        Raw<TA, N> half;
+        half.load(static_cast<const TA *>(p) + at, n);
+        __builtin_memcpy(raw.w, half.w, sizeof(half.w));
+    }
+}
+
+template <typename TA, int N>
+__device__ __forceinline__ void values_of(float (&v)[N], const Raw<float, N> &raw, bool f32) {
+    if (sizeof(TA) == 4 || f32) {
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = raw[i];
+    } else {
+        Raw<TA, N> half;
+        __builtin_memcpy(half.w, raw.w, sizeof(half.w));
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = half[i];
+    }
+}
+
+// A row in the registers of TPR threads (TPR > 64: of the workgroup, of up to TPR),
+// P pieces of N columns each: every input is read once, the sums of both norms run
+// over registers.  The row's loads are issued before the first sum, and with 8
+// columns a thread the parameters' too; with 16 these would halve the waves.
+// FULL: with layer norms or biases.
+template <typename TZ, typename TA, int N, int P, int TPR, bool FULL>
+__global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_join(Join<TZ, TA> j) {
+    constexpr int kSlots = TPR <= 64 ? 256 / TPR : 1, Q = N * P <= 8 ? P : 1;
+    constexpr bool AHEAD = N * P <= 8;
+    __shared__ float4 red[TPR > 64 ? 2 : 1][1][16];
+    uint32_t turn = 0;
+    const uint32_t threads = TPR <= 64 ? TPR : blockDim.x, waves = blockDim.x / 64;
+    const uint32_t lane = TPR <= 64 ? threadIdx.x % TPR : threadIdx.x;
+    uint32_t row = j.row0 + blockIdx.x * kSlots + (kSlots > 1 ? threadIdx.x / TPR : 0);
+    if (TPR == 64) row = __builtin_amdgcn_readfirstlane(row);
+    if (kSlots > 1 && row >= j.rows) return;
+
+    uint64_t col[P];
     int n[P];
-    const TZ *r = j.r + (int64_t)row * j.r_stride;
-    const TA *a = j.a + (int64_t)row * j.a_stride;
+    Raw<TZ, N> z_raw[P];
+    Raw<TA, N> a_raw[P];
+    Raw<float, N> g[P], w[Q], b[FULL ? Q : 1];
 #pragma unroll
     for (int p = 0; p < P; p++) {
-        const uint64_t col = (uint64_t)(p * TPR + lane) * N;
-        n[p] = piece_size(j.cols, col, N);
-        load(z[p], r + col, n[p]);
-        if (j.a) load(v[p], a + col, n[p]);
+        col[p] = (uint64_t)(p * threads + lane) * N;
+        n[p] = piece_size(j.cols, col[p], N);
+        if (j.a) a_raw[p].load(j.a + (int64_t)row * j.a_stride + col[p], n[p]);
+        z_raw[p].load(j.r + (int64_t)row * j.r_stride + col[p], n[p]);
     }
-    // mean (layer) and reciprocal deviation of the row held in x
-    auto deviation = [&](float (&x)[P][N], int kind, float eps, float &mean) {
+    const uint64_t gate_at = j.g ? (uint64_t)(row / j.gate_rows) * j.cols : 0;
+    auto parameters = [&](int p, const void *weight, const void *bias) {
+        const int q = AHEAD ? p : 0;
+        if (weight) words_of<TA>(w[q], weight, j.par_f32, col[p], n[p]);
+        if constexpr (FULL)
+            if (bias) words_of<TA>(b[q], bias, j.par_f32, col[p], n[p]);
+    };
+#pragma unroll
+    for (int p = 0; p < P; p++) {
+        if (j.g) words_of<TA>(g[p], j.g, j.gate_f32, gate_at + col[p], n[p]);
+        if (AHEAD) parameters(p, j.w1, j.b1);
+    }
+    auto affine = [&](float (&x)[N], int p, const void *weight, const void *bias) {
+        const int q = AHEAD ? p : 0;
+        if (!AHEAD) parameters(p, weight, bias);
+        float f[N];
+        if (weight) {
+            values_of<TA>(f, w[q], j.par_f32);
+#pragma unroll
+            for (int i = 0; i < N; i++) x[i] *= f[i];
+        }
+        if constexpr (FULL) {
+            if (bias) {
+                values_of<TA>(f, b[q], j.par_f32);
+#pragma unroll
+                for (int i = 0; i < N; i++) x[i] += f[i];
+            }
+        }
+    };
+    // Mean (layer) and reciprocal deviation of the row in x, whose columns past the end are 0.
+    auto deviation = [&](const float (&x)[P][N], int kind, float eps, float &mean) {
         float s[1] = {0.f};
         mean = 0.f;
-        if (kind == SPIKY_NORM_LAYER) {
+        if (FULL && kind == SPIKY_NORM_LAYER) {
 #pragma unroll
             for (int p = 0; p < P; p++)
 #pragma unroll
                 for (int i = 0; i < N; i++) s[0] += x[p][i];
-            row_sum(s);
+            row_sums<TPR, 1>(s, red, turn, waves);
             mean = s[0] * j.inv_cols;
             s[0] = 0.f;
         }
@@ -182,14 +276,22 @@ __global__ __launch_bounds__(TPR < 256 && TPR <= 64 ? 256 : TPR) void k_join(Joi
         for (int p = 0; p < P; p++)
 #pragma unroll
             for (int i = 0; i < N; i++) {
-                const float d = i < n[p] ? x[p][i] - mean : 0.f;
+                const float d = !FULL ? x[p][i] : i < n[p] ? x[p][i] - mean : 0.f;
                 s[0] += d * d;
             }
-        row_sum(s);
+        row_sums<TPR, 1>(s, red, turn, waves);
         return rsqrtf(s[0] * j.inv_cols + eps);
     };
+
+    float z[P][N];
     float4 st = {0.f, 1.f, 0.f, 1.f};
+    const uint64_t at = (uint64_t)row * j.cols;
     if (j.a) {
+        float v[P][N];
+#pragma unroll
+        for (int p = 0; p < P; p++)
+#pragma unroll
+            for (int i = 0; i < N; i++) v[p][i] = a_raw[p][i];
         if (j.post != SPIKY_NORM_NONE) {
             st.y = deviation(v, j.post, j.post_eps, st.x);
 #pragma unroll
@@ -198,39 +300,45 @@ __global__ __launch_bounds__(TPR < 256 && TPR <= 64 ? 256 : TPR) void k_join(Joi
                 for (int i = 0; i < N; i++) v[p][i] = (v[p][i] - st.x) * st.y;
         }
         const Dropper dr = dropper(j.drop);
-        const uint32_t gate_row = j.g ? row / j.gate_rows : 0;
 #pragma unroll
         for (int p = 0; p < P; p++) {
-            const uint64_t col = (uint64_t)(p * TPR + lane) * N;
-            float g[N];
-            affine_drop<TA>(v[p], j, dr, row, col, n[p]);
-            gate_of<TA>(g, j, gate_row, col, n[p]);
+            float f[N];
+            affine(v[p], p, j.w1, j.b1);
+            if (j.drops) drop(v[p], dr, row, col[p]);
 #pragma unroll
-            for (int i = 0; i < N; i++) z[p][i] = j.alpha * z[p][i] + j.beta * (g[i] * v[p][i]);
-            store(j.out + (uint64_t)row * j.cols + col, z[p], n[p]);
+            for (int i = 0; i < N; i++) f[i] = 1.f;
+            if (j.g) values_of<TA>(f, g[p], j.gate_f32);
+#pragma unroll
+            for (int i = 0; i < N; i++) z[p][i] = j.alpha * z_raw[p][i] + j.beta * (f[i] * v[p][i]);
         }
-    }
-    if (j.pre != SPIKY_NORM_NONE) {
-        // columns past the row's end hold what affine_drop made of zeros
+    } else {
 #pragma unroll
         for (int p = 0; p < P; p++)
 #pragma unroll
-            for (int i = 0; i < N; i++)
-                if (i >= n[p]) z[p][i] = 0.f;
+            for (int i = 0; i < N; i++) z[p][i] = z_raw[p][i];
+    }
+    if (AHEAD && j.pre != SPIKY_NORM_NONE)
+#pragma unroll
+        for (int p = 0; p < P; p++) parameters(p, j.w2, j.b2);
+    if (j.a)
+#pragma unroll
+        for (int p = 0; p < P; p++) store(j.out + at + col[p], z[p], n[p]);
+    if (j.pre != SPIKY_NORM_NONE) {
+        if (FULL) {
+            // columns past the row's end hold what was made of a mean's negative
+#pragma unroll
+            for (int p = 0; p < P; p++)
+#pragma unroll
+                for (int i = 0; i < N; i++)
+                    if (i >= n[p]) z[p][i] = 0.f;
+        }
         st.w = deviation(z, j.pre, j.pre_eps, st.z);
 #pragma unroll
         for (int p = 0; p < P; p++) {
-            const uint64_t col = (uint64_t)(p * TPR + lane) * N;
-            float w[N], b[N];
-            if (j.w2) param<TA>(w, j.w2, j.par_f32, col, n[p]);
-            if (j.b2) param<TA>(b, j.b2, j.par_f32, col, n[p]);
 #pragma unroll
-            for (int i = 0; i < N; i++) {
-                z[p][i] = (z[p][i] - st.z) * st.w;
-                if (j.w2) z[p][i] *= w[i];
-                if (j.b2) z[p][i] += b[i];
-            }
-            store(j.normed + (uint64_t)row * j.cols + col, z[p], n[p]);
+            for (int i = 0; i < N; i++) z[p][i] = (z[p][i] - st.z) * st.w;
+            affine(z[p], p, j.w2, j.b2);
+            store(j.normed + at + col[p], z[p], n[p]);
         }
     }
     if (j.stats && lane == 0) j.stats[row] = st;
@@ -308,37 +416,6 @@ __global__ __launch_bounds__(1024) void k_join_wide(Join<TZ, TA> j) {
 }
 
 // ---- backward --------------------------------------------------------------
-// Sums of K values over the `waves` waves of a row (TPR > 64) or its TPR lanes,
-// in every lane.  The waves' sums go through LDS, two buffers in turn: a buffer
-// is written again only after the barrier of the call in between, which its
-// readers have passed.  Lane i reads the sums of wave i % 16.
-template <int TPR, int K>
-__device__ __forceinline__ void row_sums(float (&x)[K], float4 (*lds)[(K + 3) / 4][16], uint32_t &turn,
-                                         uint32_t waves) {
-#pragma unroll
-    for (int k = 0; k < K; k++) x[k] = lanes_sum<(TPR < 64 ? TPR : 64)>(x[k]);
-    if constexpr (TPR > 64) {
-        constexpr int H = (K + 3) / 4;
-        float v[4 * H];
-#pragma unroll
-        for (int k = 0; k < 4 * H; k++) v[k] = k < K ? x[k < K ? k : 0] : 0.f;
-        if ((threadIdx.x & 63) == 0)
-#pragma unroll
-            for (int h = 0; h < H; h++)
-                lds[turn][h][threadIdx.x / 64] = make_float4(v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]);
-        __syncthreads();
-        const uint32_t wave = threadIdx.x & 15;
-#pragma unroll
-        for (int h = 0; h < H; h++) {
-            const float4 f = wave < waves ? lds[turn][h][wave] : make_float4(0.f, 0.f, 0.f, 0.f);
-            v[4 * h] = f.x, v[4 * h + 1] = f.y, v[4 * h + 2] = f.z, v[4 * h + 3] = f.w;
-        }
-#pragma unroll
-        for (int k = 0; k < K; k++) x[k] = lanes_sum<16>(v[k]);
-        turn ^= 1;
-    }
-}
-
 // The rows [row, end) of chunk number `chunk`.
 template <typename J>
 __device__ __forceinline__ void chunk_rows(const J &j, uint32_t chunk, uint32_t &row, uint32_t &end) {
@@ -394,26 +471,11 @@ struct Piece {
     }
     template <typename J>
     __device__ __forceinline__ void load_gate(const J &j, uint32_t gate_row) {
-        const uint64_t at = (uint64_t)gate_row * j.cols + col;
-        if (sizeof(TA) == 4 || j.gate_f32) {
-            g_raw.load(static_cast<const float *>(j.g) + at, n);
-        } else {
-            Raw<TA, N> half;
-            half.load(static_cast<const TA *>(j.g) + at, n);
-            __builtin_memcpy(g_raw.w, half.w, sizeof(half.w));
-        }
+        words_of<TA>(g_raw, j.g, j.gate_f32, (uint64_t)gate_row * j.cols + col, n);
     }
     template <typename J>
     __device__ __forceinline__ void take_gate(const J &j) {
-        if (sizeof(TA) == 4 || j.gate_f32) {
-#pragma unroll
-            for (int i = 0; i < N; i++) g[i] = g_raw[i];
-        } else {
-            Raw<TA, N> half;
-            __builtin_memcpy(half.w, g_raw.w, sizeof(half.w));
-#pragma unroll
-            for (int i = 0; i < N; i++) g[i] = half[i];
-        }
+        values_of<TA>(g, g_raw, j.gate_f32);
     }
     template <typename J>
     __device__ __forceinline__ void fetch(const J &j, uint32_t row, bool row_gates) {
@@ -839,30 +901,41 @@ hipError_t over_rows(J &j, uint32_t kRows, uint32_t threads, F &&launch) {
     return hipSuccess;
 }
 
-template <typename TZ, typename TA, int N, int P, int TPR>
+// W columns a thread.
+template <typename TZ, typename TA, int W, int TPR, bool FULL>
 hipError_t run_rows(Join<TZ, TA> &j, hipStream_t st) {
-    return over_rows(j, TPR <= 64 ? 256 / TPR : 1, TPR <= 64 ? 256 : TPR, [&](dim3 grid, dim3 block) {
-        k_join<TZ, TA, N, P, TPR><<<grid, block, 0, st>>>(j);
+    constexpr int N = sizeof(TA) == 4 ? 4 : 8;
+    const uint32_t threads = TPR <= 64 ? 256 : (uint32_t)((j.cols + W - 1) / W + 63) & ~63u;
+    return over_rows(j, TPR <= 64 ? 256 / TPR : 1, threads, [&](dim3 grid, dim3 block) {
+        k_join<TZ, TA, N, W / N, TPR, FULL><<<grid, block, 0, st>>>(j);
     });
+}
+
+template <typename TZ, typename TA, bool FULL>
+hipError_t run_forward(Join<TZ, TA> &j, hipStream_t st) {
+    constexpr int N = sizeof(TA) == 4 ? 4 : 8;
+    if (j.cols <= 128) return run_rows<TZ, TA, 8, 16, FULL>(j, st);
+    if (j.cols <= 256) return run_rows<TZ, TA, 8, 32, FULL>(j, st);
+    if (j.cols <= 512) return run_rows<TZ, TA, 8, 64, FULL>(j, st);
+    if (j.cols <= 1024) return run_rows<TZ, TA, 16, 64, FULL>(j, st);
+    if (j.cols <= 2048) return run_rows<TZ, TA, 8, 256, FULL>(j, st);
+    if (j.cols <= 4096) return run_rows<TZ, TA, 8, 512, FULL>(j, st);
+    if (j.cols <= 8192) return run_rows<TZ, TA, 8, 1024, FULL>(j, st);
+    if (j.cols <= 16384) return run_rows<TZ, TA, 16, 1024, FULL>(j, st);
+    return over_rows(j, 1, 1024, [&](dim3 grid, dim3 block) { k_join_wide<TZ, TA, N><<<grid, block, 0, st>>>(j); });
+}
+
+bool is_full(const spiky_lm_residual_args &a) {
+    return a.post_norm == SPIKY_NORM_LAYER || a.pre_norm == SPIKY_NORM_LAYER || a.post_bias || a.pre_bias;
 }
 
 template <typename TZ, typename TA>
 hipError_t forward(const spiky_lm_residual_args &a, const DropArgs &drop, void *out, void *normed,
                    hipStream_t st) {
-    constexpr int N = sizeof(TA) == 4 ? 4 : 8;
     Join<TZ, TA> j = view<TZ, TA>(a, drop);
     j.out = static_cast<TZ *>(out);
     j.normed = static_cast<TA *>(normed);
-    const uint64_t pieces = (a.cols + N - 1) / N;
-    if (pieces <= 16) return run_rows<TZ, TA, N, 1, 16>(j, st);
-    if (pieces <= 32) return run_rows<TZ, TA, N, 1, 32>(j, st);
-    if (pieces <= 64) return run_rows<TZ, TA, N, 1, 64>(j, st);
-    if (pieces <= 128) return run_rows<TZ, TA, N, 1, 128>(j, st);
-    if (pieces <= 256) return run_rows<TZ, TA, N, 1, 256>(j, st);
-    if (pieces <= 512) return run_rows<TZ, TA, N, 1, 512>(j, st);
-    if (pieces <= 1024) return run_rows<TZ, TA, N, 1, 1024>(j, st);
-    if (pieces <= 2048) return run_rows<TZ, TA, N, 2, 1024>(j, st);
-    return over_rows(j, 1, 1024, [&](dim3 grid, dim3 block) { k_join_wide<TZ, TA, N><<<grid, block, 0, st>>>(j); });
+    return is_full(a) ? run_forward<TZ, TA, true>(j, st) : run_forward<TZ, TA, false>(j, st);
 }
 
 // How the rows are cut into chunks, and the workspace's regions.
@@ -971,8 +1044,7 @@ hipError_t backward(const spiky_lm_residual_args &a, const DropArgs &drop, const
     j.chunk = p.chunk;
     j.span = p.span;
     j.chunks_per_span = p.chunks_per_span;
-    const bool full = a.post_norm == SPIKY_NORM_LAYER || a.pre_norm == SPIKY_NORM_LAYER || a.post_bias || a.pre_bias;
-    hipError_t err = full ? run_back<TZ, TA, true>(j, p, st) : run_back<TZ, TA, false>(j, p, st);
+    hipError_t err = is_full(a) ? run_back<TZ, TA, true>(j, p, st) : run_back<TZ, TA, false>(j, p, st);
     if (err != hipSuccess) return err;
     Sums s = {};
     void *outs[5] = {g.d_post_weight, g.d_post_bias, g.d_pre_weight, g.d_pre_bias, g.d_gate};
