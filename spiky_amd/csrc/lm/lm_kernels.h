@@ -143,14 +143,18 @@ __device__ __forceinline__ Dropper dropper(const DropArgs &a) {
             (uint32_t)(offset >> 32)};
 }
 
+__device__ __forceinline__ uint32_t xor3(uint32_t a, uint32_t b, uint32_t c) {
+    return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96);  // one instruction; the compiler takes two for a ^ b ^ c
+}
+
 __device__ __forceinline__ void drop4(float *v, const Dropper &d, uint32_t row, uint32_t group) {
     uint32_t c0 = group, c1 = row, c2 = d.o0, c3 = d.o1, k0 = d.k0, k1 = d.k1;
 #pragma unroll
     for (int i = 0; i < 7; i++) {
         const uint64_t p0 = (uint64_t)c0 * 0xD2511F53u, p1 = (uint64_t)c2 * 0xCD9E8D57u;
-        c0 = (uint32_t)(p1 >> 32) ^ c1 ^ k0;
+        c0 = xor3((uint32_t)(p1 >> 32), c1, k0);
         c1 = (uint32_t)p1;
-        c2 = (uint32_t)(p0 >> 32) ^ c3 ^ k1;
+        c2 = xor3((uint32_t)(p0 >> 32), c3, k1);
         c3 = (uint32_t)p0;
         k0 += 0x9E3779B9u;
         k1 += 0xBB67AE85u;

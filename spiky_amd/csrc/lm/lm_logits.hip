@@ -8,9 +8,14 @@ namespace lm {
 namespace {
 
 constexpr uint32_t kThreads = 256;
+// The word of an entry in LDS: flags, and in the bits below the times that it is
+// among the tokens after the prompt.  Histories short enough leave bits 18 to 29
+// for the slot of its sum of sparse biases; for others the slots have an array.
 constexpr uint32_t kSeen = 0x80000000u;    // among the prompt's tokens
 constexpr uint32_t kBiased = 0x40000000u;  // among the bias ids
-constexpr uint32_t kCount = 0x3fffffffu;   // times among the tokens after the prompt
+constexpr uint32_t kSlotShift = 18, kSlotMask = 0xfff;
+
+__host__ __device__ __forceinline__ bool slots_in_words(uint64_t history) { return history < 1u << kSlotShift; }
 
 __device__ __forceinline__ uint32_t length_at(const void *p, bool i64, uint32_t row, uint32_t most) {
     if (!p) return most;
@@ -34,29 +39,37 @@ struct Tokens {
 
     // Those past `end` are -1.
     __device__ __forceinline__ void load(const T *tokens, uint32_t at, uint32_t end) {
+        if (at + kAhead * kThreads <= end) {
+#pragma unroll
+            for (uint32_t k = 0; k < kAhead; k++) id[k] = *past(tokens + at + k * kThreads, threadIdx.x);
+            return;
+        }
 #pragma unroll
         for (uint32_t k = 0; k < kAhead; k++) {
-            const uint32_t i = at + k * kThreads + threadIdx.x;
             id[k] = (T)-1;
-            if (i < end) id[k] = tokens[i];
+            if (at + k * kThreads + threadIdx.x < end) id[k] = *past(tokens + at + k * kThreads, threadIdx.x);
         }
     }
-    // Adds those before len to the words of the chunk's entries.
+    // Adds those before len to the words of the chunk's entries.  A workgroup's
+    // kThreads are nearly always all of the prompt or all after it, and whole.
     __device__ __forceinline__ void count(uint32_t at, uint32_t len, uint32_t prompt, uint32_t base, uint32_t size,
                                           uint32_t *words) const {
 #pragma unroll
         for (uint32_t k = 0; k < kAhead; k++) {
-            if (at + k * kThreads >= len) break;
-            const uint32_t i = at + k * kThreads + threadIdx.x;
+            const uint32_t i = at + k * kThreads;
+            if (i >= len) break;
             // base < 2^31, so a negative token stays past any chunk
             const uint32_t o = (uint32_t)id[k] - base;
-            bool there = o < size && i < len;
+            bool there = o < size;
             if (sizeof(T) == 8) there = there && (uint32_t)((uint64_t)id[k] >> 32) == 0;
-            if (!there) continue;
-            if (i < prompt)
-                atomicOr(&words[o], kSeen);
-            else
-                atomicAdd(&words[o], 1u);
+            if (i >= prompt) {
+                if (i + kThreads > len) there = there && i + threadIdx.x < len;
+                if (there) atomicAdd(&words[o], 1u);
+            } else {
+                const bool said = there && i + threadIdx.x >= prompt && i + threadIdx.x < len;
+                if (there && i + threadIdx.x < prompt) atomicOr(&words[o], kSeen);
+                if (said) atomicAdd(&words[o], 1u);
+            }
         }
     }
 };
@@ -72,61 +85,75 @@ __device__ __forceinline__ float bias_value(const spiky_lm_logits_args &a, uint3
     return k < a.n_bias ? a.bias_values[(uint64_t)row * a.bias_values_stride + k] : 0.f;
 }
 
-// The sums of the row's sparse biases for the chunk's entries: sums[slots[o]] for
-// an entry o that is flagged.  The ids go by kThreads (id and value: a thread's
-// first): those in the chunk are listed in their order, and the first of each
+// The sums of the row's sparse biases for the chunk's entries.  The ids go by
+// kThreads: those in the chunk are listed in their order, and the first of each
 // entry adds up the others, so repeated ids are added in their order whatever the
 // threads do.
-__device__ __forceinline__ void add_sparse(const spiky_lm_logits_args &a, uint32_t row, uint32_t base, uint32_t size,
-                                           int64_t id, float value, uint32_t *words, uint16_t *slots, float *sums) {
-    __shared__ uint32_t list_id[kThreads];
-    __shared__ float list_value[kThreads];
-    __shared__ uint32_t wave_count[2][kThreads / 64], taken;
-    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid / 64;
-    if (tid == 0) taken = 0;
-    uint32_t turn = 0;
-    for (uint64_t k0 = 0; k0 < a.n_bias; k0 += kThreads, turn ^= 1) {
-        if (k0) id = bias_id(a, row, k0 + tid), value = bias_value(a, row, k0 + tid);
-        const uint64_t o = (uint64_t)id - base;
-        const bool there = o < size;
-        const uint64_t all = __ballot(there);
-        if (lane == 0) wave_count[turn][wave] = __popcll(all);
-        __syncthreads();
-        uint32_t at = __popcll(all & ((1ull << lane) - 1)), listed = 0;
+struct Sparse {
+    uint32_t list_id[kThreads];
+    float list_value[kThreads];
+    uint32_t wave_count[2][kThreads / 64], taken;
+
+    // Before a barrier: how many of the threads' ids are in the chunk.
+    __device__ __forceinline__ uint64_t announce(int64_t id, uint32_t turn, uint32_t base, uint32_t size) {
+        const uint64_t all = __ballot((uint64_t)id - base < size);
+        if ((threadIdx.x & 63) == 0) wave_count[turn][threadIdx.x / 64] = __popcll(all);
+        return all;
+    }
+
+    // After it.  Ends with a barrier.
+    __device__ __forceinline__ void add(const spiky_lm_logits_args &a, uint32_t row, uint32_t base, uint32_t size,
+                                        int64_t id, float value, uint64_t all, uint32_t *words, uint16_t *slots,
+                                        float *sums) {
+        const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid / 64;
+        const bool in_words = slots_in_words(a.history);
+        uint32_t turn = 0;
+        for (uint64_t k0 = 0;;) {
+            uint32_t at = __popcll(all & ((1ull << lane) - 1)), listed = 0;
 #pragma unroll
-        for (uint32_t w = 0; w < kThreads / 64; w++) {
-            if (w < wave) at += wave_count[turn][w];
-            listed += wave_count[turn][w];
-        }
-        if (listed == 0) continue;
-        if (there) {
-            list_id[at] = (uint32_t)o;
-            list_value[at] = value;
-        }
-        __syncthreads();
-        if (tid < listed) {
-            const uint32_t mine = list_id[tid];
-            bool leads = true;
-            float sum = 0.f;
-            for (uint32_t j = 0; j < listed; j++) {
-                if (list_id[j] != mine) continue;
-                leads = leads && j >= tid;
-                sum += list_value[j];
+            for (uint32_t w = 0; w < kThreads / 64; w++) {
+                if (w < wave) at += wave_count[turn][w];
+                listed += wave_count[turn][w];
             }
-            if (leads) {
-                if (words[mine] & kBiased) {  // by a round before
-                    sums[slots[mine]] += sum;
-                } else {
-                    const uint32_t slot = atomicAdd(&taken, 1u);
-                    slots[mine] = (uint16_t)slot;
-                    sums[slot] = sum;
-                    atomicOr(&words[mine], kBiased);
+            if (listed) {
+                if (all >> lane & 1) {
+                    list_id[at] = (uint32_t)id - base;
+                    list_value[at] = value;
+                }
+                __syncthreads();
+                if (tid < listed) {
+                    const uint32_t mine = list_id[tid];
+                    bool leads = true;
+                    float sum = 0.f;
+                    for (uint32_t j = 0; j < listed; j++) {
+                        if (list_id[j] != mine) continue;
+                        leads = leads && j >= tid;
+                        sum += list_value[j];
+                    }
+                    if (leads) {
+                        const uint32_t w = words[mine];
+                        if (w & kBiased) {  // by ids before these
+                            sums[in_words ? w >> kSlotShift & kSlotMask : slots[mine]] += sum;
+                        } else {
+                            const uint32_t slot = atomicAdd(&taken, 1u);
+                            sums[slot] = sum;
+                            if (!in_words) slots[mine] = (uint16_t)slot;
+                            // tokens may be counted meanwhile, in other bits
+                            atomicOr(&words[mine], kBiased | (in_words ? slot << kSlotShift : 0));
+                        }
+                    }
                 }
             }
+            k0 += kThreads;
+            if (k0 >= a.n_bias) break;
+            turn ^= 1;
+            id = bias_id(a, row, k0 + tid), value = bias_value(a, row, k0 + tid);
+            all = announce(id, turn, base, size);
+            __syncthreads();
         }
-        __syncthreads();  // the list is written again
+        __syncthreads();
     }
-}
+};
 
 // A workgroup takes a chunk of up to kThreads * P * N entries of a row.  Counts
 // of the row's tokens in the chunk, and which entries have sparse biases, are
@@ -136,11 +163,12 @@ __device__ __forceinline__ void add_sparse(const spiky_lm_logits_args &a, uint32
 template <typename TI, typename TO, int N, int P>
 __global__ __launch_bounds__(kThreads) void k_logits(spiky_lm_logits_args a) {
     constexpr uint32_t kChunk = kThreads * P * N;
-    // words where there are tokens or bias ids; slots and as many sums as may be needed where there are bias ids
+    // words where there are tokens or bias ids; with bias ids as many sums as may be needed, and slots
     extern __shared__ uint4 space[];
+    __shared__ Sparse sparse;
     uint32_t *const words = reinterpret_cast<uint32_t *>(space);
-    uint16_t *const slots = reinterpret_cast<uint16_t *>(words + kChunk);
-    float *const sums = reinterpret_cast<float *>(slots + kChunk);
+    float *const sums = reinterpret_cast<float *>(words + kChunk);
+    uint16_t *const slots = reinterpret_cast<uint16_t *>(sums + min((uint64_t)kChunk, a.n_bias));
     const uint32_t tid = threadIdx.x, row = blockIdx.y, base = blockIdx.x * kChunk;
     const uint32_t size = min(kChunk, (uint32_t)a.vocab - base);
     const bool marks = a.tokens || a.bias_ids;
@@ -203,6 +231,7 @@ __global__ __launch_bounds__(kThreads) void k_logits(spiky_lm_logits_args a) {
     // Products with reciprocals; a reciprocal past the largest number is not one.
     const float less = 1.f / rho, cool = heat > 0.f ? 1.f / heat : 1.f;
     const bool divide_heat = heat > 0.f && __builtin_isinf(cool), divide_rho = __builtin_isinf(less);
+    const uint32_t count_mask = slots_in_words(a.history) ? (1u << kSlotShift) - 1 : kBiased - 1;
     auto finish = [&](const Piece &q, uint32_t o, int n) {
         float x[N];
 #pragma unroll
@@ -231,15 +260,16 @@ __global__ __launch_bounds__(kThreads) void k_logits(spiky_lm_logits_args a) {
             if (any & kBiased) {
 #pragma unroll
                 for (int i = 0; i < N; i++)
-                    if (w[i] & kBiased) x[i] += sums[slots[o + i]];
+                    if (w[i] & kBiased)
+                        x[i] += sums[slots_in_words(a.history) ? w[i] >> kSlotShift & kSlotMask : slots[o + i]];
             }
-            if (any & (kSeen | kCount)) {
+            if (any & (kSeen | count_mask)) {
 #pragma unroll
                 for (int i = 0; i < N; i++) {
                     float y = x[i] * (x[i] > 0.f ? less : rho);
                     if (divide_rho && x[i] > 0.f) y = x[i] / rho;
-                    x[i] = w[i] & (kSeen | kCount) ? y : x[i];
-                    const uint32_t times = w[i] & kCount;
+                    x[i] = w[i] & (kSeen | count_mask) ? y : x[i];
+                    const uint32_t times = w[i] & count_mask;
                     x[i] = times ? x[i] - (phi * (float)times + pi) : x[i];
                 }
             }
@@ -272,6 +302,9 @@ __global__ __launch_bounds__(kThreads) void k_logits(spiky_lm_logits_args a) {
         for (int p = 0; p < P; p++) load(piece[p], (p * kThreads + tid) * N, N);
     if (marks) {
         for (uint32_t i = tid; i < kChunk / 4; i += kThreads) space[i] = make_uint4(0, 0, 0, 0);
+        uint64_t all = 0;
+        if (a.bias_ids) all = sparse.announce(sparse_id, 0, base, size);
+        if (tid == 0) sparse.taken = 0;
         __syncthreads();
         if (a.tokens) {
             const uint32_t len = length_at(a.lengths, a.lengths_i64, row, history);
@@ -290,8 +323,10 @@ __global__ __launch_bounds__(kThreads) void k_logits(spiky_lm_logits_args a) {
             else
                 count_all(short_ids, static_cast<const int32_t *>(a.tokens));
         }
-        if (a.bias_ids) add_sparse(a, row, base, size, sparse_id, sparse_value, words, slots, sums);
-        __syncthreads();
+        if (a.bias_ids)
+            sparse.add(a, row, base, size, sparse_id, sparse_value, all, words, slots, sums);
+        else
+            __syncthreads();
     }
     if (whole) {
 #pragma unroll
@@ -315,7 +350,9 @@ hipError_t launch(const spiky_lm_logits_args &a, hipStream_t st) {
     while (chunk > kThreads * N && (a.vocab + chunk - 1) / chunk * a.rows < 2 * kCUs) chunk /= 2;
     const uint64_t chunks = (a.vocab + chunk - 1) / chunk;
     size_t lds = a.tokens || a.bias_ids ? chunk * sizeof(uint32_t) : 0;
-    if (a.bias_ids) lds += chunk * sizeof(uint16_t) + (a.n_bias < chunk ? a.n_bias : chunk) * sizeof(float);
+    if (a.bias_ids)
+        lds += (a.n_bias < chunk ? a.n_bias : chunk) * sizeof(float) +
+               (slots_in_words(a.history) ? 0 : chunk * sizeof(uint16_t));
     // 65535 rows a launch, in y
     for (uint64_t row0 = 0; row0 < a.rows; row0 += 65535) {
         const uint32_t n = (uint32_t)(a.rows - row0 < 65535 ? a.rows - row0 : 65535);
