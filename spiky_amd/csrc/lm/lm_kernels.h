@@ -147,7 +147,8 @@ __device__ __forceinline__ uint32_t xor3(uint32_t a, uint32_t b, uint32_t c) {
     return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96);  // one instruction; the compiler takes two for a ^ b ^ c
 }
 
-__device__ __forceinline__ void drop4(float *v, const Dropper &d, uint32_t row, uint32_t group) {
+// Bit i: the group's column i is kept.
+__device__ __forceinline__ uint32_t kept4(const Dropper &d, uint32_t row, uint32_t group) {
     uint32_t c0 = group, c1 = row, c2 = d.o0, c3 = d.o1, k0 = d.k0, k1 = d.k1;
 #pragma unroll
     for (int i = 0; i < 7; i++) {
@@ -159,19 +160,30 @@ __device__ __forceinline__ void drop4(float *v, const Dropper &d, uint32_t row, 
         k0 += 0x9E3779B9u;
         k1 += 0xBB67AE85u;
     }
-    const bool any = d.scale != 0.f;
-    v[0] = any && c0 >= d.threshold ? v[0] * d.scale : 0.f;
-    v[1] = any && c1 >= d.threshold ? v[1] * d.scale : 0.f;
-    v[2] = any && c2 >= d.threshold ? v[2] * d.scale : 0.f;
-    v[3] = any && c3 >= d.threshold ? v[3] * d.scale : 0.f;
+    return (c0 >= d.threshold ? 1 : 0) | (c1 >= d.threshold ? 2 : 0) | (c2 >= d.threshold ? 4 : 0) |
+           (c3 >= d.threshold ? 8 : 0);
 }
 
 // The same for the N columns from col, a multiple of 4.
 template <int N>
-__device__ __forceinline__ void drop(float (&v)[N], const Dropper &d, uint32_t row, uint64_t col) {
-    static_assert(N % 4 == 0, "whole groups");
+__device__ __forceinline__ uint32_t kept(const Dropper &d, uint32_t row, uint64_t col) {
+    static_assert(N % 4 == 0 && N <= 32, "whole groups");
+    uint32_t bits = 0;
 #pragma unroll
-    for (int i = 0; i < N; i += 4) drop4(v + i, d, row, (uint32_t)(col / 4) + i / 4);
+    for (int i = 0; i < N; i += 4) bits |= kept4(d, row, (uint32_t)(col / 4) + i / 4) << i;
+    return d.scale != 0.f ? bits : 0;
+}
+
+// x where bit i is set, else 0, whatever x is.
+__device__ __forceinline__ float where(uint32_t bits, int i, float x) {
+    return __int_as_float(__float_as_int(x) & ((int32_t)(bits << (31 - i)) >> 31));
+}
+
+template <int N>
+__device__ __forceinline__ void drop(float (&v)[N], const Dropper &d, uint32_t row, uint64_t col) {
+    const uint32_t bits = kept<N>(d, row, col);
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = where(bits, i, v[i] * d.scale);
 }
 
 // ---- launchers -------------------------------------------------------------

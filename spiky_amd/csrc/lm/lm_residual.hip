@@ -446,7 +446,8 @@ struct Piece {
     Raw<TZ, N> z_raw, dz_raw;
     Raw<TA, N> a_raw, dh_raw;
     Raw<float, N> g_raw;  // half of the words where the gate is of a shorter type
-    float n1[N], n2[N], e[N], keep[N];
+    float n1[N], n2[N], e[N];
+    uint32_t keep;  // bit i: column i is not dropped
 
     template <typename J>
     __device__ __forceinline__ void place(const J &j, uint64_t column) {
@@ -488,10 +489,10 @@ struct Piece {
         if (row_gates) load_gate(j, row);
     }
     // v of the forward pass, and then d: a dropped element is 0 whatever it holds.
-    __device__ __forceinline__ float dropped(int i) const {
+    __device__ __forceinline__ float dropped(const Dropper &dr, int i) const {
         float v = n1[i] * w1[i];
         if (FULL) v += b1[FULL ? i : 0];
-        return keep[i] != 0.f ? v * keep[i] : 0.f;
+        return where(keep, i, v * dr.scale);
     }
     // The row's values from its loads, and the piece's share of the row's sums s;
     // add(k, v) adds v to the column sums k.
@@ -500,22 +501,19 @@ struct Piece {
                                             float (&s)[K], F &&add) {
         const float r2 = j.dh ? st.w : 0.f;
         float dw2[N], db2[FULL ? N : 1];
+        const float kept_scale = dr.scale * j.beta;
+        keep = j.drops ? kept<N>(dr, row, col) : ~0u;
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            keep[i] = 1.f;
             n1[i] = (a_raw[i] - st.x) * st.y;
-        }
-        if (j.drops) drop(keep, dr, row, col);
-#pragma unroll
-        for (int i = 0; i < N; i++) {
             float z = z_raw[i];
-            if (j.a) z = j.alpha * z + j.beta * (g[i] * dropped(i));
+            if (j.a) z = j.alpha * z + j.beta * (g[i] * dropped(dr, i));
             n2[i] = j.dh ? (z - st.z) * r2 : 0.f;
             const float dh = dh_raw[i], t = dh * w2[i];
             e[i] = dz_raw[i] + r2 * t;
             dw2[i] = dh * n2[i];
-            const float c = keep[i] * (j.beta * g[i]) * w1[i];
-            const float ce = keep[i] != 0.f ? c * e[i] : 0.f, cn = c * n1[i];
+            const float c = where(keep, i, kept_scale * g[i] * w1[i]);
+            const float ce = where(keep, i, c * e[i]), cn = c * n1[i];
             s[0] += t * n2[i];
             s[1] += ce * n1[i];
             s[2] += cn * n2[i];
@@ -534,7 +532,9 @@ struct Piece {
     }
     // The row's gradients, from its means (mean t, mean t n2, mean dn, mean dn n1).
     template <typename J, typename F>
-    __device__ __forceinline__ void finish(const J &j, const float4 &st, const float4 &m, uint32_t row, F &&add) {
+    __device__ __forceinline__ void finish(const J &j, const Dropper &dr, const float4 &st, const float4 &m,
+                                           uint32_t row, F &&add) {
+        const float kept_scale = dr.scale * j.beta;
         const float r2 = j.dh ? st.w : 0.f, alpha = j.a ? j.alpha : 1.f;
         const uint64_t at = (uint64_t)row * j.cols + col;
         float out[N], da[N], dg[N], dw1[N], db1[N];
@@ -542,8 +542,8 @@ struct Piece {
         for (int i = 0; i < N; i++) {
             const float q = e[i] - r2 * (m.x + n2[i] * m.y);
             out[i] = alpha * q;
-            dg[i] = j.beta * (dropped(i) * q);
-            db1[i] = keep[i] != 0.f ? j.beta * (g[i] * q) * keep[i] : 0.f;
+            dg[i] = j.beta * (dropped(dr, i) * q);
+            db1[i] = where(keep, i, kept_scale * (g[i] * q));
             dw1[i] = db1[i] * n1[i];
             da[i] = db1[i];
             if (j.post != SPIKY_NORM_NONE) da[i] = st.y * (db1[i] * w1[i] - m.z - n1[i] * m.w);
@@ -614,7 +614,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_join_back(Join<TZ, TA
         end = row + min(end - row, share);
     }
     if (TPR == 64) row = __builtin_amdgcn_readfirstlane(row), end = __builtin_amdgcn_readfirstlane(end);
-    const Dropper dr = dropper(j.drop);
+    const Dropper dr = dropper(j.drop);  // of scale 1 where nothing is dropped
     const bool row_gates = j.g && j.gate_rows == 1;
     uint32_t gate_row = j.g ? row / j.gate_rows : 0, in_gate = j.g ? row - gate_row * j.gate_rows : 0;
 
@@ -674,7 +674,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_join_back(Join<TZ, TA
         row_sums<TPR, K>(s, red, turn, waves);
         const float4 m = row_means<FULL>(j, now, s);
 #pragma unroll
-        for (int p = 0; p < P; p++) x[p].finish(j, now, m, row, adds_to(p));
+        for (int p = 0; p < P; p++) x[p].finish(j, dr, now, m, row, adds_to(p));
         if (j.g && !row_gates && ++in_gate == j.gate_rows) {
             // the rows of a gate end here, and with them its sum, where no other chunk has some of them
 #pragma unroll
@@ -777,7 +777,7 @@ __global__ __launch_bounds__(64) void k_join_back_cols(Join<TZ, TA> j) {
     uint32_t row, end;
     chunk_rows(j, blockIdx.y, row, end);
     if (row >= end) return;
-    const Dropper dr = dropper(j.drop);
+    const Dropper dr = dropper(j.drop);  // of scale 1 where nothing is dropped
     const bool row_gates = j.g && j.gate_rows == 1;
     uint32_t gate_row = j.g ? row / j.gate_rows : 0, in_gate = j.g ? row - gate_row * j.gate_rows : 0;
     float acc[5][N], s[K];
@@ -803,7 +803,7 @@ __global__ __launch_bounds__(64) void k_join_back_cols(Join<TZ, TA> j) {
             st = j.stats[row + 1], m = j.row_sums[row + 1];
             x.fetch(j, row + 1, row_gates);
         }
-        x.finish(j, now, means, row, add);
+        x.finish(j, dr, now, means, row, add);
         if (j.g && !row_gates && ++in_gate == j.gate_rows) {
             if (j.dgate) {
                 x.store_gate(j, gate_row, acc[kSumG]);
@@ -880,6 +880,7 @@ Join<TZ, TA> view(const spiky_lm_residual_args &a, const DropArgs &drop) {
     j.inv_cols = (float)(1.0 / (double)a.cols);
     j.drops = a.branch && a.dropout_p > 0.0;
     j.drop = drop;
+    if (!j.drops) j.drop.scale = 1.f;
     j.rows = (uint32_t)a.rows;
     j.gate_rows = a.gate ? (uint32_t)a.gate_rows : (uint32_t)a.rows;
     j.cols = a.cols;
@@ -1022,7 +1023,7 @@ hipError_t run_back(Join<TZ, TA> &j, const Plan &p, hipStream_t st) {
     else if (threads <= 512)
         k_join_back<TZ, TA, N, P, 512, FULL><<<grid, dim3(threads), 0, st>>>(j);
     else
-        k_join_back<TZ, TA, N, P, 1024, FULL><<<grid, dim3(threads), 0, st>>>(j);
+        k_join_back<TZ, TA, N, 2 * P, 512, FULL><<<grid, dim3((threads / 2 + 63) & ~63u), 0, st>>>(j);
     return hipGetLastError();
 }
 
