@@ -25,7 +25,7 @@ struct Divider {
     }
 };
 
-// A row is cut into pieces of 16 bytes (its last one may be short), and the
+// A row is cut into pieces of 16 bytes, and the
 // pieces of all rows are numbered through; thread t of a workgroup takes pieces
 // t, t + 256, ... of the workgroup's kThreads * kPieces.
 template <typename T>
@@ -47,19 +47,18 @@ __global__ __launch_bounds__(kThreads) void k_dropout(const T *__restrict__ x, i
                                                                  : row_pieces.divide((uint32_t)at);
         const uint64_t row = row0 + down;
         if (row >= rows) break;
-        const uint64_t col = (at - (uint64_t)down * row_pieces.d) * N;
-        const uint64_t left = cols - col;
-        const int n = left < N ? (int)left : N;
+        Place<N> place;
+        place.set(cols, (at - (uint64_t)down * row_pieces.d) * N);
         float v[N];
-        load(v, x + (int64_t)row * x_stride + col, n);
-        drop(v, d, (uint32_t)row, col);
+        load(v, x + (int64_t)row * x_stride + place.col, place.n);
+        drop(v, d, (uint32_t)row, place.col);
         if (sizeof(T) == 2) {
             // the product rounds to 32 bits and then to T, for every T alike: without this the
             // compiler rounds fp16 products once (v_fma_mixlo_f16)
 #pragma unroll
             for (int k = 0; k < N; k++) asm("" : "+v"(v[k]));
         }
-        store(y + row * cols + col, v, n);
+        store(y + row * cols + place.col, v, place.n);
     }
 }
 

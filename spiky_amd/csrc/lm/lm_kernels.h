@@ -46,62 +46,54 @@ __device__ __forceinline__ f16 from_f32<f16>(float x) {
     return (f16)x;
 }
 
-// N elements from p, of which the first n exist; the others read as 0.  A whole
-// piece is one load of its full width at any alignment of the element type
-// (the target's unaligned access mode); a row's last piece goes by element.
-template <typename T, int N>
-__device__ __forceinline__ void load(float (&v)[N], const T *p, int n) {
-    T t[N];
-    if (n >= N) {
-        __builtin_memcpy(t, p, sizeof(t));
-#pragma unroll
-        for (int i = 0; i < N; i++) v[i] = to_f32(t[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i++) v[i] = i < n ? to_f32(p[i]) : 0.f;
-    }
-}
-
-template <typename T, int N>
-__device__ __forceinline__ void store(T *p, const float (&v)[N], int n) {
-    T t[N];
-#pragma unroll
-    for (int i = 0; i < N; i++) t[i] = from_f32<T>(v[i]);
-    if (n >= N) {
-        __builtin_memcpy(p, t, sizeof(t));
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i++)
-            if (i < n) p[i] = t[i];
-    }
-}
-
 // The words of N elements as they were loaded, so that a load may be in flight
-// while the values of the row before are worked on.
+// while the values of the row before are worked on.  A whole piece is one load of
+// its full width at any alignment of the element type (the target's unaligned
+// access mode).
 template <typename T, int N>
 struct Raw {
-    uint32_t w[N * sizeof(T) / 4];
+    static constexpr int kWords = N * sizeof(T) / 4;
+    uint32_t w[kWords];
     __device__ __forceinline__ void clear() {
 #pragma unroll
-        for (uint32_t i = 0; i < N * sizeof(T) / 4; i++) w[i] = 0;
+        for (int i = 0; i < kWords; i++) w[i] = 0;
     }
-    // n of them exist, the others are 0.
+    // n of them exist, the others are 0.  A short piece goes element by element in
+    // a loop, which costs no registers: for rows narrower than a piece.
     __device__ __forceinline__ void load(const T *p, int n) {
         if (n >= N) {
             __builtin_memcpy(w, p, sizeof(w));
             return;
         }
+        if (n <= 0) return;
         clear();
+#pragma unroll 1
+        for (int i = n - 1; i >= 0; i--) {
+            uint32_t x = 0;
+            __builtin_memcpy(&x, p + i, sizeof(T));
+#pragma unroll
+            for (int k = kWords - 1; k > 0; k--)
+                w[k] = sizeof(T) == 4 ? w[k - 1] : w[k] << 16 | w[k - 1] >> 16;
+            w[0] = sizeof(T) == 4 ? x : w[0] << 16 | x;
+        }
+    }
+    // The same with a short piece's loads in flight at once: for the ends of rows.
+    __device__ __forceinline__ void load_end(const T *p, int n) {
+        if (n >= N) {
+            __builtin_memcpy(w, p, sizeof(w));
+            return;
+        }
+        clear();
+        if (n <= 0) return;
+        T t[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) t[i] = p[i < n ? i : 0];
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            if (i >= n) continue;
-            if (sizeof(T) == 4) {
-                __builtin_memcpy(&w[i], p + i, 4);
-            } else {
-                uint16_t h;
-                __builtin_memcpy(&h, p + i, 2);
-                w[i / 2] |= (uint32_t)h << (16 * (i % 2));
-            }
+            uint32_t x = 0;
+            __builtin_memcpy(&x, &t[i], sizeof(T));
+            x = i < n ? x : 0;
+            w[i * sizeof(T) / 4] |= sizeof(T) == 4 ? x : x << (16 * (i % 2));
         }
     }
     __device__ __forceinline__ float operator[](int i) const {
@@ -113,6 +105,62 @@ struct Raw {
             __builtin_memcpy(&t, &h, 2);
         }
         return to_f32(t);
+    }
+};
+
+// N elements from p, of which the first n exist; the others read as 0.
+template <typename T, int N>
+__device__ __forceinline__ void load(float (&v)[N], const T *p, int n) {
+    Raw<T, N> raw;
+    raw.clear();
+    raw.load(p, n);
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = raw[i];
+}
+
+// The first n of N elements, a short piece's in halves of halves.
+template <typename T, int N>
+__device__ __forceinline__ void store(T *p, const float (&v)[N], int n) {
+    T t[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) t[i] = from_f32<T>(v[i]);
+    if (n >= N) {
+        __builtin_memcpy(p, t, sizeof(t));
+        return;
+    }
+#pragma unroll
+    for (int step = N / 2; step >= 1; step /= 2) {
+        if (!(n & step)) continue;
+        __builtin_memcpy(p, t, step * sizeof(T));
+        p += step;
+#pragma unroll
+        for (int i = 0; i < step; i++) t[i] = t[i + step];
+    }
+}
+
+// A thread's piece of N columns of every row.  The last piece of a row that N does
+// not divide is the row's last N columns, and has the others of them in common
+// with the piece before: both work them out alike, and only one counts them in
+// sums, so no lane takes another path than its wave's.  Rows of fewer than N
+// columns are one short piece.
+template <int N>
+struct Place {
+    uint64_t col;   // its first column
+    uint32_t own;   // bit i: column col + i counts as this piece's
+    int n;          // columns of it that exist: N, or fewer in narrow rows; 0: no piece
+
+    __device__ __forceinline__ void set(uint64_t cols, uint64_t nominal) {
+        constexpr uint32_t kAll = N < 32 ? (1u << N) - 1 : ~0u;
+        col = nominal, own = kAll, n = N;
+        if (nominal >= cols) {
+            col = 0, own = 0, n = 0;
+        } else if (cols < N) {
+            n = (int)cols;
+            own = (1u << n) - 1;
+        } else if (nominal + N > cols) {
+            col = cols - N;
+            own = kAll & kAll << (nominal - col);
+        }
     }
 };
 
@@ -164,13 +212,15 @@ __device__ __forceinline__ uint32_t kept4(const Dropper &d, uint32_t row, uint32
            (c3 >= d.threshold ? 8 : 0);
 }
 
-// The same for the N columns from col, a multiple of 4.
+// The same for the N columns from col on.
 template <int N>
 __device__ __forceinline__ uint32_t kept(const Dropper &d, uint32_t row, uint64_t col) {
-    static_assert(N % 4 == 0 && N <= 32, "whole groups");
+    static_assert(N % 4 == 0 && N <= 28, "whole groups");
+    const uint32_t group = (uint32_t)(col / 4), within = (uint32_t)col & 3;
     uint32_t bits = 0;
 #pragma unroll
-    for (int i = 0; i < N; i += 4) bits |= kept4(d, row, (uint32_t)(col / 4) + i / 4) << i;
+    for (int i = 0; i < N; i += 4) bits |= kept4(d, row, group + i / 4) << i;
+    if (within) bits = (bits | kept4(d, row, group + N / 4) << N) >> within;
     return d.scale != 0.f ? bits : 0;
 }
 

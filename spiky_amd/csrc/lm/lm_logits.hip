@@ -200,13 +200,13 @@ __global__ __launch_bounds__(kThreads) void k_logits(spiky_lm_logits_args a) {
         uint32_t allowed[(N + 3) / 4];     // a byte an entry, or the byte that holds the piece's bits
     };
     auto load = [&](Piece &q, uint32_t o, int n) {
-        q.x.load(past(in, o), n);
+        q.x.load_end(past(in, o), n);
         if (a.bias) {
             if (a.bias_dtype == SPIKY_F32) {
-                q.bias.load(past(static_cast<const float *>(a.bias) + bias_at, o), n);
+                q.bias.load_end(past(static_cast<const float *>(a.bias) + bias_at, o), n);
             } else {
                 Raw<bf16, N> half;
-                half.load(past(static_cast<const bf16 *>(a.bias) + bias_at, o), n);
+                half.load_end(past(static_cast<const bf16 *>(a.bias) + bias_at, o), n);
                 __builtin_memcpy(q.bias.w, half.w, sizeof(half.w));
             }
         }

@@ -175,15 +175,33 @@ __device__ __forceinline__ void row_sums(float (&x)[K], float4 (*lds)[(K + 3) / 
 }
 
 // ---- forward ---------------------------------------------------------------
+// A piece of a row.  SHORT: rows may be narrower than a piece.
+template <bool SHORT, typename T, int N>
+__device__ __forceinline__ void fetch_piece(Raw<T, N> &raw, const T *p, int n) {
+    if (SHORT)
+        raw.load(p, n);
+    else if (n)
+        __builtin_memcpy(raw.w, p, sizeof(raw.w));
+}
+
+template <bool SHORT, typename T, int N>
+__device__ __forceinline__ void store_piece(T *p, const float (&v)[N], int n) {
+    if (SHORT)
+        store(p, v, n);
+    else if (n)
+        store(p, v, N);
+}
+
 // N values of a parameter or gate row: its words as loaded (half of them where it
 // is of a shorter type than float), and their values.
-template <typename TA, int N>
+template <typename TA, bool SHORT, int N>
 __device__ __forceinline__ void words_of(Raw<float, N> &raw, const void *p, bool f32, uint64_t at, int n) {
     if (sizeof(TA) == 4 || f32) {
-        raw.load(static_cast<const float *>(p) + at, n);
+        fetch_piece<SHORT>(raw, static_cast<const float *>(p) + at, n);
     } else {
         Raw<TA, N> half;
-        half.load(static_cast<const TA *>(p) + at, n);
+        __builtin_memcpy(half.w, raw.w, sizeof(half.w));
+        fetch_piece<SHORT>(half, static_cast<const TA *>(p) + at, n);
         __builtin_memcpy(raw.w, half.w, sizeof(half.w));
     }
 }
@@ -218,28 +236,31 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_join(Join<TZ, TA> j) 
     if (TPR == 64) row = __builtin_amdgcn_readfirstlane(row);
     if (kSlots > 1 && row >= j.rows) return;
 
-    uint64_t col[P];
-    int n[P];
+    Place<N> at[P];
     Raw<TZ, N> z_raw[P];
     Raw<TA, N> a_raw[P];
     Raw<float, N> g[P], w[Q], b[FULL ? Q : 1];
 #pragma unroll
     for (int p = 0; p < P; p++) {
-        col[p] = (uint64_t)(p * threads + lane) * N;
-        n[p] = piece_size(j.cols, col[p], N);
-        if (j.a) a_raw[p].load(j.a + (int64_t)row * j.a_stride + col[p], n[p]);
-        z_raw[p].load(j.r + (int64_t)row * j.r_stride + col[p], n[p]);
+        at[p].set(j.cols, (uint64_t)(p * threads + lane) * N);
+        a_raw[p].clear(), z_raw[p].clear(), g[p].clear();
+        if (AHEAD || p == 0) {
+            w[AHEAD ? p : 0].clear();
+            if (FULL) b[FULL && AHEAD ? p : 0].clear();
+        }
+        if (j.a) fetch_piece<false>(a_raw[p], j.a + (int64_t)row * j.a_stride + at[p].col, at[p].n);
+        fetch_piece<false>(z_raw[p], j.r + (int64_t)row * j.r_stride + at[p].col, at[p].n);
     }
     const uint64_t gate_at = j.g ? (uint64_t)(row / j.gate_rows) * j.cols : 0;
     auto parameters = [&](int p, const void *weight, const void *bias) {
         const int q = AHEAD ? p : 0;
-        if (weight) words_of<TA>(w[q], weight, j.par_f32, col[p], n[p]);
+        if (weight) words_of<TA, false>(w[q], weight, j.par_f32, at[p].col, at[p].n);
         if constexpr (FULL)
-            if (bias) words_of<TA>(b[q], bias, j.par_f32, col[p], n[p]);
+            if (bias) words_of<TA, false>(b[q], bias, j.par_f32, at[p].col, at[p].n);
     };
 #pragma unroll
     for (int p = 0; p < P; p++) {
-        if (j.g) words_of<TA>(g[p], j.g, j.gate_f32, gate_at + col[p], n[p]);
+        if (j.g) words_of<TA, false>(g[p], j.g, j.gate_f32, gate_at + at[p].col, at[p].n);
         if (AHEAD) parameters(p, j.w1, j.b1);
     }
     auto affine = [&](float (&x)[N], int p, const void *weight, const void *bias) {
@@ -259,7 +280,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_join(Join<TZ, TA> j) 
             }
         }
     };
-    // Mean (layer) and reciprocal deviation of the row in x, whose columns past the end are 0.
+    // Mean (layer) and reciprocal deviation of the row in x.
     auto deviation = [&](const float (&x)[P][N], int kind, float eps, float &mean) {
         float s[1] = {0.f};
         mean = 0.f;
@@ -267,7 +288,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_join(Join<TZ, TA> j) 
 #pragma unroll
             for (int p = 0; p < P; p++)
 #pragma unroll
-                for (int i = 0; i < N; i++) s[0] += x[p][i];
+                for (int i = 0; i < N; i++) s[0] += where(at[p].own, i, x[p][i]);
             row_sums<TPR, 1>(s, red, turn, waves);
             mean = s[0] * j.inv_cols;
             s[0] = 0.f;
@@ -276,7 +297,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_join(Join<TZ, TA> j) 
         for (int p = 0; p < P; p++)
 #pragma unroll
             for (int i = 0; i < N; i++) {
-                const float d = !FULL ? x[p][i] : i < n[p] ? x[p][i] - mean : 0.f;
+                const float d = where(at[p].own, i, x[p][i] - mean);
                 s[0] += d * d;
             }
         row_sums<TPR, 1>(s, red, turn, waves);
@@ -285,7 +306,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_join(Join<TZ, TA> j) 
 
     float z[P][N];
     float4 st = {0.f, 1.f, 0.f, 1.f};
-    const uint64_t at = (uint64_t)row * j.cols;
+    const uint64_t row_at = (uint64_t)row * j.cols;
     if (j.a) {
         float v[P][N];
 #pragma unroll
@@ -304,7 +325,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_join(Join<TZ, TA> j) 
         for (int p = 0; p < P; p++) {
             float f[N];
             affine(v[p], p, j.w1, j.b1);
-            if (j.drops) drop(v[p], dr, row, col[p]);
+            if (j.drops) drop(v[p], dr, row, at[p].col);
 #pragma unroll
             for (int i = 0; i < N; i++) f[i] = 1.f;
             if (j.g) values_of<TA>(f, g[p], j.gate_f32);
@@ -322,33 +343,25 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_join(Join<TZ, TA> j) 
         for (int p = 0; p < P; p++) parameters(p, j.w2, j.b2);
     if (j.a)
 #pragma unroll
-        for (int p = 0; p < P; p++) store(j.out + at + col[p], z[p], n[p]);
+        for (int p = 0; p < P; p++) store_piece<false>(j.out + row_at + at[p].col, z[p], at[p].n);
     if (j.pre != SPIKY_NORM_NONE) {
-        if (FULL) {
-            // columns past the row's end hold what was made of a mean's negative
-#pragma unroll
-            for (int p = 0; p < P; p++)
-#pragma unroll
-                for (int i = 0; i < N; i++)
-                    if (i >= n[p]) z[p][i] = 0.f;
-        }
         st.w = deviation(z, j.pre, j.pre_eps, st.z);
 #pragma unroll
         for (int p = 0; p < P; p++) {
 #pragma unroll
             for (int i = 0; i < N; i++) z[p][i] = (z[p][i] - st.z) * st.w;
             affine(z[p], p, j.w2, j.b2);
-            store(j.normed + at + col[p], z[p], n[p]);
+            store_piece<false>(j.normed + row_at + at[p].col, z[p], at[p].n);
         }
     }
     if (j.stats && lane == 0) j.stats[row] = st;
 }
 
 // Rows of any width: a workgroup walks its row once for each sum.
-template <typename TZ, typename TA, int N>
-__global__ __launch_bounds__(1024) void k_join_wide(Join<TZ, TA> j) {
+template <typename TZ, typename TA, int N, int WG>
+__global__ __launch_bounds__(WG) void k_join_any(Join<TZ, TA> j) {
     __shared__ float red[2][1][16];
-    RowSum<1024, 1> row_sum{red};
+    RowSum<WG, 1> row_sum{red};
     const uint32_t row = j.row0 + blockIdx.x;
     const TZ *r = j.r + (int64_t)row * j.r_stride;
     const TA *a = j.a + (int64_t)row * j.a_stride;
@@ -357,7 +370,7 @@ __global__ __launch_bounds__(1024) void k_join_wide(Join<TZ, TA> j) {
     float4 st = {0.f, 1.f, 0.f, 1.f};
     auto sum_of = [&](auto &&piece) {
         float s[1] = {0.f};
-        for (uint64_t col = (uint64_t)threadIdx.x * N; col < j.cols; col += 1024 * N)
+        for (uint64_t col = (uint64_t)threadIdx.x * N; col < j.cols; col += WG * N)
             s[0] += piece(col, piece_size(j.cols, col, N));
         row_sum(s);
         return s[0];
@@ -396,7 +409,7 @@ __global__ __launch_bounds__(1024) void k_join_wide(Join<TZ, TA> j) {
         for (int i = 0; i < N; i++) z[i] = j.alpha * z[i] + j.beta * (g[i] * v[i]);
     };
     if (j.pre != SPIKY_NORM_NONE) st.w = deviation(j.pre, j.pre_eps, st.z, joined);
-    for (uint64_t col = (uint64_t)threadIdx.x * N; col < j.cols; col += 1024 * N) {
+    for (uint64_t col = (uint64_t)threadIdx.x * N; col < j.cols; col += WG * N) {
         const int n = piece_size(j.cols, col, N);
         float z[N], w[N], b[N];
         joined(z, col, n);
@@ -437,11 +450,10 @@ enum { kSumW1, kSumB1, kSumW2, kSumB2, kSumG };
 // What a thread has of one piece of N columns on the way back: parameters, the
 // loads of the next row, and what the row's sums are awaited with.  FULL: with
 // layer norms or biases.
-template <typename TZ, typename TA, int N, bool FULL>
+template <typename TZ, typename TA, int N, bool FULL, bool SHORT>
 struct Piece {
     static constexpr int K = FULL ? 8 : 3;
-    uint64_t col;
-    int n;
+    Place<N> at;
     float w1[N], w2[N], b1[FULL ? N : 1], g[N];
     Raw<TZ, N> z_raw, dz_raw;
     Raw<TA, N> a_raw, dh_raw;
@@ -451,20 +463,24 @@ struct Piece {
 
     template <typename J>
     __device__ __forceinline__ void place(const J &j, uint64_t column) {
-        col = column;
-        n = piece_size(j.cols, col, N);
+        at.set(j.cols, column);
         z_raw.clear(), dz_raw.clear(), a_raw.clear(), dh_raw.clear(), g_raw.clear();
     }
-    // Columns past the row's end have weights of 0, so they add nothing to any sum.
     template <typename J>
     __device__ __forceinline__ void parameters(const J &j) {
-        if (j.w1) param<TA>(w1, j.w1, j.par_f32, col, n);
-        if (j.w2) param<TA>(w2, j.w2, j.par_f32, col, n);
+        auto values = [&](auto &v, const void *p) {
+            Raw<float, N> raw;
+            raw.clear();
+            words_of<TA, SHORT>(raw, p, j.par_f32, at.col, at.n);
+            values_of<TA>(v, raw, j.par_f32);
+        };
+        if (j.w1) values(w1, j.w1);
+        if (j.w2) values(w2, j.w2);
         if constexpr (FULL)
-            if (j.b1) param<TA>(b1, j.b1, j.par_f32, col, n);
+            if (j.b1) values(b1, j.b1);
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            if (!j.w1) w1[i] = i < n ? 1.f : 0.f;
+            if (!j.w1) w1[i] = 1.f;
             if (!j.w2) w2[i] = 1.f;
             if (FULL && !j.b1) b1[FULL ? i : 0] = 0.f;
             if (!j.g) g[i] = 1.f;
@@ -472,7 +488,7 @@ struct Piece {
     }
     template <typename J>
     __device__ __forceinline__ void load_gate(const J &j, uint32_t gate_row) {
-        words_of<TA>(g_raw, j.g, j.gate_f32, (uint64_t)gate_row * j.cols + col, n);
+        words_of<TA, SHORT>(g_raw, j.g, j.gate_f32, (uint64_t)gate_row * j.cols + at.col, at.n);
     }
     template <typename J>
     __device__ __forceinline__ void take_gate(const J &j) {
@@ -480,11 +496,11 @@ struct Piece {
     }
     template <typename J>
     __device__ __forceinline__ void fetch(const J &j, uint32_t row, bool row_gates) {
-        if (j.dz) dz_raw.load(j.dz + (int64_t)row * j.dz_stride + col, n);
-        if (j.a) a_raw.load(j.a + (int64_t)row * j.a_stride + col, n);
+        if (j.dz) fetch_piece<SHORT>(dz_raw, j.dz + (int64_t)row * j.dz_stride + at.col, at.n);
+        if (j.a) fetch_piece<SHORT>(a_raw, j.a + (int64_t)row * j.a_stride + at.col, at.n);
         if (j.dh) {
-            z_raw.load(j.r + (int64_t)row * j.r_stride + col, n);
-            dh_raw.load(j.dh + (int64_t)row * j.dh_stride + col, n);
+            fetch_piece<SHORT>(z_raw, j.r + (int64_t)row * j.r_stride + at.col, at.n);
+            fetch_piece<SHORT>(dh_raw, j.dh + (int64_t)row * j.dh_stride + at.col, at.n);
         }
         if (row_gates) load_gate(j, row);
     }
@@ -502,7 +518,8 @@ struct Piece {
         const float r2 = j.dh ? st.w : 0.f;
         float dw2[N], db2[FULL ? N : 1];
         const float kept_scale = dr.scale * j.beta;
-        keep = j.drops ? kept<N>(dr, row, col) : ~0u;
+        keep = j.drops ? kept<N>(dr, row, at.col) : ~0u;
+        const uint32_t counts = keep & at.own;
 #pragma unroll
         for (int i = 0; i < N; i++) {
             n1[i] = (a_raw[i] - st.x) * st.y;
@@ -512,14 +529,14 @@ struct Piece {
             const float dh = dh_raw[i], t = dh * w2[i];
             e[i] = dz_raw[i] + r2 * t;
             dw2[i] = dh * n2[i];
-            const float c = where(keep, i, kept_scale * g[i] * w1[i]);
-            const float ce = where(keep, i, c * e[i]), cn = c * n1[i];
-            s[0] += t * n2[i];
+            const float c = where(counts, i, kept_scale * g[i] * w1[i]), own_t = where(at.own, i, t);
+            const float ce = where(counts, i, c * e[i]), cn = c * n1[i];
+            s[0] += own_t * n2[i];
             s[1] += ce * n1[i];
             s[2] += cn * n2[i];
             if constexpr (FULL) {
                 db2[i] = dh;
-                s[3] += t;
+                s[3] += own_t;
                 s[4] += ce;
                 s[5] += c;
                 s[6] += c * n2[i];
@@ -536,7 +553,7 @@ struct Piece {
                                            uint32_t row, F &&add) {
         const float kept_scale = dr.scale * j.beta;
         const float r2 = j.dh ? st.w : 0.f, alpha = j.a ? j.alpha : 1.f;
-        const uint64_t at = (uint64_t)row * j.cols + col;
+        const uint64_t to = (uint64_t)row * j.cols + at.col;
         float out[N], da[N], dg[N], dw1[N], db1[N];
 #pragma unroll
         for (int i = 0; i < N; i++) {
@@ -548,8 +565,8 @@ struct Piece {
             da[i] = db1[i];
             if (j.post != SPIKY_NORM_NONE) da[i] = st.y * (db1[i] * w1[i] - m.z - n1[i] * m.w);
         }
-        if (j.dr) store(j.dr + at, out, n);
-        if (j.da) store(j.da + at, da, n);
+        if (j.dr) store_piece<SHORT>(j.dr + to, out, at.n);
+        if (j.da) store_piece<SHORT>(j.da + to, da, at.n);
         if (j.dgate && j.gate_rows == 1)
             store_gate(j, row, dg);
         else if (j.dgate || j.part[kSumG])
@@ -560,11 +577,11 @@ struct Piece {
     }
     template <typename J>
     __device__ __forceinline__ void store_gate(const J &j, uint32_t gate_row, const float (&dg)[N]) const {
-        const uint64_t to = (uint64_t)gate_row * j.cols + col;
+        const uint64_t to = (uint64_t)gate_row * j.cols + at.col;
         if (sizeof(TA) == 4 || j.gate_f32)
-            store(static_cast<float *>(j.dgate) + to, dg, n);
+            store_piece<SHORT>(static_cast<float *>(j.dgate) + to, dg, at.n);
         else
-            store(static_cast<TA *>(j.dgate) + to, dg, n);
+            store_piece<SHORT>(static_cast<TA *>(j.dgate) + to, dg, at.n);
     }
 };
 
@@ -620,7 +637,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_join_back(Join<TZ, TA
 
     auto slot_of = [](int k) { return k == kSumW1 ? 0 : k == kSumW2 ? 1 : k == kSumG ? 2 : 3; };
     float acc_b2[P][N];
-    Piece<TZ, TA, N, FULL> x[P];
+    Piece<TZ, TA, N, FULL, false> x[P];
     float4 st = {0.f, 1.f, 0.f, 1.f};
 #pragma unroll
     for (int p = 0; p < P; p++) {
@@ -707,19 +724,19 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_join_back(Join<TZ, TA
                     const float4 f = sums[(p * N + i) / 4][threadIdx.x];
                     v[i] = f.x, v[i + 1] = f.y, v[i + 2] = f.z, v[i + 3] = f.w;
                 }
-                store(part + x[p].col, v, x[p].n);
+                store_piece<false>(part + x[p].at.col, v, x[p].at.n);
             }
         } else {
-            // columns 4 q' .. + 3 of the row: quad q of lane l of every slot
-            for (uint32_t c = threadIdx.x * 4; c < (uint32_t)TPR * W && c < j.cols; c += 1024) {
-                const uint32_t piece = c / N, q = piece / TPR * (N / 4) + c % N / 4, l = piece % TPR;
-                float v[4] = {0.f, 0.f, 0.f, 0.f};
+            const uint32_t cols = (uint32_t)j.cols, last = (cols - 1) / N;
+            for (uint32_t c = threadIdx.x; c < cols; c += 256) {
+                const uint32_t piece = c / N;
+                const uint32_t i = piece < last ? c % N : c - (cols - N);
+                const uint32_t q = (piece / TPR * N + i) / 4, l = piece % TPR;
+                float v = 0.f;
 #pragma unroll
-                for (int slot = 0; slot < kSlots; slot++) {
-                    const float4 f = sums[q][slot * TPR + l];
-                    v[0] += f.x, v[1] += f.y, v[2] += f.z, v[3] += f.w;
-                }
-                store(part + c, v, piece_size(j.cols, c, 4));
+                for (int slot = 0; slot < kSlots; slot++)
+                    v += reinterpret_cast<const float *>(&sums[q][slot * TPR + l])[i % 4];
+                part[c] = v;
             }
         }
     };
@@ -743,7 +760,8 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_join_back(Join<TZ, TA
     }
 }
 
-// Wider rows take two passes over the inputs: the means of each row, then columns.
+// Wider rows, and those narrower than a piece, take two passes over the inputs: the
+// means of each row, then columns.
 template <typename TZ, typename TA, int N, int WG, bool FULL>
 __global__ __launch_bounds__(WG) void k_join_back_rows(Join<TZ, TA> j) {
     constexpr int K = FULL ? 8 : 3;
@@ -755,7 +773,7 @@ __global__ __launch_bounds__(WG) void k_join_back_rows(Join<TZ, TA> j) {
 #pragma unroll
     for (int k = 0; k < K; k++) s[k] = 0.f;
     for (uint64_t col = (uint64_t)threadIdx.x * N; col < j.cols; col += WG * N) {
-        Piece<TZ, TA, N, FULL> x;
+        Piece<TZ, TA, N, FULL, true> x;
         x.place(j, col);
         x.fetch(j, row, false);
         x.parameters(j);
@@ -771,9 +789,9 @@ __global__ __launch_bounds__(WG) void k_join_back_rows(Join<TZ, TA> j) {
 template <typename TZ, typename TA, int N, bool FULL>
 __global__ __launch_bounds__(64) void k_join_back_cols(Join<TZ, TA> j) {
     constexpr int K = FULL ? 8 : 3;
-    Piece<TZ, TA, N, FULL> x;
+    Piece<TZ, TA, N, FULL, true> x;
     x.place(j, ((uint64_t)blockIdx.x * 64 + threadIdx.x) * N);
-    if (x.n == 0) return;
+    if (x.at.n == 0) return;
     uint32_t row, end;
     chunk_rows(j, blockIdx.y, row, end);
     if (row >= end) return;
@@ -817,7 +835,7 @@ __global__ __launch_bounds__(64) void k_join_back_cols(Join<TZ, TA> j) {
     }
 #pragma unroll
     for (int k = 0; k < 5; k++)
-        if (j.part[k]) store(j.part[k] + (uint64_t)blockIdx.y * j.cols + x.col, acc[k], x.n);
+        if (j.part[k]) store(j.part[k] + (uint64_t)blockIdx.y * j.cols + x.at.col, acc[k], x.at.n);
 }
 
 // Column sums of the chunks' rows, in one order: out[g][c] = the sum of the
@@ -915,6 +933,8 @@ hipError_t run_rows(Join<TZ, TA> &j, hipStream_t st) {
 template <typename TZ, typename TA, bool FULL>
 hipError_t run_forward(Join<TZ, TA> &j, hipStream_t st) {
     constexpr int N = sizeof(TA) == 4 ? 4 : 8;
+    if (j.cols < 8)  // narrower than a piece
+        return over_rows(j, 1, 64, [&](dim3 grid, dim3 block) { k_join_any<TZ, TA, N, 64><<<grid, block, 0, st>>>(j); });
     if (j.cols <= 128) return run_rows<TZ, TA, 8, 16, FULL>(j, st);
     if (j.cols <= 256) return run_rows<TZ, TA, 8, 32, FULL>(j, st);
     if (j.cols <= 512) return run_rows<TZ, TA, 8, 64, FULL>(j, st);
@@ -923,7 +943,7 @@ hipError_t run_forward(Join<TZ, TA> &j, hipStream_t st) {
     if (j.cols <= 4096) return run_rows<TZ, TA, 8, 512, FULL>(j, st);
     if (j.cols <= 8192) return run_rows<TZ, TA, 8, 1024, FULL>(j, st);
     if (j.cols <= 16384) return run_rows<TZ, TA, 16, 1024, FULL>(j, st);
-    return over_rows(j, 1, 1024, [&](dim3 grid, dim3 block) { k_join_wide<TZ, TA, N><<<grid, block, 0, st>>>(j); });
+    return over_rows(j, 1, 1024, [&](dim3 grid, dim3 block) { k_join_any<TZ, TA, N, 1024><<<grid, block, 0, st>>>(j); });
 }
 
 bool is_full(const spiky_lm_residual_args &a) {
@@ -941,7 +961,7 @@ hipError_t forward(const spiky_lm_residual_args &a, const DropArgs &drop, void *
 
 // How the rows are cut into chunks, and the workspace's regions.
 struct Plan {
-    uint32_t tpr;  // lanes of a row in k_join_back, 1024 for all rows of more than 64; 0: the passes for wider rows
+    uint32_t tpr;  // lanes of a row in k_join_back, 1024 for all rows of more than 64; 0: the passes for any row
     uint32_t chunk, chunks, span, chunks_per_span;
     bool part[5];
     uint64_t row_sums, parts[5], bytes;
@@ -955,6 +975,7 @@ Plan plan(const spiky_lm_residual_args &a, const spiky_lm_residual_grads &g) {
     Plan p = {};
     const uint64_t threads = (a.cols + kBackCols - 1) / kBackCols;
     p.tpr = threads <= 16 ? 16 : threads <= 32 ? 32 : threads <= 64 ? 64 : threads <= 1024 ? 1024 : 0;
+    if (a.cols < kBackCols) p.tpr = 0;
     const uint64_t span = a.gate && g.d_gate ? a.gate_rows : a.rows;
     const uint64_t slots = p.tpr && p.tpr <= 64 ? 256 / p.tpr : 1;
     const uint64_t waves = p.tpr && p.tpr <= 64 ? 4 : (threads + 63) / 64;
