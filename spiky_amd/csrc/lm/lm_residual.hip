@@ -18,6 +18,21 @@ namespace spiky {
 namespace lm {
 namespace {
 
+// What a call has, as bits of Join::has: tests of them in a row's loop cost no
+// registers, those of the pointers two each.
+enum : uint32_t {
+    kBranch = 1, kDz = 2, kDh = 4, kDrops = 8, kPost = 16, kPostLayer = 32, kPreLayer = 64, kDr = 128, kDa = 256,
+    kGate = 512, kRowGate = 1 << 10, kDgate = 1 << 11, kRowDgate = 1 << 12, kW1 = 1 << 13, kB1 = 1 << 14, kW2 = 1 << 15,
+    kPart = 1 << 16  // and the four bits above: column sums number 0 to 4
+};
+
+// The bits where they are used: the compiler would take each test out of the row's
+// loop and keep its result in two registers over it.
+__device__ __forceinline__ uint32_t here(uint32_t has) {
+    asm("" : "+s"(has));
+    return has;
+}
+
 // The kernels' view of a call.
 template <typename TZ, typename TA>
 struct Join {
@@ -37,6 +52,7 @@ struct Join {
     TZ *out;
     TA *normed;
     // backward
+    uint32_t has;
     const TZ *dz;
     const TA *dh;
     int64_t dz_stride, dh_stride;
@@ -474,16 +490,16 @@ struct Piece {
             words_of<TA, SHORT>(raw, p, j.par_f32, at.col, at.n);
             values_of<TA>(v, raw, j.par_f32);
         };
-        if (j.w1) values(w1, j.w1);
-        if (j.w2) values(w2, j.w2);
+        if (j.has & kW1) values(w1, j.w1);
+        if (j.has & kW2) values(w2, j.w2);
         if constexpr (FULL)
-            if (j.b1) values(b1, j.b1);
+            if (j.has & kB1) values(b1, j.b1);
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            if (!j.w1) w1[i] = 1.f;
-            if (!j.w2) w2[i] = 1.f;
-            if (FULL && !j.b1) b1[FULL ? i : 0] = 0.f;
-            if (!j.g) g[i] = 1.f;
+            if (!(j.has & kW1)) w1[i] = 1.f;
+            if (!(j.has & kW2)) w2[i] = 1.f;
+            if (FULL && !(j.has & kB1)) b1[FULL ? i : 0] = 0.f;
+            if (!(j.has & kGate)) g[i] = 1.f;
         }
     }
     template <typename J>
@@ -496,9 +512,10 @@ struct Piece {
     }
     template <typename J>
     __device__ __forceinline__ void fetch(const J &j, uint32_t row, bool row_gates) {
-        if (j.dz) fetch_piece<SHORT>(dz_raw, j.dz + (int64_t)row * j.dz_stride + at.col, at.n);
-        if (j.a) fetch_piece<SHORT>(a_raw, j.a + (int64_t)row * j.a_stride + at.col, at.n);
-        if (j.dh) {
+        const uint32_t has = here(j.has);
+        if (has & kDz) fetch_piece<SHORT>(dz_raw, j.dz + (int64_t)row * j.dz_stride + at.col, at.n);
+        if (has & kBranch) fetch_piece<SHORT>(a_raw, j.a + (int64_t)row * j.a_stride + at.col, at.n);
+        if (has & kDh) {
             fetch_piece<SHORT>(z_raw, j.r + (int64_t)row * j.r_stride + at.col, at.n);
             fetch_piece<SHORT>(dh_raw, j.dh + (int64_t)row * j.dh_stride + at.col, at.n);
         }
@@ -515,17 +532,18 @@ struct Piece {
     template <typename J, typename F>
     __device__ __forceinline__ void consume(const J &j, const Dropper &dr, const float4 &st, uint32_t row,
                                             float (&s)[K], F &&add) {
-        const float r2 = j.dh ? st.w : 0.f;
+        const uint32_t has = here(j.has);
+        const float r2 = has & kDh ? st.w : 0.f;
         float dw2[N], db2[FULL ? N : 1];
         const float kept_scale = dr.scale * j.beta;
-        keep = j.drops ? kept<N>(dr, row, at.col) : ~0u;
+        keep = has & kDrops ? kept<N>(dr, row, at.col) : ~0u;
         const uint32_t counts = keep & at.own;
 #pragma unroll
         for (int i = 0; i < N; i++) {
             n1[i] = (a_raw[i] - st.x) * st.y;
             float z = z_raw[i];
-            if (j.a) z = j.alpha * z + j.beta * (g[i] * dropped(dr, i));
-            n2[i] = j.dh ? (z - st.z) * r2 : 0.f;
+            if (has & kBranch) z = j.alpha * z + j.beta * (g[i] * dropped(dr, i));
+            n2[i] = has & kDh ? (z - st.z) * r2 : 0.f;
             const float dh = dh_raw[i], t = dh * w2[i];
             e[i] = dz_raw[i] + r2 * t;
             dw2[i] = dh * n2[i];
@@ -543,16 +561,17 @@ struct Piece {
                 s[7] += cn;
             }
         }
-        if (j.part[kSumW2]) add(kSumW2, dw2);
+        if (has & kPart << kSumW2) add(kSumW2, dw2);
         if constexpr (FULL)
-            if (j.part[kSumB2]) add(kSumB2, db2);
+            if (has & kPart << kSumB2) add(kSumB2, db2);
     }
     // The row's gradients, from its means (mean t, mean t n2, mean dn, mean dn n1).
     template <typename J, typename F>
     __device__ __forceinline__ void finish(const J &j, const Dropper &dr, const float4 &st, const float4 &m,
                                            uint32_t row, F &&add) {
+        const uint32_t has = here(j.has);
         const float kept_scale = dr.scale * j.beta;
-        const float r2 = j.dh ? st.w : 0.f, alpha = j.a ? j.alpha : 1.f;
+        const float r2 = has & kDh ? st.w : 0.f, alpha = has & kBranch ? j.alpha : 1.f;
         const uint64_t to = (uint64_t)row * j.cols + at.col;
         float out[N], da[N], dg[N], dw1[N], db1[N];
 #pragma unroll
@@ -563,17 +582,17 @@ struct Piece {
             db1[i] = where(keep, i, kept_scale * (g[i] * q));
             dw1[i] = db1[i] * n1[i];
             da[i] = db1[i];
-            if (j.post != SPIKY_NORM_NONE) da[i] = st.y * (db1[i] * w1[i] - m.z - n1[i] * m.w);
+            if (has & kPost) da[i] = st.y * (db1[i] * w1[i] - m.z - n1[i] * m.w);
         }
-        if (j.dr) store_piece<SHORT>(j.dr + to, out, at.n);
-        if (j.da) store_piece<SHORT>(j.da + to, da, at.n);
-        if (j.dgate && j.gate_rows == 1)
+        if (has & kDr) store_piece<SHORT>(j.dr + to, out, at.n);
+        if (has & kDa) store_piece<SHORT>(j.da + to, da, at.n);
+        if (has & kRowDgate)
             store_gate(j, row, dg);
-        else if (j.dgate || j.part[kSumG])
+        else if (has & (kDgate | kPart << kSumG))
             add(kSumG, dg);
-        if (j.part[kSumW1]) add(kSumW1, dw1);
+        if (has & kPart << kSumW1) add(kSumW1, dw1);
         if constexpr (FULL)
-            if (j.part[kSumB1]) add(kSumB1, db1);
+            if (has & kPart << kSumB1) add(kSumB1, db1);
     }
     template <typename J>
     __device__ __forceinline__ void store_gate(const J &j, uint32_t gate_row, const float (&dg)[N]) const {
@@ -592,14 +611,15 @@ struct Piece {
 // and alike without n1.
 template <bool FULL, typename J, int K>
 __device__ __forceinline__ float4 row_means(const J &j, const float4 &st, const float (&s)[K]) {
-    const float r2 = j.dh ? st.w : 0.f;
+    const uint32_t has = here(j.has);
+    const float r2 = has & kDh ? st.w : 0.f;
     float4 m = {0.f, s[0] * j.inv_cols, 0.f, 0.f};
-    if (FULL && j.pre == SPIKY_NORM_LAYER) m.x = s[FULL ? 3 : 0] * j.inv_cols;
-    if (j.post != SPIKY_NORM_NONE) {
+    if (FULL && has & kPreLayer) m.x = s[FULL ? 3 : 0] * j.inv_cols;
+    if (has & kPost) {
         m.w = s[1] - r2 * (m.y * s[2]);
         if constexpr (FULL) {
             m.w -= r2 * (m.x * s[7]);
-            if (j.post == SPIKY_NORM_LAYER) m.z = (s[4] - r2 * (m.x * s[5] + m.y * s[6])) * j.inv_cols;
+            if (has & kPostLayer) m.z = (s[4] - r2 * (m.x * s[5] + m.y * s[6])) * j.inv_cols;
         }
         m.w *= j.inv_cols;
     }
@@ -632,8 +652,8 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_join_back(Join<TZ, TA
     }
     if (TPR == 64) row = __builtin_amdgcn_readfirstlane(row), end = __builtin_amdgcn_readfirstlane(end);
     const Dropper dr = dropper(j.drop);  // of scale 1 where nothing is dropped
-    const bool row_gates = j.g && j.gate_rows == 1;
-    uint32_t gate_row = j.g ? row / j.gate_rows : 0, in_gate = j.g ? row - gate_row * j.gate_rows : 0;
+    const bool row_gates = j.has & kRowGate;
+    uint32_t gate_row = j.has & kGate ? row / j.gate_rows : 0, in_gate = j.has & kGate ? row - gate_row * j.gate_rows : 0;
 
     auto slot_of = [](int k) { return k == kSumW1 ? 0 : k == kSumW2 ? 1 : k == kSumG ? 2 : 3; };
     float acc_b2[P][N];
@@ -652,7 +672,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_join_back(Join<TZ, TA
 #pragma unroll
     for (int p = 0; p < P; p++) {
         x[p].parameters(j);
-        if (j.g && !row_gates && row < end) x[p].load_gate(j, gate_row), x[p].take_gate(j);
+        if (j.has & kGate && !row_gates && row < end) x[p].load_gate(j, gate_row), x[p].take_gate(j);
 #pragma unroll
         for (int i = 0; i < N; i++) acc_b2[p][i] = 0.f;
     }
@@ -692,11 +712,11 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_join_back(Join<TZ, TA
         const float4 m = row_means<FULL>(j, now, s);
 #pragma unroll
         for (int p = 0; p < P; p++) x[p].finish(j, dr, now, m, row, adds_to(p));
-        if (j.g && !row_gates && ++in_gate == j.gate_rows) {
+        if (j.has & kGate && !row_gates && ++in_gate == j.gate_rows) {
             // the rows of a gate end here, and with them its sum, where no other chunk has some of them
 #pragma unroll
             for (int p = 0; p < P; p++) {
-                if (j.dgate) {
+                if (j.has & kDgate) {
                     float dg[N];
 #pragma unroll
                     for (int i = 0; i < N; i += 4) {
@@ -741,12 +761,12 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_join_back(Join<TZ, TA
         }
     };
     if (kSlots > 1) __syncthreads();
-    if (j.part[kSumW1]) write_sums(kSumW1, acc[0]);
-    if (j.part[kSumW2]) write_sums(kSumW2, acc[1]);
-    if (j.part[kSumG]) write_sums(kSumG, acc[2]);
+    if (j.has & kPart << kSumW1) write_sums(kSumW1, acc[0]);
+    if (j.has & kPart << kSumW2) write_sums(kSumW2, acc[1]);
+    if (j.has & kPart << kSumG) write_sums(kSumG, acc[2]);
     if constexpr (FULL) {
-        if (j.part[kSumB1]) write_sums(kSumB1, acc[3]);
-        if (j.part[kSumB2]) {
+        if (j.has & kPart << kSumB1) write_sums(kSumB1, acc[3]);
+        if (j.has & kPart << kSumB2) {
             if (kSlots > 1) __syncthreads();
 #pragma unroll
             for (int p = 0; p < P; p++)
@@ -777,7 +797,7 @@ __global__ __launch_bounds__(WG) void k_join_back_rows(Join<TZ, TA> j) {
         x.place(j, col);
         x.fetch(j, row, false);
         x.parameters(j);
-        if (j.g) x.load_gate(j, row / j.gate_rows), x.take_gate(j);
+        if (j.has & kGate) x.load_gate(j, row / j.gate_rows), x.take_gate(j);
         x.consume(j, dr, st, row, s, [](int, auto &) {});
     }
     uint32_t turn = 0;
@@ -796,8 +816,8 @@ __global__ __launch_bounds__(64) void k_join_back_cols(Join<TZ, TA> j) {
     chunk_rows(j, blockIdx.y, row, end);
     if (row >= end) return;
     const Dropper dr = dropper(j.drop);  // of scale 1 where nothing is dropped
-    const bool row_gates = j.g && j.gate_rows == 1;
-    uint32_t gate_row = j.g ? row / j.gate_rows : 0, in_gate = j.g ? row - gate_row * j.gate_rows : 0;
+    const bool row_gates = j.has & kRowGate;
+    uint32_t gate_row = j.has & kGate ? row / j.gate_rows : 0, in_gate = j.has & kGate ? row - gate_row * j.gate_rows : 0;
     float acc[5][N], s[K];
 #pragma unroll
     for (int k = 0; k < 5; k++)
@@ -806,7 +826,7 @@ __global__ __launch_bounds__(64) void k_join_back_cols(Join<TZ, TA> j) {
     x.fetch(j, row, row_gates);
     float4 st = j.stats[row], m = j.row_sums[row];
     x.parameters(j);
-    if (j.g && !row_gates) x.load_gate(j, gate_row), x.take_gate(j);
+    if (j.has & kGate && !row_gates) x.load_gate(j, gate_row), x.take_gate(j);
     auto add = [&](int k, const float (&v)[N]) {
 #pragma unroll
         for (int i = 0; i < N; i++) acc[k][i] += v[i];
@@ -822,8 +842,8 @@ __global__ __launch_bounds__(64) void k_join_back_cols(Join<TZ, TA> j) {
             x.fetch(j, row + 1, row_gates);
         }
         x.finish(j, dr, now, means, row, add);
-        if (j.g && !row_gates && ++in_gate == j.gate_rows) {
-            if (j.dgate) {
+        if (j.has & kGate && !row_gates && ++in_gate == j.gate_rows) {
+            if (j.has & kDgate) {
                 x.store_gate(j, gate_row, acc[kSumG]);
 #pragma unroll
                 for (int i = 0; i < N; i++) acc[kSumG][i] = 0.f;
@@ -1063,6 +1083,12 @@ hipError_t backward(const spiky_lm_residual_args &a, const DropArgs &drop, const
     j.dgate = p.part[4] ? nullptr : g.d_gate;
     j.row_sums = reinterpret_cast<float4 *>(ws + p.row_sums);
     for (int k = 0; k < 5; k++) j.part[k] = p.part[k] ? reinterpret_cast<float *>(ws + p.parts[k]) : nullptr;
+    auto bit = [](bool set, uint32_t b) { return set ? b : 0u; };
+    j.has = bit(j.a, kBranch) | bit(j.dz, kDz) | bit(j.dh, kDh) | bit(j.drops, kDrops) | bit(j.post, kPost) |
+            bit(j.post == SPIKY_NORM_LAYER, kPostLayer) | bit(j.pre == SPIKY_NORM_LAYER, kPreLayer) | bit(j.dr, kDr) |
+            bit(j.da, kDa) | bit(j.g, kGate) | bit(j.g && j.gate_rows == 1, kRowGate) | bit(j.dgate, kDgate) |
+            bit(j.dgate && j.gate_rows == 1, kRowDgate) | bit(j.w1, kW1) | bit(j.b1, kB1) | bit(j.w2, kW2);
+    for (int k = 0; k < 5; k++) j.has |= bit(j.part[k], kPart << k);
     j.chunk = p.chunk;
     j.span = p.span;
     j.chunks_per_span = p.chunks_per_span;
