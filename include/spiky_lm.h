@@ -5,7 +5,8 @@
  * the reference, which leaves these steps to torch modules.
  *
  * Every pointer is a device pointer unless its comment says host; `stream` is a
- * `hipStream_t`.  Calls launch on the stream, allocate nothing, keep nothing
+ * `hipStream_t`.  Outputs do not overlap inputs unless their comment allows it.
+ * Calls launch on the stream, allocate nothing, keep nothing
  * and never synchronise, so they can be captured into a HIP graph.  The return
  * codes are those of spiky_lut.h; the message of the last failed call on the
  * calling thread is spiky_lm_last_error().
@@ -40,13 +41,13 @@ const char *spiky_lm_last_error(void);
  * floor(p * 2^32 + 1/2).  The same call on the output's gradient is the
  * backward pass.  rng, if given, points to {seed, offset} in device memory and
  * stands for the two arguments.  x_stride: elements from one row of x to the
- * next; y has contiguous rows.  rows < 2^32, cols < 2^34. */
+ * next; y has contiguous rows.  rows < 2^32, cols <= 2^34 - 16. */
 int spiky_lm_dropout(const void *x, int64_t x_stride, void *y, uint64_t rows, uint64_t cols,
                      int dtype, double p, uint64_t seed, uint64_t offset, const int64_t *rng,
                      void *stream);
 
 /* ---- residual join ---------------------------------------------------------
- * For each row: v = post(branch) * post_weight + post_bias, d = dropout(v) as
+ * For each of rows < 2^32 rows of cols <= 2^26 columns: v = post(branch) * post_weight + post_bias, d = dropout(v) as
  * above, z = residual_scale * residual + branch_scale * gate * d, and
  * normed = pre(z) * pre_weight + pre_bias, of the sum z before it is rounded to
  * the residual's type.  Each part is left out where its pointer is null or its

@@ -27,6 +27,8 @@ int guarded(F &&f) {
     } catch (const std::exception &e) {
         g_last_error = e.what();
         return SPIKY_RUNTIME_ERROR;
+    } catch (...) {
+        return SPIKY_RUNTIME_ERROR;
     }
 }
 
@@ -57,7 +59,7 @@ spiky::lm::DropArgs check(const spiky_lm_residual_args *a) {
     require(is_type(a->res_dtype) && is_type(a->act_dtype), "unknown element type");
     require(a->res_dtype == a->act_dtype || a->res_dtype == SPIKY_F32,
             "the residual must be fp32 or have the branch's type");
-    require(a->rows < 0x100000000ull && a->cols < 0x400000000ull, "too many rows or columns");
+    require(a->rows < 0x100000000ull && a->cols <= 0x4000000ull, "too many rows or columns");
     require(a->post_norm >= SPIKY_NORM_NONE && a->post_norm <= SPIKY_NORM_LAYER &&
                 a->pre_norm >= SPIKY_NORM_NONE && a->pre_norm <= SPIKY_NORM_LAYER,
             "unknown norm");
@@ -85,7 +87,7 @@ int spiky_lm_dropout(const void *x, int64_t x_stride, void *y, uint64_t rows, ui
                      double p, uint64_t seed, uint64_t offset, const int64_t *rng, void *stream) {
     return guarded([&] {
         require(is_type(dtype), "unknown element type");
-        require(rows < 0x100000000ull && cols < 0x400000000ull, "too many rows or columns");
+        require(rows < 0x100000000ull && cols <= 0x3fffffff0ull, "too many rows or columns");
         const spiky::lm::DropArgs d = drop_args(p, seed, offset, rng);
         if (rows == 0 || cols == 0) return;
         require(x && y, "null pointer");

@@ -18,6 +18,7 @@
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/utils/object_ptr.h>
 
+#include <algorithm>
 #include <optional>
 #include <utility>
 
@@ -358,7 +359,7 @@ std::pair<Tensor, int64_t> gate_rows(const Tensor &gate, at::IntArrayRef shape) 
     if (!as_is) return {gate.expand(shape).contiguous(), 1};
     int64_t share = 1;
     for (int64_t i = k; i < dim - 1; i++) share *= shape[i];
-    return {gate.contiguous(), share};
+    return {gate.contiguous(), std::max<int64_t>(share, 1)};
 }
 
 PyObject *pair(PyObject *first, PyObject *second) {

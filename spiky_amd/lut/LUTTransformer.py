@@ -9,10 +9,15 @@ Q_j | K_i | PE_(j-i-1)); the feed-forward and unembedding layers are
 `embedding_dim` (h, w) makes each attention layer a `Conv2DLUTLayer` over the
 [h, w] grid with one receptive field covering it (sparse lookup connectivity,
 LUTTransformer.py:43-67); everything else sees E = h * w features.
+
+With `residual_join` the two joins of a block are `ResidualNorm`s (this build's own addition):
+the branch is normed, dropped out and gated, added to the residual stream, and the next layer
+reads the stream's norm.  `generate` continues byte or token sequences with `process_logits`.
 """
 import torch
 import torch.nn as nn
 
+from ..lm import ResidualNorm, process_logits
 from .LUTLayer import Conv2DLUTLayer, GradientPolicy, LUTLayer, LUTSharedContext, SynapseMeta
 
 
@@ -21,7 +26,12 @@ class LUTTransformer(nn.Module):
     (LUTTransformer.py:69-200): attention layer l is seeded seed + l*num_heads,
     its feed-forward layer seed + l*num_heads + num_heads, the unembedder seed;
     the frozen embedding is 2*U[0,1) - 1 from a generator seeded with seed
-    (else uniform(-1, 1) from the global RNG)."""
+    (else uniform(-1, 1) from the global RNG).
+
+    residual_join: None for the reference's z + dropout(branch), or a dict of ResidualNorm's
+    options (post_norm, pre_norm, bias, gate, residual_scale, branch_scale, eps) for both joins
+    of every block; their dropout is `dropout`, from counters seeded by `seed` and the join's
+    number.  It excludes use_batch_norm."""
 
     def __init__(self, vocab_size, embedding_dim, context_size, positional_dim, num_layers, num_heads,
                  n_detectors, n_anchors_per_detector, n_anchors_per_detector_attention=None,
@@ -29,7 +39,7 @@ class LUTTransformer(nn.Module):
                  do_normalise_weights=False, weights_gradient_policy: GradientPolicy = None,
                  device=None, synapse_meta=SynapseMeta(), lut_shared_context=None, seed=None,
                  summation_dtype=torch.float32, _int_rescaler=0.001, _forward_group_size=32,
-                 _backward_group_size=32, dropout=0.0, use_batch_norm=False):
+                 _backward_group_size=32, dropout=0.0, use_batch_norm=False, residual_join=None):
         super().__init__()
         if isinstance(embedding_dim, int):
             n_embeddings = embedding_dim
@@ -56,6 +66,9 @@ class LUTTransformer(nn.Module):
         self.use_batch_norm = use_batch_norm
         self.unified_pe = unified_pe
         self.no_ffn = no_ffn
+        if residual_join is not None and use_batch_norm:
+            raise ValueError("residual_join and use_batch_norm exclude each other")
+        self.residual_join = None if residual_join is None else dict(residual_join)
         self.device = torch.device("cpu") if device is None else torch.device(device)
         if lut_shared_context is None:
             lut_shared_context = LUTSharedContext()
@@ -98,6 +111,11 @@ class LUTTransformer(nn.Module):
                     sliced_product_mode=sliced_product_mode, positional_dim=positional_dim,
                     unified_pe=unified_pe, receptive_field_shape=embedding_dim,
                     receptive_field_stride_shape=embedding_dim, random_seed=attention_seed, **common)
+            if residual_join is not None:
+                # the first layer reads the embedding, so the last join's norm is the unembedder's
+                for i, name in enumerate(["attention_join"] if no_ffn else ["attention_join", "ffn_join"]):
+                    block[name] = ResidualNorm(E, dropout_p=dropout, seed=((seed or 0) << 16) + 2 * li + i,
+                                               device=self.device, **residual_join)
             block["attention_dropout"] = nn.Dropout(dropout)
             block["attention_bn"] = nn.BatchNorm1d(E, device=self.device) if use_batch_norm else None
             if not no_ffn:
@@ -139,6 +157,8 @@ class LUTTransformer(nn.Module):
         grid = not isinstance(self.embedding_dim, int)
         E = self.embedding_dim[0] * self.embedding_dim[1] if grid else self.embedding_dim
         z = self.token_embedder(tokens)
+        if self.residual_join is not None:
+            return self._forward_joined(z, B, S, E)
         if self._debug_last_forward is not None:
             self._debug_last_forward = [tokens.to(torch.float32), z.detach().clone()]
         for block in self.layers:
@@ -162,6 +182,56 @@ class LUTTransformer(nn.Module):
                     f = self._bn(block["ffn_bn"], f)
                 z = z + f
         return self.unembedder(z.reshape(B * S, 1, E)).reshape(B, S, self.vocab_size)
+
+    def _forward_joined(self, z, B, S, E):
+        def joined(join, stream, branch):
+            stream, normed = join(stream, branch.reshape(B, S, E))
+            return stream, stream if normed is None else normed
+
+        x = z
+        for block in self.layers:
+            a = block["attention_lut"](x if isinstance(self.embedding_dim, int) else x.reshape((B, S) + self.embedding_dim))
+            z, x = joined(block["attention_join"], z, a)
+            if not self.no_ffn:
+                z, x = joined(block["ffn_join"], z, block["ffn"](x.reshape(B * S, 1, E)))
+        return self.unembedder(x.reshape(B * S, 1, E)).reshape(B, S, self.vocab_size)
+
+    @torch.no_grad()
+    def generate(self, tokens, n_new, lengths=None, generator=None, **processing):
+        """Sequences [B, L + n_new] that continue tokens [B, L], of which a row's first `lengths`
+        are its prompt (all, without); a row's new tokens follow its prompt, zeros the last of
+        them.  Each new token is drawn from the softmax of the last position's logits after
+        process_logits with `processing` (penalties, biases, temperature, mask); with temperature
+        0 or less it is the largest.  A step reads the last context_size tokens, each row from its
+        own start.  generator: of torch, for the draws."""
+        B, L = tokens.shape
+        S, device = self.context_size, tokens.device
+        out = torch.cat([tokens, tokens.new_zeros(B, n_new)], 1)
+        prompt = torch.full((B,), L, dtype=torch.int64, device=device) if lengths is None else \
+            lengths.to(device=device, dtype=torch.int64)
+        if L == 0 or int(prompt.min()) < 1 or int(prompt.max()) > L:
+            raise ValueError("a prompt has 1 to L tokens")
+        out = out.masked_fill(torch.arange(L + n_new, device=device) >= prompt[:, None], 0)
+        greedy = not isinstance(processing.get("temperature", 1.0), torch.Tensor) and \
+            processing.get("temperature", 1.0) <= 0.0
+        rows, ahead = torch.arange(B, device=device), torch.arange(S, device=device)
+        was_training = self.training
+        self.eval()
+        try:
+            for i in range(n_new):
+                length = prompt + i
+                start = (length - S).clamp_min(0)
+                at = (start[:, None] + ahead).clamp_max(L + n_new - 1)
+                logits = self(out.gather(1, at))[rows, length - start - 1]
+                logits = process_logits(logits, tokens=out, lengths=length, prompt_lengths=prompt, **processing)
+                if greedy:
+                    new = logits.argmax(-1)
+                else:
+                    new = torch.multinomial(logits.softmax(-1), 1, generator=generator)[:, 0]
+                out[rows, length] = new.to(out.dtype)
+        finally:
+            self.train(was_training)
+        return out
 
     def to(self, *args, **kwargs):
         device = kwargs.get("device", args[0] if args and isinstance(args[0], (str, torch.device)) else None)
