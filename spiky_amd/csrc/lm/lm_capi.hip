@@ -63,15 +63,16 @@ spiky::lm::DropArgs check(const spiky_lm_residual_args *a) {
     require(a->post_norm >= SPIKY_NORM_NONE && a->post_norm <= SPIKY_NORM_LAYER &&
                 a->pre_norm >= SPIKY_NORM_NONE && a->pre_norm <= SPIKY_NORM_LAYER,
             "unknown norm");
+    if (a->gate)
+        require(a->gate_rows > 0 && a->rows % a->gate_rows == 0, "gate_rows must divide the rows");
+    if (a->rows == 0 || a->cols == 0) return drop_args(a->dropout_p, 0, 0, nullptr);  // null pointers say nothing then
     require(a->post_norm != SPIKY_NORM_NONE || (!a->post_weight && !a->post_bias),
             "parameters of a norm that is not applied");
     require(a->pre_norm != SPIKY_NORM_NONE || (!a->pre_weight && !a->pre_bias),
             "parameters of a norm that is not applied");
     require(a->branch || a->pre_norm != SPIKY_NORM_NONE, "neither a branch nor a norm");
     require(a->branch || (!a->gate && a->post_norm == SPIKY_NORM_NONE), "a gate or norm of no branch");
-    if (a->gate)
-        require(a->gate_rows > 0 && a->rows % a->gate_rows == 0, "gate_rows must divide the rows");
-    require(a->rows == 0 || a->cols == 0 || a->residual, "null pointer");
+    require(a->residual, "null pointer");
     return drop_args(a->branch ? a->dropout_p : 0.0, a->seed, a->offset, a->rng);
 }
 
@@ -119,13 +120,13 @@ int spiky_lm_residual_norm_backward(const spiky_lm_residual_args *args, const sp
     return guarded([&] {
         const spiky::lm::DropArgs d = check(args);
         require(grads != nullptr, "null pointer");
+        if (args->rows == 0 || args->cols == 0) return;
         require(!grads->d_normed || args->pre_norm != SPIKY_NORM_NONE, "a gradient of no output");
         require(args->branch || (!grads->d_branch && !grads->d_gate), "a gradient of no input");
         require((args->post_weight || !grads->d_post_weight) && (args->post_bias || !grads->d_post_bias) &&
                     (args->pre_weight || !grads->d_pre_weight) && (args->pre_bias || !grads->d_pre_bias) &&
                     (args->gate || !grads->d_gate),
                 "a gradient of no input");
-        if (args->rows == 0 || args->cols == 0) return;
         require(args->stats != nullptr, "the backward pass needs the forward's stats");
         const uint64_t need = spiky::lm::residual_norm_workspace(*args, *grads);
         require(grads->workspace_bytes >= need && (grads->workspace || need == 0), "residual_norm workspace too small");

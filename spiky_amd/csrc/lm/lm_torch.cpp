@@ -143,18 +143,19 @@ struct OnDevice {
 bool needs_grad(const Tensor &t) { return t.defined() && t.requires_grad(); }
 
 // Gradients of the gradients are not computed: a backward pass through these raises.
-variable_list once_differentiable(variable_list &&grads) {
-    if (!at::GradMode::is_enabled()) return std::move(grads);
-    auto stop = std::make_shared<torch::autograd::DelayedError>(
-        "trying to differentiate twice a function that was marked with once_differentiable", (int64_t)grads.size());
-    at::AutoGradMode off(false);
-    variable_list out;
-    for (size_t i = 0; i < grads.size(); i++) {
-        Tensor t = grads[i].defined() ? grads[i].detach() : Tensor();
-        if (t.defined()) torch::autograd::impl::set_gradient_edge(t, {stop, (uint32_t)i});
-        out.push_back(t);
+struct Twice : Node {
+    variable_list apply(variable_list &&) override {
+        TORCH_CHECK(false, "spiky_amd's language-model operators cannot be differentiated twice");
     }
-    return out;
+};
+
+variable_list once_differentiable(variable_list &&grads, const torch::autograd::edge_list &inputs) {
+    if (!at::GradMode::is_enabled()) return std::move(grads);
+    auto stop = std::make_shared<Twice>();
+    stop->set_next_edges(torch::autograd::edge_list(inputs));  // so that a search for them comes by here
+    for (Tensor &t : grads)
+        if (t.defined()) torch::autograd::set_history(t, stop);
+    return std::move(grads);
 }
 
 // ---- dropout ----------------------------------------------------------------
@@ -188,7 +189,7 @@ struct CounterDropoutBackward : Node {
 template <typename N>
 struct Once : N {
     variable_list apply(variable_list &&grads) override {
-        return once_differentiable(N::apply(std::move(grads)));
+        return once_differentiable(N::apply(std::move(grads)), N::next_edges());
     }
 };
 
