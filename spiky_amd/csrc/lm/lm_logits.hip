@@ -7,7 +7,8 @@ namespace spiky {
 namespace lm {
 namespace {
 
-constexpr uint32_t kThreads = 256;
+constexpr uint64_t kLong = 4096;  // tokens of a history from which 1024 threads count them
+
 // The word of an entry in LDS: flags, and in the bits below the times that it is
 // among the tokens after the prompt.  Histories short enough leave bits 18 to 29
 // for the slot of its sum of sparse biases; for others the slots have an array.
@@ -32,7 +33,7 @@ __device__ __forceinline__ T *past(T *p, uint32_t at) {
 }
 
 // The tokens a thread holds at a time: numbers at + thread, at + thread + kThreads, ...
-template <typename T>
+template <typename T, uint32_t kThreads>
 struct Tokens {
     static constexpr uint32_t kAhead = 64 / sizeof(T);
     T id[kAhead];
@@ -89,8 +90,9 @@ __device__ __forceinline__ float bias_value(const spiky_lm_logits_args &a, uint3
 // kThreads: those in the chunk are listed in their order, and the first of each
 // entry adds up the others, so repeated ids are added in their order whatever the
 // threads do.
+template <uint32_t kThreads>
 struct Sparse {
-    uint32_t list_id[kThreads];
+    alignas(16) uint32_t list_id[kThreads + 16];
     float list_value[kThreads];
     uint32_t wave_count[2][kThreads / 64], taken;
 
@@ -120,15 +122,26 @@ struct Sparse {
                     list_id[at] = (uint32_t)id - base;
                     list_value[at] = value;
                 }
+                if (tid < 16) list_id[listed + tid] = ~0u;  // the search goes by 16
                 __syncthreads();
                 if (tid < listed) {
                     const uint32_t mine = list_id[tid];
                     bool leads = true;
                     float sum = 0.f;
-                    for (uint32_t j = 0; j < listed; j++) {
-                        if (list_id[j] != mine) continue;
-                        leads = leads && j >= tid;
-                        sum += list_value[j];
+                    for (uint32_t j0 = 0; j0 < listed; j0 += 16) {
+                        uint4 ids[4];
+#pragma unroll
+                        for (int q = 0; q < 4; q++) ids[q] = *reinterpret_cast<const uint4 *>(&list_id[j0 + 4 * q]);
+                        uint32_t same = 0;
+#pragma unroll
+                        for (int q = 0; q < 4; q++)
+                            same |= (ids[q].x == mine ? 1u : 0u) << 4 * q | (ids[q].y == mine ? 2u : 0u) << 4 * q |
+                                    (ids[q].z == mine ? 4u : 0u) << 4 * q | (ids[q].w == mine ? 8u : 0u) << 4 * q;
+                        for (; same; same &= same - 1) {
+                            const uint32_t j = j0 + __builtin_ctz(same);
+                            leads = leads && j >= tid;
+                            sum += list_value[j];
+                        }
                     }
                     if (leads) {
                         const uint32_t w = words[mine];
@@ -155,17 +168,17 @@ struct Sparse {
     }
 };
 
-// A workgroup takes a chunk of up to kThreads * P * N entries of a row.  Counts
+// A workgroup of kThreads takes a chunk of up to kThreads * P * N entries of a row.  Counts
 // of the row's tokens in the chunk, and which entries have sparse biases, are
 // words in LDS, so the logits are read and written once and no count is kept in
 // memory.  Loads are issued in the order in which they are waited for: tokens,
 // logits, bias, mask.
-template <typename TI, typename TO, int N, int P>
-__global__ __launch_bounds__(kThreads) void k_logits(spiky_lm_logits_args a) {
+template <typename TI, typename TO, int N, int P, uint32_t kThreads>
+__global__ __launch_bounds__(kThreads, kThreads == 256 ? 7 : 1) void k_logits(spiky_lm_logits_args a) {
     constexpr uint32_t kChunk = kThreads * P * N;
     // words where there are tokens or bias ids; with bias ids as many sums as may be needed, and slots
     extern __shared__ uint4 space[];
-    __shared__ Sparse sparse;
+    __shared__ Sparse<kThreads> sparse;
     uint32_t *const words = reinterpret_cast<uint32_t *>(space);
     float *const sums = reinterpret_cast<float *>(words + kChunk);
     uint16_t *const slots = reinterpret_cast<uint16_t *>(sums + min((uint64_t)kChunk, a.n_bias));
@@ -178,8 +191,8 @@ __global__ __launch_bounds__(kThreads) void k_logits(spiky_lm_logits_args a) {
 
     const uint32_t history = (uint32_t)a.history;
     const uint64_t first = (uint64_t)row * a.tokens_stride;
-    Tokens<int32_t> short_ids;
-    Tokens<int64_t> long_ids;
+    Tokens<int32_t, kThreads> short_ids;
+    Tokens<int64_t, kThreads> long_ids;
     if (a.tokens) {
         if (a.tokens_i64)
             long_ids.load(static_cast<const int64_t *>(a.tokens) + first, 0, history);
@@ -343,11 +356,11 @@ __global__ __launch_bounds__(kThreads) void k_logits(spiky_lm_logits_args a) {
 
 template <typename TI, typename TO>
 hipError_t launch(const spiky_lm_logits_args &a, hipStream_t st) {
-    // enough workgroups for the chip, but no more than a row's history is worth reading for
     constexpr int N = sizeof(TO) == 4 ? 4 : 8, kMost = 16 / N;
     // enough workgroups for the chip, but no more than a row's history is worth reading for
-    uint64_t chunk = kThreads * 16;
-    while (chunk > kThreads * N && (a.vocab + chunk - 1) / chunk * a.rows < 2 * kCUs) chunk /= 2;
+    const bool wide = a.tokens && a.history > kLong && (a.vocab + 4095) / 4096 * a.rows < 2 * kCUs;
+    uint64_t chunk = wide ? 1024 * N : 256 * 16;
+    while (!wide && chunk > 256 * N && (a.vocab + chunk - 1) / chunk * a.rows < 2 * kCUs) chunk /= 2;
     const uint64_t chunks = (a.vocab + chunk - 1) / chunk;
     size_t lds = a.tokens || a.bias_ids ? chunk * sizeof(uint32_t) : 0;
     if (a.bias_ids)
@@ -375,12 +388,14 @@ hipError_t launch(const spiky_lm_logits_args &a, hipStream_t st) {
         skip(part.bias_values, a.bias_values_stride * 4);
         skip(part.mask, a.mask_stride * (a.mask_bits ? 4 : 1));
         const dim3 grid((uint32_t)chunks, n);
-        if (chunk == kThreads * 16)
-            k_logits<TI, TO, N, kMost><<<grid, dim3(kThreads), lds, st>>>(part);
-        else if (chunk == kThreads * 8)
-            k_logits<TI, TO, N, kMost / 2><<<grid, dim3(kThreads), lds, st>>>(part);
+        if (wide)
+            k_logits<TI, TO, N, 1, 1024><<<grid, dim3(1024), lds, st>>>(part);
+        else if (chunk == 256 * 16)
+            k_logits<TI, TO, N, kMost, 256><<<grid, dim3(256), lds, st>>>(part);
+        else if (chunk == 256 * 8)
+            k_logits<TI, TO, N, kMost / 2, 256><<<grid, dim3(256), lds, st>>>(part);
         else
-            k_logits<TI, TO, N, 1><<<grid, dim3(kThreads), lds, st>>>(part);
+            k_logits<TI, TO, N, 1, 256><<<grid, dim3(256), lds, st>>>(part);
         const hipError_t err = hipGetLastError();
         if (err != hipSuccess) return err;
     }
