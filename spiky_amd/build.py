@@ -50,7 +50,7 @@ def build_binding(verbose=False):
                "/opt/rocm/include", sysconfig.get_paths()["include"]]
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__",
            "-DUSE_ROCM", *(f for i in include for f in ("-isystem", i)), os.path.join(CSRC, BINDING_SOURCE), "-o", tmp,
-           "-L" + os.path.join(torch, "lib"), "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python", "-L" + HERE,
+           "-L" + os.path.join(torch, "lib"), "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch_python", "-L" + HERE,
            "-l:" + os.path.basename(LIB), "-Wl,-rpath,$ORIGIN"]
     if verbose:
         print(" ".join(cmd), flush=True)

@@ -6,6 +6,7 @@
 // launches.  Python functions over ctypes took 92-103 us for a pass of the
 // residual join and its gradients whose kernels take 33.
 #include <ATen/ATen.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
 #include <c10/hip/HIPStream.h>
@@ -134,6 +135,11 @@ int64_t rows_of(const Tensor &t) {
     return cols ? t.numel() / cols : 0;
 }
 
+// An uninitialised tensor, without the dispatcher's way to the same call.
+Tensor fresh(at::IntArrayRef sizes, ScalarType type, c10::Device device) {
+    return at::detail::empty_cuda(sizes, type, device, std::nullopt);
+}
+
 struct OnDevice {
     c10::DeviceGuard guard;
     void *stream;
@@ -162,7 +168,7 @@ variable_list once_differentiable(variable_list &&grads, const torch::autograd::
 Tensor apply_dropout(const Tensor &given, double p, uint64_t seed, uint64_t offset, const Tensor &state) {
     OnDevice on(given.device());
     auto [x, stride] = as_rows(given);
-    Tensor y = at::empty(x.sizes(), x.options().requires_grad(false));
+    Tensor y = fresh(x.sizes(), x.scalar_type(), x.device());
     check(spiky_lm_dropout(x.data_ptr(), stride, y.data_ptr(), rows_of(x), x.dim() ? x.size(-1) : 1,
                            type_code(x, "x"), p, seed, offset, static_cast<const int64_t *>(pointer(state)),
                            on.stream));
@@ -273,8 +279,8 @@ std::pair<Tensor, Tensor> join_forward(const How &how, const Inputs &in, const T
     OnDevice on(in[kRes].device());
     Tensor res, branch, out, normed;
     const spiky_lm_residual_args a = join_args(how, in, state, stats, res, branch);
-    if (branch.defined()) out = at::empty(res.sizes(), res.options().requires_grad(false));
-    if (how.pre) normed = at::empty(res.sizes(), res.options().dtype(how.dtype).requires_grad(false));
+    if (branch.defined()) out = fresh(res.sizes(), res.scalar_type(), res.device());
+    if (how.pre) normed = fresh(res.sizes(), how.dtype, res.device());
     check(spiky_lm_residual_norm(&a, pointer(out), pointer(normed), on.stream));
     return {out, normed};
 }
@@ -304,8 +310,8 @@ struct ResidualNormBackward : Node {
         for (int i = 0; i < kInputs; i++) {
             if (!has[i] || !task_should_compute_output(i)) continue;
             const bool zero = a.rows == 0 || a.cols == 0 || (idle && (i == kPreWeight || i == kPreBias));
-            const auto options = in[i].options().requires_grad(false);
-            out[i] = zero ? at::zeros(in[i].sizes(), options) : at::empty(in[i].sizes(), options);
+            out[i] = zero ? at::zeros(in[i].sizes(), in[i].options().requires_grad(false))
+                          : fresh(in[i].sizes(), in[i].scalar_type(), in[i].device());
         }
         if (d_out.defined()) std::tie(d_out, g.d_out_stride) = as_rows(d_out);
         if (d_normed.defined()) std::tie(d_normed, g.d_normed_stride) = as_rows(d_normed);
@@ -319,7 +325,7 @@ struct ResidualNormBackward : Node {
         g.d_pre_weight = idle ? nullptr : pointer(out[kPreWeight]);
         g.d_pre_bias = idle ? nullptr : pointer(out[kPreBias]);
         g.workspace_bytes = spiky_lm_residual_norm_workspace(&a, &g);
-        Tensor workspace = at::empty({(int64_t)g.workspace_bytes}, res.options().dtype(at::kByte).requires_grad(false));
+        Tensor workspace = fresh({(int64_t)g.workspace_bytes}, at::kByte, res.device());
         g.workspace = workspace.data_ptr();
         check(spiky_lm_residual_norm_backward(&a, &g, on.stream));
         return out;
@@ -458,7 +464,7 @@ PyObject *residual_norm(PyObject *, PyObject *const *args, Py_ssize_t n) {
         auto node = std::make_shared<Once<ResidualNormBackward>>();
         {
             at::AutoGradMode off(false);
-            node->stats = at::empty({rows_of(res), 4}, res.options().dtype(at::kFloat).requires_grad(false));
+            node->stats = fresh({rows_of(res), 4}, at::kFloat, device);
             result = join_forward(how, in, g.state, node->stats);
         }
         node->how = how;
@@ -525,7 +531,7 @@ PyObject *process_logits(PyObject *, PyObject *const *args, Py_ssize_t n) {
     if (!out.defined()) {
         const ScalarType t = dtype.value_or(logits.scalar_type());
         TORCH_CHECK_VALUE(fits(t), "dtype must be ", logits.scalar_type(), " or float32, got ", t);
-        out = at::empty({rows, vocab}, logits.options().dtype(t).requires_grad(false));
+        out = fresh({rows, vocab}, t, device);
     } else {
         TORCH_CHECK_VALUE(out.sizes() == logits.sizes() && fits(out.scalar_type()) &&
                               (!dtype || *dtype == out.scalar_type()),
