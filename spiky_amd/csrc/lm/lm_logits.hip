@@ -18,9 +18,17 @@ constexpr uint32_t kSlotShift = 18, kSlotMask = 0xfff;
 
 __host__ __device__ __forceinline__ bool slots_in_words(uint64_t history) { return history < 1u << kSlotShift; }
 
+// A value that no one writes during the launch, read the same by all lanes: a
+// scalar load, which does not queue with the lanes' loads.
+template <typename T>
+__device__ __forceinline__ T scalar(const T *p) {
+    typedef __attribute__((address_space(4))) const T *Constant;
+    return *(Constant)(uintptr_t)p;
+}
+
 __device__ __forceinline__ uint32_t length_at(const void *p, bool i64, uint32_t row, uint32_t most) {
     if (!p) return most;
-    const int64_t n = i64 ? static_cast<const int64_t *>(p)[row] : static_cast<const int32_t *>(p)[row];
+    const int64_t n = i64 ? scalar(static_cast<const int64_t *>(p) + row) : scalar(static_cast<const int32_t *>(p) + row);
     return n < 0 ? 0 : n < (int64_t)most ? (uint32_t)n : most;
 }
 
@@ -172,7 +180,7 @@ struct Sparse {
 // of the row's tokens in the chunk, and which entries have sparse biases, are
 // words in LDS, so the logits are read and written once and no count is kept in
 // memory.  Loads are issued in the order in which they are waited for: tokens,
-// logits, bias, mask.
+// sparse biases, logits, bias, mask.
 template <typename TI, typename TO, int N, int P, uint32_t kThreads>
 __global__ __launch_bounds__(kThreads, kThreads == 256 ? 7 : 1) void k_logits(spiky_lm_logits_args a) {
     constexpr uint32_t kChunk = kThreads * P * N;
@@ -202,10 +210,10 @@ __global__ __launch_bounds__(kThreads, kThreads == 256 ? 7 : 1) void k_logits(sp
     int64_t sparse_id = -1;
     float sparse_value = 0.f;
     if (a.bias_ids) sparse_id = bias_id(a, row, tid), sparse_value = bias_value(a, row, tid);
-    const float rho = a.repetition_rows ? a.repetition_rows[row] : a.repetition;
-    const float phi = a.frequency_rows ? a.frequency_rows[row] : a.frequency;
-    const float pi = a.presence_rows ? a.presence_rows[row] : a.presence;
-    const float heat = a.temperature_rows ? a.temperature_rows[row] : a.temperature;
+    const float rho = a.repetition_rows ? scalar(a.repetition_rows + row) : a.repetition;
+    const float phi = a.frequency_rows ? scalar(a.frequency_rows + row) : a.frequency;
+    const float pi = a.presence_rows ? scalar(a.presence_rows + row) : a.presence;
+    const float heat = a.temperature_rows ? scalar(a.temperature_rows + row) : a.temperature;
 
     struct Piece {
         Raw<TI, N> x;
@@ -241,9 +249,11 @@ __global__ __launch_bounds__(kThreads, kThreads == 256 ? 7 : 1) void k_logits(sp
             }
         }
     };
-    // Products with reciprocals; a reciprocal past the largest number is not one.
-    const float less = 1.f / rho, cool = heat > 0.f ? 1.f / heat : 1.f;
-    const bool divide_heat = heat > 0.f && __builtin_isinf(cool), divide_rho = __builtin_isinf(less);
+    // Products with reciprocals.  Those of subnormal numbers would pass the largest: a penalty is scaled
+    // to a normal one first, and so is what it divides; a temperature divides.
+    const float lift = rho < 0x1p-126f ? 0x1p24f : 1.f, less = 1.f / (rho * lift);
+    const float cool = heat > 0.f ? 1.f / heat : 1.f;
+    const bool divide_heat = heat > 0.f && __builtin_isinf(cool);
     const uint32_t count_mask = slots_in_words(a.history) ? (1u << kSlotShift) - 1 : kBiased - 1;
     auto finish = [&](const Piece &q, uint32_t o, int n) {
         float x[N];
@@ -279,10 +289,9 @@ __global__ __launch_bounds__(kThreads, kThreads == 256 ? 7 : 1) void k_logits(sp
             if (any & (kSeen | count_mask)) {
 #pragma unroll
                 for (int i = 0; i < N; i++) {
-                    float y = x[i] * (x[i] > 0.f ? less : rho);
-                    if (divide_rho && x[i] > 0.f) y = x[i] / rho;
-                    x[i] = w[i] & (kSeen | count_mask) ? y : x[i];
                     const uint32_t times = w[i] & count_mask;
+                    const float y = x[i] > 0.f ? x[i] * lift * less : x[i] * rho;
+                    x[i] = w[i] & (kSeen | count_mask) ? y : x[i];
                     x[i] = times ? x[i] - (phi * (float)times + pi) : x[i];
                 }
             }
@@ -298,7 +307,10 @@ __global__ __launch_bounds__(kThreads, kThreads == 256 ? 7 : 1) void k_logits(sp
             if (a.mask_bits) {
                 const uint32_t bits = q.allowed[0] >> (o % 8);
 #pragma unroll
-                for (int i = 0; i < N; i++) x[i] = bits >> i & 1 ? x[i] : -__builtin_inff();
+                for (int i = 0; i < N; i++) {
+                    const uint32_t keep = (uint32_t)((int32_t)(bits << (31 - i)) >> 31);
+                    x[i] = __uint_as_float((__float_as_uint(x[i]) & keep) | (0xff800000u & ~keep));
+                }
             } else {
 #pragma unroll
                 for (int i = 0; i < N; i++)
@@ -313,6 +325,11 @@ __global__ __launch_bounds__(kThreads, kThreads == 256 ? 7 : 1) void k_logits(sp
     if (whole)
 #pragma unroll
         for (int p = 0; p < P; p++) load(piece[p], (p * kThreads + tid) * N, N);
+    uint32_t len = 0, prompt = 0;
+    if (a.tokens) {
+        len = length_at(a.lengths, a.lengths_i64, row, history);
+        if (a.prompt_lengths) prompt = length_at(a.prompt_lengths, a.lengths_i64, row, len);
+    }
     if (marks) {
         for (uint32_t i = tid; i < kChunk / 4; i += kThreads) space[i] = make_uint4(0, 0, 0, 0);
         uint64_t all = 0;
@@ -320,8 +337,6 @@ __global__ __launch_bounds__(kThreads, kThreads == 256 ? 7 : 1) void k_logits(sp
         if (tid == 0) sparse.taken = 0;
         __syncthreads();
         if (a.tokens) {
-            const uint32_t len = length_at(a.lengths, a.lengths_i64, row, history);
-            const uint32_t prompt = a.prompt_lengths ? length_at(a.prompt_lengths, a.lengths_i64, row, len) : 0;
             auto count_all = [&](auto &ids, auto *tokens) {
                 uint32_t at = 0;
                 while (true) {
