@@ -40,6 +40,26 @@ __device__ __forceinline__ T *past(T *p, uint32_t at) {
     return reinterpret_cast<T *>(reinterpret_cast<C *>(p) + at * (uint32_t)sizeof(T));
 }
 
+// Stores a piece past the caches' ordinary replacement: a row's bias and tokens, which other
+// workgroups read again, stay in L2.  512 rows of 152000 take 100 us against 130, and with a
+// reader of the result after it (which finds less of it in the last cache) 218 against 222;
+// 64 rows of 130000 and a reader 25.3 against 26.8, 4 rows 8.0 against 8.1.
+template <typename T, int N>
+__device__ __forceinline__ void stream_out(T *p, const float (&v)[N], int n) {
+    static_assert(N * sizeof(T) == 16, "16-byte pieces");
+    if (n < N) {
+        store(p, v, n);
+        return;
+    }
+    typedef uint32_t Piece __attribute__((ext_vector_type(4), aligned(2)));
+    T t[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) t[i] = from_f32<T>(v[i]);
+    Piece q;
+    __builtin_memcpy(&q, t, sizeof(q));
+    __builtin_nontemporal_store(q, reinterpret_cast<Piece *>(p));
+}
+
 // The tokens a thread holds at a time: numbers at + thread, at + thread + kThreads, ...
 template <typename T, uint32_t kThreads>
 struct Tokens {
@@ -317,7 +337,7 @@ __global__ __launch_bounds__(kThreads, kThreads == 256 ? 7 : 1) void k_logits(sp
                     x[i] = q.allowed[i / 4] >> (8 * (i % 4)) & 0xff ? x[i] : -__builtin_inff();
             }
         }
-        store(past(out, o), x, n);
+        stream_out(past(out, o), x, n);
     };
 
     const bool whole = size == kChunk;
