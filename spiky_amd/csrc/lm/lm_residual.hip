@@ -864,18 +864,20 @@ struct Sums {
     const float *part[5];
     void *out[5];
     bool f32[5];
-    uint32_t count[5], groups[5];
+    uint32_t count[5], groups[5];  // groups: 0 where there is no sum
 };
 
 // A workgroup takes 32 columns, its thread (k, c) every 32nd row from k on.
 template <typename TA>
 __global__ __launch_bounds__(1024) void k_join_sums(Sums s, uint64_t cols) {
     __shared__ float lds[32][33];
-    const int k = blockIdx.z;
-    if (!s.part[k] || blockIdx.y >= s.groups[k]) return;
+    // blockIdx.y counts through the groups of all sums
+    uint32_t group = blockIdx.y;
+    int k = 0;
+    while (group >= s.groups[k]) group -= s.groups[k++];
     const uint32_t c = threadIdx.x & 31, first = threadIdx.x / 32, count = s.count[k];
     const uint64_t col = (uint64_t)blockIdx.x * 32 + c;
-    const float *p = s.part[k] + (uint64_t)blockIdx.y * count * cols + col;
+    const float *p = s.part[k] + (uint64_t)group * count * cols + col;
     float sum = 0.f;
     if (col < cols)
 #pragma unroll 8
@@ -883,11 +885,10 @@ __global__ __launch_bounds__(1024) void k_join_sums(Sums s, uint64_t cols) {
     lds[first][c] = sum;
     __syncthreads();
     // row `first` of the transposed sums: its 32 lanes hold one column's
-    sum = lds[c][first];
-    sum = lanes_sum<32>(sum);
+    sum = lanes_sum<32>(lds[c][first]);
     const uint64_t to = (uint64_t)blockIdx.x * 32 + first;
     if (c != 0 || to >= cols) return;
-    const uint64_t at = (uint64_t)blockIdx.y * cols + to;
+    const uint64_t at = (uint64_t)group * cols + to;
     if (s.f32[k])
         static_cast<float *>(s.out[k])[at] = sum;
     else
@@ -1102,11 +1103,11 @@ hipError_t backward(const spiky_lm_residual_args &a, const DropArgs &drop, const
         s.out[k] = outs[k];
         s.f32[k] = k == 4 ? j.gate_f32 : j.par_f32;
         s.count[k] = k == 4 ? p.chunks_per_span : p.chunks;
-        s.groups[k] = k == 4 && p.chunks_per_span ? p.chunks / p.chunks_per_span : 1;
-        if (s.part[k] && s.groups[k] > groups) groups = s.groups[k];
+        s.groups[k] = !s.part[k] ? 0 : k == 4 && p.chunks_per_span ? p.chunks / p.chunks_per_span : 1;
+        groups += s.groups[k];
     }
     if (groups == 0) return hipSuccess;
-    k_join_sums<TA><<<dim3((uint32_t)((a.cols + 31) / 32), groups, 5), dim3(1024), 0, st>>>(s, a.cols);
+    k_join_sums<TA><<<dim3((uint32_t)((a.cols + 31) / 32), groups), dim3(1024), 0, st>>>(s, a.cols);
     return hipGetLastError();
 }
 
