@@ -7,7 +7,10 @@ namespace spiky {
 namespace lm {
 namespace {
 
-constexpr uint64_t kLong = 4096;  // tokens of a history from which 1024 threads count them
+// Tokens of a history from which 1024 threads count them where workgroups are few: 128 rows of
+// 8991 entries with 31972 tokens take 25 us against 30, but 46 rows of 97950 with 22483, whose
+// chunks of 256 threads fill the chip, 36 against 27.
+constexpr uint64_t kLong = 4096;
 
 // The word of an entry in LDS: flags, and in the bits below the times that it is
 // among the tokens after the prompt.  Histories short enough leave bits 18 to 29
@@ -41,9 +44,10 @@ __device__ __forceinline__ T *past(T *p, uint32_t at) {
 }
 
 // Stores a piece past the caches' ordinary replacement: a row's bias and tokens, which other
-// workgroups read again, stay in L2.  512 rows of 152000 take 100 us against 130, and with a
-// reader of the result after it (which finds less of it in the last cache) 218 against 222;
-// 64 rows of 130000 and a reader 25.3 against 26.8, 4 rows 8.0 against 8.1.
+// workgroups read again, stay in L2.  512 rows of 152000, stored so and as usual: 97 and 130 us
+// where the last cache holds the inputs, 128 and 130 where it does not; with a reader of the
+// result behind the call, which then finds less of it there, 218 and 222, 64 rows of 130000
+// 25.3 and 26.8, 4 rows 8.0 and 8.1.
 template <typename T, int N>
 __device__ __forceinline__ void stream_out(T *p, const float (&v)[N], int n) {
     static_assert(N * sizeof(T) == 16, "16-byte pieces");
@@ -197,10 +201,15 @@ struct Sparse {
 };
 
 // A workgroup of kThreads takes a chunk of up to kThreads * P * N entries of a row.  Counts
-// of the row's tokens in the chunk, and which entries have sparse biases, are
-// words in LDS, so the logits are read and written once and no count is kept in
-// memory.  Loads are issued in the order in which they are waited for: tokens,
-// sparse biases, logits, bias, mask.
+// of the row's tokens in the chunk, and which entries have sparse biases, are words in LDS, so
+// the logits are read and written once and no count is kept in memory.  Loads are issued in the
+// order in which they are waited for: tokens, sparse biases, logits, bias, mask.
+//
+// 512 rows of 152000 bf16 logits to fp32: 78 us without more (6.0 TB/s); 4096 tokens a row add
+// 17, a shared bias 13, a mask 2 and 64 sparse biases 3, all of them together 50, where the
+// waves wait for each other's phases and for L2, which reads a row's tokens for each of its
+// chunks.  256 threads are faster than 512 and 1024 there (all together, in an earlier form:
+// 166, 198, 242), for barriers hold fewer waves; 8 pieces a thread no faster than 4 (144, 141).
 template <typename TI, typename TO, int N, int P, uint32_t kThreads>
 __global__ __launch_bounds__(kThreads, kThreads == 256 ? 7 : 1) void k_logits(spiky_lm_logits_args a) {
     constexpr uint32_t kChunk = kThreads * P * N;

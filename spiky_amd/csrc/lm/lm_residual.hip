@@ -12,6 +12,12 @@
 //   da = r1 (dn - [mean dn] - n1 mean(dn n1))
 // ([..] in layer norms only).  z is formed again from r and a, not read back
 // from its rounded copy, so n2 is the forward's own.
+//
+// Both directions are bound by memory where the work is large: 16384 rows of 4096,
+// bf16 beside an fp32 residual, take 160 us forward (805 MB, 5.0 TB/s; a large copy
+// runs at 4.9 to 5.4) and 265 us backward (1.24 GB, 4.7 TB/s), with the vector unit
+// busy half of the time, a third of that with the dropout's generator.  A backward
+// pass in two passes over the inputs took 808.  Small calls are bound by the host.
 #include "lm_kernels.h"
 
 namespace spiky {
@@ -97,34 +103,6 @@ __device__ __forceinline__ float lanes_sum(float x) {
     }
     return x;
 }
-
-// Sums of K values over the TPR threads of a row.  Rows of more than a wave go
-// through LDS, two buffers in turn: a buffer is written again only after the
-// barrier of the call in between, which its readers have passed.
-template <int TPR, int K>
-struct RowSum {
-    static constexpr int kWaves = TPR / 64;
-    float (*lds)[K][16];
-    int turn = 0;
-    __device__ __forceinline__ void operator()(float (&x)[K]) {
-#pragma unroll
-        for (int k = 0; k < K; k++) x[k] = lanes_sum<(TPR < 64 ? TPR : 64)>(x[k]);
-        if constexpr (TPR > 64) {
-            if ((threadIdx.x & 63) == 0)
-#pragma unroll
-                for (int k = 0; k < K; k++) lds[turn][k][threadIdx.x / 64] = x[k];
-            __syncthreads();
-#pragma unroll
-            for (int k = 0; k < K; k++) {
-                float s = 0.f;
-#pragma unroll
-                for (int w = 0; w < kWaves; w++) s += lds[turn][k][w];
-                x[k] = s;
-            }
-            turn ^= 1;
-        }
-    }
-};
 
 __device__ __forceinline__ int piece_size(uint64_t cols, uint64_t col, int n) {
     return col >= cols ? 0 : cols - col < (uint64_t)n ? (int)(cols - col) : n;
@@ -238,8 +216,11 @@ __device__ __forceinline__ void values_of(float (&v)[N], const Raw<float, N> &ra
 // A row in the registers of TPR threads (TPR > 64: of the workgroup, of up to TPR),
 // P pieces of N columns each: every input is read once, the sums of both norms run
 // over registers.  The row's loads are issued before the first sum, and with 8
-// columns a thread the parameters' too; with 16 these would halve the waves.
-// FULL: with layer norms or biases.
+// columns a thread the parameters' too; with 16 these would halve the waves (2597
+// rows of 9564: 119 us so, 107 without).  A workgroup has one round of rows and
+// leaves: walking many with the parameters in registers and the next row's loads
+// ahead needs twice the registers, so half the waves (16384 rows of 8192 bf16: 287
+// us against 232).  FULL: with layer norms or biases.
 template <typename TZ, typename TA, int N, int P, int TPR, bool FULL>
 __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_join(Join<TZ, TA> j) {
     constexpr int kSlots = TPR <= 64 ? 256 / TPR : 1, Q = N * P <= 8 ? P : 1;
@@ -376,8 +357,8 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_join(Join<TZ, TA> j) 
 // Rows of any width: a workgroup walks its row once for each sum.
 template <typename TZ, typename TA, int N, int WG>
 __global__ __launch_bounds__(WG) void k_join_any(Join<TZ, TA> j) {
-    __shared__ float red[2][1][16];
-    RowSum<WG, 1> row_sum{red};
+    __shared__ float4 red[2][1][16];
+    uint32_t turn = 0;
     const uint32_t row = j.row0 + blockIdx.x;
     const TZ *r = j.r + (int64_t)row * j.r_stride;
     const TA *a = j.a + (int64_t)row * j.a_stride;
@@ -388,7 +369,7 @@ __global__ __launch_bounds__(WG) void k_join_any(Join<TZ, TA> j) {
         float s[1] = {0.f};
         for (uint64_t col = (uint64_t)threadIdx.x * N; col < j.cols; col += WG * N)
             s[0] += piece(col, piece_size(j.cols, col, N));
-        row_sum(s);
+        row_sums<WG, 1>(s, red, turn, WG / 64);
         return s[0];
     };
     auto deviation = [&](int kind, float eps, float &mean, auto &&read) {
@@ -626,18 +607,21 @@ __device__ __forceinline__ float4 row_means(const J &j, const float4 &st, const 
     return m;
 }
 
-// Rows of up to 1024 * N * P columns: a workgroup walks the rows of its chunk (a
-// slot of TPR lanes its share of them), a thread always with the same columns,
-// so every input crosses HBM once.  Parameters stay in registers; column sums are
-// in LDS, each thread's its own, which costs a read and a write of LDS a row and
-// frees the registers that more waves need.  The next row's loads are issued
-// before the reduction, into the registers that this row's left.
+// Rows of 8 to 8192 columns: a workgroup walks the rows of its chunk (a slot of TPR
+// lanes its share of them), a thread always with the same columns, so every input
+// crosses HBM once.  Parameters stay in registers; column sums are in LDS, each
+// thread's its own: a read and a write of LDS a row, a tenth of the time that the
+// row takes in HBM, for registers that make 3 waves of 2 to a SIMD (33822 rows of
+// 640 fp32 with layer norms 234 -> 161 us).  The next row's loads are issued before
+// the reduction, into the registers that this row's left.  Above 4096 columns 512
+// threads have 16 columns each: 1024 of 8 may use 128 registers, and spill (8192
+// rows of 8192: 370 us against 255; with layer norms 445 and 410).
 template <typename TZ, typename TA, int N, int P, int TPR, bool FULL>
 __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_join_back(Join<TZ, TA> j) {
     constexpr int kThreads = TPR <= 64 ? 256 : TPR, kSlots = TPR <= 64 ? 256 / TPR : 1;
     constexpr int W = N * P, K = FULL ? 8 : 3, kQuads = W / 4;
     __shared__ float4 red[TPR > 64 ? 2 : 1][(K + 3) / 4][16];
-    // sums of w1, w2, g and, FULL, b1; those of b2 stay in registers, where 1024 threads have no LDS for them
+    // sums of w1, w2, g and, FULL, b1; five of 8192 columns would not fit, so those of b2 stay in registers
     constexpr int kInLds = FULL ? 4 : 3;
     __shared__ float4 acc[kInLds][kQuads][kThreads];
     const uint32_t threads = TPR <= 64 ? TPR : blockDim.x, waves = blockDim.x / 64;
@@ -781,7 +765,8 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_join_back(Join<TZ, TA
 }
 
 // Wider rows, and those narrower than a piece, take two passes over the inputs: the
-// means of each row, then columns.
+// means of each row, then columns.  1392 rows of 10700 fp16: 32 and 40 us, for 41 of
+// HBM in one pass; neither a thread's registers nor the LDS hold such a row's sums.
 template <typename TZ, typename TA, int N, int WG, bool FULL>
 __global__ __launch_bounds__(WG) void k_join_back_rows(Join<TZ, TA> j) {
     constexpr int K = FULL ? 8 : 3;
@@ -941,7 +926,9 @@ hipError_t over_rows(J &j, uint32_t kRows, uint32_t threads, F &&launch) {
     return hipSuccess;
 }
 
-// W columns a thread.
+// W columns a thread.  Rows of up to 1024 columns have a wave, which needs no
+// barrier: 33822 rows of 640 fp32 take 85 us against 118 in workgroups of 160
+// threads, 14400 of 646 fp16 38 against 42.
 template <typename TZ, typename TA, int W, int TPR, bool FULL>
 hipError_t run_rows(Join<TZ, TA> &j, hipStream_t st) {
     constexpr int N = sizeof(TA) == 4 ? 4 : 8;
@@ -982,7 +969,7 @@ hipError_t forward(const spiky_lm_residual_args &a, const DropArgs &drop, void *
 
 // How the rows are cut into chunks, and the workspace's regions.
 struct Plan {
-    uint32_t tpr;  // lanes of a row in k_join_back, 1024 for all rows of more than 64; 0: the passes for any row
+    uint32_t tpr;  // lanes of a row in k_join_back, 1024: a workgroup's; 0: the passes for any row
     uint32_t chunk, chunks, span, chunks_per_span;
     bool part[5];
     uint64_t row_sums, parts[5], bytes;
@@ -990,7 +977,7 @@ struct Plan {
 
 // Columns of a thread of k_join_back.
 constexpr uint64_t kBackCols = 8;
-constexpr uint64_t kLeast = 4;
+constexpr uint64_t kLeast = 8;
 
 Plan plan(const spiky_lm_residual_args &a, const spiky_lm_residual_grads &g) {
     Plan p = {};
@@ -1002,7 +989,9 @@ Plan plan(const spiky_lm_residual_args &a, const spiky_lm_residual_grads &g) {
     const uint64_t waves = p.tpr && p.tpr <= 64 ? 4 : (threads + 63) / 64;
     uint64_t chunk;
     if (p.tpr) {
-        // 16 waves to a CU, where each has kLeast rows of its own
+        // 16 waves to a CU, where each has kLeast rows of its own; at least one workgroup to a CU.  Fewer
+        // rows to more workgroups: 1024 rows of 4096 in 512 workgroups 34 us, in 256 27; 8192 rows of 1024
+        // with 4 rows to a workgroup 35 and 7.4 for the sums, with 8 35 and 4.5
         const uint64_t most = kCUs * (waves > 8 ? 1 : 16 / waves);
         chunk = (a.rows + most - 1) / most;
         const uint64_t one_each = (a.rows + kCUs - 1) / kCUs, least = kLeast * slots;
