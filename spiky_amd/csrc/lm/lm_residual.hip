@@ -85,14 +85,14 @@ __device__ __forceinline__ float add_dpp(float x) {
     return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
 }
 
-// Sum over groups of L lanes (16, 32 or 64), in every lane: exchanges inside
+// Sum over groups of L lanes (8, 16, 32 or 64), in every lane: exchanges inside
 // quads, eights and sixteens by DPP, then between rows of 16 and halves.
 template <int L>
 __device__ __forceinline__ float lanes_sum(float x) {
     x = add_dpp<0xB1>(x);   // quad_perm 1 0 3 2
     x = add_dpp<0x4E>(x);   // quad_perm 2 3 0 1
     x = add_dpp<0x141>(x);  // row_half_mirror
-    x = add_dpp<0x140>(x);  // row_mirror
+    if (L >= 16) x = add_dpp<0x140>(x);  // row_mirror
     if (L >= 32) {
         auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
         x = __uint_as_float(s[0]) + __uint_as_float(s[1]);
@@ -928,7 +928,9 @@ hipError_t over_rows(J &j, uint32_t kRows, uint32_t threads, F &&launch) {
 
 // W columns a thread.  Rows of up to 1024 columns have a wave, which needs no
 // barrier: 33822 rows of 640 fp32 take 85 us against 118 in workgroups of 160
-// threads, 14400 of 646 fp16 38 against 42.
+// threads, 14400 of 646 fp16 38 against 42.  Narrower ones have as few lanes as hold
+// them (262144 rows of 64 bf16 beside fp32 with 8 lanes 38 us forward, 68 backward,
+// with 16 54 and 94).
 template <typename TZ, typename TA, int W, int TPR, bool FULL>
 hipError_t run_rows(Join<TZ, TA> &j, hipStream_t st) {
     constexpr int N = sizeof(TA) == 4 ? 4 : 8;
@@ -943,6 +945,7 @@ hipError_t run_forward(Join<TZ, TA> &j, hipStream_t st) {
     constexpr int N = sizeof(TA) == 4 ? 4 : 8;
     if (j.cols < 8)  // narrower than a piece
         return over_rows(j, 1, 64, [&](dim3 grid, dim3 block) { k_join_any<TZ, TA, N, 64><<<grid, block, 0, st>>>(j); });
+    if (j.cols <= 64) return run_rows<TZ, TA, 8, 8, FULL>(j, st);
     if (j.cols <= 128) return run_rows<TZ, TA, 8, 16, FULL>(j, st);
     if (j.cols <= 256) return run_rows<TZ, TA, 8, 32, FULL>(j, st);
     if (j.cols <= 512) return run_rows<TZ, TA, 8, 64, FULL>(j, st);
@@ -982,7 +985,7 @@ constexpr uint64_t kLeast = 8;
 Plan plan(const spiky_lm_residual_args &a, const spiky_lm_residual_grads &g) {
     Plan p = {};
     const uint64_t threads = (a.cols + kBackCols - 1) / kBackCols;
-    p.tpr = threads <= 16 ? 16 : threads <= 32 ? 32 : threads <= 64 ? 64 : threads <= 1024 ? 1024 : 0;
+    p.tpr = threads <= 8 ? 8 : threads <= 16 ? 16 : threads <= 32 ? 32 : threads <= 64 ? 64 : threads <= 1024 ? 1024 : 0;
     if (a.cols < kBackCols) p.tpr = 0;
     const uint64_t span = a.gate && g.d_gate ? a.gate_rows : a.rows;
     const uint64_t slots = p.tpr && p.tpr <= 64 ? 256 / p.tpr : 1;
@@ -1041,7 +1044,9 @@ hipError_t run_back(Join<TZ, TA> &j, const Plan &p, hipStream_t st) {
     }
     const dim3 grid(p.chunks);
     const uint32_t threads = (uint32_t)((j.cols + kBackCols - 1) / kBackCols + 63) & ~63u;
-    if (p.tpr == 16)
+    if (p.tpr == 8)
+        k_join_back<TZ, TA, N, P, 8, FULL><<<grid, dim3(256), 0, st>>>(j);
+    else if (p.tpr == 16)
         k_join_back<TZ, TA, N, P, 16, FULL><<<grid, dim3(256), 0, st>>>(j);
     else if (p.tpr == 32)
         k_join_back<TZ, TA, N, P, 32, FULL><<<grid, dim3(256), 0, st>>>(j);

@@ -68,6 +68,21 @@ def test_unneeded_columns_of_other_lanes_do_not_leak(cuda_device):
             assert torch.equal(counter_dropout(a, 0.2, 1), counter_dropout(a.contiguous(), 0.2, 1))
 
 
+def test_rows_past_32_bits_of_elements(cuda_device):
+    """Rows are worked out alike wherever they lie: the last of 2^32 elements and some, forward and backward."""
+    rows, D = (1 << 19) + 3, 8192
+    r, a, dz, dh = (torch.empty(rows, D, dtype=torch.bfloat16, device=cuda_device).normal_() for _ in range(4))
+    w = torch.randn(D, device=cuda_device).to(torch.bfloat16)
+
+    def step(at):
+        v, b = r[at].detach().requires_grad_(), a[at].detach().requires_grad_()
+        z, h = residual_norm(v, b, post_norm="rms", post_weight=w, pre_norm="rms", pre_weight=w)
+        return [z.detach(), h.detach(), *torch.autograd.grad([z, h], [v, b], [dz[at], dh[at]])]
+
+    whole, end = step(slice(None)), step(slice(rows - 5, rows))
+    assert all(torch.equal(x[-5:], y) for x, y in zip(whole, end))
+
+
 def test_a_gate_of_no_rows(cuda_device):
     for shape, gate in (((0, 8), (8,)), ((3, 0, 8), (3, 1, 8)), ((2, 0), (0,))):
         g = torch.ones(gate, device=cuda_device, requires_grad=True)
