@@ -14,12 +14,15 @@ constexpr uint64_t kLong = 4096;
 
 // The word of an entry in LDS: flags, and in the bits below the times that it is
 // among the tokens after the prompt.  Histories short enough leave bits 18 to 29
-// for the slot of its sum of sparse biases; for others the slots have an array.
+// for the slot of its sum of sparse biases, if there are no more of these; for
+// others the slots have an array.
 constexpr uint32_t kSeen = 0x80000000u;    // among the prompt's tokens
 constexpr uint32_t kBiased = 0x40000000u;  // among the bias ids
 constexpr uint32_t kSlotShift = 18, kSlotMask = 0xfff;
 
-__host__ __device__ __forceinline__ bool slots_in_words(uint64_t history) { return history < 1u << kSlotShift; }
+__host__ __device__ __forceinline__ bool slots_in_words(uint64_t history, uint64_t n_bias) {
+    return history < 1u << kSlotShift && n_bias <= kSlotMask + 1;
+}
 
 // A value that no one writes during the launch, read the same by all lanes: a
 // scalar load, which does not queue with the lanes' loads.
@@ -140,7 +143,7 @@ struct Sparse {
                                         int64_t id, float value, uint64_t all, uint32_t *words, uint16_t *slots,
                                         float *sums) {
         const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid / 64;
-        const bool in_words = slots_in_words(a.history);
+        const bool in_words = slots_in_words(a.history, a.n_bias);
         uint32_t turn = 0;
         for (uint64_t k0 = 0;;) {
             uint32_t at = __popcll(all & ((1ull << lane) - 1)), listed = 0;
@@ -283,7 +286,7 @@ __global__ __launch_bounds__(kThreads, kThreads == 256 ? 7 : 1) void k_logits(sp
     const float lift = rho < 0x1p-126f ? 0x1p24f : 1.f, less = 1.f / (rho * lift);
     const float cool = heat > 0.f ? 1.f / heat : 1.f;
     const bool divide_heat = heat > 0.f && __builtin_isinf(cool);
-    const uint32_t count_mask = slots_in_words(a.history) ? (1u << kSlotShift) - 1 : kBiased - 1;
+    const uint32_t count_mask = slots_in_words(a.history, a.n_bias) ? (1u << kSlotShift) - 1 : kBiased - 1;
     auto finish = [&](const Piece &q, uint32_t o, int n) {
         float x[N];
 #pragma unroll
@@ -313,7 +316,7 @@ __global__ __launch_bounds__(kThreads, kThreads == 256 ? 7 : 1) void k_logits(sp
 #pragma unroll
                 for (int i = 0; i < N; i++)
                     if (w[i] & kBiased)
-                        x[i] += sums[slots_in_words(a.history) ? w[i] >> kSlotShift & kSlotMask : slots[o + i]];
+                        x[i] += sums[slots_in_words(a.history, a.n_bias) ? w[i] >> kSlotShift & kSlotMask : slots[o + i]];
             }
             if (any & (kSeen | count_mask)) {
 #pragma unroll
@@ -409,7 +412,7 @@ hipError_t launch(const spiky_lm_logits_args &a, hipStream_t st) {
     size_t lds = a.tokens || a.bias_ids ? chunk * sizeof(uint32_t) : 0;
     if (a.bias_ids)
         lds += (a.n_bias < chunk ? a.n_bias : chunk) * sizeof(float) +
-               (slots_in_words(a.history) ? 0 : chunk * sizeof(uint16_t));
+               (slots_in_words(a.history, a.n_bias) ? 0 : chunk * sizeof(uint16_t));
     // 65535 rows a launch, in y
     for (uint64_t row0 = 0; row0 < a.rows; row0 += 65535) {
         const uint32_t n = (uint32_t)(a.rows - row0 < 65535 ? a.rows - row0 : 65535);

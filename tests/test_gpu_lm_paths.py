@@ -174,6 +174,14 @@ def test_more_sparse_biases_than_a_chunk_has_entries(cuda_device, K):
         check_logits(cuda_device, s["x"], ids=s["ids"], values=s["values"] * 2.0 ** -6)
 
 
+def test_more_sparse_biases_than_slots_in_a_chunk_of_a_long_history(cuda_device):
+    """1024 threads have chunks of 8192 entries of two bytes: more entries with a bias than a word has slots for."""
+    s = make(2, 8192, 5000, K=9000, seed=4)
+    s["ids"][0] = torch.arange(9000) % 8192
+    check_logits(cuda_device, s["x"].to(torch.bfloat16), tokens=s["tokens"], rho=1.2, frequency=0.5, ids=s["ids"],
+                 values=s["values"])
+
+
 @pytest.mark.parametrize("B", [1, 40, 700])
 @pytest.mark.parametrize("V", [1023, 1024, 1025, 2049, 4095, 4096, 4097, 9000])
 def test_vocabularies_around_a_chunk(cuda_device, B, V):
@@ -204,6 +212,24 @@ def test_logits_in_place_are_seen_by_autograd(cuda_device):
     with pytest.raises(ValueError, match="overlap"):
         process_logits(x, out=torch.zeros(1, 50, device=cuda_device).expand(2, 50))
     assert not process_logits(leaf).requires_grad
+
+
+def test_steps_leave_nothing_behind(cuda_device):
+    x = torch.randn(64, 256, device=cuda_device, requires_grad=True)
+    w = torch.ones(256, device=cuda_device, requires_grad=True)
+    state = torch.tensor([1, 2], dtype=torch.int64, device=cuda_device)
+
+    def step():
+        z, h = residual_norm(x, counter_dropout(x, 0.1, state), pre_norm="rms", pre_weight=w, dropout_p=0.1, seed=state)
+        torch.autograd.grad(z.sum() + process_logits(h.detach(), temperature=2.0).sum() + h.sum(), [x, w])
+
+    step()
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    for _ in range(20):
+        step()
+    torch.cuda.synchronize()
+    assert torch.cuda.memory_allocated() == before
 
 
 def test_module_counts_only_training_calls(cuda_device):
