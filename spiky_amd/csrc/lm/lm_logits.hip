@@ -7,10 +7,13 @@ namespace spiky {
 namespace lm {
 namespace {
 
-// Tokens of a history from which 1024 threads count them where workgroups are few: 128 rows of
-// 8991 entries with 31972 tokens take 25 us against 30, but 46 rows of 97950 with 22483, whose
-// chunks of 256 threads fill the chip, 36 against 27.
+// Tokens of a history from which 1024 threads count them: where workgroups are few (128 rows of
+// 8991 entries with 31972 tokens take 25 us against 30), and, from twice as many on, where
+// chunks of 16384 entries and more, which read it less often, fill the chip (256 rows of 152000:
+// 6000 tokens 53 us against 49, 8192 55 both, 16384 60 against 88, 32768 80 against 156).  In
+// between the chunks of 256 threads are faster (46 rows of 97950 with 22483: 27 against 36).
 constexpr uint64_t kLong = 4096;
+constexpr size_t kMostLds = 150000;  // of 160 KiB, beside a list of sparse biases
 
 // The word of an entry in LDS: flags, and in the bits below the times that it is
 // among the tokens after the prompt.  Histories short enough leave bits 18 to 29
@@ -203,10 +206,11 @@ struct Sparse {
     }
 };
 
-// A workgroup of kThreads takes a chunk of up to kThreads * P * N entries of a row.  Counts
+// A workgroup of kThreads takes a chunk of a row, of kThreads * P * N entries or others.  Counts
 // of the row's tokens in the chunk, and which entries have sparse biases, are words in LDS, so
 // the logits are read and written once and no count is kept in memory.  Loads are issued in the
-// order in which they are waited for: tokens, sparse biases, logits, bias, mask.
+// order in which they are waited for: tokens, sparse biases, logits, bias, mask; in chunks of
+// another size the last three by the piece, after the counts.
 //
 // 512 rows of 152000 bf16 logits to fp32: 78 us without more (6.0 TB/s); 4096 tokens a row add
 // 17, a shared bias 13, a mask 2 and 64 sparse biases 3, all of them together 50, where the
@@ -214,16 +218,15 @@ struct Sparse {
 // chunks.  256 threads are faster than 512 and 1024 there (all together, in an earlier form:
 // 166, 198, 242), for barriers hold fewer waves; 8 pieces a thread no faster than 4 (144, 141).
 template <typename TI, typename TO, int N, int P, uint32_t kThreads>
-__global__ __launch_bounds__(kThreads, kThreads == 256 ? 7 : 1) void k_logits(spiky_lm_logits_args a) {
-    constexpr uint32_t kChunk = kThreads * P * N;
+__global__ __launch_bounds__(kThreads, kThreads == 256 ? 7 : 1) void k_logits(spiky_lm_logits_args a, uint32_t chunk) {
     // words where there are tokens or bias ids; with bias ids as many sums as may be needed, and slots
     extern __shared__ uint4 space[];
     __shared__ Sparse<kThreads> sparse;
     uint32_t *const words = reinterpret_cast<uint32_t *>(space);
-    float *const sums = reinterpret_cast<float *>(words + kChunk);
-    uint16_t *const slots = reinterpret_cast<uint16_t *>(sums + min((uint64_t)kChunk, a.n_bias));
-    const uint32_t tid = threadIdx.x, row = blockIdx.y, base = blockIdx.x * kChunk;
-    const uint32_t size = min(kChunk, (uint32_t)a.vocab - base);
+    float *const sums = reinterpret_cast<float *>(words + chunk);
+    uint16_t *const slots = reinterpret_cast<uint16_t *>(sums + min((uint64_t)chunk, a.n_bias));
+    const uint32_t tid = threadIdx.x, row = blockIdx.y, base = blockIdx.x * chunk;
+    const uint32_t size = min(chunk, (uint32_t)a.vocab - base);
     const bool marks = a.tokens || a.bias_ids;
     const TI *in = static_cast<const TI *>(a.logits) + (int64_t)row * a.logits_stride + base;
     TO *out = static_cast<TO *>(a.out) + (int64_t)row * a.out_stride + base;
@@ -352,7 +355,7 @@ __global__ __launch_bounds__(kThreads, kThreads == 256 ? 7 : 1) void k_logits(sp
         stream_out(past(out, o), x, n);
     };
 
-    const bool whole = size == kChunk;
+    const bool whole = size == kThreads * P * N;
     Piece piece[P];
     if (whole)
 #pragma unroll
@@ -363,7 +366,7 @@ __global__ __launch_bounds__(kThreads, kThreads == 256 ? 7 : 1) void k_logits(sp
         if (a.prompt_lengths) prompt = length_at(a.prompt_lengths, a.lengths_i64, row, len);
     }
     if (marks) {
-        for (uint32_t i = tid; i < kChunk / 4; i += kThreads) space[i] = make_uint4(0, 0, 0, 0);
+        for (uint32_t i = tid; i < chunk / 4; i += kThreads) space[i] = make_uint4(0, 0, 0, 0);
         uint64_t all = 0;
         if (a.bias_ids) all = sparse.announce(sparse_id, 0, base, size);
         if (tid == 0) sparse.taken = 0;
@@ -405,14 +408,20 @@ template <typename TI, typename TO>
 hipError_t launch(const spiky_lm_logits_args &a, hipStream_t st) {
     constexpr int N = sizeof(TO) == 4 ? 4 : 8, kMost = 16 / N;
     // enough workgroups for the chip, but no more than a row's history is worth reading for
-    const bool wide = a.tokens && a.history > kLong && (a.vocab + 4095) / 4096 * a.rows < 2 * kCUs;
-    uint64_t chunk = wide ? 1024 * N : 256 * 16;
-    while (!wide && chunk > 256 * N && (a.vocab + chunk - 1) / chunk * a.rows < 2 * kCUs) chunk /= 2;
+    auto workgroups = [&](uint64_t entries) { return (a.vocab + entries - 1) / entries * a.rows; };
+    const bool wide = a.tokens && a.history > kLong &&
+                      (workgroups(4096) < 2 * kCUs || (a.history >= 2 * kLong && workgroups(16384) >= 2 * kCUs));
+    uint64_t chunk = wide ? 32768 : 256 * 16;
+    auto lds_of = [&](uint64_t entries) {
+        size_t bytes = a.tokens || a.bias_ids ? entries * sizeof(uint32_t) : 0;
+        if (a.bias_ids)
+            bytes += (a.n_bias < entries ? a.n_bias : entries) * sizeof(float) +
+                     (slots_in_words(a.history, a.n_bias) ? 0 : entries * sizeof(uint16_t));
+        return bytes;
+    };
+    while (chunk > (wide ? 1024 : 256) * N && (workgroups(chunk) < 2 * kCUs || lds_of(chunk) > kMostLds)) chunk /= 2;
     const uint64_t chunks = (a.vocab + chunk - 1) / chunk;
-    size_t lds = a.tokens || a.bias_ids ? chunk * sizeof(uint32_t) : 0;
-    if (a.bias_ids)
-        lds += (a.n_bias < chunk ? a.n_bias : chunk) * sizeof(float) +
-               (slots_in_words(a.history, a.n_bias) ? 0 : chunk * sizeof(uint16_t));
+    const size_t lds = lds_of(chunk);
     // 65535 rows a launch, in y
     for (uint64_t row0 = 0; row0 < a.rows; row0 += 65535) {
         const uint32_t n = (uint32_t)(a.rows - row0 < 65535 ? a.rows - row0 : 65535);
@@ -436,13 +445,13 @@ hipError_t launch(const spiky_lm_logits_args &a, hipStream_t st) {
         skip(part.mask, a.mask_stride * (a.mask_bits ? 4 : 1));
         const dim3 grid((uint32_t)chunks, n);
         if (wide)
-            k_logits<TI, TO, N, 1, 1024><<<grid, dim3(1024), lds, st>>>(part);
+            k_logits<TI, TO, N, 1, 1024><<<grid, dim3(1024), lds, st>>>(part, (uint32_t)chunk);
         else if (chunk == 256 * 16)
-            k_logits<TI, TO, N, kMost, 256><<<grid, dim3(256), lds, st>>>(part);
+            k_logits<TI, TO, N, kMost, 256><<<grid, dim3(256), lds, st>>>(part, (uint32_t)chunk);
         else if (chunk == 256 * 8)
-            k_logits<TI, TO, N, kMost / 2, 256><<<grid, dim3(256), lds, st>>>(part);
+            k_logits<TI, TO, N, kMost / 2, 256><<<grid, dim3(256), lds, st>>>(part, (uint32_t)chunk);
         else
-            k_logits<TI, TO, N, 1, 256><<<grid, dim3(256), lds, st>>>(part);
+            k_logits<TI, TO, N, 1, 256><<<grid, dim3(256), lds, st>>>(part, (uint32_t)chunk);
         const hipError_t err = hipGetLastError();
         if (err != hipSuccess) return err;
     }

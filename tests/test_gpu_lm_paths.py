@@ -182,6 +182,23 @@ def test_more_sparse_biases_than_slots_in_a_chunk_of_a_long_history(cuda_device)
                  values=s["values"])
 
 
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,V,L", [(60, 150001, 8192), (520, 16385, 8200), (3, 33000, 9000), (130, 20000, 4097)])
+def test_long_histories_of_many_rows(cuda_device, out, B, V, L):
+    s = make(B, V, L, K=100, token=torch.int32)
+    check_logits(cuda_device, s["x"].to(torch.bfloat16), dtype=out, tokens=s["tokens"], lengths=s["lengths"],
+                 prompts=s["prompts"], rho=1.3, presence=0.5, frequency=0.125, ids=s["ids"], values=s["values"],
+                 mask=torch.rand(V, generator=s["gen"]) < 0.7)
+
+
+@pytest.mark.parametrize("B,K", [(110, 100), (110, 9000), (30, 40000)])
+def test_chunks_that_fill_the_lds(cuda_device, B, K):
+    """The largest chunks, and with as many sparse biases smaller ones."""
+    s = make(B, 150001, 8192, K=K, token=torch.int32)
+    check_logits(cuda_device, s["x"], tokens=s["tokens"], lengths=s["lengths"], rho=1.3, frequency=0.125, ids=s["ids"],
+                 values=s["values"] * 2.0 ** -6)
+
+
 @pytest.mark.parametrize("B", [1, 40, 700])
 @pytest.mark.parametrize("V", [1023, 1024, 1025, 2049, 4095, 4096, 4097, 9000])
 def test_vocabularies_around_a_chunk(cuda_device, B, V):
