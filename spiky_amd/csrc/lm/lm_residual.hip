@@ -446,12 +446,12 @@ enum { kSumW1, kSumB1, kSumW2, kSumB2, kSumG };
 
 // What a thread has of one piece of N columns on the way back: parameters, the
 // loads of the next row, and what the row's sums are awaited with.  FULL: with
-// layer norms or biases.
-template <typename TZ, typename TA, int N, bool FULL, bool SHORT>
+// layer norms or biases.  LEAN: w2 and b1 are read again for every row.
+template <typename TZ, typename TA, int N, bool FULL, bool SHORT, bool LEAN = false>
 struct Piece {
     static constexpr int K = FULL ? 8 : 3;
     Place<N> at;
-    float w1[N], w2[N], b1[FULL ? N : 1], g[N];
+    float w1[N], w2[LEAN ? 1 : N], b1[FULL && !LEAN ? N : 1], g[N];
     Raw<TZ, N> z_raw, dz_raw;
     Raw<TA, N> a_raw, dh_raw;
     Raw<float, N> g_raw;  // half of the words where the gate is of a shorter type
@@ -464,24 +464,25 @@ struct Piece {
         z_raw.clear(), dz_raw.clear(), a_raw.clear(), dh_raw.clear(), g_raw.clear();
     }
     template <typename J>
-    __device__ __forceinline__ void parameters(const J &j) {
-        auto values = [&](auto &v, const void *p) {
+    __device__ __forceinline__ void parameter(float (&v)[N], const J &j, const void *p, bool there, float absent) const {
+        if (there) {
             Raw<float, N> raw;
             raw.clear();
             words_of<TA, SHORT>(raw, p, j.par_f32, at.col, at.n);
             values_of<TA>(v, raw, j.par_f32);
-        };
-        if (j.has & kW1) values(w1, j.w1);
-        if (j.has & kW2) values(w2, j.w2);
-        if constexpr (FULL)
-            if (j.has & kB1) values(b1, j.b1);
+        } else {
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-            if (!(j.has & kW1)) w1[i] = 1.f;
-            if (!(j.has & kW2)) w2[i] = 1.f;
-            if (FULL && !(j.has & kB1)) b1[FULL ? i : 0] = 0.f;
-            if (!(j.has & kGate)) g[i] = 1.f;
+            for (int i = 0; i < N; i++) v[i] = absent;
         }
+    }
+    template <typename J>
+    __device__ __forceinline__ void parameters(const J &j) {
+        parameter(w1, j, j.w1, j.has & kW1, 1.f);
+        if constexpr (!LEAN) parameter(w2, j, j.w2, j.has & kW2, 1.f);
+        if constexpr (FULL && !LEAN) parameter(b1, j, j.b1, j.has & kB1, 0.f);
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            if (!(j.has & kGate)) g[i] = 1.f;
     }
     template <typename J>
     __device__ __forceinline__ void load_gate(const J &j, uint32_t gate_row) {
@@ -503,10 +504,30 @@ struct Piece {
         if (row_gates) load_gate(j, row);
     }
     // v of the forward pass, and then d: a dropped element is 0 whatever it holds.
-    __device__ __forceinline__ float dropped(const Dropper &dr, int i) const {
+    __device__ __forceinline__ float dropped(const Dropper &dr, int i, const float (&b)[N]) const {
         float v = n1[i] * w1[i];
-        if (FULL) v += b1[FULL ? i : 0];
+        if (FULL) v += b[i];
         return where(keep, i, v * dr.scale);
+    }
+    // The post norm's bias, and the pre norm's weight, as the row's sums want them.
+    template <typename J>
+    __device__ __forceinline__ void bias_of(float (&v)[N], const J &j, uint32_t has) const {
+        if constexpr (!FULL) return;
+        if constexpr (LEAN) {
+            parameter(v, j, j.b1, has & kB1, 0.f);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i++) v[i] = b1[FULL && !LEAN ? i : 0];
+        }
+    }
+    template <typename J>
+    __device__ __forceinline__ void weight_of(float (&v)[N], const J &j, uint32_t has) const {
+        if constexpr (LEAN) {
+            parameter(v, j, j.w2, has & kW2, 1.f);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i++) v[i] = w2[LEAN ? 0 : i];
+        }
     }
     // The row's values from its loads, and the piece's share of the row's sums s;
     // add(k, v) adds v to the column sums k.
@@ -515,7 +536,9 @@ struct Piece {
                                             float (&s)[K], F &&add) {
         const uint32_t has = here(j.has);
         const float r2 = has & kDh ? st.w : 0.f;
-        float dw2[N], db2[FULL ? N : 1];
+        float dw2[N], db2[FULL ? N : 1], b[N], w[N];
+        bias_of(b, j, has);
+        weight_of(w, j, has);
         const float kept_scale = dr.scale * j.beta;
         keep = has & kDrops ? kept<N>(dr, row, at.col) : ~0u;
         const uint32_t counts = keep & at.own;
@@ -523,9 +546,9 @@ struct Piece {
         for (int i = 0; i < N; i++) {
             n1[i] = (a_raw[i] - st.x) * st.y;
             float z = z_raw[i];
-            if (has & kBranch) z = j.alpha * z + j.beta * (g[i] * dropped(dr, i));
+            if (has & kBranch) z = j.alpha * z + j.beta * (g[i] * dropped(dr, i, b));
             n2[i] = has & kDh ? (z - st.z) * r2 : 0.f;
-            const float dh = dh_raw[i], t = dh * w2[i];
+            const float dh = dh_raw[i], t = dh * w[i];
             e[i] = dz_raw[i] + r2 * t;
             dw2[i] = dh * n2[i];
             const float c = where(counts, i, kept_scale * g[i] * w1[i]), own_t = where(at.own, i, t);
@@ -554,12 +577,13 @@ struct Piece {
         const float kept_scale = dr.scale * j.beta;
         const float r2 = has & kDh ? st.w : 0.f, alpha = has & kBranch ? j.alpha : 1.f;
         const uint64_t to = (uint64_t)row * j.cols + at.col;
-        float out[N], da[N], dg[N], dw1[N], db1[N];
+        float out[N], da[N], dg[N], dw1[N], db1[N], b[N];
+        bias_of(b, j, has);
 #pragma unroll
         for (int i = 0; i < N; i++) {
             const float q = e[i] - r2 * (m.x + n2[i] * m.y);
             out[i] = alpha * q;
-            dg[i] = j.beta * (dropped(dr, i) * q);
+            dg[i] = j.beta * (dropped(dr, i, b) * q);
             db1[i] = where(keep, i, kept_scale * (g[i] * q));
             dw1[i] = db1[i] * n1[i];
             da[i] = db1[i];
@@ -615,7 +639,8 @@ __device__ __forceinline__ float4 row_means(const J &j, const float4 &st, const 
 // 640 fp32 with layer norms 234 -> 161 us).  The next row's loads are issued before
 // the reduction, into the registers that this row's left.  Above 4096 columns 512
 // threads have 16 columns each: 1024 of 8 may use 128 registers, and spill (8192
-// rows of 8192: 370 us against 255; with layer norms 445 and 410).
+// rows of 8192: 370 us against 255).  With layer norms these would still spill (410
+// us), and read w2 and b1 again for every row instead (341).
 template <typename TZ, typename TA, int N, int P, int TPR, bool FULL>
 __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_join_back(Join<TZ, TA> j) {
     constexpr int kThreads = TPR <= 64 ? 256 : TPR, kSlots = TPR <= 64 ? 256 / TPR : 1;
@@ -641,7 +666,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_join_back(Join<TZ, TA
 
     auto slot_of = [](int k) { return k == kSumW1 ? 0 : k == kSumW2 ? 1 : k == kSumG ? 2 : 3; };
     float acc_b2[P][N];
-    Piece<TZ, TA, N, FULL, false> x[P];
+    Piece<TZ, TA, N, FULL, false, FULL && (N * P > 8)> x[P];
     float4 st = {0.f, 1.f, 0.f, 1.f};
 #pragma unroll
     for (int p = 0; p < P; p++) {
