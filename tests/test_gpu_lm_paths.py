@@ -231,6 +231,16 @@ def test_logits_in_place_are_seen_by_autograd(cuda_device):
     assert not process_logits(leaf).requires_grad
 
 
+def test_inference_mode(cuda_device):
+    x, w = torch.randn(6, 96, device=cuda_device, requires_grad=True), torch.ones(96, device=cuda_device, requires_grad=True)
+    want = [counter_dropout(x, 0.5, 1), *residual_norm(x, x, pre_norm="rms", pre_weight=w), process_logits(x, temperature=2.0)]
+    with torch.inference_mode():
+        got = [counter_dropout(x, 0.5, 1), *residual_norm(x, x, pre_norm="rms", pre_weight=w)]
+        y = x.clone()
+        got.append(process_logits(y, out=y, temperature=2.0))
+    assert all(torch.equal(a, b) for a, b in zip(want, got)) and not any(t.requires_grad for t in got)
+
+
 def test_steps_leave_nothing_behind(cuda_device):
     x = torch.randn(64, 256, device=cuda_device, requires_grad=True)
     w = torch.ones(256, device=cuda_device, requires_grad=True)
