@@ -212,11 +212,12 @@ struct Sparse {
 // order in which they are waited for: tokens, sparse biases, logits, bias, mask; in chunks of
 // another size the last three by the piece, after the counts.
 //
-// 512 rows of 152000 bf16 logits to fp32: 78 us without more (6.0 TB/s); 4096 tokens a row add
-// 17, a shared bias 13, a mask 2 and 64 sparse biases 3, all of them together 50, where the
-// waves wait for each other's phases and for L2, which reads a row's tokens for each of its
-// chunks.  256 threads are faster than 512 and 1024 there (all together, in an earlier form:
-// 166, 198, 242), for barriers hold fewer waves; 8 pieces a thread no faster than 4 (144, 141).
+// 512 rows of 152000 bf16 logits to fp32, inputs not in the caches: 76 us without more (6.1
+// TB/s); 4096 tokens a row add 14, a shared bias 15, a mask 2 and 64 sparse biases 5, all of
+// them together 58, where the waves wait for each other's phases and for L2, which reads a
+// row's tokens for each of its chunks.  256 threads are faster than 512 and 1024 there (all
+// together, in an earlier form: 166, 198, 242), for barriers hold fewer waves; 8 pieces a
+// thread no faster than 4 (144, 141).
 template <typename TI, typename TO, int N, int P, uint32_t kThreads>
 __global__ __launch_bounds__(kThreads, kThreads == 256 ? 7 : 1) void k_logits(spiky_lm_logits_args a, uint32_t chunk) {
     // words where there are tokens or bias ids; with bias ids as many sums as may be needed, and slots
@@ -225,7 +226,17 @@ __global__ __launch_bounds__(kThreads, kThreads == 256 ? 7 : 1) void k_logits(sp
     uint32_t *const words = reinterpret_cast<uint32_t *>(space);
     float *const sums = reinterpret_cast<float *>(words + chunk);
     uint16_t *const slots = reinterpret_cast<uint16_t *>(sums + min((uint64_t)chunk, a.n_bias));
-    const uint32_t tid = threadIdx.x, row = blockIdx.y, base = blockIdx.x * chunk;
+    // Workgroups go round the 8 XCDs in their order: the chunks of a row, which read the same
+    // tokens, to one of them, as far as rows come in eights (512 rows of 152000 with 4096 tokens,
+    // nothing else set: 90 us against 95).  A chunk of all rows before the next one would share
+    // the bias, but reads the logits in too many places at once (all set: 143 against 134).
+    uint32_t row = blockIdx.y, number = blockIdx.x;
+    if (row < (gridDim.y & ~7u)) {
+        const uint32_t at = blockIdx.y * gridDim.x + blockIdx.x, step = at / 8;
+        row = step / gridDim.x * 8 + at % 8;
+        number = step % gridDim.x;
+    }
+    const uint32_t tid = threadIdx.x, base = number * chunk;
     const uint32_t size = min(chunk, (uint32_t)a.vocab - base);
     const bool marks = a.tokens || a.bias_ids;
     const TI *in = static_cast<const TI *>(a.logits) + (int64_t)row * a.logits_stride + base;
