@@ -9,6 +9,7 @@
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
@@ -146,6 +147,24 @@ struct OnDevice {
     explicit OnDevice(c10::Device d) : guard(d), stream(c10::hip::getCurrentHIPStream(d.index()).stream()) {}
 };
 
+// Gradients in a capture cannot go to a node that was recorded on the default stream
+// (a leaf's, kept alive by an eager graph): autograd would make that stream wait for
+// the captured one, which ends the process.  So the backward call raises first.
+void check_capture(const Node &node, c10::Device device) {
+    const c10::Stream standard = c10::hip::getDefaultHIPStream(device.index()).unwrap();
+    if (c10::hip::getCurrentHIPStream(device.index()).unwrap() == standard) return;  // which is never captured
+    bool stands = false;
+    for (size_t i = 0; i < node.num_outputs(); i++) {
+        if (!node.task_should_compute_output(i)) continue;
+        const auto stream = node.next_edge(i).function->stream();
+        stands = stands || (stream && stream->id() == standard.id() && stream->device_index() == device.index());
+    }
+    if (!stands) return;
+    TORCH_CHECK(c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None,
+                "a gradient belongs to the default stream, which a captured backward pass cannot reach: drop eager "
+                "graphs of the same leaves before the capture, or run them on a side stream");
+}
+
 bool needs_grad(const Tensor &t) { return t.defined() && t.requires_grad(); }
 
 // Gradients of the gradients are not computed: a backward pass through these raises.
@@ -183,6 +202,7 @@ struct CounterDropoutBackward : Node {
 
     variable_list apply(variable_list &&grads) override {
         if (!grads[0].defined()) return {Tensor()};
+        check_capture(*this, grads[0].device());
         at::AutoGradMode off(false);
         const Tensor s = has_state ? state.unpack() : Tensor();
         Tensor dx = apply_dropout(grads[0], p, seed, offset, s);
@@ -301,6 +321,7 @@ struct ResidualNormBackward : Node {
             if (has[i]) in[i] = saved[i].unpack();
         const Tensor rng = has_state ? state.unpack() : Tensor();
         TORCH_CHECK(stats.defined(), torch::autograd::ERR_BACKWARD_TWICE);
+        check_capture(*this, in[kRes].device());
         OnDevice on(in[kRes].device());
         Tensor res, branch;
         const spiky_lm_residual_args a = join_args(how, in, rng, stats, res, branch);

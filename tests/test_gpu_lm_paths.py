@@ -231,6 +231,33 @@ def test_logits_in_place_are_seen_by_autograd(cuda_device):
     assert not process_logits(leaf).requires_grad
 
 
+def test_a_capture_beside_an_eager_graph_of_the_same_leaves_is_refused(cuda_device):
+    """The eager graph's leaves belong to the default stream; without it the capture is made."""
+    w = torch.ones(64, device=cuda_device, requires_grad=True)
+    x, dy = torch.randn(4, 64, device=cuda_device), torch.randn(4, 64, device=cuda_device)
+    calls = (lambda: residual_norm(x, pre_norm="rms", pre_weight=w)[1], lambda: counter_dropout(w, 0.5, 1))
+    for call in calls:
+        call()
+        eager = call()
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="belongs to the default stream"):
+            with torch.cuda.graph(graph):
+                y = call()  # forward alone may be captured
+                torch.autograd.grad(y, w, dy[:y.shape[0]] if y.dim() == 2 else dy[0])
+        del eager, graph, y
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = call()
+            (dw,) = torch.autograd.grad(y, w, dy[:y.shape[0]] if y.dim() == 2 else dy[0])
+        for _ in range(3):
+            x.normal_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y.detach(), call().detach())
+        del y, dw
+
+
 def test_inference_mode(cuda_device):
     x, w = torch.randn(6, 96, device=cuda_device, requires_grad=True), torch.ones(96, device=cuda_device, requires_grad=True)
     want = [counter_dropout(x, 0.5, 1), *residual_norm(x, x, pre_norm="rms", pre_weight=w), process_logits(x, temperature=2.0)]
