@@ -201,7 +201,7 @@ class LUTTransformer(nn.Module):
         """Sequences [B, L + n_new] that continue tokens [B, L], of which a row's first `lengths`
         are its prompt (all, without); a row's new tokens follow its prompt, zeros the last of
         them.  Each new token is drawn from the softmax of the last position's logits after
-        process_logits with `processing` (penalties, biases, temperature, mask); with temperature
+        process_logits with `processing` (penalties, biases, temperature, mask); in rows of temperature
         0 or less it is the largest.  A step reads the last context_size tokens, each row from its
         own start.  generator: of torch, for the draws."""
         B, L = tokens.shape
@@ -212,8 +212,7 @@ class LUTTransformer(nn.Module):
         if L == 0 or int(prompt.min()) < 1 or int(prompt.max()) > L:
             raise ValueError("a prompt has 1 to L tokens")
         out = out.masked_fill(torch.arange(L + n_new, device=device) >= prompt[:, None], 0)
-        greedy = not isinstance(processing.get("temperature", 1.0), torch.Tensor) and \
-            processing.get("temperature", 1.0) <= 0.0
+        cold = processing.get("temperature", 1.0) <= 0.0  # a truth value, or one for each row
         rows, ahead = torch.arange(B, device=device), torch.arange(S, device=device)
         was_training = self.training
         self.eval()
@@ -224,10 +223,13 @@ class LUTTransformer(nn.Module):
                 at = (start[:, None] + ahead).clamp_max(L + n_new - 1)
                 logits = self(out.gather(1, at))[rows, length - start - 1]
                 logits = process_logits(logits, tokens=out, lengths=length, prompt_lengths=prompt, **processing)
-                if greedy:
-                    new = logits.argmax(-1)
-                else:
+                each = isinstance(cold, torch.Tensor)
+                if each or not cold:
                     new = torch.multinomial(logits.softmax(-1), 1, generator=generator)[:, 0]
+                if each:
+                    new = torch.where(cold, logits.argmax(-1), new)
+                elif cold:
+                    new = logits.argmax(-1)
                 out[rows, length] = new.to(out.dtype)
         finally:
             self.train(was_training)

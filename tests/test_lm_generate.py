@@ -1,0 +1,65 @@
+"""LUTTransformer.generate on the CPU: a table of logits for the layers, plain torch for process_logits."""
+import math
+import sys
+
+import numpy as np
+import pytest
+import torch
+
+from spiky_amd import LUTTransformer
+
+VOCAB, CONTEXT = 7, 4
+
+
+class Table(LUTTransformer):
+    """The logits of a position are its token's row of a table."""
+
+    def __init__(self, table):
+        torch.nn.Module.__init__(self)
+        self.context_size = CONTEXT
+        self.table = torch.nn.Parameter(table)
+
+    def forward(self, tokens):
+        return self.table[tokens.long()]
+
+
+def plain(logits, *, tokens=None, lengths=None, prompt_lengths=None, temperature=1.0, mask=None):
+    """process_logits with a temperature and a mask alone."""
+    t = torch.as_tensor(temperature, dtype=logits.dtype).reshape(-1, 1)
+    x = torch.where(t > 0, logits / torch.where(t > 0, t, 1.0), logits)
+    return x if mask is None else torch.where(mask, x, -math.inf)
+
+
+@pytest.fixture
+def model(monkeypatch):
+    monkeypatch.setattr(sys.modules[LUTTransformer.__module__], "process_logits", plain)
+    # flat rows, in which a draw seldom meets the largest, and each token's largest another one
+    return Table(torch.eye(VOCAB)[(torch.arange(VOCAB) * 3 + 1) % VOCAB] * 0.1)
+
+
+def greedy(model, tokens, n_new):
+    out = tokens.tolist()
+    for row in out:
+        for _ in range(n_new):
+            row.append(int(model.table[row[-1]].argmax()))
+    return torch.tensor(out)
+
+
+def test_each_row_has_its_own_temperature(model):
+    """Rows of temperature 0 or less get the largest whatever the other rows do, and those are drawn."""
+    prompt = torch.tensor([[1, 2], [3, 4], [5, 6], [0, 1]])
+    want = greedy(model, prompt, 20)
+    temperature = torch.tensor([0.0, 1.0, -1.0, 1.0])
+    out = model.generate(prompt, 20, generator=torch.Generator().manual_seed(0), temperature=temperature)
+    assert torch.equal(out[[0, 2]], want[[0, 2]])
+    assert not torch.equal(out[1], want[1]) and not torch.equal(out[3], want[3])
+    for cold in (torch.zeros(4), 0.0, np.float32(0.0)):
+        assert torch.equal(model.generate(prompt, 20, temperature=cold), want)
+
+
+def test_rows_without_a_temperature_of_their_own_are_drawn_as_ever(model):
+    """A tensor of one temperature draws what the number draws."""
+    prompt = torch.tensor([[1, 2], [3, 4]])
+    one, each = (model.generate(prompt, 9, generator=torch.Generator().manual_seed(4), temperature=t)
+                 for t in (0.5, torch.full((2,), 0.5)))
+    assert torch.equal(one, each)
