@@ -14,6 +14,8 @@ With `residual_join` the two joins of a block are `ResidualNorm`s (this build's 
 the branch is normed, dropped out and gated, added to the residual stream, and the next layer
 reads the stream's norm.  `generate` continues byte or token sequences with `process_logits`.
 """
+import math
+
 import torch
 import torch.nn as nn
 
@@ -203,7 +205,8 @@ class LUTTransformer(nn.Module):
         them.  Each new token is drawn from the softmax of the last position's logits after
         process_logits with `processing` (penalties, biases, temperature, mask); in rows of temperature
         0 or less it is the largest.  A step reads the last context_size tokens, each row from its
-        own start.  generator: of torch, for the draws."""
+        own start.  Raises where a step leaves a row nothing to choose from.  generator: of torch,
+        for the draws."""
         B, L = tokens.shape
         S, device = self.context_size, tokens.device
         out = torch.cat([tokens, tokens.new_zeros(B, n_new)], 1)
@@ -214,6 +217,7 @@ class LUTTransformer(nn.Module):
         out = out.masked_fill(torch.arange(L + n_new, device=device) >= prompt[:, None], 0)
         cold = processing.get("temperature", 1.0) <= 0.0  # a truth value, or one for each row
         rows, ahead = torch.arange(B, device=device), torch.arange(S, device=device)
+        stuck = torch.zeros(B, dtype=torch.bool, device=device)
         was_training = self.training
         self.eval()
         try:
@@ -224,15 +228,25 @@ class LUTTransformer(nn.Module):
                 logits = self(out.gather(1, at))[rows, length - start - 1]
                 logits = process_logits(logits, tokens=out, lengths=length, prompt_lengths=prompt, **processing)
                 each = isinstance(cold, torch.Tensor)
+                none = ~(logits.amax(-1) > -math.inf)
                 if each or not cold:
-                    new = torch.multinomial(logits.softmax(-1), 1, generator=generator)[:, 0]
+                    p = logits.softmax(-1)
+                    if each:
+                        none |= ~cold & p[:, 0].isnan()
+                    else:
+                        none |= p[:, 0].isnan()
+                    # NaN in a row's largest or sum is in all of p: a draw from that would end the process
+                    new = torch.multinomial(p.nan_to_num(nan=1.0), 1, generator=generator)[:, 0]
                 if each:
                     new = torch.where(cold, logits.argmax(-1), new)
                 elif cold:
                     new = logits.argmax(-1)
                 out[rows, length] = new.to(out.dtype)
+                stuck |= none
         finally:
             self.train(was_training)
+        if bool(stuck.any()):
+            raise ValueError("no token to choose: the mask leaves nothing of a row, or its logits are NaN or infinite")
         return out
 
     def to(self, *args, **kwargs):

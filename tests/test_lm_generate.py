@@ -63,3 +63,28 @@ def test_rows_without_a_temperature_of_their_own_are_drawn_as_ever(model):
     one, each = (model.generate(prompt, 9, generator=torch.Generator().manual_seed(4), temperature=t)
                  for t in (0.5, torch.full((2,), 0.5)))
     assert torch.equal(one, each)
+
+
+@pytest.mark.parametrize("temperature", [1.0, 0.0, torch.tensor([1.0, 0.0, 0.7])])
+def test_a_row_without_a_token_to_choose_raises(model, temperature, monkeypatch):
+    """A mask that leaves nothing, and NaN: raised by the host, with no draw from what is no distribution."""
+    draw, prompt = torch.multinomial, torch.tensor([[1, 2], [3, 4], [5, 6]])
+    drawn = []
+
+    def checked(p, *args, **kw):
+        drawn.append(bool(torch.isfinite(p).all() and (p.sum(-1) > 0).all()))
+        return draw(p, *args, **kw)
+
+    monkeypatch.setattr(torch, "multinomial", checked)
+    for row in range(3):
+        mask = torch.ones(3, VOCAB, dtype=torch.bool)
+        mask[row] = False
+        with pytest.raises(ValueError, match="no token"):
+            model.generate(prompt, 3, temperature=temperature, mask=mask)
+        mask[row, 2] = True
+        assert model.generate(prompt, 3, temperature=temperature, mask=mask)[row, 2:].tolist() == [2, 2, 2]
+    with torch.no_grad():
+        model.table[4, 1] = math.nan
+    with pytest.raises(ValueError, match="no token"):
+        model.generate(prompt, 3, temperature=temperature)
+    assert all(drawn)
