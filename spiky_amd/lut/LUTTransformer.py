@@ -218,7 +218,7 @@ class LUTTransformer(nn.Module):
         cold = processing.get("temperature", 1.0) <= 0.0  # a truth value, or one for each row
         rows, ahead = torch.arange(B, device=device), torch.arange(S, device=device)
         stuck = torch.zeros(B, dtype=torch.bool, device=device)
-        was_training = self.training
+        training = [m for m in self.modules() if m.training]
         self.eval()
         try:
             for i in range(n_new):
@@ -244,7 +244,8 @@ class LUTTransformer(nn.Module):
                 out[rows, length] = new.to(out.dtype)
                 stuck |= none
         finally:
-            self.train(was_training)
+            for m in training:  # not train(), which takes along modules held in evaluation
+                m.training = True
         if bool(stuck.any()):
             raise ValueError("no token to choose: the mask leaves nothing of a row, or its logits are NaN or infinite")
         return out

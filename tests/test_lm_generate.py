@@ -88,3 +88,16 @@ def test_a_row_without_a_token_to_choose_raises(model, temperature, monkeypatch)
     with pytest.raises(ValueError, match="no token"):
         model.generate(prompt, 3, temperature=temperature)
     assert all(drawn)
+
+
+def test_submodules_keep_their_mode(model):
+    """What was held in evaluation stays there."""
+    model.frozen, model.other = torch.nn.Dropout(0.5).eval(), torch.nn.Dropout(0.5)
+    for training in (True, False):
+        model.training = training
+        model.generate(torch.tensor([[1, 2]]), 2)
+        assert model.training is training and not model.frozen.training and model.other.training
+    modes = []
+    model.register_forward_pre_hook(lambda m, _: modes.extend(x.training for x in m.modules()))
+    model.generate(torch.tensor([[1, 2]]), 2)
+    assert modes and not any(modes)
