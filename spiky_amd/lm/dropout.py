@@ -2,7 +2,7 @@
 import torch
 
 from .. import _native
-from .common import check_probability
+from .common import CountedMasks, check_probability
 
 
 def counter_dropout(x, p, seed, offset=0):
@@ -20,30 +20,23 @@ def counter_dropout(x, p, seed, offset=0):
     return _native.lm().dropout(x, p, seed, offset)
 
 
-class CounterDropout(torch.nn.Module):
+class CounterDropout(CountedMasks, torch.nn.Module):
     """nn.Dropout over counter_dropout: call number n of a module in training uses offset n.
 
     Modules of one model take different seeds.  The calls' number is part of the state dict, so a
-    resumed run goes on with masks that it has not used."""
+    resumed run goes on with masks that it has not used.  Inside a backward pass (recomputed by
+    torch.utils.checkpoint) a call raises, unless the model has mask_counters."""
 
     def __init__(self, p=0.5, seed=0):
         super().__init__()
         check_probability(p)
         self.p = float(p)
-        self.seed = int(seed)
-        self.calls = 0
-
-    def get_extra_state(self):
-        return {"seed": self.seed, "calls": self.calls}
-
-    def set_extra_state(self, state):
-        self.seed, self.calls = int(state["seed"]), int(state["calls"])
+        self.count_masks(seed)
 
     def forward(self, x):
         if not self.training or self.p == 0.0:
             return x
-        self.calls += 1
-        return counter_dropout(x, self.p, self.seed, self.calls)
+        return counter_dropout(x, self.p, *self.next_mask())
 
     def extra_repr(self):
         return f"p={self.p}, seed={self.seed}"

@@ -3,7 +3,7 @@ norm before the next block, in one pass over the rows."""
 import torch
 
 from .. import _native
-from .common import check_probability
+from .common import CountedMasks, check_probability
 
 _NORMS = (None, "rms", "layer")
 
@@ -34,7 +34,7 @@ def residual_norm(residual, branch=None, *, post_norm=None, post_weight=None, po
                                       dtype)
 
 
-class ResidualNorm(torch.nn.Module):
+class ResidualNorm(CountedMasks, torch.nn.Module):
     """The residual join of one block, with its parameters.
 
     post_norm, pre_norm: None, "rms" or "layer" over `dim` features, each with a weight (from 1)
@@ -51,7 +51,8 @@ class ResidualNorm(torch.nn.Module):
                 raise ValueError(f"a norm must be None, 'rms' or 'layer', got {norm!r}")
         self.dim, self.post_norm, self.pre_norm = dim, post_norm, pre_norm
         self.residual_scale, self.branch_scale, self.eps = residual_scale, branch_scale, eps
-        self.dropout_p, self.seed, self.calls = float(dropout_p), int(seed), 0
+        self.dropout_p = float(dropout_p)
+        self.count_masks(seed)
 
         def parameter(there, value):
             if not there:
@@ -64,20 +65,13 @@ class ResidualNorm(torch.nn.Module):
         self.pre_weight = parameter(pre_norm, 1.0)
         self.pre_bias = parameter(pre_norm and bias, 0.0)
 
-    def get_extra_state(self):
-        return {"seed": self.seed, "calls": self.calls}
-
-    def set_extra_state(self, state):
-        self.seed, self.calls = int(state["seed"]), int(state["calls"])
-
     def forward(self, residual, branch):
         p = self.dropout_p if self.training else 0.0
-        if p:
-            self.calls += 1
+        seed, offset = self.next_mask() if p else (0, 0)
         return residual_norm(residual, branch, post_norm=self.post_norm, post_weight=self.post_weight,
                              post_bias=self.post_bias, post_eps=self.eps, gate=self.gate,
                              residual_scale=self.residual_scale, branch_scale=self.branch_scale, dropout_p=p,
-                             seed=self.seed, offset=self.calls, pre_norm=self.pre_norm,
+                             seed=seed, offset=offset, pre_norm=self.pre_norm,
                              pre_weight=self.pre_weight, pre_bias=self.pre_bias, pre_eps=self.eps)
 
     def extra_repr(self):
