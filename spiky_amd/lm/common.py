@@ -42,14 +42,17 @@ class CountedMasks:
         seed = (int(state["seed"]) + (1 << 63)) % (1 << 64) - (1 << 63)
         return torch.tensor([seed, int(state["calls"]) + 1], dtype=torch.int64)
 
-    def next_mask(self):
-        """(seed, offset) of a call in training."""
+    def next_mask(self, x):
+        """(seed, offset) of a call in training on x."""
         if self.counter is not None:
             return self.counter, 0
         if torch._C._current_graph_task_id() != -1:
             # a recomputed forward pass (torch.utils.checkpoint): counted again, its mask would be another one
             raise RuntimeError("dropout inside a backward pass cannot tell which call it repeats: give the model "
                                "counters with spiky_amd.mask_counters, or pass seed and offset to the functions")
+        if x.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the number of a captured dropout would be the same in every replay: give the model "
+                               "counters with spiky_amd.mask_counters, or pass a seed tensor to the functions")
         self.calls += 1
         return self.seed, self.calls
 
@@ -59,8 +62,9 @@ def mask_counters(model, device):
     and ResidualNorm of `model`, in the order of its modules, and takes the place of their own counts.
 
     The modules read it when their kernels run, so a recomputed forward pass (torch.utils.checkpoint) has
-    the masks of the first one.  The program advances it after each step's backward pass, with
-    `counters[:, 1] += 1`; until then every call of a module has the same mask.  State dicts save and load it."""
+    the masks of the first one, and each replay of a captured step its own.  The program advances it after
+    each step's backward pass, in the capture or between replays, with `counters[:, 1] += 1`; until then
+    every call of a module has the same mask.  State dicts save and load it, in place."""
     modules = [m for m in model.modules() if isinstance(m, CountedMasks)]
     rows = [m.next_count(m.get_extra_state()) for m in modules]
     counters = torch.stack(rows) if rows else torch.zeros(0, 2, dtype=torch.int64)

@@ -25,7 +25,8 @@ class CounterDropout(CountedMasks, torch.nn.Module):
 
     Modules of one model take different seeds.  The calls' number is part of the state dict, so a
     resumed run goes on with masks that it has not used.  Inside a backward pass (recomputed by
-    torch.utils.checkpoint) a call raises, unless the model has mask_counters."""
+    torch.utils.checkpoint) and in a captured graph a call raises, unless the model has
+    mask_counters."""
 
     def __init__(self, p=0.5, seed=0):
         super().__init__()
@@ -36,7 +37,7 @@ class CounterDropout(CountedMasks, torch.nn.Module):
     def forward(self, x):
         if not self.training or self.p == 0.0:
             return x
-        return counter_dropout(x, self.p, *self.next_mask())
+        return counter_dropout(x, self.p, *self.next_mask(x))
 
     def extra_repr(self):
         return f"p={self.p}, seed={self.seed}"

@@ -67,7 +67,7 @@ class ResidualNorm(CountedMasks, torch.nn.Module):
 
     def forward(self, residual, branch):
         p = self.dropout_p if self.training else 0.0
-        seed, offset = self.next_mask() if p else (0, 0)
+        seed, offset = self.next_mask(residual) if p else (0, 0)
         return residual_norm(residual, branch, post_norm=self.post_norm, post_weight=self.post_weight,
                              post_bias=self.post_bias, post_eps=self.eps, gate=self.gate,
                              residual_scale=self.residual_scale, branch_scale=self.branch_scale, dropout_p=p,

@@ -1,4 +1,4 @@
-"""The masks of CounterDropout and ResidualNorm in recomputed steps, on the CPU: plain operators in the
+"""The masks of CounterDropout and ResidualNorm in recomputed and captured steps, on the CPU: plain operators in the
 place of the library's."""
 import copy
 import sys
@@ -94,3 +94,25 @@ def test_counters_and_numbers_are_one_state():
     assert twin.drop.counter is None and twin.drop.calls == 2 and counted.drop.counter is not None
     assert torch.equal(spiky_amd.mask_counters(counted, "cpu"), counters)
     assert spiky_amd.mask_counters(torch.nn.Linear(2, 2), "cpu").shape == (0, 2)
+
+
+def test_a_captured_call_that_is_counted_raises(monkeypatch):
+    """Its number would be part of the graph: every replay would drop the same elements."""
+    class Captured(torch.Tensor):
+        is_cuda = True
+
+    x, capturing = torch.randn(4, 16).as_subclass(Captured), [True]
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    drop, join = CounterDropout(0.5), ResidualNorm(16, dropout_p=0.5)
+    calls = (lambda: drop(x), lambda: join(x, x))
+    for call in calls:
+        with pytest.raises(RuntimeError, match="mask_counters"):
+            call()
+    assert (drop.calls, join.calls) == (0, 0)
+    spiky_amd.mask_counters(drop, "cpu"), spiky_amd.mask_counters(join, "cpu")
+    for call in calls:
+        call()
+    capturing[0] = False
+    CounterDropout(0.5)(x)
+    capturing[0] = True
+    join.eval()(x, x), drop.eval()(x)
