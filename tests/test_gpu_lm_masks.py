@@ -46,6 +46,15 @@ def test_a_counted_recomputation_raises(cuda_device, reentrant):
         y.sum().backward()
 
 
+def filled(model):
+    """The model with tables of normal values: they start as zeros, and the logits with them."""
+    gen = torch.Generator(model.device).manual_seed(6)
+    with torch.no_grad():
+        for layer in model._lut_layers():
+            layer._weights.normal_(0.0, 0.5, generator=gen)
+    return model
+
+
 def check_model_step(got, want):
     """The logits bit for bit.  Gradients pass four layers, whose fp32 atomics come in any order: sums of
     some thousand terms, each off by half a step of 2^-24 of the sum of magnitudes, taken as at most
@@ -60,7 +69,7 @@ def test_a_recomputed_model_is_the_whole_one(cuda_device):
     join = dict(post_norm="rms", pre_norm="rms", gate=0.5)
     results = []
     for recomputed in (False, True):
-        m = small(cuda_device, dropout=0.2, residual_join=join)
+        m = filled(small(cuda_device, dropout=0.2, residual_join=join))
         if recomputed:
             mask_counters(m, cuda_device)
         y = checkpoint(m, tokens, use_reentrant=False) if recomputed else m(tokens)
@@ -138,7 +147,7 @@ def test_a_counted_call_in_a_capture_raises(cuda_device):
 def test_replays_of_a_captured_model_have_the_eager_models_masks(cuda_device):
     tokens = torch.randint(0, 50, (4, 8), device=cuda_device)
     how = dict(dropout=0.2, residual_join=dict(post_norm="rms", pre_norm="rms", gate=0.5))
-    eager, m = small(cuda_device, **how), small(cuda_device, **how)
+    eager, m = filled(small(cuda_device, **how)), filled(small(cuda_device, **how))
     counters = mask_counters(m, cuda_device)
     start = counters.clone()
 
