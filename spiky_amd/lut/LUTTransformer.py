@@ -32,8 +32,9 @@ class LUTTransformer(nn.Module):
 
     residual_join: None for the reference's z + dropout(branch), or a dict of ResidualNorm's
     options (post_norm, pre_norm, bias, gate, residual_scale, branch_scale, eps) for both joins
-    of every block; their dropout is `dropout`, from counters seeded by `seed` and the join's
-    number.  It excludes use_batch_norm."""
+    of every block; their dropout is `dropout`, from counters seeded by `dropout_seed` (without it
+    `seed`) and the join's number: data-parallel ranks have one `seed`, for equal weights, and
+    each a `dropout_seed`.  It excludes use_batch_norm."""
 
     def __init__(self, vocab_size, embedding_dim, context_size, positional_dim, num_layers, num_heads,
                  n_detectors, n_anchors_per_detector, n_anchors_per_detector_attention=None,
@@ -41,7 +42,8 @@ class LUTTransformer(nn.Module):
                  do_normalise_weights=False, weights_gradient_policy: GradientPolicy = None,
                  device=None, synapse_meta=SynapseMeta(), lut_shared_context=None, seed=None,
                  summation_dtype=torch.float32, _int_rescaler=0.001, _forward_group_size=32,
-                 _backward_group_size=32, dropout=0.0, use_batch_norm=False, residual_join=None):
+                 _backward_group_size=32, dropout=0.0, use_batch_norm=False, residual_join=None,
+                 dropout_seed=None):
         super().__init__()
         if isinstance(embedding_dim, int):
             n_embeddings = embedding_dim
@@ -115,9 +117,8 @@ class LUTTransformer(nn.Module):
                     receptive_field_stride_shape=embedding_dim, random_seed=attention_seed, **common)
             if residual_join is not None:
                 # the first layer reads the embedding, so the last join's norm is the unembedder's
-                for i, name in enumerate(["attention_join"] if no_ffn else ["attention_join", "ffn_join"]):
-                    block[name] = ResidualNorm(E, dropout_p=dropout, seed=((seed or 0) << 16) + 2 * li + i,
-                                               device=self.device, **residual_join)
+                for name in ["attention_join"] if no_ffn else ["attention_join", "ffn_join"]:
+                    block[name] = ResidualNorm(E, dropout_p=dropout, device=self.device, **residual_join)
             block["attention_dropout"] = nn.Dropout(dropout)
             block["attention_bn"] = nn.BatchNorm1d(E, device=self.device) if use_batch_norm else None
             if not no_ffn:
@@ -132,6 +133,16 @@ class LUTTransformer(nn.Module):
                                    n_detectors=n_detectors, n_outputs=vocab_size, sequence_length=1,
                                    random_seed=seed, **common)
         self._debug_last_forward = None
+        self.seed_dropout((seed or 0) if dropout_seed is None else dropout_seed)
+
+    def seed_dropout(self, seed):
+        """Seeds the masks of the joins as dropout_seed does, for a rank that has loaded a state dict of
+        another; the numbers of their calls stay."""
+        for li, block in enumerate(self.layers):
+            for i, name in enumerate(["attention_join", "ffn_join"]):
+                if name in block:
+                    join = block[name]
+                    join.set_extra_state({**join.get_extra_state(), "seed": (seed << 16) + 2 * li + i})
 
     def _lut_layers(self):
         for block in self.layers:

@@ -8,7 +8,7 @@ import torch
 from torch.utils.checkpoint import checkpoint
 
 import spiky_amd
-from spiky_amd import CounterDropout, ResidualNorm
+from spiky_amd import CounterDropout, LUTTransformer, ResidualNorm
 import lm_plain
 
 
@@ -116,3 +116,40 @@ def test_a_captured_call_that_is_counted_raises(monkeypatch):
     CounterDropout(0.5)(x)
     capturing[0] = True
     join.eval()(x, x), drop.eval()(x)
+
+
+JOIN = dict(vocab_size=20, embedding_dim=16, context_size=4, positional_dim=2, num_layers=2, num_heads=2, n_detectors=4,
+            n_anchors_per_detector=3, dropout=0.25, residual_join={})
+
+
+def joins(model):
+    return [m for m in model.modules() if isinstance(m, ResidualNorm)]
+
+
+def test_ranks_of_equal_weights_have_masks_of_their_own():
+    """dropout_seed is the masks' alone; without it they follow seed, as they did."""
+    one, two, plain = (LUTTransformer(seed=5, **kw, **JOIN) for kw in (dict(dropout_seed=1), dict(dropout_seed=2), {}))
+    for (name, a), b in zip(one.state_dict().items(), two.state_dict().values()):
+        assert name.endswith("_extra_state") or torch.equal(a, b), name
+    for p, q in zip(one._lut_layers(), two._lut_layers()):
+        assert torch.equal(p._detector_anchors, q._detector_anchors)
+    assert not {m.seed for m in joins(one)} & {m.seed for m in joins(two)}
+    assert len({m.seed for m in joins(one)}) == 4
+    assert [m.seed for m in joins(plain)] == [(5 << 16) + n for n in range(4)]
+    assert [m.seed for m in joins(LUTTransformer(**JOIN))] == list(range(4))
+
+
+@pytest.mark.parametrize("counted", [True, False])
+def test_a_rank_keeps_its_masks_over_another_ones_checkpoint(counted):
+    """A state dict brings its own seeds; seed_dropout gives them back, and leaves the numbers of the calls."""
+    one, two = (LUTTransformer(seed=5, dropout_seed=n, **JOIN) for n in (1, 2))
+    if counted:
+        counters = spiky_amd.mask_counters(two, "cpu")
+    want = [m.get_extra_state()["seed"] for m in joins(two)]
+    for m in joins(one):
+        m.calls = 7
+    two.load_state_dict(one.state_dict())
+    two.seed_dropout(2)
+    assert [m.get_extra_state() for m in joins(two)] == [{"seed": s, "calls": 7} for s in want]
+    if counted:
+        assert counters.tolist() == [[s, 8] for s in want]
