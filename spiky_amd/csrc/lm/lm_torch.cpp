@@ -59,6 +59,13 @@ const Tensor &device_tensor(PyObject *o, const char *name) {
     return t;
 }
 
+// Forward-mode derivatives are not computed, and a result without a tangent would count as constant.
+void check_tangent(PyObject *o, const char *name) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!THPVariable_Check(o) || !THPVariable_Unpack(o)._fw_grad(0).defined(),
+                                "spiky_amd's language-model operators have no forward-mode derivatives, but tensor ",
+                                name, " has a tangent");
+}
+
 // Undefined for None.
 Tensor device_tensor(PyObject *o, const char *name, c10::Device device) {
     if (o == Py_None) return Tensor();
@@ -222,6 +229,7 @@ struct Once : N {
 PyObject *dropout(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     TORCH_CHECK_TYPE(n == 4, "dropout takes 4 arguments");
+    check_tangent(args[0], "x");
     const Tensor &x = device_tensor(args[0], "x");
     type_code(x, "x");
     const double p = probability(args[1]);
@@ -411,6 +419,11 @@ PyObject *residual_norm(PyObject *, PyObject *const *args, Py_ssize_t n) {
         Residual, Branch, PostNorm, PostWeight, PostBias, PostEps, Gate, ResidualScale, BranchScale, DropoutP, Seed,
         Offset, PreNorm, PreWeight, PreBias, PreEps, Dtype
     };
+    const std::pair<int, const char *> differentiable[] = {
+        {Residual, "residual"}, {Branch, "branch"},         {PostWeight, "post_weight"}, {PostBias, "post_bias"},
+        {Gate, "gate"},         {PreWeight, "pre_weight"}, {PreBias, "pre_bias"},
+    };
+    for (const auto &[arg, name] : differentiable) check_tangent(args[arg], name);
     Inputs in;
     in[kRes] = device_tensor(args[Residual], "residual");
     const Tensor &res = in[kRes];

@@ -16,7 +16,8 @@ def counter_dropout(x, p, seed, offset=0):
 
     x: float32, bfloat16 or float16 on a HIP device, any shape.  seed, offset: whole numbers of
     64 bits, or seed an int64 device tensor of [seed, offset], read when the kernels run (for
-    graphs whose replays advance it in place, after the backward pass)."""
+    graphs whose replays advance it in place, after the backward pass).  Tensors with forward-mode
+    tangents are refused."""
     return _native.lm().dropout(x, p, seed, offset)
 
 

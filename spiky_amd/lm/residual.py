@@ -28,7 +28,7 @@ def residual_norm(residual, branch=None, *, post_norm=None, post_weight=None, po
     branch's type; so is the gate, of any shape that broadcasts to the branch's: [D], [B, 1, D]
     and full gates are read as they are.  dropout_p, seed and offset are counter_dropout's, over
     the branch.  All sums and intermediate values are 32-bit; gradients, of every tensor, do not
-    depend on the order in which workgroups run."""
+    depend on the order in which workgroups run.  Tensors with forward-mode tangents are refused."""
     return _native.lm().residual_norm(residual, branch, post_norm, post_weight, post_bias, post_eps, gate, residual_scale,
                                       branch_scale, dropout_p, seed, offset, pre_norm, pre_weight, pre_bias, pre_eps,
                                       dtype)
