@@ -6,6 +6,7 @@
 // launches.  Python functions over ctypes took 92-103 us for a pass of the
 // residual join and its gradients whose kernels take 33.
 #include <ATen/ATen.h>
+#include <ATen/TracerMode.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
@@ -57,6 +58,12 @@ const Tensor &device_tensor(PyObject *o, const char *name) {
     const Tensor &t = THPVariable_Unpack(o);
     TORCH_CHECK(t.device().is_cuda(), "tensor ", name, " must be on CUDA");
     return t;
+}
+
+// A trace sees torch's own calls alone, and would keep the results here as constants.
+void check_trace() {
+    TORCH_CHECK(!at::tracer::impl::is_dispatch_enabled(),
+                "spiky_amd's language-model operators cannot be traced by torch.jit.trace");
 }
 
 // Forward-mode derivatives are not computed, and a result without a tangent would count as constant.
@@ -229,6 +236,7 @@ struct Once : N {
 PyObject *dropout(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     TORCH_CHECK_TYPE(n == 4, "dropout takes 4 arguments");
+    check_trace();
     check_tangent(args[0], "x");
     const Tensor &x = device_tensor(args[0], "x");
     type_code(x, "x");
@@ -415,6 +423,7 @@ PyObject *wrapped(const Tensor &t) {
 PyObject *residual_norm(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     TORCH_CHECK_TYPE(n == 17, "residual_norm takes 17 arguments");
+    check_trace();
     enum {
         Residual, Branch, PostNorm, PostWeight, PostBias, PostEps, Gate, ResidualScale, BranchScale, DropoutP, Seed,
         Offset, PreNorm, PreWeight, PreBias, PreEps, Dtype
@@ -539,6 +548,7 @@ std::pair<Tensor, int64_t> by_row(const Tensor &t, const char *name, int64_t row
 PyObject *process_logits(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     TORCH_CHECK_TYPE(n == 14, "process_logits takes 14 arguments");
+    check_trace();
     enum {
         Logits, TokenIds, Lengths, PromptLengths, Repetition, Presence, Frequency, Bias, BiasIds, BiasValues,
         Temperature, Mask, Out, Dtype

@@ -3,7 +3,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from spiky_amd import counter_dropout, residual_norm
+from spiky_amd import counter_dropout, process_logits, residual_norm
 
 
 def test_tangents_are_refused():
@@ -21,3 +21,14 @@ def test_tangents_are_refused():
                 call()
     with pytest.raises(RuntimeError, match="must be on CUDA"):
         counter_dropout(forward_ad.unpack_dual(x).primal, 0.5, 1)
+
+
+def test_traces_are_refused():
+    """torch.jit.trace would keep the results of its example inputs as constants."""
+    x = torch.randn(4, 8)
+    for call in (lambda x: counter_dropout(x, 0.5, 1), lambda x: residual_norm(x, x, pre_norm="rms")[1],
+                 lambda x: process_logits(x, temperature=2.0)):
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            torch.jit.trace(call, x)
+        with pytest.raises(RuntimeError, match="must be on CUDA"):
+            call(x)
