@@ -528,6 +528,34 @@ PyObject *residual_norm(PyObject *, PyObject *const *args, Py_ssize_t n) {
 }
 
 // ---- logits -----------------------------------------------------------------
+// n rows of `width` bytes in memory, `step` bytes apart.
+struct Span {
+    uintptr_t at = 0;
+    int64_t n = 0, step = 0, width = 0;
+};
+
+// The rows of a tensor with contiguous columns, `stride` elements apart; one row for all where that is 0.
+Span span_of(const Tensor &t, int64_t stride) {
+    if (!t.defined() || t.numel() == 0) return {};
+    const int64_t size = (int64_t)t.element_size(), rows = t.dim() == 2 ? t.size(0) : 1;
+    return {reinterpret_cast<uintptr_t>(t.data_ptr()), stride ? rows : 1, stride * size, t.size(-1) * size};
+}
+
+// Rows of both are in the order of their addresses, so one walk along them meets any two that overlap.
+bool overlap(const Span &a, const Span &b) {
+    if (a.at + (a.n - 1) * a.step + a.width <= b.at || b.at + (b.n - 1) * b.step + b.width <= a.at) return false;
+    for (int64_t i = 0, j = 0; i < a.n && j < b.n;) {
+        const uintptr_t from_a = a.at + i * a.step, from_b = b.at + j * b.step;
+        if (from_a + a.width <= from_b)
+            i++;
+        else if (from_b + b.width <= from_a)
+            j++;
+        else
+            return true;
+    }
+    return false;
+}
+
 bool is_index(const Tensor &t, const char *name) {
     const bool wide = t.scalar_type() == at::kLong;
     TORCH_CHECK(wide || t.scalar_type() == at::kInt, "tensor ", name, " must have dtype int32 or int64, got ",
@@ -583,7 +611,8 @@ PyObject *process_logits(PyObject *, PyObject *const *args, Py_ssize_t n) {
         TORCH_CHECK_VALUE(vocab <= 1 || out.stride(1) == 1, "out must have contiguous columns");
         TORCH_CHECK_VALUE(rows <= 1 || out.stride(0) >= vocab, "the rows of out must not overlap");
         TORCH_CHECK_VALUE(out.data_ptr() != logits.data_ptr() ||
-                              (out.scalar_type() == logits.scalar_type() && out.stride(0) == logits.stride(0)),
+                              (out.scalar_type() == logits.scalar_type() &&
+                               (rows <= 1 || out.stride(0) == logits.stride(0))),
                           "out may be logits, but not another view of them");
         TORCH_CHECK_VALUE(!out.requires_grad(), "out must not require a gradient");
     }
@@ -684,8 +713,35 @@ PyObject *process_logits(PyObject *, PyObject *const *args, Py_ssize_t n) {
                           mask.sizes());
         a.mask = mask.data_ptr();
     }
+    if (args[Out] == Py_None) {
+        check(spiky_lm_process_logits(&a, on.stream));
+        return THPVariable_Wrap(out);
+    }
+    // Workgroups read the row's settings, tokens and biases at any time, and other elements of the rest than
+    // they write.  Logits, or a bias, in the very place of the result are read by the lane that writes there.
+    const Span to = span_of(out, a.out_stride);
+    auto apart = [&](const Tensor &t, int64_t stride, const char *name, bool by_element = false) {
+        const Span from = span_of(t, stride);
+        const bool in_place = by_element && from.at == to.at && from.width == to.width && from.n == to.n &&
+                              (to.n == 1 || from.step == to.step);
+        TORCH_CHECK_VALUE(in_place || !overlap(from, to), "out must not overlap ", name);
+    };
+    apart(logits, a.logits_stride, "logits other than as the same tensor", true);
+    apart(bias, a.bias_stride, "bias", true);
+    apart(mask, a.mask_stride, "mask");
+    apart(tokens, a.tokens_stride, "tokens");
+    apart(ids, a.bias_ids_stride, "bias_ids");
+    apart(values, a.bias_values_stride, "bias_values");
+    const std::pair<const Tensor &, const char *> by_rows[] = {
+        {lengths, "lengths"},
+        {prompts, "prompt_lengths"},
+        {repetition, "repetition_penalty"},
+        {presence, "presence_penalty"},
+        {frequency, "frequency_penalty"},
+        {temperature, "temperature"},
+    };
+    for (const auto &[t, name] : by_rows) apart(t, 0, name);
     check(spiky_lm_process_logits(&a, on.stream));
-    if (args[Out] == Py_None) return THPVariable_Wrap(out);
     if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
     Py_INCREF(args[Out]);
     return args[Out];
@@ -709,6 +765,14 @@ PyObject *rows_of_gate(PyObject *, PyObject *const *args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+PyObject *rows_overlap(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK(n == 2 && THPVariable_Check(args[0]) && THPVariable_Check(args[1]), "two tensors of rows");
+    const Tensor &a = THPVariable_Unpack(args[0]), &b = THPVariable_Unpack(args[1]);
+    return PyBool_FromLong(overlap(span_of(a, a.stride(0)), span_of(b, b.stride(0))));
+    END_HANDLE_TH_ERRORS
+}
+
 template <typename F>
 PyCFunction fast(F *f) {
     return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f));
@@ -720,6 +784,7 @@ PyMethodDef methods[] = {
     {"process_logits", fast(process_logits), METH_FASTCALL, "the arguments of spiky_amd.process_logits, in its order"},
     {"rows_of_tensor", rows_of_tensor, METH_O, "the tensor as rows of its last dimension, and their distance"},
     {"rows_of_gate", fast(rows_of_gate), METH_FASTCALL, "the gate as read for a branch, and the rows that share one"},
+    {"rows_overlap", fast(rows_overlap), METH_FASTCALL, "whether rows of two matrices share memory"},
     {nullptr, nullptr, 0, nullptr},
 };
 

@@ -26,7 +26,8 @@ def process_logits(logits, *, tokens=None, lengths=None, prompt_lengths=None, re
     True where allowed, or int32 [ceil(V / 32)] or [B, ceil(V / 32)] with entry v in bit v % 32 of
     word v // 32.
 
-    Returns a tensor of the logits' type, or of `dtype` float32, or `out`, which may be `logits`.
+    Returns a tensor of the logits' type, or of `dtype` float32, or `out`, which may be `logits` and
+    else shares no memory with them or another argument.
     There is no gradient."""
     return _native.lm().process_logits(logits, tokens, lengths, prompt_lengths, repetition_penalty, presence_penalty,
                                        frequency_penalty, bias, bias_ids, bias_values, temperature, mask, out, dtype)

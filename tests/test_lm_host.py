@@ -173,3 +173,22 @@ def test_logits_entry_refuses(change, message):
     for k, v in change.items():
         setattr(a, k, v)
     refuse(_native.lib().spiky_lm_process_logits(a, None), message)
+
+
+def test_rows_that_overlap():
+    """Rows of two views of one memory, against the elements that they share."""
+    base = torch.arange(240)
+    views = {f"{at}:{n}x{width}/{step}": base.as_strided((n, width), (step, 1), at)
+             for at in (0, 1, 7, 8, 20, 60) for n, width, step in ((1, 8, 8), (3, 8, 8), (4, 5, 12), (2, 10, 24), (5, 6, 0),
+                                                                    (3, 0, 9), (6, 7, 5))}
+    halves = torch.zeros(480, dtype=torch.int32)
+    assert not _native.lm().rows_overlap(base[:24].reshape(3, 8), halves[:24].reshape(3, 8))
+    for a in views.values():
+        for b in views.values():
+            assert _native.lm().rows_overlap(a, b) == bool(set(a.flatten().tolist()) & set(b.flatten().tolist())), (a, b)
+    # of other types: the bytes count
+    bytes_ = base.view(torch.int8)
+    assert _native.lm().rows_overlap(base[4:8].reshape(1, 4), bytes_[63:64].reshape(1, 1))
+    assert not _native.lm().rows_overlap(base[4:8].reshape(1, 4), bytes_[64:70].reshape(1, 6))
+    assert not _native.lm().rows_overlap(base[4:8].reshape(1, 4), bytes_[20:32].reshape(1, 12))
+    assert _native.lm().rows_overlap(base[4:8].reshape(1, 4), bytes_[20:33].reshape(1, 13))
