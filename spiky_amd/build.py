@@ -1,6 +1,7 @@
 """Build libspiky_lut.so (the HIP kernels + C ABI) in-tree for gfx950.
 
-Run as ``python -m spiky_amd.build`` or through ``__graft_entry__.build()``.
+Run as ``python -m spiky_amd.build`` or through ``__graft_entry__.build()``; without torch, a host
+compiler or Python's headers, for hosts in C or C++, as ``python spiky_amd/build.py --library``.
 The library lands next to this file so that it travels with the source tree.
 """
 import importlib.util
@@ -44,7 +45,10 @@ def _hipcc():
 
 def build_binding(verbose=False):
     """Compile the torch binding against the library, which must be there."""
-    torch = os.path.dirname(importlib.util.find_spec("torch").origin)
+    found = importlib.util.find_spec("torch")
+    if found is None:
+        raise RuntimeError("the torch binding needs torch, which is not found")
+    torch = os.path.dirname(found.origin)
     tmp = BINDING + ".tmp"
     include = [os.path.join(torch, "include"), os.path.join(torch, "include", "torch", "csrc", "api", "include"),
                "/opt/rocm/include", sysconfig.get_paths()["include"]]
@@ -59,8 +63,9 @@ def build_binding(verbose=False):
     return BINDING
 
 
-def build(verbose=False):
-    """Compile every source to an object, link the shared library, then build the torch binding."""
+def build(verbose=False, binding=None):
+    """Compile every source to an object, link the shared library, then build the torch binding:
+    where torch is found, or always (binding=True) or never (False).  The library needs hipcc alone."""
     hipcc = _hipcc()
     objs = []
     os.makedirs(os.path.join(HERE, "_build"), exist_ok=True)
@@ -80,10 +85,15 @@ def build(verbose=False):
         print(" ".join(cmd), flush=True)
     subprocess.check_call(cmd)
     os.replace(tmp, LIB)
-    build_binding(verbose)
+    if binding is None:
+        binding = importlib.util.find_spec("torch") is not None
+        if not binding:
+            print("torch not found: built without the torch binding", file=sys.stderr)
+    if binding:
+        build_binding(verbose)
     return LIB
 
 
 if __name__ == "__main__":
-    build(verbose="-v" in sys.argv)
+    build(verbose="-v" in sys.argv, binding=False if "--library" in sys.argv else None)
     print(LIB)
