@@ -170,10 +170,10 @@ class LUTTransformer(nn.Module):
         grid = not isinstance(self.embedding_dim, int)
         E = self.embedding_dim[0] * self.embedding_dim[1] if grid else self.embedding_dim
         z = self.token_embedder(tokens)
-        if self.residual_join is not None:
-            return self._forward_joined(z, B, S, E)
         if self._debug_last_forward is not None:
             self._debug_last_forward = [tokens.to(torch.float32), z.detach().clone()]
+        if self.residual_join is not None:
+            return self._forward_joined(z, B, S, E)
         for block in self.layers:
             if grid:
                 z = z.reshape((B, S) + self.embedding_dim)
@@ -198,6 +198,8 @@ class LUTTransformer(nn.Module):
 
     def _forward_joined(self, z, B, S, E):
         def joined(join, stream, branch):
+            if self._debug_last_forward is not None:
+                self._debug_last_forward.append(branch.detach().clone())
             stream, normed = join(stream, branch.reshape(B, S, E))
             return stream, stream if normed is None else normed
 
@@ -206,7 +208,7 @@ class LUTTransformer(nn.Module):
             a = block["attention_lut"](x if isinstance(self.embedding_dim, int) else x.reshape((B, S) + self.embedding_dim))
             z, x = joined(block["attention_join"], z, a)
             if not self.no_ffn:
-                z, x = joined(block["ffn_join"], z, block["ffn"](x.reshape(B * S, 1, E)))
+                z, x = joined(block["ffn_join"], z, block["ffn"](x.reshape(B * S, 1, E)).reshape(B, S, E))
         return self.unembedder(x.reshape(B * S, 1, E)).reshape(B, S, self.vocab_size)
 
     @torch.no_grad()
