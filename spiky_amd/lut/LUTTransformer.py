@@ -36,6 +36,8 @@ class LUTTransformer(nn.Module):
     `seed`) and the join's number: data-parallel ranks have one `seed`, for equal weights, and
     each a `dropout_seed`.  It excludes use_batch_norm."""
 
+    residual_join = None  # of models that were pickled before there was one
+
     def __init__(self, vocab_size, embedding_dim, context_size, positional_dim, num_layers, num_heads,
                  n_detectors, n_anchors_per_detector, n_anchors_per_detector_attention=None,
                  no_ffn=False, concatenation_product=True, sliced_product_mode=False, unified_pe=False,

@@ -1,4 +1,5 @@
 """LUTTransformer's joined forward on the CPU, with plain layers and a plain join in the library's place."""
+import pickle
 import sys
 
 import pytest
@@ -54,3 +55,12 @@ def test_a_joined_forward_keeps_what_the_plain_one_does(embedding_dim, no_ffn):
         seen.append([out, *m._debug_last_forward])
     assert len(seen[0]) == len(seen[1]) == 3 + (2 if no_ffn else 4)
     assert all(a.shape == b.shape and torch.equal(a, b) for a, b in zip(*seen))
+
+
+def test_a_model_pickled_without_joins_runs():
+    """One of before there were joins has no attribute of them."""
+    m = model()
+    want = m(torch.arange(B * S).reshape(B, S))
+    del m.__dict__["residual_join"]
+    old = pickle.loads(pickle.dumps(m))
+    assert "residual_join" not in old.__dict__ and torch.equal(old(torch.arange(B * S).reshape(B, S)), want)
