@@ -297,7 +297,7 @@ __global__ __launch_bounds__(kThreads, kThreads == 256 ? 7 : 1) void k_logits(sp
     };
     // Products with reciprocals.  Those of subnormal numbers would pass the largest: a penalty is scaled
     // to a normal one first, and so is what it divides; a temperature divides.
-    const float lift = rho < 0x1p-126f ? 0x1p24f : 1.f, less = 1.f / (rho * lift);
+    const float lift = fabsf(rho) < 0x1p-126f ? 0x1p24f : 1.f, less = 1.f / (rho * lift);
     const float cool = heat > 0.f ? 1.f / heat : 1.f;
     const bool divide_heat = heat > 0.f && __builtin_isinf(cool);
     const uint32_t count_mask = slots_in_words(a.history, a.n_bias) ? (1u << kSlotShift) - 1 : kBiased - 1;
