@@ -53,11 +53,14 @@ int type_code(const Tensor &t, const char *name) {
     return code;
 }
 
-const Tensor &device_tensor(PyObject *o, const char *name) {
+// With its memory's values: torch keeps the sign of imaginary parts of conjugates beside them.
+Tensor settled(const Tensor &t) { return t.is_neg() ? t.resolve_neg() : t; }
+
+Tensor device_tensor(PyObject *o, const char *name) {
     TORCH_CHECK(THPVariable_Check(o), "tensor ", name, " must be a torch.Tensor");
     const Tensor &t = THPVariable_Unpack(o);
     TORCH_CHECK(t.device().is_cuda(), "tensor ", name, " must be on CUDA");
-    return t;
+    return settled(t);
 }
 
 // A trace sees torch's own calls alone, and would keep the results here as constants.
@@ -76,7 +79,7 @@ void check_tangent(PyObject *o, const char *name) {
 // Undefined for None.
 Tensor device_tensor(PyObject *o, const char *name, c10::Device device) {
     if (o == Py_None) return Tensor();
-    const Tensor &t = device_tensor(o, name);
+    Tensor t = device_tensor(o, name);
     TORCH_CHECK(t.device() == device, "tensor ", name, " must be on ", device, ", got ", t.device());
     return t;
 }
@@ -125,7 +128,8 @@ Generator generator(PyObject *seed, PyObject *offset, c10::Device device) {
 // The tensor seen as rows of its last dimension, and the elements from row to
 // row.  Rows at one distance with contiguous columns stay where they are; others
 // are copied.
-std::pair<Tensor, int64_t> as_rows(const Tensor &t) {
+std::pair<Tensor, int64_t> as_rows(const Tensor &given) {
+    const Tensor t = settled(given);
     const int64_t dim = t.dim();
     const int64_t cols = dim ? t.size(-1) : 1;
     if (t.is_contiguous()) return {t, cols};
@@ -238,7 +242,7 @@ PyObject *dropout(PyObject *, PyObject *const *args, Py_ssize_t n) {
     TORCH_CHECK_TYPE(n == 4, "dropout takes 4 arguments");
     check_trace();
     check_tangent(args[0], "x");
-    const Tensor &x = device_tensor(args[0], "x");
+    const Tensor x = device_tensor(args[0], "x");
     type_code(x, "x");
     const double p = probability(args[1]);
     const Generator g = generator(args[2], args[3], x.device());
@@ -599,6 +603,8 @@ PyObject *process_logits(PyObject *, PyObject *const *args, Py_ssize_t n) {
         dtype = reinterpret_cast<THPDtype *>(args[Dtype])->scalar_type;
     }
     auto fits = [&](ScalarType t) { return t == logits.scalar_type() || t == at::kFloat; };
+    TORCH_CHECK_VALUE(!THPVariable_Check(args[Out]) || !THPVariable_Unpack(args[Out]).is_neg(),
+                      "out must hold its values' signs");
     Tensor out = device_tensor(args[Out], "out", device);
     if (!out.defined()) {
         const ScalarType t = dtype.value_or(logits.scalar_type());
