@@ -100,6 +100,8 @@ int spiky_lm_residual_norm_backward(const spiky_lm_residual_args *args,
  *   x -= frequency * n + presence * (n > 0)        n: times v is among tokens prompt_lengths[b]..lengths[b]
  *   x /= temperature                               unless temperature <= 0
  *   x  = -infinity                                 where the mask leaves v out
+ * Quotients are products with the divisor's reciprocal: one rounding of 32 bits more than a division.  That
+ * of a divisor past 2^126 is subnormal and has two bits fewer; one that would overflow is not used.
  * Tokens and bias ids outside [0, vocab) count nowhere.  out may be logits. */
 typedef struct {
     uint64_t rows, vocab;

@@ -218,6 +218,10 @@ struct Sparse {
 // row's tokens for each of its chunks.  256 threads are faster than 512 and 1024 there (all
 // together, in an earlier form: 166, 198, 242), for barriers hold fewer waves; 8 pieces a
 // thread no faster than 4 (144, 141).
+//
+// The bound of 7 waves is measured for 2-byte logits to fp32, which spill nothing under it (127 us
+// with everything set, 98 of HBM).  Under it fp32 to fp32 spills 46 registers (225 us, 129 of HBM) and
+// a 2-byte result 16 (125 us, 66 of HBM); other bounds have not been measured for these.
 template <typename TI, typename TO, int N, int P, uint32_t kThreads>
 __global__ __launch_bounds__(kThreads, kThreads == 256 ? 7 : 1) void k_logits(spiky_lm_logits_args a, uint32_t chunk) {
     // words where there are tokens or bias ids; with bias ids as many sums as may be needed, and slots

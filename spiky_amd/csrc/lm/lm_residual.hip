@@ -14,8 +14,9 @@
 // from its rounded copy, so n2 is the forward's own.
 //
 // Both directions are bound by memory where the work is large: 16384 rows of 4096,
-// bf16 beside an fp32 residual, take 160 us forward (805 MB, 5.0 TB/s; a large copy
-// runs at 4.9 to 5.4) and 265 us backward (1.24 GB, 4.7 TB/s), with the vector unit
+// bf16 beside an fp32 residual, take 155-176 us forward (805 MB, 4.6-5.2 TB/s; a large
+// copy runs at 4.9 to 5.4) and 268-299 us backward (1.24 GB, 4.1-4.6 TB/s), the less in a
+// process that has worked on nothing else, with the vector unit
 // busy half of the time, a third of that with the dropout's generator.  A backward
 // pass in two passes over the inputs took 808.  Small calls are bound by the host.
 #include "lm_kernels.h"
@@ -638,9 +639,11 @@ __device__ __forceinline__ float4 row_means(const J &j, const float4 &st, const 
 // row takes in HBM, for registers that make 3 waves of 2 to a SIMD (33822 rows of
 // 640 fp32 with layer norms 234 -> 161 us).  The next row's loads are issued before
 // the reduction, into the registers that this row's left.  Above 4096 columns 512
-// threads have 16 columns each: 1024 of 8 may use 128 registers, and spill (8192
-// rows of 8192: 370 us against 255).  With layer norms these would still spill (410
-// us), and read w2 and b1 again for every row instead (341).
+// threads have 16 columns each.  All of these spill: 14 registers with rms norms beside
+// fp32, 22 to 37 with layer norms, 86 and 112 for fp32.  1024 threads of 8, which may use
+// 128 registers, spilled more when they were compared (8192 rows of 8192 bf16: 370 us
+// against 255), before a call's parts were bits and parameters could be read again.  With
+// layer norms w2 and b1 are read again for every row (410 -> 341 us).
 template <typename TZ, typename TA, int N, int P, int TPR, bool FULL>
 __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_join_back(Join<TZ, TA> j) {
     constexpr int kThreads = TPR <= 64 ? 256 : TPR, kSlots = TPR <= 64 ? 256 / TPR : 1;
@@ -791,7 +794,9 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_join_back(Join<TZ, TA
 
 // Wider rows, and those narrower than a piece, take two passes over the inputs: the
 // means of each row, then columns.  1392 rows of 10700 fp16: 32 and 40 us, for 41 of
-// HBM in one pass; neither a thread's registers nor the LDS hold such a row's sums.
+// HBM in one pass.  A thread's registers do not hold such a row's inputs and sums; a row
+// of 2-byte elements in LDS, its column sums in registers, would fit to 16384 columns and
+// has not been built.
 template <typename TZ, typename TA, int N, int WG, bool FULL>
 __global__ __launch_bounds__(WG) void k_join_back_rows(Join<TZ, TA> j) {
     constexpr int K = FULL ? 8 : 3;
