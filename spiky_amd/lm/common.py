@@ -14,6 +14,7 @@ class CountedMasks:
     [seed, offset] that the operators read and the program advances."""
 
     counter = None
+    counter_version = None  # of the counter in the last forward pass
 
     def count_masks(self, seed):
         self.seed, self.calls = int(seed), 0
@@ -33,7 +34,8 @@ class CountedMasks:
         # copies and pickles count for themselves: nobody advances a copy of the counter
         state = dict(self.__dict__)
         state.update(self.get_extra_state())
-        state.pop("counter", None)
+        for name in ("counter", "counter_version"):
+            state.pop(name, None)
         return state
 
     @staticmethod
@@ -44,10 +46,17 @@ class CountedMasks:
 
     def next_mask(self, x):
         """(seed, offset) of a call in training on x."""
+        recomputed = torch._C._current_graph_task_id() != -1  # inside a backward pass (torch.utils.checkpoint)
         if self.counter is not None:
+            version = 0 if self.counter.is_inference() else self.counter._version
+            if not recomputed:
+                self.counter_version = version
+            elif self.counter_version not in (None, version):
+                raise RuntimeError("mask counters have changed since the forward pass that a backward pass repeats: "
+                                   "advance them after the backward pass")
             return self.counter, 0
-        if torch._C._current_graph_task_id() != -1:
-            # a recomputed forward pass (torch.utils.checkpoint): counted again, its mask would be another one
+        if recomputed:
+            # counted again, its mask would be another one
             raise RuntimeError("dropout inside a backward pass cannot tell which call it repeats: give the model "
                                "counters with spiky_amd.mask_counters, or pass seed and offset to the functions")
         if x.is_cuda and torch.cuda.is_current_stream_capturing():
@@ -70,5 +79,5 @@ def mask_counters(model, device):
     counters = torch.stack(rows) if rows else torch.zeros(0, 2, dtype=torch.int64)
     counters = counters.to(device)
     for m, row in zip(modules, counters):
-        m.counter = row
+        m.counter, m.counter_version = row, None
     return counters

@@ -153,3 +153,19 @@ def test_a_rank_keeps_its_masks_over_another_ones_checkpoint(counted):
     assert [m.get_extra_state() for m in joins(two)] == [{"seed": s, "calls": 7} for s in want]
     if counted:
         assert counters.tolist() == [[s, 8] for s in want]
+
+
+@pytest.mark.parametrize("reentrant", [True, False])
+def test_counters_that_move_before_the_backward_pass_raise(reentrant):
+    """The recomputed call would read the next mask."""
+    net, x = Net(), torch.randn(4, 16, requires_grad=True)
+    counters = spiky_amd.mask_counters(net, "cpu")
+    for _ in range(2):
+        y = checkpoint(net, x, use_reentrant=reentrant)
+        counters[:, 1] += 1
+        with pytest.raises(RuntimeError, match="after the backward pass"):
+            y.sum().backward()
+        y = checkpoint(net, x, use_reentrant=reentrant)
+        y.sum().backward()
+        counters[:, 1] += 1
+    copy.deepcopy(net)(x).sum().backward()
