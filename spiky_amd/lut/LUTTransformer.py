@@ -121,14 +121,16 @@ class LUTTransformer(nn.Module):
                 # the first layer reads the embedding, so the last join's norm is the unembedder's
                 for name in ["attention_join"] if no_ffn else ["attention_join", "ffn_join"]:
                     block[name] = ResidualNorm(E, dropout_p=dropout, device=self.device, **residual_join)
-            block["attention_dropout"] = nn.Dropout(dropout)
+            else:
+                block["attention_dropout"] = nn.Dropout(dropout)
             block["attention_bn"] = nn.BatchNorm1d(E, device=self.device) if use_batch_norm else None
             if not no_ffn:
                 block["ffn"] = LUTLayer(
                     n_inputs=E, n_anchors_per_detector=n_anchors_per_detector, n_detectors=n_detectors,
                     n_outputs=E, sequence_length=1,
                     random_seed=None if seed is None else seed + li * num_heads + num_heads, **common)
-                block["ffn_dropout"] = nn.Dropout(dropout)
+                if residual_join is None:
+                    block["ffn_dropout"] = nn.Dropout(dropout)
                 block["ffn_bn"] = nn.BatchNorm1d(E, device=self.device) if use_batch_norm else None
             self.layers.append(block)
         self.unembedder = LUTLayer(n_inputs=E, n_anchors_per_detector=n_anchors_per_detector,

@@ -64,3 +64,13 @@ def test_a_model_pickled_without_joins_runs():
     del m.__dict__["residual_join"]
     old = pickle.loads(pickle.dumps(m))
     assert "residual_join" not in old.__dict__ and torch.equal(old(torch.arange(B * S).reshape(B, S)), want)
+
+
+def test_joins_have_the_dropout_of_a_joined_model():
+    """No module is made that no call reaches."""
+    def dropouts(m):
+        return [x for x in m.modules() if isinstance(x, torch.nn.Dropout)]
+
+    assert len(dropouts(model(dropout=0.1))) == 4 and not dropouts(model(dropout=0.1, residual_join={}))
+    joined = model(dropout=0.1, residual_join={})
+    assert [x.dropout_p for x in joined.modules() if isinstance(x, ResidualNorm)] == [0.1] * 4
