@@ -1,5 +1,5 @@
 """Loader of libspiky_lut.so, the HIP kernels behind the C ABI in include/spiky_lut.h
-and include/spiky_lm.h.
+and include/spiky_lm.h and include/spiky_lm_tokens.h.
 
 The library is built in-tree (``python -m spiky_amd.build``).  There is no
 fallback: if the library is missing or fails to load, every device entry point
@@ -108,6 +108,27 @@ class LmLogitsArgs(ctypes.Structure):
                 ("n_bias", _u64), ("bias_ids_i64", _i32), ("mask", _vp), ("mask_stride", _i64), ("mask_bits", _i32)]
 
 
+# include/spiky_lm_tokens.h
+class LmEmbedArgs(ctypes.Structure):
+    """spiky_lm_embed_args"""
+    _fields_ = [("n", _u64), ("vocab", _u64), ("cols", _u64), ("tokens_i64", _i32), ("weight_dtype", _i32),
+                ("out_dtype", _i32), ("tokens", _vp), ("weight", _vp), ("weight_stride", _i64), ("scale", _f64)]
+
+
+class LmBeamsArgs(ctypes.Structure):
+    """spiky_lm_beams_args"""
+    _fields_ = [("searches", _u64), ("beams", _u64), ("vocab", _u64), ("n", _u64), ("dtype", _i32),
+                ("lengths_i64", _i32), ("logits", _vp), ("search_stride", _i64), ("beam_stride", _i64),
+                ("scores", _vp), ("finished", _vp), ("lengths", _vp), ("length_penalty", _f64), ("pad", _i64),
+                ("out_scores", _vp), ("out_parents", _vp), ("out_tokens", _vp)]
+
+
+class LmState(ctypes.Structure):
+    """spiky_lm_state"""
+    _fields_ = [("in", _vp), ("out", _vp), ("runs", _u64), ("run_bytes", _u64), ("in_search", _i64),
+                ("in_beam", _i64), ("in_run", _i64), ("out_search", _i64), ("out_beam", _i64), ("out_run", _i64)]
+
+
 _LM_SIGNATURES = {
     "spiky_lm_last_error": ([], ctypes.c_char_p),
     "spiky_lm_dropout": ([_vp, _i64, _vp, _u64, _u64, _i32, _f64, _u64, _u64, _vp, _vp], _i32),
@@ -116,6 +137,12 @@ _LM_SIGNATURES = {
     "spiky_lm_residual_norm_backward": (
         [ctypes.POINTER(LmResidualArgs), ctypes.POINTER(LmResidualGrads), _vp], _i32),
     "spiky_lm_process_logits": ([ctypes.POINTER(LmLogitsArgs), _vp], _i32),
+    "spiky_lm_embed": ([ctypes.POINTER(LmEmbedArgs), _vp, _vp], _i32),
+    "spiky_lm_embed_workspace": ([ctypes.POINTER(LmEmbedArgs)], _u64),
+    "spiky_lm_embed_backward": ([ctypes.POINTER(LmEmbedArgs), _vp, _i64, _vp, _vp, _u64, _vp], _i32),
+    "spiky_lm_beam_select_workspace": ([ctypes.POINTER(LmBeamsArgs)], _u64),
+    "spiky_lm_beam_select": ([ctypes.POINTER(LmBeamsArgs), _vp, _u64, _vp], _i32),
+    "spiky_lm_reorder": ([ctypes.POINTER(LmState), _u64, _vp, _i32, _u64, _u64, _u64, _vp], _i32),
 }
 
 
@@ -151,7 +178,8 @@ def lib():
 
 
 def lm():
-    """The torch binding of include/spiky_lm.h (csrc/lm/lm_torch.cpp); raises if it is absent."""
+    """The torch binding of include/spiky_lm.h and include/spiky_lm_tokens.h (csrc/lm/lm_torch.cpp,
+    csrc/lm/lm_tokens_torch.cpp); raises if it is absent."""
     global _lm
     if _lm is None:
         lib()

@@ -15,7 +15,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libspiky_lut.so")
 SOURCES = ["lut_fc.hip", "lut_tm.hip", "lut_seq.hip", "lut_sparse.hip", "lut_densify.hip", "lut_product.hip", "lut_seq_sparse.hip",
            "lut_builder.hip", "lut_capi.hip", "lm/lm_dropout.hip", "lm/lm_residual.hip", "lm/lm_logits.hip",
-           "lm/lm_capi.hip"]
+           "lm/lm_embed.hip", "lm/lm_beams.hip", "lm/lm_capi.hip"]
 ARCH = os.environ.get("SPIKY_OFFLOAD_ARCH", "gfx950")
 
 HIPCC_FLAGS = [
@@ -33,7 +33,7 @@ HIPCC_FLAGS = [
 
 # The operators on torch tensors: host code, which calls the library.
 BINDING = os.path.join(HERE, "_lm_torch.so")
-BINDING_SOURCE = os.path.join("lm", "lm_torch.cpp")
+BINDING_SOURCES = [os.path.join("lm", "lm_torch.cpp"), os.path.join("lm", "lm_tokens_torch.cpp")]
 
 
 def _hipcc():
@@ -53,7 +53,7 @@ def build_binding(verbose=False):
     include = [os.path.join(torch, "include"), os.path.join(torch, "include", "torch", "csrc", "api", "include"),
                "/opt/rocm/include", sysconfig.get_paths()["include"]]
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__",
-           "-DUSE_ROCM", *(f for i in include for f in ("-isystem", i)), os.path.join(CSRC, BINDING_SOURCE), "-o", tmp,
+           "-DUSE_ROCM", *(f for i in include for f in ("-isystem", i)), *(os.path.join(CSRC, s) for s in BINDING_SOURCES), "-o", tmp,
            "-L" + os.path.join(torch, "lib"), "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch_python", "-L" + HERE,
            "-l:" + os.path.basename(LIB), "-Wl,-rpath,$ORIGIN"]
     if verbose:

@@ -1,0 +1,379 @@
+// lm_beams.hip -- the selection of a beam search and the reordering of its states (gfx950).
+#include "lm_tokens.h"
+
+namespace spiky {
+namespace lm {
+namespace {
+
+constexpr int kThreads = 256, kWaves = kThreads / 64, kPieces = 4;
+constexpr uint32_t kMostBeams = 64;
+
+// ---- selection -----------------------------------------------------------------
+// A beam's logits are cut into slices, a workgroup each, which stays in registers: its largest
+// value, the sum of exponentials relative to that, and its n first candidates.  A second launch
+// joins the slices of each search's beams.
+template <typename T>
+constexpr uint32_t slice_size() {
+    return kThreads * kPieces * (16 / sizeof(T));
+}
+
+// A beam's part of the workspace: per slice the largest value and the sum, then n logits and tokens.
+struct Parts {
+    float2 *stats;      // [rows][slices]
+    float *logits;      // [rows][slices][n], from the largest; -infinity where there are fewer
+    uint32_t *tokens;
+    uint32_t slices, n;
+};
+
+// Before which a candidate of the same beam comes: the larger logit, then the lower token.
+__device__ __forceinline__ bool before(float x, uint32_t token, float y, uint32_t other) {
+    return x > y || (x == y && token < other);
+}
+
+// What a beam takes part with.
+enum Kind : uint32_t { kNothing, kLive, kFinished };
+
+__device__ __forceinline__ Kind kind_of(const spiky_lm_beams_args &a, uint64_t row) {
+    if (a.scores[row] == -INFINITY) return kNothing;
+    return a.finished && a.finished[row] ? kFinished : kLive;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void k_beam_slices(const spiky_lm_beams_args a, const Parts parts) {
+    constexpr int N = 16 / sizeof(T);
+    __shared__ float wave_value[2][kWaves];
+    __shared__ uint32_t wave_token[2][kWaves];
+    const uint64_t row = blockIdx.y + (uint64_t)blockIdx.z * 32768;
+    if (row >= a.searches * a.beams || kind_of(a, row) != kLive) return;
+    const uint32_t slice = blockIdx.x, wave = threadIdx.x / 64, lane = threadIdx.x & 63;
+    const T *x = static_cast<const T *>(a.logits) + (int64_t)(row / a.beams) * a.search_stride +
+                 (int64_t)(row % a.beams) * a.beam_stride;
+    float v[kPieces][N];
+    uint32_t col[kPieces];
+    float top = -INFINITY;
+#pragma unroll
+    for (int p = 0; p < kPieces; p++) {
+        Place<N> place;
+        place.set(a.vocab, (uint64_t)slice * slice_size<T>() + (p * kThreads + threadIdx.x) * N);
+        load(v[p], x + place.col, place.n);
+        col[p] = (uint32_t)place.col;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            v[p][i] = place.own >> i & 1 ? v[p][i] : -INFINITY;
+            top = fmaxf(top, v[p][i]);
+        }
+    }
+    for (int k = 32; k >= 1; k /= 2) top = fmaxf(top, __shfl_xor(top, k));
+    if (lane == 0) wave_value[0][wave] = top;
+    __syncthreads();
+    for (int w = 0; w < kWaves; w++) top = fmaxf(top, wave_value[0][w]);
+    const float from = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+#pragma unroll
+    for (int p = 0; p < kPieces; p++)
+#pragma unroll
+        for (int i = 0; i < N; i++) sum += __expf(v[p][i] - from);
+    for (int k = 32; k >= 1; k /= 2) sum += __shfl_xor(sum, k);
+    if (lane == 0) wave_value[1][wave] = sum;
+    __syncthreads();
+    const uint64_t at = row * parts.slices + slice;
+    if (threadIdx.x == 0) {
+        sum = 0.f;
+        for (int w = 0; w < kWaves; w++) sum += wave_value[1][w];
+        parts.stats[at] = make_float2(top, sum);
+    }
+    __syncthreads();
+    float last = INFINITY;
+    uint32_t last_token = ~0u;
+    for (uint32_t r = 0; r < parts.n; r++) {
+        float best = -INFINITY;
+        uint32_t token = ~0u;
+#pragma unroll
+        for (int p = 0; p < kPieces; p++)
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const bool left = before(last, last_token, v[p][i], col[p] + i) || r == 0;
+                if (left && before(v[p][i], col[p] + i, best, token) && v[p][i] > -INFINITY) {
+                    best = v[p][i];
+                    token = col[p] + i;
+                }
+            }
+        auto take = [&](float y, uint32_t other) {
+            if (before(y, other, best, token)) {
+                best = y;
+                token = other;
+            }
+        };
+        for (int k = 32; k >= 1; k /= 2) take(__shfl_xor(best, k), __shfl_xor(token, k));
+        if (lane == 0) {
+            wave_value[r & 1][wave] = best;
+            wave_token[r & 1][wave] = token;
+        }
+        __syncthreads();
+        for (int w = 0; w < kWaves; w++) take(wave_value[r & 1][w], wave_token[r & 1][w]);
+        if (threadIdx.x == 0) {
+            parts.logits[at * parts.n + r] = best;
+            parts.tokens[at * parts.n + r] = token;
+        }
+        last = best;
+        last_token = token;
+    }
+}
+
+// A candidate of a search.
+struct Candidate {
+    double rank, score;
+    float logit;
+    uint32_t beam, token;
+
+    __device__ __forceinline__ bool before(const Candidate &o) const {
+        if (rank != o.rank) return rank > o.rank;
+        if (beam != o.beam) return beam < o.beam;
+        return lm::before(logit, token, o.logit, o.token);
+    }
+};
+
+template <typename T>
+__device__ __forceinline__ T from_lane_xor(T x, int mask) {
+    static_assert(sizeof(T) % 4 == 0, "words");
+    uint32_t w[sizeof(T) / 4];
+    __builtin_memcpy(w, &x, sizeof(T));
+#pragma unroll
+    for (uint32_t i = 0; i < sizeof(T) / 4; i++) w[i] = __shfl_xor(w[i], mask);
+    __builtin_memcpy(&x, w, sizeof(T));
+    return x;
+}
+
+// What turns a beam's logits into ranks and scores.
+struct Beam {
+    double top, log_sum, score, length;
+    uint32_t kind;  // of Kind
+    bool unknown;   // its scores are NaN
+};
+
+__global__ __launch_bounds__(kThreads) void k_beam_join(const spiky_lm_beams_args a, const Parts parts) {
+    __shared__ Beam beams[kMostBeams];
+    __shared__ Candidate wave_best[2][kWaves];
+    const uint64_t search = blockIdx.x, row0 = search * a.beams;
+    const uint32_t wave = threadIdx.x / 64, lane = threadIdx.x & 63;
+    for (uint32_t k = wave; k < a.beams; k += kWaves) {
+        const uint64_t row = row0 + k;
+        Beam b;
+        b.kind = kind_of(a, row);
+        b.score = a.scores[row];
+        b.unknown = false;
+        b.top = -INFINITY;
+        double sum = 0.0;
+        if (b.kind == kLive) {
+            float top = -INFINITY;
+            for (uint32_t s = lane; s < parts.slices; s += 64) top = fmaxf(top, parts.stats[row * parts.slices + s].x);
+            for (int i = 32; i >= 1; i /= 2) top = fmaxf(top, __shfl_xor(top, i));
+            b.top = top;
+            for (uint32_t s = lane; s < parts.slices; s += 64) {
+                const float2 part = parts.stats[row * parts.slices + s];
+                if (part.x > -INFINITY || part.y != part.y) sum += part.y * exp(part.x - b.top);
+            }
+            for (int i = 32; i >= 1; i /= 2) sum += from_lane_xor(sum, i);
+            b.unknown = sum != sum || b.score != b.score || b.score == INFINITY;
+            if (!b.unknown && b.top == -INFINITY) b.kind = kNothing;
+        }
+        b.log_sum = log(sum);
+        b.length = 1.0;
+        if (a.lengths && a.length_penalty != 0.0) {
+            const int64_t n = a.lengths_i64 ? static_cast<const int64_t *>(a.lengths)[row]
+                                            : static_cast<const int32_t *>(a.lengths)[row];
+            const double grown = (double)n + (b.kind == kFinished ? 0.0 : 1.0);
+            b.length = pow(grown < 1.0 ? 1.0 : grown, a.length_penalty);
+        }
+        if (lane == 0) beams[k] = b;
+    }
+    __syncthreads();
+    const uint64_t each = (uint64_t)parts.slices * parts.n, all = a.beams * each;
+    const Candidate none = {-INFINITY, -INFINITY, -INFINITY, ~0u, ~0u};
+    // Candidate number i of the search, or none.
+    auto candidate = [&](uint64_t i) {
+        Candidate c = none;
+        const uint32_t k = (uint32_t)(i / each);
+        const uint64_t o = i - k * each;
+        const Beam &b = beams[k];
+        if (b.kind == kNothing) return c;
+        if (b.kind == kFinished) {
+            if (o != 0) return c;
+            c.token = 0;
+            c.score = b.score;
+        } else if (b.unknown) {
+            if (o >= parts.n || o >= a.vocab) return c;
+            c.token = (uint32_t)o;
+            c.score = NAN;
+        } else {
+            c.logit = parts.logits[row0 * each + i];
+            if (c.logit == -INFINITY) return c;
+            c.token = parts.tokens[row0 * each + i];
+            c.score = c.logit - b.top - b.log_sum + b.score;
+        }
+        c.beam = k;
+        c.rank = c.score / b.length;
+        if (c.rank != c.rank) c.rank = INFINITY;
+        return c;
+    };
+    Candidate last = none;
+    for (uint32_t r = 0; r < a.n; r++) {
+        Candidate best = none;
+        for (uint64_t i = threadIdx.x; i < all; i += kThreads) {
+            const Candidate c = candidate(i);
+            if (c.beam != ~0u && (r == 0 || last.before(c)) && c.before(best)) best = c;
+        }
+        for (int k = 32; k >= 1; k /= 2) {
+            const Candidate c = from_lane_xor(best, k);
+            if (c.before(best)) best = c;
+        }
+        if (lane == 0) wave_best[r & 1][wave] = best;
+        __syncthreads();
+        for (int w = 0; w < kWaves; w++)
+            if (wave_best[r & 1][w].before(best)) best = wave_best[r & 1][w];
+        if (threadIdx.x == 0) {
+            const bool there = best.beam != ~0u;
+            a.out_scores[search * a.n + r] = there ? (float)best.score : -INFINITY;
+            a.out_parents[search * a.n + r] = there ? best.beam : 0;
+            a.out_tokens[search * a.n + r] = there && beams[best.beam].kind == kLive ? best.token : a.pad;
+        }
+        last = best;
+    }
+}
+
+uint32_t slices_of(const spiky_lm_beams_args &a) {
+    const uint32_t size = a.dtype == SPIKY_F32 ? slice_size<float>() : slice_size<bf16>();
+    return a.vocab ? (uint32_t)((a.vocab + size - 1) / size) : 1;  // a finished beam needs one too
+}
+
+// ---- reordering -----------------------------------------------------------------
+// A thread takes the same 16 bytes of all beams of a search, loads those that go on and stores
+// them: so the result may lie in the place of the input.
+constexpr int kMostStates = 16;  // of a launch, by value
+
+struct State {
+    spiky_lm_state s;
+    Divider pieces;  // of a run
+};
+
+struct States {
+    State of[kMostStates];
+};
+
+template <typename V, int kBeams>
+__device__ __forceinline__ void move(const char *in, char *out, int64_t in_beam, int64_t out_beam,
+                                     const uint32_t *parents, uint32_t beams, uint32_t n, bool in_place) {
+    for (uint32_t j0 = 0; j0 < n; j0 += kBeams) {
+        V v[kBeams];
+#pragma unroll
+        for (int j = 0; j < kBeams; j++) {
+            if (j0 + j >= n) break;
+            const uint32_t p = parents[j0 + j];
+            if (p < beams && !(in_place && p == j0 + j))
+                __builtin_memcpy(&v[j], in + (int64_t)p * in_beam, sizeof(V));
+            else
+                v[j] = V();
+        }
+#pragma unroll
+        for (int j = 0; j < kBeams; j++) {
+            if (j0 + j >= n) break;
+            if (!(in_place && parents[j0 + j] == j0 + j))
+                __builtin_memcpy(out + (int64_t)(j0 + j) * out_beam, &v[j], sizeof(V));
+        }
+    }
+}
+
+typedef uint32_t Words4 __attribute__((ext_vector_type(4)));
+
+template <int kBeams>
+__global__ __launch_bounds__(kThreads) void k_reorder(const States states, const void *parents_, bool i64,
+                                                      uint32_t beams, uint32_t n, uint64_t first) {
+    extern __shared__ uint32_t parents[];  // ~0: none
+    const uint64_t search = first + blockIdx.y;
+    for (uint32_t j = threadIdx.x; j < n; j += kThreads) {
+        const uint64_t at = search * n + j;
+        const int64_t p = i64 ? static_cast<const int64_t *>(parents_)[at] : static_cast<const int32_t *>(parents_)[at];
+        parents[j] = p >= 0 && p < (int64_t)beams ? (uint32_t)p : ~0u;
+    }
+    __syncthreads();
+    const State &state = states.of[blockIdx.z];
+    const spiky_lm_state &s = state.s;
+    const bool in_place = s.in == s.out;
+    for (uint64_t i = (uint64_t)blockIdx.x * kThreads + threadIdx.x; i < s.runs * state.pieces.d;
+         i += (uint64_t)gridDim.x * kThreads) {
+        const uint64_t run = i < 0x100000000ull ? state.pieces.divide((uint32_t)i) : i / state.pieces.d;
+        const uint64_t at = (i - run * state.pieces.d) * 16;
+        const char *in = static_cast<const char *>(s.in) + (int64_t)search * s.in_search + (int64_t)run * s.in_run + at;
+        char *out = static_cast<char *>(s.out) + (int64_t)search * s.out_search + (int64_t)run * s.out_run + at;
+        const uint64_t left = s.run_bytes - at;
+        if (left >= 16) {
+            move<Words4, kBeams>(in, out, s.in_beam, s.out_beam, parents, beams, n, in_place);
+            continue;
+        }
+        // the end of a run: other threads' pieces may be written already, so it keeps to its own
+        uint32_t o = 0;
+        if (left & 8) move<uint64_t, kBeams>(in, out, s.in_beam, s.out_beam, parents, beams, n, in_place), o += 8;
+        if (left & 4) move<uint32_t, kBeams>(in + o, out + o, s.in_beam, s.out_beam, parents, beams, n, in_place), o += 4;
+        if (left & 2) move<uint16_t, kBeams>(in + o, out + o, s.in_beam, s.out_beam, parents, beams, n, in_place), o += 2;
+        if (left & 1) move<uint8_t, kBeams>(in + o, out + o, s.in_beam, s.out_beam, parents, beams, n, in_place);
+    }
+}
+
+}  // namespace
+
+uint64_t beam_select_workspace(const spiky_lm_beams_args &a) {
+    return a.searches * a.beams * slices_of(a) * (sizeof(float2) + a.n * 8);
+}
+
+hipError_t launch_beam_select(const spiky_lm_beams_args &a, void *workspace, hipStream_t st) {
+    Parts parts;
+    const uint64_t rows = a.searches * a.beams;
+    parts.slices = slices_of(a);
+    parts.n = (uint32_t)a.n;
+    parts.stats = static_cast<float2 *>(workspace);
+    parts.logits = reinterpret_cast<float *>(parts.stats + rows * parts.slices);
+    parts.tokens = reinterpret_cast<uint32_t *>(parts.logits + rows * parts.slices * a.n);
+    const dim3 grid(parts.slices, (uint32_t)min(rows, (uint64_t)32768), (uint32_t)((rows + 32767) / 32768));
+    if (a.dtype == SPIKY_F32)
+        k_beam_slices<float><<<grid, dim3(kThreads), 0, st>>>(a, parts);
+    else if (a.dtype == SPIKY_BF16)
+        k_beam_slices<bf16><<<grid, dim3(kThreads), 0, st>>>(a, parts);
+    else
+        k_beam_slices<f16><<<grid, dim3(kThreads), 0, st>>>(a, parts);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    k_beam_join<<<dim3((uint32_t)a.searches), dim3(kThreads), 0, st>>>(a, parts);
+    return hipGetLastError();
+}
+
+hipError_t launch_reorder(const spiky_lm_state *states, uint64_t count, const void *parents, bool parents_i64,
+                          uint64_t searches, uint64_t beams, uint64_t n, hipStream_t st) {
+    for (uint64_t at = 0; at < count; at += kMostStates) {
+        const uint64_t here = min(count - at, (uint64_t)kMostStates);
+        States group = {};
+        uint64_t most = 0;
+        for (uint64_t i = 0; i < here; i++) {
+            const uint64_t pieces = (states[at + i].run_bytes + 15) / 16;
+            group.of[i] = {states[at + i], Divider((uint32_t)max(pieces, (uint64_t)1))};
+            if (pieces == 0) group.of[i].s.runs = 0;
+            most = max(most, group.of[i].s.runs * pieces);
+        }
+        if (most == 0) continue;
+        const uint64_t groups = min((most + kThreads - 1) / kThreads, (uint64_t)16384);
+        for (uint64_t first = 0; first < searches; first += 32768) {
+            const dim3 grid((uint32_t)groups, (uint32_t)min(searches - first, (uint64_t)32768), (uint32_t)here);
+            auto go = [&](auto kernel) {
+                kernel<<<grid, dim3(kThreads), n * 4, st>>>(group, parents, parents_i64, (uint32_t)beams, (uint32_t)n,
+                                                            first);
+                return hipGetLastError();
+            };
+            const hipError_t e = n <= 4 ? go(k_reorder<4>) : n <= 8 ? go(k_reorder<8>) : n <= 16 ? go(k_reorder<16>)
+                                 : n <= 32 ? go(k_reorder<32>) : go(k_reorder<64>);
+            if (e != hipSuccess) return e;
+        }
+    }
+    return hipSuccess;
+}
+
+}  // namespace lm
+}  // namespace spiky

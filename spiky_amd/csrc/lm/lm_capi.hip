@@ -1,11 +1,12 @@
-// lm_capi.hip -- the C ABI of include/spiky_lm.h: host validation, and dispatch
-// to the kernels on the caller's stream.  Nothing here allocates or synchronises.
+// lm_capi.hip -- the C ABI of include/spiky_lm.h and include/spiky_lm_tokens.h: host
+// validation, and dispatch to the kernels on the caller's stream.  Nothing here allocates or synchronises.
 #include <cmath>
 #include <stdexcept>
 #include <string>
 
 #include "../../../include/spiky_lut.h"
 #include "lm_kernels.h"
+#include "lm_tokens.h"
 
 namespace {
 
@@ -74,6 +75,29 @@ spiky::lm::DropArgs check(const spiky_lm_residual_args *a) {
     require(a->branch || (!a->gate && a->post_norm == SPIKY_NORM_NONE), "a gate or norm of no branch");
     require(a->residual, "null pointer");
     return drop_args(a->branch ? a->dropout_p : 0.0, a->seed, a->offset, a->rng);
+}
+
+void check(const spiky_lm_embed_args *a) {
+    require(a != nullptr, "null pointer");
+    require(is_type(a->weight_dtype) && is_type(a->out_dtype), "unknown element type");
+    require(a->weight_dtype == a->out_dtype || a->weight_dtype == SPIKY_F32 || a->out_dtype == SPIKY_F32,
+            "the table and the result must have one type, or one of them fp32");
+    require(a->n < 0x80000000ull && a->vocab < 0x80000000ull && a->cols <= 0x4000000ull,
+            "too many tokens, rows or columns");
+}
+
+void check(const spiky_lm_beams_args *a) {
+    require(a != nullptr, "null pointer");
+    require(is_type(a->dtype), "unknown element type");
+    require(a->beams >= 1 && a->beams <= 64 && a->n >= 1 && a->n <= 64, "beams and n must be 1 to 64");
+    require(a->vocab < 0x80000000ull && a->searches < 0x1000000ull / a->beams, "too many searches or entries");
+    require(a->length_penalty >= -8.0 && a->length_penalty <= 8.0, "the length penalty must be -8 to 8");
+}
+
+void check(const spiky_lm_state &s) {
+    require(s.run_bytes < (1ull << 35), "too long a run");
+    require(s.runs == 0 || s.run_bytes == 0 || (s.in && s.out), "null pointer");
+    require(s.runs == 0 || (s.run_bytes + 15) / 16 <= (1ull << 56) / s.runs, "too large a state");
 }
 
 hipStream_t as_stream(void *s) { return reinterpret_cast<hipStream_t>(s); }
@@ -149,6 +173,75 @@ int spiky_lm_process_logits(const spiky_lm_logits_args *a, void *stream) {
         if (a->rows == 0 || a->vocab == 0) return;
         require(a->logits && a->out, "null pointer");
         check_launch(spiky::lm::launch_process_logits(*a, as_stream(stream)), "process_logits");
+    });
+}
+
+int spiky_lm_embed(const spiky_lm_embed_args *a, void *out, void *stream) {
+    return guarded([&] {
+        check(a);
+        if (a->n == 0 || a->cols == 0) return;
+        require(a->tokens && (a->weight || a->vocab == 0) && out, "null pointer");
+        check_launch(spiky::lm::launch_embed(*a, out, as_stream(stream)), "embed");
+    });
+}
+
+uint64_t spiky_lm_embed_workspace(const spiky_lm_embed_args *a) {
+    uint64_t bytes = 0;
+    guarded([&] {
+        check(a);
+        if (a->vocab > 0 && a->cols > 0) bytes = spiky::lm::embed_workspace(*a);
+    });
+    return bytes;
+}
+
+int spiky_lm_embed_backward(const spiky_lm_embed_args *a, const void *d_out, int64_t d_out_stride, void *d_weight,
+                            void *workspace, uint64_t workspace_bytes, void *stream) {
+    return guarded([&] {
+        check(a);
+        if (a->vocab == 0 || a->cols == 0) return;
+        require(d_weight && (a->n == 0 || (a->tokens && d_out)), "null pointer");
+        require(workspace && workspace_bytes >= spiky::lm::embed_workspace(*a), "embed workspace too small");
+        check_launch(spiky::lm::launch_embed_backward(*a, d_out, d_out_stride, d_weight, workspace, as_stream(stream)),
+                     "embed_backward");
+    });
+}
+
+uint64_t spiky_lm_beam_select_workspace(const spiky_lm_beams_args *a) {
+    uint64_t bytes = 0;
+    guarded([&] {
+        check(a);
+        bytes = spiky::lm::beam_select_workspace(*a);
+    });
+    return bytes;
+}
+
+int spiky_lm_beam_select(const spiky_lm_beams_args *a, void *workspace, uint64_t workspace_bytes, void *stream) {
+    return guarded([&] {
+        check(a);
+        if (a->searches == 0) return;
+        require(a->scores && a->out_scores && a->out_parents && a->out_tokens && (a->logits || a->vocab == 0),
+                "null pointer");
+        const uint64_t need = spiky::lm::beam_select_workspace(*a);
+        require(workspace_bytes >= need && (workspace || need == 0), "beam_select workspace too small");
+        check_launch(spiky::lm::launch_beam_select(*a, workspace, as_stream(stream)), "beam_select");
+    });
+}
+
+int spiky_lm_reorder(const spiky_lm_state *states, uint64_t count, const void *parents, int parents_i64,
+                     uint64_t searches, uint64_t beams, uint64_t n, void *stream) {
+    return guarded([&] {
+        require(states || count == 0, "null pointer");
+        require(searches < 0x80000000ull && beams < 0x80000000ull && n <= 4096, "too many searches or beams");
+        for (uint64_t i = 0; i < count; i++) {
+            check(states[i]);
+            require(states[i].in != states[i].out || states[i].runs == 0 || (n == beams && n <= 64),
+                    "in place, n must be the number of beams, at most 64");
+        }
+        if (searches == 0 || n == 0) return;
+        require(parents != nullptr, "null pointer");
+        check_launch(spiky::lm::launch_reorder(states, count, parents, parents_i64 != 0, searches, beams, n,
+                                               as_stream(stream)),
+                     "reorder");
     });
 }
 

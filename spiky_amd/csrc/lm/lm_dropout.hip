@@ -8,23 +8,6 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kPieces = 4;  // 16-byte pieces of a thread
 
-// x / d for x < 2^32 by a product and two shifts (Granlund and Montgomery,
-// "Division by invariant integers using multiplication", 1994).
-struct Divider {
-    uint32_t d, m, s1, s2;
-    explicit Divider(uint32_t d_) : d(d_) {
-        uint32_t l = 0;
-        while (l < 32 && ((uint64_t)1 << l) < d) l++;
-        m = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << l) - d)) / d + 1);
-        s1 = l < 1 ? l : 1;
-        s2 = l < 1 ? 0 : l - 1;
-    }
-    __device__ __forceinline__ uint32_t divide(uint32_t x) const {
-        const uint32_t t = __umulhi(m, x);
-        return (t + ((x - t) >> s1)) >> s2;
-    }
-};
-
 // Reads and writes once: 16384 x 8192 bf16 take 96 us, 5.6 TB/s (a large copy runs
 // at 4.9 to 5.4).  The generator's 14 products of 32 x 32 bits for four columns make
 // most of 44.6 M vector instructions, 73 us at one in 4 cycles.  A row is cut into pieces of 16 bytes, and the

@@ -1,0 +1,238 @@
+// lm_embed.hip -- token embeddings and their gradient (gfx950).
+#include "lm_tokens.h"
+
+namespace spiky {
+namespace lm {
+namespace {
+
+constexpr int kThreads = 256;
+
+template <typename A, typename B>
+constexpr int piece() {  // columns of a piece: 16 bytes of the narrower type
+    return 16 / (sizeof(A) < sizeof(B) ? sizeof(A) : sizeof(B));
+}
+
+// ---- lookup ------------------------------------------------------------------
+// Reads the distinct rows and writes every one: bound by HBM where it is large.  The pieces of
+// all rows are numbered through as in dropout; a thread takes kPieces of them.
+template <typename Tok, typename W, typename T, int kPieces>
+__global__ __launch_bounds__(kThreads) void k_embed(const Tok *__restrict__ tokens, const W *__restrict__ weight,
+                                                    int64_t stride, T *__restrict__ out, uint64_t n, uint64_t vocab,
+                                                    uint64_t cols, Divider row_pieces, float scale) {
+    constexpr int N = piece<W, T>();
+    const uint64_t first = (uint64_t)blockIdx.x * (kThreads * kPieces);
+    const uint64_t row0 = first < 0x100000000ull ? row_pieces.divide((uint32_t)first) : first / row_pieces.d;
+    const uint32_t piece0 = (uint32_t)(first - row0 * row_pieces.d);
+#pragma unroll
+    for (int i = 0; i < kPieces; i++) {
+        const uint64_t at = (uint64_t)piece0 + i * kThreads + threadIdx.x;
+        // a long row ends at most once in the workgroup's pieces, a short one's numbers fit 32 bits
+        const uint32_t down = row_pieces.d >= kThreads * kPieces ? at >= row_pieces.d
+                                                                 : row_pieces.divide((uint32_t)at);
+        const uint64_t row = row0 + down;
+        if (row >= n) break;
+        Place<N> place;
+        place.set(cols, (at - (uint64_t)down * row_pieces.d) * N);
+        const int64_t token = tokens[row];
+        float v[N];
+        if ((uint64_t)token < vocab) {
+            load(v, weight + token * stride + place.col, place.n);
+#pragma unroll
+            for (int k = 0; k < N; k++) {
+                v[k] *= scale;
+                // the product rounds to 32 bits and then to T, for every T alike
+                if (sizeof(T) == 2) asm("" : "+v"(v[k]));
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < N; k++) v[k] = 0.f;
+        }
+        store(out + row * cols + place.col, v, place.n);
+    }
+}
+
+template <typename Tok, typename W, typename T>
+hipError_t lookup(const spiky_lm_embed_args &a, void *out, hipStream_t st) {
+    constexpr uint64_t N = piece<W, T>();
+    const uint64_t row_pieces = (a.cols + N - 1) / N, pieces = a.n * row_pieces;
+    const Divider by((uint32_t)row_pieces);
+    auto go = [&](auto kernel, uint64_t each) {
+        const uint64_t groups = (pieces + each - 1) / each;
+        if (groups * kThreads > 0xffffffffull) return hipErrorInvalidValue;
+        kernel<<<dim3((uint32_t)groups), dim3(kThreads), 0, st>>>(
+            static_cast<const Tok *>(a.tokens), static_cast<const W *>(a.weight), a.weight_stride,
+            static_cast<T *>(out), a.n, a.vocab, a.cols, by, (float)a.scale);
+        return hipGetLastError();
+    };
+    return go(k_embed<Tok, W, T, 4>, kThreads * 4);
+}
+
+// ---- gradient ------------------------------------------------------------------
+// The tokens' positions, sorted by token and for each token in ascending order, and where each
+// token's begin: start [vocab + 1], order [start[vocab]].  One launch without any exchange between
+// workgroups: a workgroup owns `range` consecutive tokens of the vocabulary, reads all n, counts its
+// own for each wave's share of the positions and those below its range, adds up, and reads them
+// again to place its own.  Tokens outside the vocabulary are in no range.
+constexpr int kSortWaves = 16, kMostRange = 1024;
+
+template <typename Tok>
+__global__ __launch_bounds__(kSortWaves * 64) void k_embed_sort(const Tok *__restrict__ tokens, uint32_t n,
+                                                                uint32_t vocab, uint32_t range,
+                                                                uint32_t *__restrict__ start,
+                                                                uint32_t *__restrict__ order) {
+    extern __shared__ uint32_t counts[];  // [kSortWaves][range]
+    __shared__ uint32_t below_of[kSortWaves], sum_of[kSortWaves];
+    const uint32_t wave = threadIdx.x / 64, lane = threadIdx.x & 63;
+    const uint32_t base = blockIdx.x * range, size = min(range, vocab - base);
+    for (uint32_t i = threadIdx.x; i < kSortWaves * range; i += kSortWaves * 64) counts[i] = 0;
+    __syncthreads();
+    const uint32_t share = (n / (kSortWaves * 64) + 1) * 64;
+    const uint32_t begin = min(wave * share, n), end = min(begin + share, n);
+    uint32_t *mine = counts + wave * range, below = 0;
+    constexpr int kAhead = 8;
+    // fn(position of the wave's lane 0, offset in the range or past it, token is below the range)
+    auto each = [&](auto fn) {
+        for (uint32_t at = begin; at < end; at += 64 * kAhead) {
+            Tok id[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; k++) {
+                const uint32_t i = at + k * 64 + lane;
+                id[k] = i < end ? tokens[i] : (Tok)-1;
+            }
+#pragma unroll
+            for (int k = 0; k < kAhead; k++) {
+                // base < 2^31, so a negative token stays past any range
+                const uint64_t o = (uint64_t)(int64_t)id[k] - base;
+                fn(at + k * 64, o < size ? (uint32_t)o : ~0u, id[k] >= 0 && id[k] < (Tok)base);
+            }
+        }
+    };
+    each([&](uint32_t, uint32_t o, bool lower) {
+        if (o != ~0u) atomicAdd(&mine[o], 1u);
+        below += lower;
+    });
+    for (int k = 32; k >= 1; k /= 2) below += __shfl_xor(below, k);
+    if (lane == 0) below_of[wave] = below;
+    __syncthreads();
+    uint32_t total = 0;
+    if (threadIdx.x < size)
+        for (int w = 0; w < kSortWaves; w++) total += counts[w * range + threadIdx.x];
+    uint32_t upto = total;
+    for (int k = 1; k < 64; k *= 2) {
+        const uint32_t x = __shfl_up(upto, k);
+        if (lane >= (uint32_t)k) upto += x;
+    }
+    if (lane == 63) sum_of[wave] = upto;
+    __syncthreads();
+    uint32_t at = upto - total;
+    for (uint32_t w = 0; w < kSortWaves; w++) at += below_of[w] + (w < wave ? sum_of[w] : 0);
+    if (threadIdx.x < size) {
+        start[base + threadIdx.x] = at;
+        if (base + threadIdx.x == vocab - 1) start[vocab] = at + total;
+        for (int w = 0; w < kSortWaves; w++) {
+            const uint32_t c = counts[w * range + threadIdx.x];
+            counts[w * range + threadIdx.x] = at;
+            at += c;
+        }
+    }
+    __syncthreads();
+    each([&](uint32_t first, uint32_t o, bool) {
+        for (uint64_t left = __ballot(o != ~0u); left;) {
+            const uint32_t leader = __builtin_ctzll(left);
+            const uint32_t token = __builtin_amdgcn_readlane(o, leader);
+            const uint64_t same = __ballot(o == token);
+            uint32_t place = 0;
+            if (lane == leader) place = atomicAdd(&mine[token], (uint32_t)__popcll(same));
+            place = __builtin_amdgcn_readlane(place, leader);
+            if (o == token) order[place + __popcll(same & (((uint64_t)1 << lane) - 1))] = first + lane;
+            left &= ~same;
+        }
+    });
+}
+
+// A row of the table's gradient: the sum over its token's positions.  `lanes` threads, a power of
+// two, take the pieces of a row.
+template <typename T, typename W>
+__global__ __launch_bounds__(kThreads) void k_embed_sum(const T *__restrict__ d_out, int64_t stride,
+                                                        const uint32_t *__restrict__ start,
+                                                        const uint32_t *__restrict__ order, W *__restrict__ d_weight,
+                                                        uint32_t vocab, uint64_t cols, uint32_t lanes, float scale) {
+    constexpr int N = piece<W, T>();
+    Place<N> place;
+    place.set(cols, ((uint64_t)blockIdx.y * lanes + (threadIdx.x & (lanes - 1))) * N);
+    const uint32_t rows = kThreads / lanes;
+    for (uint64_t row = (uint64_t)blockIdx.x * rows + threadIdx.x / lanes; row < vocab; row += (uint64_t)gridDim.x * rows) {
+        const uint32_t from = start[row], to = start[row + 1];
+        if (place.n == 0) continue;
+        float sum[N] = {};
+        for (uint32_t i = from; i < to; i++) {
+            float v[N];
+            load(v, d_out + (int64_t)order[i] * stride + place.col, place.n);
+#pragma unroll
+            for (int k = 0; k < N; k++) sum[k] += v[k];
+        }
+#pragma unroll
+        for (int k = 0; k < N; k++) sum[k] *= scale;
+        store(d_weight + row * cols + place.col, sum, place.n);
+    }
+}
+
+uint64_t order_at(const spiky_lm_embed_args &a) { return (a.vocab + 1) * 4; }
+
+template <typename Tok>
+hipError_t sort(const spiky_lm_embed_args &a, uint32_t *start, uint32_t *order, hipStream_t st) {
+    const uint32_t vocab = (uint32_t)a.vocab;
+    const uint32_t range = min(max((vocab + kCUs - 1) / kCUs, 1u), (uint32_t)kMostRange);
+    k_embed_sort<Tok><<<dim3((vocab + range - 1) / range), dim3(kSortWaves * 64), kSortWaves * range * 4, st>>>(
+        static_cast<const Tok *>(a.tokens), (uint32_t)a.n, vocab, range, start, order);
+    return hipGetLastError();
+}
+
+template <typename W, typename T>
+hipError_t sums(const spiky_lm_embed_args &a, const void *d_out, int64_t stride, void *d_weight, const uint32_t *start,
+                const uint32_t *order, hipStream_t st) {
+    constexpr uint64_t N = piece<W, T>();
+    const uint64_t pieces = (a.cols + N - 1) / N;
+    uint32_t lanes = 1;
+    while (lanes < pieces && lanes < kThreads) lanes *= 2;
+    const uint64_t groups = (a.vocab * lanes + kThreads - 1) / kThreads;
+    const dim3 grid((uint32_t)min(groups, (uint64_t)1 << 18), (uint32_t)((pieces + lanes - 1) / lanes));
+    k_embed_sum<T, W><<<grid, dim3(kThreads), 0, st>>>(static_cast<const T *>(d_out), stride, start, order,
+                                                       static_cast<W *>(d_weight), (uint32_t)a.vocab, a.cols, lanes,
+                                                       (float)a.scale);
+    return hipGetLastError();
+}
+
+// go(a value of the table's type, a value of out's)
+template <typename F>
+hipError_t by_types(int weight, int out, F &&go) {
+    if (weight == SPIKY_F32)
+        return out == SPIKY_F32 ? go(0.f, 0.f) : out == SPIKY_BF16 ? go(0.f, bf16()) : go(0.f, f16());
+    if (weight == SPIKY_BF16) return out == SPIKY_F32 ? go(bf16(), 0.f) : go(bf16(), bf16());
+    return out == SPIKY_F32 ? go(f16(), 0.f) : go(f16(), f16());
+}
+
+}  // namespace
+
+hipError_t launch_embed(const spiky_lm_embed_args &a, void *out, hipStream_t st) {
+    return by_types(a.weight_dtype, a.out_dtype, [&](auto w, auto t) {
+        return a.tokens_i64 ? lookup<int64_t, decltype(w), decltype(t)>(a, out, st)
+                            : lookup<int32_t, decltype(w), decltype(t)>(a, out, st);
+    });
+}
+
+uint64_t embed_workspace(const spiky_lm_embed_args &a) { return order_at(a) + a.n * 4; }
+
+hipError_t launch_embed_backward(const spiky_lm_embed_args &a, const void *d_out, int64_t d_out_stride, void *d_weight,
+                                 void *workspace, hipStream_t st) {
+    uint32_t *start = static_cast<uint32_t *>(workspace);
+    uint32_t *order = reinterpret_cast<uint32_t *>(static_cast<char *>(workspace) + order_at(a));
+    const hipError_t e = a.tokens_i64 ? sort<int64_t>(a, start, order, st) : sort<int32_t>(a, start, order, st);
+    if (e != hipSuccess) return e;
+    return by_types(a.weight_dtype, a.out_dtype, [&](auto w, auto t) {
+        return sums<decltype(w), decltype(t)>(a, d_out, d_out_stride, d_weight, start, order, st);
+    });
+}
+
+}  // namespace lm
+}  // namespace spiky

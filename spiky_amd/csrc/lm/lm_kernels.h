@@ -164,6 +164,24 @@ struct Place {
     }
 };
 
+// x / d for x < 2^32 by a product and two shifts (Granlund and Montgomery,
+// "Division by invariant integers using multiplication", 1994).
+struct Divider {
+    uint32_t d, m, s1, s2;
+    Divider() : Divider(1) {}
+    explicit Divider(uint32_t d_) : d(d_) {
+        uint32_t l = 0;
+        while (l < 32 && ((uint64_t)1 << l) < d) l++;
+        m = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << l) - d)) / d + 1);
+        s1 = l < 1 ? l : 1;
+        s2 = l < 1 ? 0 : l - 1;
+    }
+    __device__ __forceinline__ uint32_t divide(uint32_t x) const {
+        const uint32_t t = __umulhi(m, x);
+        return (t + ((x - t) >> s1)) >> s2;
+    }
+};
+
 // ---- dropout ---------------------------------------------------------------
 // The kept elements of a tensor are a function of (seed, offset, row, column)
 // alone: 7 rounds of Philox4x32 (Salmon, Moraes, Dror, Shaw, "Parallel random

@@ -5,201 +5,11 @@
 // A training step of a small model is bound by what the host does between
 // launches.  Python functions over ctypes took 92-103 us for a pass of the
 // residual join and its gradients whose kernels take 33.
-#include <ATen/ATen.h>
-#include <ATen/TracerMode.h>
-#include <ATen/hip/EmptyTensor.h>
-#include <c10/core/DeviceGuard.h>
-#include <c10/core/GradMode.h>
-#include <c10/hip/HIPGraphsC10Utils.h>
-#include <c10/hip/HIPStream.h>
-#include <torch/csrc/Dtype.h>
-#include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/function.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
-#include <torch/csrc/autograd/functions/utils.h>
-#include <torch/csrc/autograd/python_variable.h>
-#include <torch/csrc/autograd/saved_variable.h>
-#include <torch/csrc/utils/object_ptr.h>
-
-#include <algorithm>
-#include <optional>
-#include <utility>
-
-#include "../../../include/spiky_lm.h"
-#include "../../../include/spiky_lut.h"
+#include "lm_torch.h"
 
 namespace {
 
-using at::ScalarType;
-using at::Tensor;
-using torch::autograd::Node;
-using torch::autograd::SavedVariable;
-using torch::autograd::variable_list;
-
-// ---- checks and views -------------------------------------------------------
-void check(int status) {
-    if (status == SPIKY_OK) return;
-    TORCH_CHECK_VALUE(status != SPIKY_VALUE_ERROR, spiky_lm_last_error());
-    TORCH_CHECK(false, spiky_lm_last_error());
-}
-
-int type_code(ScalarType t) {
-    return t == at::kFloat ? SPIKY_F32 : t == at::kBFloat16 ? SPIKY_BF16 : t == at::kHalf ? SPIKY_F16 : -1;
-}
-
-int type_code(const Tensor &t, const char *name) {
-    const int code = type_code(t.scalar_type());
-    TORCH_CHECK(code >= 0, "tensor ", name, " must be float32, bfloat16 or float16, got ", t.scalar_type());
-    return code;
-}
-
-// With its memory's values: torch keeps the sign of imaginary parts of conjugates beside them.
-Tensor settled(const Tensor &t) { return t.is_neg() ? t.resolve_neg() : t; }
-
-Tensor device_tensor(PyObject *o, const char *name) {
-    TORCH_CHECK(THPVariable_Check(o), "tensor ", name, " must be a torch.Tensor");
-    const Tensor &t = THPVariable_Unpack(o);
-    TORCH_CHECK(t.device().is_cuda(), "tensor ", name, " must be on CUDA");
-    return settled(t);
-}
-
-// A trace sees torch's own calls alone, and would keep the results here as constants.
-void check_trace() {
-    TORCH_CHECK(!at::tracer::impl::is_dispatch_enabled(),
-                "spiky_amd's language-model operators cannot be traced by torch.jit.trace");
-}
-
-// Forward-mode derivatives are not computed, and a result without a tangent would count as constant.
-void check_tangent(PyObject *o, const char *name) {
-    TORCH_CHECK_NOT_IMPLEMENTED(!THPVariable_Check(o) || !THPVariable_Unpack(o)._fw_grad(0).defined(),
-                                "spiky_amd's language-model operators have no forward-mode derivatives, but tensor ",
-                                name, " has a tangent");
-}
-
-// Undefined for None.
-Tensor device_tensor(PyObject *o, const char *name, c10::Device device) {
-    if (o == Py_None) return Tensor();
-    Tensor t = device_tensor(o, name);
-    TORCH_CHECK(t.device() == device, "tensor ", name, " must be on ", device, ", got ", t.device());
-    return t;
-}
-
-void *pointer(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
-
-double number(PyObject *o) {
-    const double v = PyFloat_AsDouble(o);
-    if (v == -1.0 && PyErr_Occurred()) throw python_error();
-    return v;
-}
-
-uint64_t bits64(PyObject *o) {
-    THPObjectPtr index(PyNumber_Index(o));
-    if (!index) throw python_error();
-    const uint64_t v = PyLong_AsUnsignedLongLongMask(index.get());
-    if (v == (uint64_t)-1 && PyErr_Occurred()) throw python_error();
-    return v;
-}
-
-double probability(PyObject *o) {
-    const double p = number(o);
-    TORCH_CHECK_VALUE(p >= 0.0 && p <= 1.0, "dropout probability must be between 0 and 1, got ", p);
-    return p;
-}
-
-struct Generator {
-    uint64_t seed = 0, offset = 0;
-    Tensor state;  // [seed, offset] in device memory, in their place
-};
-
-Generator generator(PyObject *seed, PyObject *offset, c10::Device device) {
-    Generator g;
-    if (!THPVariable_Check(seed)) {
-        g.seed = bits64(seed);
-        g.offset = bits64(offset);
-        return g;
-    }
-    g.state = device_tensor(seed, "seed", device);
-    TORCH_CHECK(g.state.scalar_type() == at::kLong && g.state.numel() == 2 && g.state.is_contiguous(),
-                "tensor seed must be a contiguous int64 tensor of [seed, offset]");
-    TORCH_CHECK_VALUE(bits64(offset) == 0, "offset is the second element of a seed tensor");
-    return g;
-}
-
-// The tensor seen as rows of its last dimension, and the elements from row to
-// row.  Rows at one distance with contiguous columns stay where they are; others
-// are copied.
-std::pair<Tensor, int64_t> as_rows(const Tensor &given) {
-    const Tensor t = settled(given);
-    const int64_t dim = t.dim();
-    const int64_t cols = dim ? t.size(-1) : 1;
-    if (t.is_contiguous()) return {t, cols};
-    if (dim && t.stride(-1) == 1 && t.numel()) {
-        int64_t step = -1, reach = 0;  // from the innermost dimension of more than one
-        bool even = true;
-        for (int64_t k = dim - 2; k >= 0; k--) {
-            if (t.size(k) == 1) continue;
-            if (step < 0)
-                step = t.stride(k);
-            else if (t.stride(k) != reach)
-                even = false;
-            reach = t.stride(k) * t.size(k);
-        }
-        if (even) return {t, step < 0 ? cols : step};
-    }
-    return {t.contiguous(), cols};
-}
-
-int64_t rows_of(const Tensor &t) {
-    const int64_t cols = t.dim() ? t.size(-1) : 1;
-    return cols ? t.numel() / cols : 0;
-}
-
-// An uninitialised tensor, without the dispatcher's way to the same call.
-Tensor fresh(at::IntArrayRef sizes, ScalarType type, c10::Device device) {
-    return at::detail::empty_cuda(sizes, type, device, std::nullopt);
-}
-
-struct OnDevice {
-    c10::DeviceGuard guard;
-    void *stream;
-    explicit OnDevice(c10::Device d) : guard(d), stream(c10::hip::getCurrentHIPStream(d.index()).stream()) {}
-};
-
-// Gradients in a capture cannot go to a node that was recorded on the default stream
-// (a leaf's, kept alive by an eager graph): autograd would make that stream wait for
-// the captured one, which ends the process.  So the backward call raises first.
-void check_capture(const Node &node, c10::Device device) {
-    const c10::Stream standard = c10::hip::getDefaultHIPStream(device.index()).unwrap();
-    if (c10::hip::getCurrentHIPStream(device.index()).unwrap() == standard) return;  // which is never captured
-    bool stands = false;
-    for (size_t i = 0; i < node.num_outputs(); i++) {
-        if (!node.task_should_compute_output(i)) continue;
-        const auto stream = node.next_edge(i).function->stream();
-        stands = stands || (stream && stream->id() == standard.id() && stream->device_index() == device.index());
-    }
-    if (!stands) return;
-    TORCH_CHECK(c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None,
-                "a gradient belongs to the default stream, which a captured backward pass cannot reach: drop eager "
-                "graphs of the same leaves before the capture, or run them on a side stream");
-}
-
-bool needs_grad(const Tensor &t) { return t.defined() && t.requires_grad(); }
-
-// Gradients of the gradients are not computed: a backward pass through these raises.
-struct Twice : Node {
-    variable_list apply(variable_list &&) override {
-        TORCH_CHECK(false, "spiky_amd's language-model operators cannot be differentiated twice");
-    }
-};
-
-variable_list once_differentiable(variable_list &&grads, const torch::autograd::edge_list &inputs) {
-    if (!at::GradMode::is_enabled()) return std::move(grads);
-    auto stop = std::make_shared<Twice>();
-    stop->set_next_edges(torch::autograd::edge_list(inputs));  // so that a search for them comes by here
-    for (Tensor &t : grads)
-        if (t.defined()) torch::autograd::set_history(t, stop);
-    return std::move(grads);
-}
+using namespace lm_torch;
 
 // ---- dropout ----------------------------------------------------------------
 Tensor apply_dropout(const Tensor &given, double p, uint64_t seed, uint64_t offset, const Tensor &state) {
@@ -229,13 +39,6 @@ struct CounterDropoutBackward : Node {
     void release_variables() override { state.reset_data(); }
 };
 
-// Runs a node's gradients, and marks them where a graph of them is asked for.
-template <typename N>
-struct Once : N {
-    variable_list apply(variable_list &&grads) override {
-        return once_differentiable(N::apply(std::move(grads)), N::next_edges());
-    }
-};
 
 PyObject *dropout(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
@@ -410,19 +213,6 @@ std::pair<Tensor, int64_t> gate_rows(const Tensor &gate, at::IntArrayRef shape) 
     return {gate.contiguous(), std::max<int64_t>(share, 1)};
 }
 
-PyObject *pair(PyObject *first, PyObject *second) {
-    PyObject *t = PyTuple_New(2);
-    if (!t) throw python_error();
-    PyTuple_SET_ITEM(t, 0, first);
-    PyTuple_SET_ITEM(t, 1, second);
-    return t;
-}
-
-PyObject *wrapped(const Tensor &t) {
-    if (t.defined()) return THPVariable_Wrap(t);
-    Py_INCREF(Py_None);
-    return Py_None;
-}
 
 PyObject *residual_norm(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
@@ -532,50 +322,6 @@ PyObject *residual_norm(PyObject *, PyObject *const *args, Py_ssize_t n) {
 }
 
 // ---- logits -----------------------------------------------------------------
-// n rows of `width` bytes in memory, `step` bytes apart.
-struct Span {
-    uintptr_t at = 0;
-    int64_t n = 0, step = 0, width = 0;
-};
-
-// The rows of a tensor with contiguous columns, `stride` elements apart; one row for all where that is 0.
-Span span_of(const Tensor &t, int64_t stride) {
-    if (!t.defined() || t.numel() == 0) return {};
-    const int64_t size = (int64_t)t.element_size(), rows = t.dim() == 2 ? t.size(0) : 1;
-    return {reinterpret_cast<uintptr_t>(t.data_ptr()), stride ? rows : 1, stride * size, t.size(-1) * size};
-}
-
-// Rows of both are in the order of their addresses, so one walk along them meets any two that overlap.
-bool overlap(const Span &a, const Span &b) {
-    if (a.at + (a.n - 1) * a.step + a.width <= b.at || b.at + (b.n - 1) * b.step + b.width <= a.at) return false;
-    for (int64_t i = 0, j = 0; i < a.n && j < b.n;) {
-        const uintptr_t from_a = a.at + i * a.step, from_b = b.at + j * b.step;
-        if (from_a + a.width <= from_b)
-            i++;
-        else if (from_b + b.width <= from_a)
-            j++;
-        else
-            return true;
-    }
-    return false;
-}
-
-bool is_index(const Tensor &t, const char *name) {
-    const bool wide = t.scalar_type() == at::kLong;
-    TORCH_CHECK(wide || t.scalar_type() == at::kInt, "tensor ", name, " must have dtype int32 or int64, got ",
-                t.scalar_type());
-    return wide;
-}
-
-// [n] for every row, or [rows, n]: with contiguous columns, and the distance of its rows.
-std::pair<Tensor, int64_t> by_row(const Tensor &t, const char *name, int64_t rows) {
-    TORCH_CHECK_VALUE(t.dim() == 1 || (t.dim() == 2 && t.size(0) == rows), name, " must be [n] or [", rows,
-                      ", n], got ", t.sizes());
-    if (t.dim() == 1) return {t.contiguous(), 0};
-    Tensor c = t.size(1) > 1 && t.stride(1) != 1 ? t.contiguous() : t;
-    const int64_t stride = c.stride(0);
-    return {c, stride};
-}
 
 PyObject *process_logits(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
@@ -788,6 +534,9 @@ PyMethodDef methods[] = {
     {"dropout", fast(dropout), METH_FASTCALL, "x, p, seed, offset"},
     {"residual_norm", fast(residual_norm), METH_FASTCALL, "the arguments of spiky_amd.residual_norm, in its order"},
     {"process_logits", fast(process_logits), METH_FASTCALL, "the arguments of spiky_amd.process_logits, in its order"},
+    {"embed_tokens", fast(embed_tokens), METH_FASTCALL, "the arguments of spiky_amd.embed_tokens, in its order"},
+    {"beam_select", fast(beam_select), METH_FASTCALL, "the arguments of spiky_amd.beam_select, in its order"},
+    {"reorder_states", fast(reorder_states), METH_FASTCALL, "the arguments of spiky_amd.reorder_states, in its order"},
     {"rows_of_tensor", rows_of_tensor, METH_O, "the tensor as rows of its last dimension, and their distance"},
     {"rows_of_gate", fast(rows_of_gate), METH_FASTCALL, "the gate as read for a branch, and the rows that share one"},
     {"rows_overlap", fast(rows_overlap), METH_FASTCALL, "whether rows of two matrices share memory"},

@@ -12,14 +12,16 @@ LUTTransformer.py:43-67); everything else sees E = h * w features.
 
 With `residual_join` the two joins of a block are `ResidualNorm`s (this build's own addition):
 the branch is normed, dropped out and gated, added to the residual stream, and the next layer
-reads the stream's norm.  `generate` continues byte or token sequences with `process_logits`.
+reads the stream's norm.  With `train_embedding` or an `embedding_scale` the token embedding is a
+`TokenEmbedding`.  `generate` continues byte or token sequences with `process_logits`, and
+`generate_beams` searches for the likeliest continuations with `beam_select` and `reorder_states`.
 """
 import math
 
 import torch
 import torch.nn as nn
 
-from ..lm import ResidualNorm, process_logits
+from ..lm import ResidualNorm, TokenEmbedding, beam_select, process_logits, reorder_states
 from .LUTLayer import Conv2DLUTLayer, GradientPolicy, LUTLayer, LUTSharedContext, SynapseMeta
 
 
@@ -34,7 +36,10 @@ class LUTTransformer(nn.Module):
     options (post_norm, pre_norm, bias, gate, residual_scale, branch_scale, eps) for both joins
     of every block; their dropout is `dropout`, from counters seeded by `dropout_seed` (without it
     `seed`) and the join's number: data-parallel ranks have one `seed`, for equal weights, and
-    each a `dropout_seed`.  It excludes use_batch_norm."""
+    each a `dropout_seed`.  It excludes use_batch_norm.
+
+    train_embedding: the embedding is a parameter that learns (the reference's is frozen).
+    embedding_scale: a number that the embeddings are multiplied by."""
 
     residual_join = None  # of models that were pickled before there was one
 
@@ -45,7 +50,7 @@ class LUTTransformer(nn.Module):
                  device=None, synapse_meta=SynapseMeta(), lut_shared_context=None, seed=None,
                  summation_dtype=torch.float32, _int_rescaler=0.001, _forward_group_size=32,
                  _backward_group_size=32, dropout=0.0, use_batch_norm=False, residual_join=None,
-                 dropout_seed=None):
+                 dropout_seed=None, train_embedding=False, embedding_scale=1.0):
         super().__init__()
         if isinstance(embedding_dim, int):
             n_embeddings = embedding_dim
@@ -82,8 +87,11 @@ class LUTTransformer(nn.Module):
         self.lut_shared_context = lut_shared_context
 
         E = n_embeddings
-        self.token_embedder = nn.Embedding(vocab_size, E, device=self.device)
-        self.token_embedder.weight.requires_grad_(False)
+        if train_embedding or embedding_scale != 1.0:
+            self.token_embedder = TokenEmbedding(vocab_size, E, embedding_scale, device=self.device)
+        else:
+            self.token_embedder = nn.Embedding(vocab_size, E, device=self.device)
+        self.token_embedder.weight.requires_grad_(bool(train_embedding))
         with torch.no_grad():
             if seed is not None:
                 gen = torch.Generator(device=self.device)
@@ -266,6 +274,72 @@ class LUTTransformer(nn.Module):
         if bool(stuck.any()):
             raise ValueError("no token to choose: the mask leaves nothing of a row, or its logits are NaN or infinite")
         return out
+
+    @torch.no_grad()
+    def generate_beams(self, tokens, n_new, beams, lengths=None, end=None, length_penalty=0.0, **processing):
+        """(sequences [B, beams, L + n_new], scores [B, beams]): the continuations of tokens [B, L] that a
+        beam search with `beams` beams finds, the best first.  A row's first `lengths` tokens are its
+        prompt (all, without); a beam's new tokens follow the prompt, zeros the last of them.  A beam that
+        has chosen the token `end` has finished: zeros follow it, and the search ends before n_new tokens
+        where all have.  Scores are the sums of the new tokens' log-probabilities under the logits after
+        process_logits with `processing`; beams are ordered by score / (new tokens) ** length_penalty.
+        Of a prompt with fewer continuations than beams, the last have the score -infinity.  Raises where a
+        search is left with no continuation, or with logits of NaN or infinity."""
+        B, L = tokens.shape
+        K, S, device = beams, self.context_size, tokens.device
+        prompt = torch.full((B,), L, dtype=torch.int64, device=device) if lengths is None else \
+            lengths.to(device=device, dtype=torch.int64)
+        if L == 0 or int(prompt.min()) < 1 or int(prompt.max()) > L:
+            raise ValueError("a prompt has 1 to L tokens")
+        out = torch.cat([tokens, tokens.new_zeros(B, n_new)], 1)
+        out = out.masked_fill(torch.arange(L + n_new, device=device) >= prompt[:, None], 0)
+        out = out[:, None].expand(B, K, L + n_new).contiguous()
+        # all beams are alike at first: one of them is alive
+        scores = torch.full((B, K), -math.inf, device=device)
+        scores[:, 0] = 0.0
+        finished = torch.zeros(B, K, dtype=torch.bool, device=device)
+        grown = torch.zeros(B, K, dtype=torch.int64, device=device)
+        prompts = prompt[:, None].expand(B, K).reshape(-1)
+        rows, ahead = torch.arange(B * K, device=device), torch.arange(S, device=device)
+        stuck = torch.zeros(B, dtype=torch.bool, device=device)
+        # one value for each prompt is one for each of its beams
+        processing = {k: v.repeat_interleave(K, 0) if self._by_prompt(k, v, B) else v for k, v in processing.items()}
+        training = [m for m in self.modules() if m.training]
+        self.eval()
+        try:
+            for i in range(n_new):
+                flat = out.view(B * K, -1)
+                length = prompts + grown.view(-1)
+                start = (length - S).clamp_min(0)
+                at = (start[:, None] + ahead).clamp_max(L + n_new - 1)
+                logits = self(flat.gather(1, at))[rows, length - start - 1]
+                logits = process_logits(logits, tokens=flat, lengths=length, prompt_lengths=prompts, **processing)
+                scores, parents, new = beam_select(logits.view(B, K, -1), scores, finished=finished, lengths=grown,
+                                                   length_penalty=length_penalty)
+                reorder_states([out, finished, grown], parents, out=[out, finished, grown])
+                # a finished beam's position holds a zero, and a beam that is not there nothing to read
+                position = (prompt[:, None] + grown).clamp_max(L + n_new - 1)
+                last = out.gather(2, position[:, :, None])[:, :, 0]
+                out.scatter_(2, position[:, :, None], torch.where(finished, last, new.to(out.dtype))[:, :, None])
+                grown += ~finished
+                if end is not None:
+                    finished |= new == end
+                stuck |= scores[:, 0].isnan() | (scores[:, 0] == -math.inf)
+                if end is not None and bool((finished | (scores == -math.inf)).all()):
+                    break
+        finally:
+            for m in training:  # not train(), which takes along modules held in evaluation
+                m.training = True
+        if bool(stuck.any()):
+            raise ValueError("no continuation to choose: the mask leaves nothing of a row, or its logits are NaN or infinite")
+        return out, scores
+
+    @staticmethod
+    def _by_prompt(name, value, B):
+        """Whether an option of process_logits has one value, or row, for each prompt."""
+        if not isinstance(value, torch.Tensor):
+            return False
+        return value.dim() == (1 if name.endswith("penalty") or name == "temperature" else 2) and value.shape[0] == B
 
     def to(self, *args, **kwargs):
         device = kwargs.get("device", args[0] if args and isinstance(args[0], (str, torch.device)) else None)
