@@ -23,7 +23,7 @@ extern "C" {
  * out[i] = scale * weight[tokens[i]], each product rounded to 32 bits and then to
  * out's type; zeros where a token is outside [0, vocab). */
 typedef struct {
-    uint64_t n, vocab, cols;   /* tokens, rows and columns of the table: n < 2^31, vocab < 2^31, cols <= 2^26 */
+    uint64_t n, vocab, cols;   /* tokens, rows and columns of the table: n < 2^31, vocab < 2^31, cols <= 2^23 */
     int tokens_i64;            /* tokens are int64; else int32 */
     int weight_dtype;          /* of the table and its gradient */
     int out_dtype;             /* of out and its gradient: weight_dtype, or one of the two is F32 */

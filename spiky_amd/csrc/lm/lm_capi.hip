@@ -82,7 +82,7 @@ void check(const spiky_lm_embed_args *a) {
     require(is_type(a->weight_dtype) && is_type(a->out_dtype), "unknown element type");
     require(a->weight_dtype == a->out_dtype || a->weight_dtype == SPIKY_F32 || a->out_dtype == SPIKY_F32,
             "the table and the result must have one type, or one of them fp32");
-    require(a->n < 0x80000000ull && a->vocab < 0x80000000ull && a->cols <= 0x4000000ull,
+    require(a->n < 0x80000000ull && a->vocab < 0x80000000ull && a->cols <= 0x800000ull,
             "too many tokens, rows or columns");
 }
 

@@ -70,10 +70,19 @@ hipError_t lookup(const spiky_lm_embed_args &a, void *out, hipStream_t st) {
 // ---- gradient ------------------------------------------------------------------
 // The tokens' positions, sorted by token and for each token in ascending order, and where each
 // token's begin: start [vocab + 1], order [start[vocab]].  One launch without any exchange between
-// workgroups: a workgroup owns `range` consecutive tokens of the vocabulary, reads all n, counts its
-// own for each wave's share of the positions and those below its range, adds up, and reads them
-// again to place its own.  Tokens outside the vocabulary are in no range.
+// workgroups: a workgroup owns `range` consecutive tokens of the vocabulary, reads all n, lists its
+// own for each wave's share of the positions, counts these and the ones below its range, adds up,
+// and places its own.  A wave with more of its own than its list holds reads its share again.
+// Tokens outside the vocabulary are in no range.
 constexpr int kSortWaves = 16, kMostRange = 1024;
+constexpr uint32_t kList = 512;                        // of a wave
+constexpr uint32_t kListShare = 0xffffffffu / kMostRange;  // positions of a share that a list's words can tell apart
+
+// A token as 32 bits: those outside any vocabulary stay outside.
+__device__ __forceinline__ uint32_t narrow(int64_t token) {
+    return (uint64_t)token >> 32 ? ~0u : (uint32_t)token;
+}
+__device__ __forceinline__ uint32_t narrow(int32_t token) { return (uint32_t)token; }
 
 template <typename Tok>
 __global__ __launch_bounds__(kSortWaves * 64) void k_embed_sort(const Tok *__restrict__ tokens, uint32_t n,
@@ -81,35 +90,50 @@ __global__ __launch_bounds__(kSortWaves * 64) void k_embed_sort(const Tok *__res
                                                                 uint32_t *__restrict__ start,
                                                                 uint32_t *__restrict__ order) {
     extern __shared__ uint32_t counts[];  // [kSortWaves][range]
-    __shared__ uint32_t below_of[kSortWaves], sum_of[kSortWaves];
+    __shared__ uint32_t lists[kSortWaves][kList], below_of[kSortWaves], sum_of[kSortWaves];
     const uint32_t wave = threadIdx.x / 64, lane = threadIdx.x & 63;
+    const uint64_t lower = ((uint64_t)1 << lane) - 1;
     const uint32_t base = blockIdx.x * range, size = min(range, vocab - base);
     for (uint32_t i = threadIdx.x; i < kSortWaves * range; i += kSortWaves * 64) counts[i] = 0;
     __syncthreads();
     const uint32_t share = (n / (kSortWaves * 64) + 1) * 64;
     const uint32_t begin = min(wave * share, n), end = min(begin + share, n);
-    uint32_t *mine = counts + wave * range, below = 0;
+    uint32_t *mine = counts + wave * range, *list = lists[wave], below = 0, listed = 0;
     constexpr int kAhead = 8;
-    // fn(position of the wave's lane 0, offset in the range or past it, token is below the range)
+    // fn(position of the wave's lane 0, the lane's token)
     auto each = [&](auto fn) {
+        if (begin >= end) return;
+        Tok id[kAhead], next[kAhead];  // no lane's load hangs on a condition: all are in flight at once
+#pragma unroll
+        for (int k = 0; k < kAhead; k++) next[k] = tokens[min(begin + k * 64 + lane, end - 1)];
         for (uint32_t at = begin; at < end; at += 64 * kAhead) {
-            Tok id[kAhead];
 #pragma unroll
-            for (int k = 0; k < kAhead; k++) {
-                const uint32_t i = at + k * 64 + lane;
-                id[k] = i < end ? tokens[i] : (Tok)-1;
-            }
+            for (int k = 0; k < kAhead; k++) id[k] = next[k];
 #pragma unroll
-            for (int k = 0; k < kAhead; k++) {
-                // base < 2^31, so a negative token stays past any range
-                const uint64_t o = (uint64_t)(int64_t)id[k] - base;
-                fn(at + k * 64, o < size ? (uint32_t)o : ~0u, id[k] >= 0 && id[k] < (Tok)base);
-            }
+            for (int k = 0; k < kAhead; k++) next[k] = tokens[min(at + (kAhead + k) * 64 + lane, end - 1)];
+#pragma unroll
+            for (int k = 0; k < kAhead; k++) fn(at + k * 64, at + k * 64 + lane < end ? narrow(id[k]) : ~0u);
         }
     };
-    each([&](uint32_t, uint32_t o, bool lower) {
-        if (o != ~0u) atomicAdd(&mine[o], 1u);
-        below += lower;
+    each([&](uint32_t first, uint32_t id) {
+        const uint32_t o = id - base;
+        below += id < base;  // base <= vocab, so tokens outside are not
+        const uint64_t own = __ballot(o < size);
+        if (own == 0) return;
+        // many lanes with one token, as where a batch is padded with it, count as one: 32768 times one
+        // token take KK us against 43
+        uint32_t counted = ~0u;
+        if (__popcll(own) >= 16) {
+            counted = __builtin_amdgcn_readlane(o, __builtin_ctzll(own));
+            const uint64_t same = __ballot(o == counted);
+            if (lane == 0) atomicAdd(&mine[counted], (uint32_t)__popcll(same));
+        }
+        if (o < size) {
+            if (o != counted) atomicAdd(&mine[o], 1u);
+            const uint32_t at = listed + __popcll(own & lower);
+            if (at < kList) list[at] = (first - begin + lane) * kMostRange + o;
+        }
+        listed += __popcll(own);
     });
     for (int k = 32; k >= 1; k /= 2) below += __shfl_xor(below, k);
     if (lane == 0) below_of[wave] = below;
@@ -136,18 +160,27 @@ __global__ __launch_bounds__(kSortWaves * 64) void k_embed_sort(const Tok *__res
         }
     }
     __syncthreads();
-    each([&](uint32_t first, uint32_t o, bool) {
+    // Places the lanes' positions whose tokens are o in the range, or none where that is ~0.
+    auto place = [&](uint32_t position, uint32_t o) {
         for (uint64_t left = __ballot(o != ~0u); left;) {
             const uint32_t leader = __builtin_ctzll(left);
             const uint32_t token = __builtin_amdgcn_readlane(o, leader);
             const uint64_t same = __ballot(o == token);
-            uint32_t place = 0;
-            if (lane == leader) place = atomicAdd(&mine[token], (uint32_t)__popcll(same));
-            place = __builtin_amdgcn_readlane(place, leader);
-            if (o == token) order[place + __popcll(same & (((uint64_t)1 << lane) - 1))] = first + lane;
+            uint32_t to = 0;
+            if (lane == leader) to = atomicAdd(&mine[token], (uint32_t)__popcll(same));
+            to = __builtin_amdgcn_readlane(to, leader);
+            if (o == token) order[to + __popcll(same & lower)] = position;
             left &= ~same;
         }
-    });
+    };
+    if (listed <= kList && share <= kListShare) {
+        for (uint32_t i = 0; i < listed; i += 64) {
+            const uint32_t word = i + lane < listed ? list[i + lane] : ~0u;
+            place(begin + word / kMostRange, word == ~0u ? ~0u : word % kMostRange);
+        }
+    } else {
+        each([&](uint32_t first, uint32_t id) { place(first + lane, id - base < size ? id - base : ~0u); });
+    }
 }
 
 // Positions of a token that are added up one after the other: tokens with more ("frequent") go in
@@ -155,6 +188,8 @@ __global__ __launch_bounds__(kSortWaves * 64) void k_embed_sort(const Tok *__res
 // frequent token stands at every tenth position or so: as one row's sum it took 1.9 ms of 32768
 // tokens' gradient, ten times the rest.
 constexpr uint32_t kChunk = 32;
+constexpr uint64_t kManyGroups = 64 * kCUs;
+constexpr uint64_t kLastCache = 256u << 20;  // bytes; what is written past it does not stay there for its reader
 
 // The sum over positions [from, to) of the columns at d_out; `from < to`.
 template <int N, typename T>
@@ -199,12 +234,10 @@ __device__ __forceinline__ Run run_at(const Tok *tokens, const uint32_t *start, 
 
 // The first `chunks` workgroups of x take chunk blockIdx.x of the sorted positions: the runs of its
 // first and its last one are the only frequent ones that it can hold a part of, since these are
-// longer; their sums go to partial [2 * chunk] and [2 * chunk + 1].  The others take kRows rows of
-// the table's gradient, of tokens that are not frequent.  `lanes` threads, a power of two, take the
+// longer; their sums go to partial [2 * chunk] and [2 * chunk + 1].  The others take
+// kRows rows a thread of the table's gradient, of tokens that are not frequent.  `lanes` threads, a power of two, take the
 // pieces of a row.
-constexpr uint32_t kRows = 8;
-
-template <typename Tok, typename T, typename W>
+template <typename Tok, typename T, typename W, uint32_t kRows, bool kStream>
 __global__ __launch_bounds__(kThreads) void k_embed_sum(const Tok *__restrict__ tokens, const T *__restrict__ d_out,
                                                         int64_t stride, const uint32_t *__restrict__ start,
                                                         const uint32_t *__restrict__ order, W *__restrict__ d_weight,
@@ -251,13 +284,19 @@ __global__ __launch_bounds__(kThreads) void k_embed_sum(const Tok *__restrict__ 
         }
 #pragma unroll
         for (int k = 0; k < N; k++) sum[k] *= scale;
-        store(d_weight + (row0 + r * rows) * cols + place.col, sum, place.n);
+        W *to_row = d_weight + (row0 + r * rows) * cols + place.col;
+        if (kStream)
+            stream_out(to_row, sum, place.n);
+        else
+            store(to_row, sum, place.n);
     }
 }
 
-// The rows of frequent tokens, from their chunks' sums: workgroup x adds up the run that begins in
-// chunk x and goes on into the next one, 64 lanes a group of columns, wave w the sums number w,
-// w + 4, ... of the run.
+// The rows of frequent tokens, from their chunks' sums: workgroup x adds up the runs that begin in
+// kJoined chunks from x * kJoined on and go on into the next one, 64 lanes a group of columns, wave w the
+// sums number w, w + 4, ... of a run.
+constexpr uint32_t kJoined = 8;
+
 template <typename Tok, typename W>
 __global__ __launch_bounds__(kThreads) void k_embed_join(const Tok *__restrict__ tokens,
                                                          const uint32_t *__restrict__ start,
@@ -267,39 +306,47 @@ __global__ __launch_bounds__(kThreads) void k_embed_join(const Tok *__restrict__
     constexpr int N = 4, kAhead = 8;
     constexpr uint32_t kWaves = kThreads / 64;
     __shared__ float sums[kWaves - 1][N][64];
-    const uint32_t chunk = blockIdx.x, n = start[vocab], wave = threadIdx.x / 64, lane = threadIdx.x & 63;
-    if (chunk * kChunk >= n) return;
-    const uint32_t end = min((chunk + 1) * kChunk, n);
-    const Run run = run_at(tokens, start, order, end - 1);
-    if (!run.frequent || run.from < chunk * kChunk) return;
+    const uint32_t n = start[vocab], wave = threadIdx.x / 64, lane = threadIdx.x & 63;
+    const uint32_t chunk0 = blockIdx.x * kJoined;
+    // a lane a chunk, the same in all waves
+    Run mine = {0, 0, false};
+    if (lane < kJoined && (chunk0 + lane) * kChunk < n) {
+        mine = run_at(tokens, start, order, min((chunk0 + lane + 1) * kChunk, n) - 1);
+        mine.frequent = mine.frequent && mine.from >= (chunk0 + lane) * kChunk;
+    }
     Place<N> place;
     place.set(cols, ((uint64_t)blockIdx.y * 64 + lane) * N);
-    const uint32_t parts = (run.to - 1) / kChunk - chunk + 1;
-    // a run that begins inside its first chunk is that one's last
-    const uint32_t skew = run.from > chunk * kChunk ? 1 : 0;
-    const float *p = partial + (uint64_t)chunk * 2 * cols + place.col;
-    float sum[N] = {};
-    for (uint32_t i = wave; i < parts; i += kWaves * kAhead) {
-        Raw<float, N> raw[kAhead];
+    for (uint64_t found = __ballot(mine.frequent); found; found &= found - 1) {
+        const uint32_t l = __builtin_ctzll(found), chunk = chunk0 + l;
+        const uint32_t from = __builtin_amdgcn_readlane(mine.from, l), to = __builtin_amdgcn_readlane(mine.to, l);
+        const uint32_t parts = (to - 1) / kChunk - chunk + 1;
+        // a run that begins inside its first chunk is that one's last
+        const uint32_t skew = from > chunk * kChunk ? 1 : 0;
+        const float *p = partial + (uint64_t)chunk * 2 * cols + place.col;
+        float sum[N] = {};
+        for (uint32_t i = wave; i < parts; i += kWaves * kAhead) {
+            Raw<float, N> raw[kAhead];
 #pragma unroll
-        for (uint32_t j = 0; j < kAhead; j++) {
-            const uint32_t k = i + j * kWaves;
-            raw[j].clear();
-            if (k < parts) raw[j].load(p + ((uint64_t)k * 2 + (k == 0 ? skew : 0)) * cols, place.n);
+            for (uint32_t j = 0; j < kAhead; j++) {
+                const uint32_t k = i + j * kWaves;
+                raw[j].clear();
+                if (k < parts) raw[j].load(p + ((uint64_t)k * 2 + (k == 0 ? skew : 0)) * cols, place.n);
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < kAhead; j++)
+#pragma unroll
+                for (int k = 0; k < N; k++) sum[k] += raw[j][k];
         }
-#pragma unroll
-        for (uint32_t j = 0; j < kAhead; j++)
-#pragma unroll
-            for (int k = 0; k < N; k++) sum[k] += raw[j][k];
+        __syncthreads();  // the sums of the run before are read
+        if (wave > 0)
+            for (int k = 0; k < N; k++) sums[wave - 1][k][lane] = sum[k];
+        __syncthreads();
+        if (wave > 0 || place.n == 0) continue;
+        for (uint32_t w = 0; w < kWaves - 1; w++)
+            for (int k = 0; k < N; k++) sum[k] += sums[w][k][lane];
+        for (int k = 0; k < N; k++) sum[k] *= scale;
+        store(d_weight + (uint64_t)tokens[order[from]] * cols + place.col, sum, place.n);
     }
-    if (wave > 0)
-        for (int k = 0; k < N; k++) sums[wave - 1][k][lane] = sum[k];
-    __syncthreads();
-    if (wave > 0 || place.n == 0) return;
-    for (uint32_t w = 0; w < kWaves - 1; w++)
-        for (int k = 0; k < N; k++) sum[k] += sums[w][k][lane];
-    for (int k = 0; k < N; k++) sum[k] *= scale;
-    store(d_weight + (uint64_t)tokens[order[run.from]] * cols + place.col, sum, place.n);
 }
 
 // The workspace: starts, order, and the chunks' sums.
@@ -332,15 +379,22 @@ hipError_t sums(const spiky_lm_embed_args &a, const void *d_out_, int64_t stride
     uint32_t lanes = 1;
     while (lanes < pieces && lanes < kThreads) lanes *= 2;
     const uint32_t rows = kThreads / lanes, chunks = (uint32_t)chunks_of(a), groups = (chunks + rows - 1) / rows;
-    const uint64_t all = groups + (a.vocab + rows * kRows - 1) / (rows * kRows);
-    if (all * kThreads > 0xffffffffull) return hipErrorInvalidValue;
-    const dim3 grid((uint32_t)all, (uint32_t)((pieces + lanes - 1) / lanes));
-    k_embed_sum<Tok, T, W><<<grid, dim3(kThreads), 0, st>>>(tokens, d_out, stride, start, order, d_weight, partial,
-                                                            (uint32_t)a.vocab, a.cols, chunks, groups, lanes,
-                                                            (float)a.scale);
-    const hipError_t e = hipGetLastError();
+    const uint64_t slabs = (pieces + lanes - 1) / lanes;
+    auto go = [&](auto kernel, uint64_t each) {
+        const uint64_t all = groups + (a.vocab + rows * each - 1) / (rows * each);
+        if (all * kThreads > 0xffffffffull) return hipErrorInvalidValue;
+        kernel<<<dim3((uint32_t)all, (uint32_t)slabs), dim3(kThreads), 0, st>>>(
+            tokens, d_out, stride, start, order, d_weight, partial, (uint32_t)a.vocab, a.cols, chunks, groups, lanes,
+            (float)a.scale);
+        return hipGetLastError();
+    };
+    // several rows to a thread where there are enough: most have no token, and only their zeros to write
+    const bool many = a.vocab / rows * slabs >= kManyGroups;
+    const bool stream = a.vocab * a.cols * sizeof(W) >= kLastCache * 2;
+    const hipError_t e = many ? stream ? go(k_embed_sum<Tok, T, W, 4, true>, 4) : go(k_embed_sum<Tok, T, W, 4, false>, 4)
+                              : go(k_embed_sum<Tok, T, W, 1, false>, 1);
     if (e != hipSuccess || chunks == 0) return e;
-    k_embed_join<Tok, W><<<dim3(chunks, (uint32_t)((a.cols + 255) / 256)), dim3(kThreads), 0, st>>>(
+    k_embed_join<Tok, W><<<dim3((chunks + kJoined - 1) / kJoined, (uint32_t)((a.cols + 255) / 256)), dim3(kThreads), 0, st>>>(
         tokens, start, order, d_weight, partial, (uint32_t)a.vocab, a.cols, (float)a.scale);
     return hipGetLastError();
 }
