@@ -38,72 +38,50 @@ __device__ __forceinline__ Kind kind_of(const spiky_lm_beams_args &a, uint64_t r
     return a.finished && a.finished[row] ? kFinished : kLive;
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void k_beam_slices(const spiky_lm_beams_args a, const Parts parts) {
-    constexpr int N = 16 / sizeof(T);
+// Floats as whole numbers in their order, without NaN; both zeros are one.
+__device__ __forceinline__ uint32_t ordered(float x) {
+    const uint32_t u = __float_as_uint(x + 0.f);
+    return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+}
+
+// A number that at least n of the wave's 64 values reach, in its upper `bits` bits: the largest such.
+template <int bits>
+__device__ __forceinline__ uint32_t reached_by(uint32_t value, uint32_t n) {
+    uint32_t found = 0;
+#pragma unroll
+    for (int i = 31; i > 31 - bits; i--) {
+        const uint32_t more = found | 1u << i;
+        if (__popcll(__ballot(value >= more)) >= n) found = more;
+    }
+    return found;
+}
+
+constexpr uint32_t kMostListed = 1024;
+
+// The slice's n first candidates, one round for each: for lists that too many candidates would be
+// on, as where most logits are equal.
+template <int N>
+__device__ __forceinline__ void first_by_rounds(const float (&v)[kPieces][N], const uint32_t (&col)[kPieces],
+                                                float *logits, uint32_t *tokens, uint32_t n) {
     __shared__ float wave_value[2][kWaves];
     __shared__ uint32_t wave_token[2][kWaves];
-    const uint64_t row = blockIdx.y + (uint64_t)blockIdx.z * 32768;
-    if (row >= a.searches * a.beams || kind_of(a, row) != kLive) return;
-    const uint32_t slice = blockIdx.x, wave = threadIdx.x / 64, lane = threadIdx.x & 63;
-    const T *x = static_cast<const T *>(a.logits) + (int64_t)(row / a.beams) * a.search_stride +
-                 (int64_t)(row % a.beams) * a.beam_stride;
-    float v[kPieces][N];
-    uint32_t col[kPieces];
-    float top = -INFINITY;
-#pragma unroll
-    for (int p = 0; p < kPieces; p++) {
-        Place<N> place;
-        place.set(a.vocab, (uint64_t)slice * slice_size<T>() + (p * kThreads + threadIdx.x) * N);
-        load(v[p], x + place.col, place.n);
-        col[p] = (uint32_t)place.col;
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            v[p][i] = place.own >> i & 1 ? v[p][i] : -INFINITY;
-            top = fmaxf(top, v[p][i]);
-        }
-    }
-    for (int k = 32; k >= 1; k /= 2) top = fmaxf(top, __shfl_xor(top, k));
-    if (lane == 0) wave_value[0][wave] = top;
-    __syncthreads();
-    for (int w = 0; w < kWaves; w++) top = fmaxf(top, wave_value[0][w]);
-    const float from = top == -INFINITY ? 0.f : top;
-    float sum = 0.f;
-#pragma unroll
-    for (int p = 0; p < kPieces; p++)
-#pragma unroll
-        for (int i = 0; i < N; i++) sum += __expf(v[p][i] - from);
-    for (int k = 32; k >= 1; k /= 2) sum += __shfl_xor(sum, k);
-    if (lane == 0) wave_value[1][wave] = sum;
-    __syncthreads();
-    const uint64_t at = row * parts.slices + slice;
-    if (threadIdx.x == 0) {
-        sum = 0.f;
-        for (int w = 0; w < kWaves; w++) sum += wave_value[1][w];
-        parts.stats[at] = make_float2(top, sum);
-    }
-    __syncthreads();
+    const uint32_t wave = threadIdx.x / 64, lane = threadIdx.x & 63;
     float last = INFINITY;
-    uint32_t last_token = ~0u;
-    for (uint32_t r = 0; r < parts.n; r++) {
+    uint32_t last_token = 0;
+    for (uint32_t r = 0; r < n; r++) {
         float best = -INFINITY;
         uint32_t token = ~0u;
-#pragma unroll
-        for (int p = 0; p < kPieces; p++)
-#pragma unroll
-            for (int i = 0; i < N; i++) {
-                const bool left = before(last, last_token, v[p][i], col[p] + i) || r == 0;
-                if (left && before(v[p][i], col[p] + i, best, token) && v[p][i] > -INFINITY) {
-                    best = v[p][i];
-                    token = col[p] + i;
-                }
-            }
         auto take = [&](float y, uint32_t other) {
             if (before(y, other, best, token)) {
                 best = y;
                 token = other;
             }
         };
+#pragma unroll
+        for (int p = 0; p < kPieces; p++)
+#pragma unroll
+            for (int i = 0; i < N; i++)
+                if (before(last, last_token, v[p][i], col[p] + i) && v[p][i] > -INFINITY) take(v[p][i], col[p] + i);
         for (int k = 32; k >= 1; k /= 2) take(__shfl_xor(best, k), __shfl_xor(token, k));
         if (lane == 0) {
             wave_value[r & 1][wave] = best;
@@ -112,11 +90,118 @@ __global__ __launch_bounds__(kThreads) void k_beam_slices(const spiky_lm_beams_a
         __syncthreads();
         for (int w = 0; w < kWaves; w++) take(wave_value[r & 1][w], wave_token[r & 1][w]);
         if (threadIdx.x == 0) {
-            parts.logits[at * parts.n + r] = best;
-            parts.tokens[at * parts.n + r] = token;
+            logits[r] = best;
+            tokens[r] = token;
         }
         last = best;
         last_token = token;
+    }
+}
+
+// The n first candidates are among the values that reach a threshold which n of 64 groups of lanes
+// reach with their largest: a few more than n of random logits.  These are listed, and each counts
+// those before it.  n rounds over the registers, each with a barrier, took 410 us where this takes KK
+// (512 beams of 152000 bf16, n = 16).
+template <typename T>
+__global__ __launch_bounds__(kThreads) void k_beam_slices(const spiky_lm_beams_args a, const Parts parts) {
+    constexpr int N = 16 / sizeof(T);
+    __shared__ float group_top[64], wave_sum[kWaves];
+    __shared__ uint64_t list[kMostListed];
+    __shared__ uint32_t threshold, listed;
+    const uint64_t row = blockIdx.y + (uint64_t)blockIdx.z * 32768;
+    if (row >= a.searches * a.beams || kind_of(a, row) != kLive) return;
+    const uint32_t slice = blockIdx.x, wave = threadIdx.x / 64, lane = threadIdx.x & 63;
+    const T *x = static_cast<const T *>(a.logits) + (int64_t)(row / a.beams) * a.search_stride +
+                 (int64_t)(row % a.beams) * a.beam_stride;
+    float v[kPieces][N];
+    uint32_t col[kPieces];
+    const uint64_t first = (uint64_t)slice * slice_size<T>();
+    if (first + slice_size<T>() <= a.vocab) {
+        Raw<T, N> raw[kPieces];
+#pragma unroll
+        for (int p = 0; p < kPieces; p++) {
+            col[p] = (uint32_t)first + (p * kThreads + threadIdx.x) * N;
+            raw[p].load(x + col[p], N);
+        }
+#pragma unroll
+        for (int p = 0; p < kPieces; p++)
+#pragma unroll
+            for (int i = 0; i < N; i++) v[p][i] = raw[p][i];
+    } else {
+#pragma unroll
+        for (int p = 0; p < kPieces; p++) {
+            Place<N> place;
+            place.set(a.vocab, first + (p * kThreads + threadIdx.x) * N);
+            load(v[p], x + place.col, place.n);
+            col[p] = (uint32_t)place.col;
+#pragma unroll
+            for (int i = 0; i < N; i++) v[p][i] = place.own >> i & 1 ? v[p][i] : -INFINITY;
+        }
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int p = 0; p < kPieces; p++)
+#pragma unroll
+        for (int i = 0; i < N; i++) top = fmaxf(top, v[p][i]);
+    top = fmaxf(top, __shfl_xor(top, 1));
+    top = fmaxf(top, __shfl_xor(top, 2));
+    if ((lane & 3) == 0) group_top[threadIdx.x / 4] = top;
+    if (threadIdx.x == 0) listed = 0;
+    __syncthreads();
+    const float of_group = group_top[lane];
+    top = of_group;
+    for (int k = 32; k >= 1; k /= 2) top = fmaxf(top, __shfl_xor(top, k));
+    if (wave == 0) {
+        const uint32_t t = reached_by<16>(ordered(of_group), parts.n);
+        if (lane == 0) threshold = t;
+    }
+    const float from = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+#pragma unroll
+    for (int p = 0; p < kPieces; p++)
+#pragma unroll
+        for (int i = 0; i < N; i++) sum += __expf(v[p][i] - from);
+    for (int k = 32; k >= 1; k /= 2) sum += __shfl_xor(sum, k);
+    if (lane == 0) wave_sum[wave] = sum;
+    __syncthreads();
+    const uint64_t at = row * parts.slices + slice;
+    if (threadIdx.x == 0) {
+        sum = 0.f;
+        for (int w = 0; w < kWaves; w++) sum += wave_sum[w];
+        parts.stats[at] = make_float2(top, sum);
+    }
+    const uint32_t least = threshold;
+#pragma unroll
+    for (int p = 0; p < kPieces; p++)
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            // NaN in a beam makes its candidates known without a list
+            if (ordered(v[p][i]) >= least && v[p][i] > -INFINITY) {
+                const uint32_t k = atomicAdd(&listed, 1u);
+                if (k < kMostListed) list[k] = (uint64_t)ordered(v[p][i]) << 32 | (uint32_t)~(col[p] + i);
+            }
+        }
+    __syncthreads();
+    const uint32_t count = listed;
+    float *logits = parts.logits + at * parts.n;
+    uint32_t *tokens = parts.tokens + at * parts.n;
+    if (count > kMostListed) {
+        first_by_rounds<N>(v, col, logits, tokens, parts.n);
+        return;
+    }
+    for (uint32_t i = threadIdx.x; i < max(count, parts.n); i += kThreads) {
+        if (i >= count) {
+            logits[i] = -INFINITY;
+            continue;
+        }
+        const uint64_t own = list[i];
+        uint32_t rank = 0;
+        for (uint32_t k = 0; k < count; k++) rank += list[k] > own;
+        if (rank < parts.n) {
+            const uint32_t u = (uint32_t)(own >> 32);
+            logits[rank] = __uint_as_float(u ^ (~(uint32_t)((int32_t)u >> 31) | 0x80000000u));
+            tokens[rank] = ~(uint32_t)own;
+        }
     }
 }
 
@@ -151,12 +236,26 @@ struct Beam {
     bool unknown;   // its scores are NaN
 };
 
-__global__ __launch_bounds__(kThreads) void k_beam_join(const spiky_lm_beams_args a, const Parts parts) {
+constexpr int kJoinThreads = 512, kJoinWaves = kJoinThreads / 64;
+
+// The same of doubles.
+__device__ __forceinline__ uint64_t ordered(double x) {
+    const uint64_t u = (uint64_t)__double_as_longlong(x + 0.0);
+    return u ^ ((uint64_t)((int64_t)u >> 63) | (uint64_t)1 << 63);
+}
+
+// A workgroup a search.  As in a slice, candidates that reach what n groups of candidates reach are
+// listed, and each counts those before it; the groups are made of the first candidates of the
+// slices' lists.
+__global__ __launch_bounds__(kJoinThreads) void k_beam_join(const spiky_lm_beams_args a, const Parts parts) {
+    constexpr uint32_t kMost = 512;
     __shared__ Beam beams[kMostBeams];
-    __shared__ Candidate wave_best[2][kWaves];
+    __shared__ Candidate list[kMost], wave_best[2][kJoinWaves];
+    __shared__ uint64_t group_top[kJoinWaves][64];
+    __shared__ uint32_t threshold, listed;
     const uint64_t search = blockIdx.x, row0 = search * a.beams;
     const uint32_t wave = threadIdx.x / 64, lane = threadIdx.x & 63;
-    for (uint32_t k = wave; k < a.beams; k += kWaves) {
+    for (uint32_t k = wave; k < a.beams; k += kJoinWaves) {
         const uint64_t row = row0 + k;
         Beam b;
         b.kind = kind_of(a, row);
@@ -187,40 +286,84 @@ __global__ __launch_bounds__(kThreads) void k_beam_join(const spiky_lm_beams_arg
         }
         if (lane == 0) beams[k] = b;
     }
+    if (threadIdx.x == 0) listed = 0;
     __syncthreads();
-    const uint64_t each = (uint64_t)parts.slices * parts.n, all = a.beams * each;
+    const uint64_t lists = a.beams * parts.slices;
     const Candidate none = {-INFINITY, -INFINITY, -INFINITY, ~0u, ~0u};
-    // Candidate number i of the search, or none.
-    auto candidate = [&](uint64_t i) {
+    // Candidate `o` of list `l` of the search, or none.
+    auto candidate = [&](uint64_t l, uint32_t o) {
         Candidate c = none;
-        const uint32_t k = (uint32_t)(i / each);
-        const uint64_t o = i - k * each;
+        const uint32_t k = (uint32_t)(l / parts.slices);
+        const uint64_t slice = l - (uint64_t)k * parts.slices;
         const Beam &b = beams[k];
         if (b.kind == kNothing) return c;
         if (b.kind == kFinished) {
-            if (o != 0) return c;
+            if (slice > 0 || o > 0) return c;
             c.token = 0;
             c.score = b.score;
         } else if (b.unknown) {
-            if (o >= parts.n || o >= a.vocab) return c;
-            c.token = (uint32_t)o;
+            if (slice > 0 || o >= a.vocab) return c;
+            c.token = o;
             c.score = NAN;
         } else {
-            c.logit = parts.logits[row0 * each + i];
+            const uint64_t at = (row0 * parts.slices + l) * parts.n + o;
+            c.logit = parts.logits[at];
             if (c.logit == -INFINITY) return c;
-            c.token = parts.tokens[row0 * each + i];
+            c.token = parts.tokens[at];
             c.score = c.logit - b.top - b.log_sum + b.score;
         }
         c.beam = k;
-        c.rank = c.score / b.length;
+        c.rank = b.length == 1.0 ? c.score : c.score / b.length;
         if (c.rank != c.rank) c.rank = INFINITY;
         return c;
     };
+    // the first `heads` of each list: n or more in all, so that n of the 64 groups hold one
+    const uint32_t heads = (uint32_t)((parts.n + lists - 1) / lists);
+    uint64_t top = 0;
+    for (uint64_t i = threadIdx.x; i < lists * heads; i += kJoinThreads)
+        top = max(top, ordered(candidate(i / heads, (uint32_t)(i % heads)).rank));
+    group_top[wave][lane] = top;
+    __syncthreads();
+    if (wave == 0) {
+        for (int w = 1; w < kJoinWaves; w++) top = max(top, group_top[w][lane]);
+        const uint32_t t = reached_by<24>((uint32_t)(top >> 32), parts.n);
+        if (lane == 0) threshold = t;
+    }
+    __syncthreads();
+    const uint32_t least = threshold;
+    for (uint64_t i = threadIdx.x; i < lists * parts.n; i += kJoinThreads) {
+        const Candidate c = candidate(i / parts.n, (uint32_t)(i % parts.n));
+        if (c.beam == ~0u || ordered(c.rank) >> 32 < least) continue;
+        const uint32_t k = atomicAdd(&listed, 1u);
+        if (k < kMost) list[k] = c;
+    }
+    __syncthreads();
+    const uint32_t count = listed;
+    auto write = [&](uint32_t r, const Candidate &c) {
+        const bool there = c.beam != ~0u;
+        a.out_scores[search * a.n + r] = there ? (float)c.score : -INFINITY;
+        a.out_parents[search * a.n + r] = there ? c.beam : 0;
+        a.out_tokens[search * a.n + r] = there && beams[c.beam].kind == kLive ? c.token : a.pad;
+    };
+    if (count <= kMost) {
+        for (uint32_t i = threadIdx.x; i < max(count, parts.n); i += kJoinThreads) {
+            if (i >= count) {
+                write(i, none);
+                continue;
+            }
+            const Candidate own = list[i];
+            uint32_t rank = 0;
+            for (uint32_t k = 0; k < count; k++) rank += list[k].before(own);
+            if (rank < parts.n) write(rank, own);
+        }
+        return;
+    }
+    // too many of one rank: a round for each
     Candidate last = none;
     for (uint32_t r = 0; r < a.n; r++) {
         Candidate best = none;
-        for (uint64_t i = threadIdx.x; i < all; i += kThreads) {
-            const Candidate c = candidate(i);
+        for (uint64_t i = threadIdx.x; i < lists * parts.n; i += kJoinThreads) {
+            const Candidate c = candidate(i / parts.n, (uint32_t)(i % parts.n));
             if (c.beam != ~0u && (r == 0 || last.before(c)) && c.before(best)) best = c;
         }
         for (int k = 32; k >= 1; k /= 2) {
@@ -229,14 +372,9 @@ __global__ __launch_bounds__(kThreads) void k_beam_join(const spiky_lm_beams_arg
         }
         if (lane == 0) wave_best[r & 1][wave] = best;
         __syncthreads();
-        for (int w = 0; w < kWaves; w++)
+        for (int w = 0; w < kJoinWaves; w++)
             if (wave_best[r & 1][w].before(best)) best = wave_best[r & 1][w];
-        if (threadIdx.x == 0) {
-            const bool there = best.beam != ~0u;
-            a.out_scores[search * a.n + r] = there ? (float)best.score : -INFINITY;
-            a.out_parents[search * a.n + r] = there ? best.beam : 0;
-            a.out_tokens[search * a.n + r] = there && beams[best.beam].kind == kLive ? best.token : a.pad;
-        }
+        if (threadIdx.x == 0) write(r, best);
         last = best;
     }
 }
@@ -342,7 +480,7 @@ hipError_t launch_beam_select(const spiky_lm_beams_args &a, void *workspace, hip
         k_beam_slices<f16><<<grid, dim3(kThreads), 0, st>>>(a, parts);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    k_beam_join<<<dim3((uint32_t)a.searches), dim3(kThreads), 0, st>>>(a, parts);
+    k_beam_join<<<dim3((uint32_t)a.searches), dim3(kJoinThreads), 0, st>>>(a, parts);
     return hipGetLastError();
 }
 

@@ -235,3 +235,14 @@ def test_refusals(cuda_device, case):
 def test_no_searches(cuda_device):
     got = beam_select(torch.zeros(0, 3, 8, device=cuda_device), torch.zeros(0, 3, device=cuda_device), 2)
     assert [t.shape for t in got] == [(0, 2)] * 3
+
+
+def test_zeros_of_both_signs_are_equal(cuda_device):
+    for dtype in (F, B, H):
+        x = torch.zeros(1, 2, 9000, dtype=dtype)
+        x[:, :, ::2] = -0.0
+        got = run(cuda_device, x, torch.zeros(1, 2), 5)
+        assert got[2].tolist() == [[0, 1, 2, 3, 4]]
+        x[:, :, 100:] = -1.0
+        got = run(cuda_device, x, torch.tensor([[-0.0, 0.0]]), 5)
+        assert got[2].tolist() == [[0, 1, 2, 3, 4]] and got[1].tolist() == [[0] * 5]
