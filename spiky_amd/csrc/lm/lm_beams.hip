@@ -44,6 +44,10 @@ __device__ __forceinline__ uint32_t ordered(float x) {
     return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
 }
 
+__device__ __forceinline__ float from_ordered(uint32_t u) {
+    return __uint_as_float(u ^ (~(uint32_t)((int32_t)u >> 31) | 0x80000000u));
+}
+
 // A number that at least n of the wave's 64 values reach, in its upper `bits` bits: the largest such.
 template <int bits>
 __device__ __forceinline__ uint32_t reached_by(uint32_t value, uint32_t n) {
@@ -58,11 +62,11 @@ __device__ __forceinline__ uint32_t reached_by(uint32_t value, uint32_t n) {
 
 constexpr uint32_t kMostListed = 1024;
 
-// The slice's n first candidates, one round for each: for lists that too many candidates would be
-// on, as where most logits are equal.
-template <int N>
-__device__ __forceinline__ void first_by_rounds(const float (&v)[kPieces][N], const uint32_t (&col)[kPieces],
-                                                float *logits, uint32_t *tokens, uint32_t n) {
+// The n first candidates of `size` logits from column `first` on, one round over them for each: for
+// lists that too many candidates would be on, as where most logits are equal.
+template <typename T>
+__device__ __forceinline__ void first_by_rounds(const T *x, uint32_t first, uint32_t size, float *logits,
+                                                uint32_t *tokens, uint32_t n) {
     __shared__ float wave_value[2][kWaves];
     __shared__ uint32_t wave_token[2][kWaves];
     const uint32_t wave = threadIdx.x / 64, lane = threadIdx.x & 63;
@@ -77,11 +81,11 @@ __device__ __forceinline__ void first_by_rounds(const float (&v)[kPieces][N], co
                 token = other;
             }
         };
-#pragma unroll
-        for (int p = 0; p < kPieces; p++)
-#pragma unroll
-            for (int i = 0; i < N; i++)
-                if (before(last, last_token, v[p][i], col[p] + i) && v[p][i] > -INFINITY) take(v[p][i], col[p] + i);
+#pragma unroll 4
+        for (uint32_t i = threadIdx.x; i < size; i += kThreads) {
+            const float y = to_f32(x[first + i]);
+            if (before(last, last_token, y, first + i) && y > -INFINITY) take(y, first + i);
+        }
         for (int k = 32; k >= 1; k /= 2) take(__shfl_xor(best, k), __shfl_xor(token, k));
         if (lane == 0) {
             wave_value[r & 1][wave] = best;
@@ -107,12 +111,14 @@ __global__ __launch_bounds__(kThreads) void k_beam_slices(const spiky_lm_beams_a
     constexpr int N = 16 / sizeof(T);
     __shared__ float group_top[64], wave_sum[kWaves];
     __shared__ uint64_t list[kMostListed];
-    __shared__ uint32_t threshold, listed;
-    const uint64_t row = blockIdx.y + (uint64_t)blockIdx.z * 32768;
-    if (row >= a.searches * a.beams || kind_of(a, row) != kLive) return;
+    __shared__ float threshold;
+    __shared__ uint32_t listed;
+    const uint32_t row = blockIdx.y + blockIdx.z * 32768, beams = (uint32_t)a.beams;  // searches * beams < 2^24
+    if (row >= (uint32_t)a.searches * beams || kind_of(a, row) != kLive) return;
     const uint32_t slice = blockIdx.x, wave = threadIdx.x / 64, lane = threadIdx.x & 63;
-    const T *x = static_cast<const T *>(a.logits) + (int64_t)(row / a.beams) * a.search_stride +
-                 (int64_t)(row % a.beams) * a.beam_stride;
+    const uint32_t search = row / beams;
+    const T *x = static_cast<const T *>(a.logits) + (int64_t)search * a.search_stride +
+                 (int64_t)(row - search * beams) * a.beam_stride;
     float v[kPieces][N];
     uint32_t col[kPieces];
     const uint64_t first = (uint64_t)slice * slice_size<T>();
@@ -153,7 +159,7 @@ __global__ __launch_bounds__(kThreads) void k_beam_slices(const spiky_lm_beams_a
     for (int k = 32; k >= 1; k /= 2) top = fmaxf(top, __shfl_xor(top, k));
     if (wave == 0) {
         const uint32_t t = reached_by<16>(ordered(of_group), parts.n);
-        if (lane == 0) threshold = t;
+        if (lane == 0) threshold = from_ordered(max(t, ordered(-__FLT_MAX__)));  // -infinity is no candidate
     }
     const float from = top == -INFINITY ? 0.f : top;
     float sum = 0.f;
@@ -164,29 +170,36 @@ __global__ __launch_bounds__(kThreads) void k_beam_slices(const spiky_lm_beams_a
     for (int k = 32; k >= 1; k /= 2) sum += __shfl_xor(sum, k);
     if (lane == 0) wave_sum[wave] = sum;
     __syncthreads();
-    const uint64_t at = row * parts.slices + slice;
+    const uint64_t at = (uint64_t)row * parts.slices + slice;
     if (threadIdx.x == 0) {
         sum = 0.f;
         for (int w = 0; w < kWaves; w++) sum += wave_sum[w];
         parts.stats[at] = make_float2(top, sum);
     }
-    const uint32_t least = threshold;
+    // bit kPieces * N - 1 of `reached`: the first value's.  Few lanes have one, and read its logit again.
+    // NaN reaches nothing: it makes its beam's candidates known without a list.
+    const float least = threshold;
+    uint32_t reached = 0;
 #pragma unroll
     for (int p = 0; p < kPieces; p++)
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-            // NaN in a beam makes its candidates known without a list
-            if (ordered(v[p][i]) >= least && v[p][i] > -INFINITY) {
-                const uint32_t k = atomicAdd(&listed, 1u);
-                if (k < kMostListed) list[k] = (uint64_t)ordered(v[p][i]) << 32 | (uint32_t)~(col[p] + i);
-            }
-        }
+        for (int i = 0; i < N; i++) reached += reached + (v[p][i] >= least);
+    while (reached) {
+        const uint32_t i = kPieces * N - 1 - __builtin_ctz(reached), p = i / N;
+        uint32_t from = col[0];
+#pragma unroll
+        for (int k = 1; k < kPieces; k++) from = p == k ? col[k] : from;
+        const uint32_t c = from + i % N, k = atomicAdd(&listed, 1u);
+        if (k < kMostListed) list[k] = (uint64_t)ordered(to_f32(x[c])) << 32 | (uint32_t)~c;
+        reached &= reached - 1;
+    }
     __syncthreads();
     const uint32_t count = listed;
     float *logits = parts.logits + at * parts.n;
     uint32_t *tokens = parts.tokens + at * parts.n;
     if (count > kMostListed) {
-        first_by_rounds<N>(v, col, logits, tokens, parts.n);
+        first_by_rounds(x, (uint32_t)first, (uint32_t)min((uint64_t)slice_size<T>(), a.vocab - first), logits, tokens,
+                        parts.n);
         return;
     }
     for (uint32_t i = threadIdx.x; i < max(count, parts.n); i += kThreads) {
@@ -198,8 +211,7 @@ __global__ __launch_bounds__(kThreads) void k_beam_slices(const spiky_lm_beams_a
         uint32_t rank = 0;
         for (uint32_t k = 0; k < count; k++) rank += list[k] > own;
         if (rank < parts.n) {
-            const uint32_t u = (uint32_t)(own >> 32);
-            logits[rank] = __uint_as_float(u ^ (~(uint32_t)((int32_t)u >> 31) | 0x80000000u));
+            logits[rank] = from_ordered((uint32_t)(own >> 32));
             tokens[rank] = ~(uint32_t)own;
         }
     }
@@ -238,112 +250,161 @@ struct Beam {
 
 constexpr int kJoinThreads = 512, kJoinWaves = kJoinThreads / 64;
 
-// The same of doubles.
-__device__ __forceinline__ uint64_t ordered(double x) {
-    const uint64_t u = (uint64_t)__double_as_longlong(x + 0.0);
-    return u ^ ((uint64_t)((int64_t)u >> 63) | (uint64_t)1 << 63);
+// The natural logarithm of a positive normal number: of its mantissa m in [0.7, 1.5), 2 artanh z with
+// z = (m - 1) / (m + 1), |z| < 0.2, as its series up to z^21 / 21.  The library's functions of
+// doubles are several times as long, and a launch that runs once waits for its instructions.
+__device__ __forceinline__ double log_of(double x) {
+    uint64_t u = (uint64_t)__double_as_longlong(x);
+    const uint64_t half = (u >> 51) & 1;  // m >= 1.5 goes down by 2
+    const int64_t e = (int64_t)(u >> 52) - 1023 + (int64_t)half;
+    u = (u & 0xfffffffffffffull) | (uint64_t)(1023 - half) << 52;
+    const double m = __longlong_as_double((int64_t)u), z = (m - 1.0) / (m + 1.0), w = z * z;
+    double p = 1.0 / 21;
+#pragma unroll
+    for (int k = 19; k >= 1; k -= 2) p = fma(p, w, 1.0 / k);
+    return fma((double)e, 0.693147180559945309417, 2.0 * z * p);
+}
+
+// exp(x) for |x| < 700: 2^k times the series of what is left, |r| < 0.35, up to r^14 / 14!.  The
+// logarithm of 2 is its first 36 bits, whose product with k has no rounding, and the rest.
+__device__ __forceinline__ double exp_of(double x) {
+    const double k = rint(x * 1.44269504088896340736);
+    const double r = fma(k, -0x1.cf79abc9e3b3ap-40, fma(k, -0x1.62e42fefa0000p-1, x));
+    double p = 1.0;
+#pragma unroll
+    for (int i = 14; i >= 1; i--) p = fma(p * (1.0 / i), r, 1.0);
+    return __longlong_as_double(__double_as_longlong(p) + ((int64_t)k << 52));
 }
 
 // A workgroup a search.  As in a slice, candidates that reach what n groups of candidates reach are
 // listed, and each counts those before it; the groups are made of the first candidates of the
-// slices' lists.
+// slices' lists.  Bound by latency: what does not hang on anything is read first, the beams' values
+// and a thread's first logits.
 __global__ __launch_bounds__(kJoinThreads) void k_beam_join(const spiky_lm_beams_args a, const Parts parts) {
-    constexpr uint32_t kMost = 512;
+    constexpr uint32_t kMost = 512, kAhead = 4;
     __shared__ Beam beams[kMostBeams];
     __shared__ Candidate list[kMost], wave_best[2][kJoinWaves];
-    __shared__ uint64_t group_top[kJoinWaves][64];
-    __shared__ uint32_t threshold, listed;
-    const uint64_t search = blockIdx.x, row0 = search * a.beams;
+    __shared__ uint32_t group_top[64], threshold, listed;
+    const uint32_t search = blockIdx.x, row0 = search * (uint32_t)a.beams;  // searches * beams < 2^24
     const uint32_t wave = threadIdx.x / 64, lane = threadIdx.x & 63;
+    const uint32_t lists = (uint32_t)a.beams * parts.slices;  // at most 64 * 2^19
+    const float *logits = parts.logits + (uint64_t)row0 * parts.slices * parts.n;
+    const uint32_t *tokens = parts.tokens + (uint64_t)row0 * parts.slices * parts.n;
+    float ahead[kAhead];
+    uint32_t ahead_token[kAhead];
+#pragma unroll
+    for (uint32_t o = 0; o < kAhead; o++) {
+        const uint64_t at = (uint64_t)min(threadIdx.x, lists - 1) * parts.n + min(o, parts.n - 1);
+        ahead[o] = logits[at];  // of no use where the list's beam is not alive
+        ahead_token[o] = tokens[at];
+    }
     for (uint32_t k = wave; k < a.beams; k += kJoinWaves) {
-        const uint64_t row = row0 + k;
-        Beam b;
-        b.kind = kind_of(a, row);
-        b.score = a.scores[row];
-        b.unknown = false;
-        b.top = -INFINITY;
-        double sum = 0.0;
-        if (b.kind == kLive) {
-            float top = -INFINITY;
-            for (uint32_t s = lane; s < parts.slices; s += 64) top = fmaxf(top, parts.stats[row * parts.slices + s].x);
-            for (int i = 32; i >= 1; i /= 2) top = fmaxf(top, __shfl_xor(top, i));
-            b.top = top;
-            for (uint32_t s = lane; s < parts.slices; s += 64) {
-                const float2 part = parts.stats[row * parts.slices + s];
-                if (part.x > -INFINITY || part.y != part.y) sum += part.y * exp(part.x - b.top);
-            }
-            for (int i = 32; i >= 1; i /= 2) sum += from_lane_xor(sum, i);
-            b.unknown = sum != sum || b.score != b.score || b.score == INFINITY;
-            if (!b.unknown && b.top == -INFINITY) b.kind = kNothing;
-        }
-        b.log_sum = log(sum);
-        b.length = 1.0;
+        const uint32_t row = row0 + k;
+        const float score = a.scores[row];
+        const bool done = a.finished && a.finished[row];
+        const float2 none = make_float2(-INFINITY, 0.f);
+        const float2 *stats = parts.stats + (uint64_t)row * parts.slices;
+        const float2 own = lane < parts.slices ? stats[lane] : none;
+        double grown = 1.0;
         if (a.lengths && a.length_penalty != 0.0) {
             const int64_t n = a.lengths_i64 ? static_cast<const int64_t *>(a.lengths)[row]
                                             : static_cast<const int32_t *>(a.lengths)[row];
-            const double grown = (double)n + (b.kind == kFinished ? 0.0 : 1.0);
-            b.length = pow(grown < 1.0 ? 1.0 : grown, a.length_penalty);
+            grown = fmax((double)n + (done ? 0.0 : 1.0), 1.0);
         }
+        Beam b;
+        b.kind = score == -INFINITY ? kNothing : done ? kFinished : kLive;
+        b.score = score;
+        b.unknown = false;
+        float top = own.x;
+        double sum = 0.0;
+        if (b.kind == kLive) {
+            for (uint32_t s = lane + 64; s < parts.slices; s += 64) top = fmaxf(top, stats[s].x);
+            for (int i = 32; i >= 1; i /= 2) top = fmaxf(top, __shfl_xor(top, i));
+            auto add = [&](const float2 &part) {
+                if (part.x > -INFINITY || part.y != part.y) sum += (double)part.y * (double)__expf(part.x - top);
+            };
+            add(own);
+            for (uint32_t s = lane + 64; s < parts.slices; s += 64) add(stats[s]);
+            for (int i = 32; i >= 1; i /= 2) sum += from_lane_xor(sum, i);
+            b.unknown = sum != sum || score != score || score == INFINITY;
+            if (!b.unknown && top == -INFINITY) b.kind = kNothing;
+        }
+        b.top = top;
+        b.log_sum = log_of(sum);
+        b.length = grown == 1.0 ? 1.0 : exp_of(a.length_penalty * log_of(grown));
         if (lane == 0) beams[k] = b;
     }
     if (threadIdx.x == 0) listed = 0;
+    if (threadIdx.x < 64) group_top[threadIdx.x] = 0;
     __syncthreads();
-    const uint64_t lists = a.beams * parts.slices;
     const Candidate none = {-INFINITY, -INFINITY, -INFINITY, ~0u, ~0u};
-    // Candidate `o` of list `l` of the search, or none.
-    auto candidate = [&](uint64_t l, uint32_t o) {
+    // Candidate `o` of list `l`, or none, from its logit and token.
+    auto made = [&](uint32_t l, uint32_t o, float logit, uint32_t token) {
         Candidate c = none;
-        const uint32_t k = (uint32_t)(l / parts.slices);
-        const uint64_t slice = l - (uint64_t)k * parts.slices;
+        const uint32_t k = l / parts.slices;
         const Beam &b = beams[k];
         if (b.kind == kNothing) return c;
         if (b.kind == kFinished) {
-            if (slice > 0 || o > 0) return c;
+            if (l != k * parts.slices || o > 0) return c;
             c.token = 0;
             c.score = b.score;
         } else if (b.unknown) {
-            if (slice > 0 || o >= a.vocab) return c;
+            if (l != k * parts.slices || o >= a.vocab) return c;
             c.token = o;
             c.score = NAN;
         } else {
-            const uint64_t at = (row0 * parts.slices + l) * parts.n + o;
-            c.logit = parts.logits[at];
-            if (c.logit == -INFINITY) return c;
-            c.token = parts.tokens[at];
-            c.score = c.logit - b.top - b.log_sum + b.score;
+            if (logit == -INFINITY) return c;
+            c.logit = logit;
+            c.token = token;
+            c.score = logit - b.top - b.log_sum + b.score;
         }
         c.beam = k;
         c.rank = b.length == 1.0 ? c.score : c.score / b.length;
         if (c.rank != c.rank) c.rank = INFINITY;
         return c;
     };
+    auto candidate = [&](uint32_t l, uint32_t o) {
+        const uint64_t at = (uint64_t)l * parts.n + o;
+        return made(l, o, logits[at], tokens[at]);
+    };
+    // Calls fn(number, candidate) for the first `most` of the thread's lists, kAhead at a time, up to
+    // the first that fn returns false for, since those behind it are no better.
+    auto each = [&](uint32_t most, auto fn) {
+        for (uint32_t l = threadIdx.x; l < lists; l += kJoinThreads) {
+            bool more = true;
+#pragma unroll
+            for (uint32_t o = 0; o < kAhead; o++)
+                if (o < most && more)
+                    more = fn(l * most + o, l == threadIdx.x ? made(l, o, ahead[o], ahead_token[o]) : candidate(l, o));
+            for (uint32_t o = kAhead; o < most && more; o++) more = fn(l * most + o, candidate(l, o));
+        }
+    };
     // the first `heads` of each list: n or more in all, so that n of the 64 groups hold one
-    const uint32_t heads = (uint32_t)((parts.n + lists - 1) / lists);
-    uint64_t top = 0;
-    for (uint64_t i = threadIdx.x; i < lists * heads; i += kJoinThreads)
-        top = max(top, ordered(candidate(i / heads, (uint32_t)(i % heads)).rank));
-    group_top[wave][lane] = top;
+    each((parts.n + lists - 1) / lists, [&](uint32_t i, const Candidate &c) {
+        atomicMax(&group_top[i & 63], ordered((float)c.rank));
+        return true;
+    });
     __syncthreads();
     if (wave == 0) {
-        for (int w = 1; w < kJoinWaves; w++) top = max(top, group_top[w][lane]);
-        const uint32_t t = reached_by<24>((uint32_t)(top >> 32), parts.n);
+        const uint32_t t = reached_by<20>(group_top[lane], parts.n);
         if (lane == 0) threshold = t;
     }
     __syncthreads();
     const uint32_t least = threshold;
-    for (uint64_t i = threadIdx.x; i < lists * parts.n; i += kJoinThreads) {
-        const Candidate c = candidate(i / parts.n, (uint32_t)(i % parts.n));
-        if (c.beam == ~0u || ordered(c.rank) >> 32 < least) continue;
+    each(parts.n, [&](uint32_t, const Candidate &c) {
+        if (c.beam == ~0u || ordered((float)c.rank) < least) return false;
         const uint32_t k = atomicAdd(&listed, 1u);
         if (k < kMost) list[k] = c;
-    }
+        return true;
+    });
     __syncthreads();
     const uint32_t count = listed;
     auto write = [&](uint32_t r, const Candidate &c) {
         const bool there = c.beam != ~0u;
-        a.out_scores[search * a.n + r] = there ? (float)c.score : -INFINITY;
-        a.out_parents[search * a.n + r] = there ? c.beam : 0;
-        a.out_tokens[search * a.n + r] = there && beams[c.beam].kind == kLive ? c.token : a.pad;
+        const uint64_t at = (uint64_t)search * parts.n + r;
+        a.out_scores[at] = there ? (float)c.score : -INFINITY;
+        a.out_parents[at] = there ? c.beam : 0;
+        a.out_tokens[at] = there && beams[c.beam].kind == kLive ? c.token : a.pad;
     };
     if (count <= kMost) {
         for (uint32_t i = threadIdx.x; i < max(count, parts.n); i += kJoinThreads) {
@@ -360,10 +421,10 @@ __global__ __launch_bounds__(kJoinThreads) void k_beam_join(const spiky_lm_beams
     }
     // too many of one rank: a round for each
     Candidate last = none;
-    for (uint32_t r = 0; r < a.n; r++) {
+    for (uint32_t r = 0; r < parts.n; r++) {
         Candidate best = none;
-        for (uint64_t i = threadIdx.x; i < lists * parts.n; i += kJoinThreads) {
-            const Candidate c = candidate(i / parts.n, (uint32_t)(i % parts.n));
+        for (uint32_t i = threadIdx.x; i < lists * parts.n; i += kJoinThreads) {  // fewer than 2^31
+            const Candidate c = candidate(i / parts.n, i % parts.n);
             if (c.beam != ~0u && (r == 0 || last.before(c)) && c.before(best)) best = c;
         }
         for (int k = 32; k >= 1; k /= 2) {
