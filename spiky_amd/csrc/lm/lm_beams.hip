@@ -1,4 +1,6 @@
 // lm_beams.hip -- the selection of a beam search and the reordering of its states (gfx950).
+#include <type_traits>
+
 #include "lm_tokens.h"
 
 namespace spiky {
@@ -23,6 +25,7 @@ struct Parts {
     float *logits;      // [rows][slices][n], from the largest; -infinity where there are fewer
     uint32_t *tokens;
     uint32_t slices, n;
+    Divider by_n, by_slices, by_beams;
 };
 
 // Before which a candidate of the same beam comes: the larger logit, then the lower token.
@@ -44,8 +47,15 @@ __device__ __forceinline__ uint32_t ordered(float x) {
     return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
 }
 
+// The float of such a number.
 __device__ __forceinline__ float from_ordered(uint32_t u) {
     return __uint_as_float(u ^ (~(uint32_t)((int32_t)u >> 31) | 0x80000000u));
+}
+
+// The same of doubles.
+__device__ __forceinline__ uint64_t ordered(double x) {
+    const uint64_t u = (uint64_t)__double_as_longlong(x + 0.0);
+    return u ^ ((uint64_t)((int64_t)u >> 63) | (uint64_t)1 << 63);
 }
 
 // A number that at least n of the wave's 64 values reach, in its upper `bits` bits: the largest such.
@@ -58,6 +68,38 @@ __device__ __forceinline__ uint32_t reached_by(uint32_t value, uint32_t n) {
         if (__popcll(__ballot(value >= more)) >= n) found = more;
     }
     return found;
+}
+
+// The lane's value combined with those of its row of 16 lanes and of the rows before: lane 63 has all.
+// DPP moves instead of shuffles, which go through LDS and take an address each.
+template <typename F>
+__device__ __forceinline__ float over_wave(float x, float none, F f) {
+    auto step = [&](auto ctrl, auto rows) {
+        x = f(x, __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(none), __float_as_int(x), decltype(ctrl)::value,
+                                                            decltype(rows)::value, 0xf, false)));
+    };
+    using All = std::integral_constant<int, 0xf>;
+    step(std::integral_constant<int, 0x111>(), All());  // row_shr 1, 2, 4, 8
+    step(std::integral_constant<int, 0x112>(), All());
+    step(std::integral_constant<int, 0x114>(), All());
+    step(std::integral_constant<int, 0x118>(), All());
+    step(std::integral_constant<int, 0x142>(), std::integral_constant<int, 0xa>());  // row_bcast 15 into rows 1 and 3
+    step(std::integral_constant<int, 0x143>(), std::integral_constant<int, 0xc>());  // row_bcast 31 into rows 2 and 3
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
+}
+
+__device__ __forceinline__ float wave_max(float x) {
+    return over_wave(x, -INFINITY, [](float a, float b) { return fmaxf(a, b); });
+}
+
+__device__ __forceinline__ float wave_sum_of(float x) {
+    return over_wave(x, 0.f, [](float a, float b) { return a + b; });
+}
+
+// The largest of the lane's four.
+__device__ __forceinline__ float quad_max(float x) {
+    x = fmaxf(x, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0xb1, 0xf, 0xf, false)));  // quad_perm 1 0 3 2
+    return fmaxf(x, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x4e, 0xf, 0xf, false)));  // 2 3 0 1
 }
 
 constexpr uint32_t kMostListed = 1024;
@@ -102,72 +144,77 @@ __device__ __forceinline__ void first_by_rounds(const T *x, uint32_t first, uint
     }
 }
 
-// The n first candidates are among the values that reach a threshold which n of 64 groups of lanes
-// reach with their largest: a few more than n of random logits.  These are listed, and each counts
-// those before it.  n rounds over the registers, each with a barrier, took 410 us where this takes KK
-// (512 beams of 152000 bf16, n = 16).
+constexpr float kLog2E = 1.44269504088896340736f;
+
+// The n first candidates are in units, a lane's logits, whose largest reaches a threshold that n of 64
+// groups of lanes reach: few more than n units.  The logits of these that reach it too, of random ones
+// few more than n again, are listed, and each counts those before it.  n rounds over the registers,
+// each with a barrier, took 410 us where this takes KK (512 beams of 152000 bf16, n = 16, 30 % of
+// them finished, 109 MB).  Slices of a wave each, without barriers and with the next logits in
+// flight, take 32: all are at the same point at a time, and what the choice takes at a slice's end
+// has nothing beside it.  Per logit a conversion, half a maximum, a product and sum, a power of 2 (four
+// times as long) and a sum.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void k_beam_slices(const spiky_lm_beams_args a, const Parts parts) {
     constexpr int N = 16 / sizeof(T);
-    __shared__ float group_top[64], wave_sum[kWaves];
+    constexpr uint32_t kUnit = kPieces * N;
+    __shared__ float group_top[64], wave_sum[kWaves], threshold;
     __shared__ uint64_t list[kMostListed];
-    __shared__ float threshold;
-    __shared__ uint32_t listed;
+    __shared__ uint32_t units[kThreads], n_units, listed;
     const uint32_t row = blockIdx.y + blockIdx.z * 32768, beams = (uint32_t)a.beams;  // searches * beams < 2^24
     if (row >= (uint32_t)a.searches * beams || kind_of(a, row) != kLive) return;
     const uint32_t slice = blockIdx.x, wave = threadIdx.x / 64, lane = threadIdx.x & 63;
-    const uint32_t search = row / beams;
+    const uint32_t vocab = (uint32_t)a.vocab, search = parts.by_beams.divide(row), first = slice * slice_size<T>();
     const T *x = static_cast<const T *>(a.logits) + (int64_t)search * a.search_stride +
                  (int64_t)(row - search * beams) * a.beam_stride;
-    float v[kPieces][N];
-    uint32_t col[kPieces];
-    const uint64_t first = (uint64_t)slice * slice_size<T>();
-    if (first + slice_size<T>() <= a.vocab) {
+    float v[kUnit];
+    if (vocab - first >= slice_size<T>()) {
         Raw<T, N> raw[kPieces];
 #pragma unroll
-        for (int p = 0; p < kPieces; p++) {
-            col[p] = (uint32_t)first + (p * kThreads + threadIdx.x) * N;
-            raw[p].load(x + col[p], N);
-        }
+        for (int p = 0; p < kPieces; p++) raw[p].load(x + first + (p * kThreads + threadIdx.x) * N, N);
 #pragma unroll
         for (int p = 0; p < kPieces; p++)
 #pragma unroll
-            for (int i = 0; i < N; i++) v[p][i] = raw[p][i];
+            for (int i = 0; i < N; i++) v[p * N + i] = raw[p][i];
     } else {
 #pragma unroll
         for (int p = 0; p < kPieces; p++) {
             Place<N> place;
-            place.set(a.vocab, first + (p * kThreads + threadIdx.x) * N);
-            load(v[p], x + place.col, place.n);
-            col[p] = (uint32_t)place.col;
+            place.set(vocab, (uint64_t)first + (p * kThreads + threadIdx.x) * N);
+            float y[N];
+            load(y, x + place.col, place.n);
 #pragma unroll
-            for (int i = 0; i < N; i++) v[p][i] = place.own >> i & 1 ? v[p][i] : -INFINITY;
+            for (int i = 0; i < N; i++) {
+                // the last piece's columns in their places, in front of which it has others'
+                v[p * N + i] = place.own >> i & 1 ? y[i] : -INFINITY;
+            }
         }
     }
-    float top = -INFINITY;
+    float here = v[0];
 #pragma unroll
-    for (int p = 0; p < kPieces; p++)
-#pragma unroll
-        for (int i = 0; i < N; i++) top = fmaxf(top, v[p][i]);
-    top = fmaxf(top, __shfl_xor(top, 1));
-    top = fmaxf(top, __shfl_xor(top, 2));
+    for (uint32_t i = 1; i < kUnit; i++) here = fmaxf(here, v[i]);
+    float top = quad_max(here);
     if ((lane & 3) == 0) group_top[threadIdx.x / 4] = top;
-    if (threadIdx.x == 0) listed = 0;
+    if (threadIdx.x == 0) listed = n_units = 0;
     __syncthreads();
     const float of_group = group_top[lane];
-    top = of_group;
-    for (int k = 32; k >= 1; k /= 2) top = fmaxf(top, __shfl_xor(top, k));
+    top = wave_max(of_group);
     if (wave == 0) {
         const uint32_t t = reached_by<16>(ordered(of_group), parts.n);
         if (lane == 0) threshold = from_ordered(max(t, ordered(-__FLT_MAX__)));  // -infinity is no candidate
     }
-    const float from = top == -INFINITY ? 0.f : top;
     float sum = 0.f;
+    if (fabsf(top) <= 1e6f) {  // relative to 2^power, and in the end to exp(top)
+        const float power = rintf(top * kLog2E);
 #pragma unroll
-    for (int p = 0; p < kPieces; p++)
+        for (uint32_t i = 0; i < kUnit; i++) sum += __builtin_amdgcn_exp2f(fmaf(v[i], kLog2E, -power));
+        sum *= __builtin_amdgcn_exp2f(fmaf(-top, kLog2E, power));
+    } else {  // whose power of 2 has no fraction left
+        const float from = top == -INFINITY ? 0.f : top;
 #pragma unroll
-        for (int i = 0; i < N; i++) sum += __expf(v[p][i] - from);
-    for (int k = 32; k >= 1; k /= 2) sum += __shfl_xor(sum, k);
+        for (uint32_t i = 0; i < kUnit; i++) sum += __builtin_amdgcn_exp2f((v[i] - from) * kLog2E);
+    }
+    sum = wave_sum_of(sum);
     if (lane == 0) wave_sum[wave] = sum;
     __syncthreads();
     const uint64_t at = (uint64_t)row * parts.slices + slice;
@@ -176,30 +223,35 @@ __global__ __launch_bounds__(kThreads) void k_beam_slices(const spiky_lm_beams_a
         for (int w = 0; w < kWaves; w++) sum += wave_sum[w];
         parts.stats[at] = make_float2(top, sum);
     }
-    // bit kPieces * N - 1 of `reached`: the first value's.  Few lanes have one, and read its logit again.
-    // NaN reaches nothing: it makes its beam's candidates known without a list.
+    // NaN reaches nothing: it makes its beam's candidates known without a list
     const float least = threshold;
-    uint32_t reached = 0;
+    if (here >= least) units[atomicAdd(&n_units, 1u)] = threadIdx.x;
+    __syncthreads();
+    // a unit's logits are read again, a few by each thread
+    constexpr uint32_t kAhead = 4;
+    const uint32_t all = n_units * kUnit;
+    for (uint32_t i = threadIdx.x; i < all; i += kThreads * kAhead) {
+        T y[kAhead];
+        uint32_t col[kAhead];
 #pragma unroll
-    for (int p = 0; p < kPieces; p++)
+        for (uint32_t j = 0; j < kAhead; j++) {
+            const uint32_t o = min(i + j * kThreads, all - 1), e = o % kUnit;
+            col[j] = first + (e / N * kThreads + units[o / kUnit]) * N + e % N;
+            y[j] = x[min(col[j], vocab - 1)];
+        }
 #pragma unroll
-        for (int i = 0; i < N; i++) reached += reached + (v[p][i] >= least);
-    while (reached) {
-        const uint32_t i = kPieces * N - 1 - __builtin_ctz(reached), p = i / N;
-        uint32_t from = col[0];
-#pragma unroll
-        for (int k = 1; k < kPieces; k++) from = p == k ? col[k] : from;
-        const uint32_t c = from + i % N, k = atomicAdd(&listed, 1u);
-        if (k < kMostListed) list[k] = (uint64_t)ordered(to_f32(x[c])) << 32 | (uint32_t)~c;
-        reached &= reached - 1;
+        for (uint32_t j = 0; j < kAhead; j++) {
+            if (i + j * kThreads >= all || col[j] >= vocab || !(to_f32(y[j]) >= least)) continue;
+            const uint32_t k = atomicAdd(&listed, 1u);
+            if (k < kMostListed) list[k] = (uint64_t)ordered(to_f32(y[j])) << 32 | (uint32_t)~col[j];
+        }
     }
     __syncthreads();
     const uint32_t count = listed;
     float *logits = parts.logits + at * parts.n;
     uint32_t *tokens = parts.tokens + at * parts.n;
     if (count > kMostListed) {
-        first_by_rounds(x, (uint32_t)first, (uint32_t)min((uint64_t)slice_size<T>(), a.vocab - first), logits, tokens,
-                        parts.n);
+        first_by_rounds(x, first, min(slice_size<T>(), vocab - first), logits, tokens, parts.n);
         return;
     }
     for (uint32_t i = threadIdx.x; i < max(count, parts.n); i += kThreads) {
@@ -209,6 +261,7 @@ __global__ __launch_bounds__(kThreads) void k_beam_slices(const spiky_lm_beams_a
         }
         const uint64_t own = list[i];
         uint32_t rank = 0;
+#pragma unroll 4
         for (uint32_t k = 0; k < count; k++) rank += list[k] > own;
         if (rank < parts.n) {
             logits[rank] = from_ordered((uint32_t)(own >> 32));
@@ -217,16 +270,16 @@ __global__ __launch_bounds__(kThreads) void k_beam_slices(const spiky_lm_beams_a
     }
 }
 
-// A candidate of a search.
+// A candidate of a search, as numbers that it is compared by: the largest `first`, then the smallest
+// `second` and the lowest token come first.
 struct Candidate {
-    double rank, score;
-    float logit;
-    uint32_t beam, token;
+    uint64_t first;   // the rank, ordered; 0: no candidate
+    uint64_t second;  // the beam, and the logit against its order
+    uint32_t token;
+    float score;
 
     __device__ __forceinline__ bool before(const Candidate &o) const {
-        if (rank != o.rank) return rank > o.rank;
-        if (beam != o.beam) return beam < o.beam;
-        return lm::before(logit, token, o.logit, o.token);
+        return (first > o.first) | ((first == o.first) & ((second < o.second) | ((second == o.second) & (token < o.token))));
     }
 };
 
@@ -281,23 +334,23 @@ __device__ __forceinline__ double exp_of(double x) {
 // slices' lists.  Bound by latency: what does not hang on anything is read first, the beams' values
 // and a thread's first logits.
 __global__ __launch_bounds__(kJoinThreads) void k_beam_join(const spiky_lm_beams_args a, const Parts parts) {
-    constexpr uint32_t kMost = 512, kAhead = 4;
+    constexpr uint32_t kMost = 512;
     __shared__ Beam beams[kMostBeams];
     __shared__ Candidate list[kMost], wave_best[2][kJoinWaves];
-    __shared__ uint32_t group_top[64], threshold, listed;
+    __shared__ uint32_t ranks[kMost];
+    __shared__ uint32_t group_top[64], open_list[kMost], threshold, open, listed;
     const uint32_t search = blockIdx.x, row0 = search * (uint32_t)a.beams;  // searches * beams < 2^24
     const uint32_t wave = threadIdx.x / 64, lane = threadIdx.x & 63;
-    const uint32_t lists = (uint32_t)a.beams * parts.slices;  // at most 64 * 2^19
+    const uint32_t lists = (uint32_t)a.beams * parts.slices;
     const float *logits = parts.logits + (uint64_t)row0 * parts.slices * parts.n;
     const uint32_t *tokens = parts.tokens + (uint64_t)row0 * parts.slices * parts.n;
-    float ahead[kAhead];
-    uint32_t ahead_token[kAhead];
-#pragma unroll
-    for (uint32_t o = 0; o < kAhead; o++) {
-        const uint64_t at = (uint64_t)min(threadIdx.x, lists - 1) * parts.n + min(o, parts.n - 1);
-        ahead[o] = logits[at];  // of no use where the list's beam is not alive
-        ahead_token[o] = tokens[at];
-    }
+    // the first `heads` candidates of each list: n or more in all, and enough for the groups
+    const uint32_t heads = min(parts.n, (63 + lists) / lists);
+    // Where the first heads number i lie: list i / heads, candidate i % heads.
+    auto head_at = [&](uint32_t i) { return heads == 1 ? i * parts.n : i / heads * parts.n + i % heads; };
+    const uint32_t first_at = head_at(min(threadIdx.x, lists * heads - 1));
+    const float first_logit = logits[first_at];  // of no use where the list's beam is not alive
+    const uint32_t first_token = tokens[first_at];
     for (uint32_t k = wave; k < a.beams; k += kJoinWaves) {
         const uint32_t row = row0 + k;
         const float score = a.scores[row];
@@ -326,7 +379,7 @@ __global__ __launch_bounds__(kJoinThreads) void k_beam_join(const spiky_lm_beams
             add(own);
             for (uint32_t s = lane + 64; s < parts.slices; s += 64) add(stats[s]);
             for (int i = 32; i >= 1; i /= 2) sum += from_lane_xor(sum, i);
-            b.unknown = sum != sum || score != score || score == INFINITY;
+            b.unknown = sum != sum || top == INFINITY || score != score || score == INFINITY;
             if (!b.unknown && top == -INFINITY) b.kind = kNothing;
         }
         b.top = top;
@@ -334,115 +387,125 @@ __global__ __launch_bounds__(kJoinThreads) void k_beam_join(const spiky_lm_beams
         b.length = grown == 1.0 ? 1.0 : exp_of(a.length_penalty * log_of(grown));
         if (lane == 0) beams[k] = b;
     }
-    if (threadIdx.x == 0) listed = 0;
+    if (threadIdx.x == 0) listed = open = 0;
     if (threadIdx.x < 64) group_top[threadIdx.x] = 0;
     __syncthreads();
-    const Candidate none = {-INFINITY, -INFINITY, -INFINITY, ~0u, ~0u};
+    const Candidate none = {0, ~(uint64_t)0, ~0u, -INFINITY};
     // Candidate `o` of list `l`, or none, from its logit and token.
     auto made = [&](uint32_t l, uint32_t o, float logit, uint32_t token) {
-        Candidate c = none;
-        const uint32_t k = l / parts.slices;
+        const uint32_t k = parts.by_slices.divide(l);
         const Beam &b = beams[k];
-        if (b.kind == kNothing) return c;
-        if (b.kind == kFinished) {
-            if (l != k * parts.slices || o > 0) return c;
-            c.token = 0;
-            c.score = b.score;
-        } else if (b.unknown) {
-            if (l != k * parts.slices || o >= a.vocab) return c;
-            c.token = o;
-            c.score = NAN;
-        } else {
-            if (logit == -INFINITY) return c;
-            c.logit = logit;
-            c.token = token;
-            c.score = logit - b.top - b.log_sum + b.score;
+        const bool only = l == k * parts.slices;  // what finished and unknown beams have is in their first list
+        bool there = logit > -INFINITY;
+        double score = logit - b.top - b.log_sum + b.score;
+        if (b.kind != kLive || b.unknown) {
+            there = only && b.kind != kNothing && (b.kind == kFinished ? o == 0 : o < a.vocab);
+            score = b.kind == kFinished ? b.score : NAN;
+            token = b.kind == kFinished ? 0 : o;
+            logit = 0.f;
         }
-        c.beam = k;
-        c.rank = b.length == 1.0 ? c.score : c.score / b.length;
-        if (c.rank != c.rank) c.rank = INFINITY;
-        return c;
+        double rank = b.length == 1.0 ? score : score / b.length;
+        rank = rank != rank ? INFINITY : rank;
+        if (!there) return none;
+        return Candidate{ordered(rank), (uint64_t)k << 32 | (uint32_t)~ordered(logit), token, (float)score};
     };
-    auto candidate = [&](uint32_t l, uint32_t o) {
-        const uint64_t at = (uint64_t)l * parts.n + o;
-        return made(l, o, logits[at], tokens[at]);
+    // The rank in 32 bits, rounded alike for all: what reaches a threshold in 64 reaches it here.
+    auto coarse = [](const Candidate &c) { return (uint32_t)(c.first >> 32); };
+    // The candidate at `at` of the search's part of the workspace, at most 64 * 2^19 * 64 = 2^31 long.
+    auto candidate = [&](uint32_t at) {
+        const uint32_t l = parts.by_n.divide(at);
+        return made(l, at - l * parts.n, logits[at], tokens[at]);
     };
-    // Calls fn(number, candidate) for the first `most` of the thread's lists, kAhead at a time, up to
-    // the first that fn returns false for, since those behind it are no better.
-    auto each = [&](uint32_t most, auto fn) {
-        for (uint32_t l = threadIdx.x; l < lists; l += kJoinThreads) {
-            bool more = true;
-#pragma unroll
-            for (uint32_t o = 0; o < kAhead; o++)
-                if (o < most && more)
-                    more = fn(l * most + o, l == threadIdx.x ? made(l, o, ahead[o], ahead_token[o]) : candidate(l, o));
-            for (uint32_t o = kAhead; o < most && more; o++) more = fn(l * most + o, candidate(l, o));
-        }
-    };
-    // the first `heads` of each list: n or more in all, so that n of the 64 groups hold one
-    each((parts.n + lists - 1) / lists, [&](uint32_t i, const Candidate &c) {
-        atomicMax(&group_top[i & 63], ordered((float)c.rank));
-        return true;
-    });
+    // The heads are in 64 groups; n or more of these hold one.
+    for (uint32_t i = threadIdx.x; i < lists * heads; i += kJoinThreads) {
+        const uint32_t at = head_at(i), l = parts.by_n.divide(at);
+        const Candidate c = i == threadIdx.x ? made(l, at - l * parts.n, first_logit, first_token) : candidate(at);
+        atomicMax(&group_top[i & 63], coarse(c));
+    }
     __syncthreads();
     if (wave == 0) {
         const uint32_t t = reached_by<20>(group_top[lane], parts.n);
         if (lane == 0) threshold = t;
     }
     __syncthreads();
+    // the lists whose first candidate reaches the threshold, and of these the candidates that do
     const uint32_t least = threshold;
-    each(parts.n, [&](uint32_t, const Candidate &c) {
-        if (c.beam == ~0u || ordered((float)c.rank) < least) return false;
+    for (uint32_t l = threadIdx.x; l < lists; l += kJoinThreads) {
+        const Candidate c = l == threadIdx.x && heads == 1 ? made(l, 0, first_logit, first_token) : candidate(l * parts.n);
+        if (!c.first || coarse(c) < least) continue;
+        const uint32_t k = atomicAdd(&open, 1u);
+        if (k < kMost) open_list[k] = l;
+    }
+    __syncthreads();
+    const bool every = open > kMost;
+    for (uint32_t i = threadIdx.x; i < (every ? lists : open) * parts.n; i += kJoinThreads) {
+        const uint32_t l = parts.by_n.divide(i);
+        const Candidate c = candidate(every ? i : open_list[l] * parts.n + (i - l * parts.n));
+        if (!c.first || coarse(c) < least) continue;
         const uint32_t k = atomicAdd(&listed, 1u);
-        if (k < kMost) list[k] = c;
-        return true;
-    });
+        if (k < kMost) {
+            list[k] = c;
+            ranks[k] = 0;
+        }
+    }
     __syncthreads();
     const uint32_t count = listed;
     auto write = [&](uint32_t r, const Candidate &c) {
-        const bool there = c.beam != ~0u;
         const uint64_t at = (uint64_t)search * parts.n + r;
-        a.out_scores[at] = there ? (float)c.score : -INFINITY;
-        a.out_parents[at] = there ? c.beam : 0;
-        a.out_tokens[at] = there && beams[c.beam].kind == kLive ? c.token : a.pad;
+        const uint32_t beam = c.first ? (uint32_t)(c.second >> 32) : 0;
+        a.out_scores[at] = c.score;
+        a.out_parents[at] = beam;
+        a.out_tokens[at] = c.first && beams[beam].kind == kLive ? c.token : a.pad;
     };
     if (count <= kMost) {
-        for (uint32_t i = threadIdx.x; i < max(count, parts.n); i += kJoinThreads) {
-            if (i >= count) {
-                write(i, none);
-                continue;
-            }
+        // as many threads to a candidate as there are
+        uint32_t shares = 1;
+        while (2 * shares * count <= kJoinThreads && shares < 16) shares *= 2;
+        const uint32_t i = threadIdx.x / shares;
+        if (i < count) {
             const Candidate own = list[i];
             uint32_t rank = 0;
-            for (uint32_t k = 0; k < count; k++) rank += list[k].before(own);
-            if (rank < parts.n) write(rank, own);
+#pragma unroll 4
+            for (uint32_t k = threadIdx.x % shares; k < count; k += shares) rank += list[k].before(own);
+            atomicAdd(&ranks[i], rank);
         }
+        __syncthreads();
+        if (threadIdx.x < count && ranks[threadIdx.x] < parts.n) write(ranks[threadIdx.x], list[threadIdx.x]);
+        if (threadIdx.x >= count && threadIdx.x < parts.n) write(threadIdx.x, none);
         return;
     }
     // too many of one rank: a round for each
-    Candidate last = none;
+    Candidate last = {~(uint64_t)0, 0, 0, 0.f};
+#pragma unroll 1
     for (uint32_t r = 0; r < parts.n; r++) {
         Candidate best = none;
-        for (uint32_t i = threadIdx.x; i < lists * parts.n; i += kJoinThreads) {  // fewer than 2^31
-            const Candidate c = candidate(i / parts.n, i % parts.n);
-            if (c.beam != ~0u && (r == 0 || last.before(c)) && c.before(best)) best = c;
+#pragma unroll 1
+        for (uint32_t i = threadIdx.x; i < lists * parts.n; i += kJoinThreads) {
+            const Candidate c = candidate(i);
+            if (c.first && last.before(c) && c.before(best)) best = c;
         }
+#pragma unroll 1
         for (int k = 32; k >= 1; k /= 2) {
             const Candidate c = from_lane_xor(best, k);
             if (c.before(best)) best = c;
         }
         if (lane == 0) wave_best[r & 1][wave] = best;
         __syncthreads();
+#pragma unroll 1
         for (int w = 0; w < kJoinWaves; w++)
             if (wave_best[r & 1][w].before(best)) best = wave_best[r & 1][w];
         if (threadIdx.x == 0) write(r, best);
-        last = best;
+        last = best.first ? best : Candidate{0, 0, 0, 0.f};
     }
 }
 
-uint32_t slices_of(const spiky_lm_beams_args &a) {
-    const uint32_t size = a.dtype == SPIKY_F32 ? slice_size<float>() : slice_size<bf16>();
-    return a.vocab ? (uint32_t)((a.vocab + size - 1) / size) : 1;  // a finished beam needs one too
+void cut(const spiky_lm_beams_args &a, Parts &parts) {
+    const uint64_t size = a.dtype == SPIKY_F32 ? slice_size<float>() : slice_size<bf16>();
+    parts.slices = (uint32_t)max((a.vocab + size - 1) / size, (uint64_t)1);  // a finished beam needs a list too
+    parts.n = (uint32_t)a.n;
+    parts.by_n = Divider(parts.n);
+    parts.by_slices = Divider(parts.slices);
+    parts.by_beams = Divider((uint32_t)a.beams);
 }
 
 // ---- reordering -----------------------------------------------------------------
@@ -521,14 +584,15 @@ __global__ __launch_bounds__(kThreads) void k_reorder(const States states, const
 }  // namespace
 
 uint64_t beam_select_workspace(const spiky_lm_beams_args &a) {
-    return a.searches * a.beams * slices_of(a) * (sizeof(float2) + a.n * 8);
+    Parts parts;
+    cut(a, parts);
+    return a.searches * a.beams * parts.slices * (sizeof(float2) + a.n * 8);
 }
 
 hipError_t launch_beam_select(const spiky_lm_beams_args &a, void *workspace, hipStream_t st) {
     Parts parts;
+    cut(a, parts);
     const uint64_t rows = a.searches * a.beams;
-    parts.slices = slices_of(a);
-    parts.n = (uint32_t)a.n;
     parts.stats = static_cast<float2 *>(workspace);
     parts.logits = reinterpret_cast<float *>(parts.stats + rows * parts.slices);
     parts.tokens = reinterpret_cast<uint32_t *>(parts.logits + rows * parts.slices * a.n);
