@@ -522,7 +522,7 @@ struct States {
     State of[kMostStates];
 };
 
-template <typename V, int kBeams>
+template <typename V, int kBeams, bool kStream = false>
 __device__ __forceinline__ void move(const char *in, char *out, int64_t in_beam, int64_t out_beam,
                                      const uint32_t *parents, uint32_t beams, uint32_t n, bool in_place) {
     for (uint32_t j0 = 0; j0 < n; j0 += kBeams) {
@@ -539,15 +539,21 @@ __device__ __forceinline__ void move(const char *in, char *out, int64_t in_beam,
 #pragma unroll
         for (int j = 0; j < kBeams; j++) {
             if (j0 + j >= n) break;
-            if (!(in_place && parents[j0 + j] == j0 + j))
-                __builtin_memcpy(out + (int64_t)(j0 + j) * out_beam, &v[j], sizeof(V));
+            if (in_place && parents[j0 + j] == j0 + j) continue;
+            char *to = out + (int64_t)(j0 + j) * out_beam;
+            if constexpr (kStream) {
+                typedef V Anywhere __attribute__((aligned(1)));
+                __builtin_nontemporal_store(v[j], reinterpret_cast<Anywhere *>(to));
+            } else {
+                __builtin_memcpy(to, &v[j], sizeof(V));
+            }
         }
     }
 }
 
 typedef uint32_t Words4 __attribute__((ext_vector_type(4)));
 
-template <int kBeams>
+template <int kBeams, bool kStream>
 __global__ __launch_bounds__(kThreads) void k_reorder(const States states, const void *parents_, bool i64,
                                                       uint32_t beams, uint32_t n, uint64_t first) {
     extern __shared__ uint32_t parents[];  // ~0: none
@@ -564,15 +570,17 @@ __global__ __launch_bounds__(kThreads) void k_reorder(const States states, const
     for (uint64_t i = (uint64_t)blockIdx.x * kThreads + threadIdx.x; i < s.runs * state.pieces.d;
          i += (uint64_t)gridDim.x * kThreads) {
         const uint64_t run = i < 0x100000000ull ? state.pieces.divide((uint32_t)i) : i / state.pieces.d;
-        const uint64_t at = (i - run * state.pieces.d) * 16;
+        uint64_t at = (i - run * state.pieces.d) * 16;
+        // the end of a run: its last 16 bytes, which have some in common with the piece before.  In place
+        // that one may be written already, and the end keeps to its own, in halves of halves.
+        if (!in_place && s.run_bytes >= 16) at = min(at, s.run_bytes - 16);
         const char *in = static_cast<const char *>(s.in) + (int64_t)search * s.in_search + (int64_t)run * s.in_run + at;
         char *out = static_cast<char *>(s.out) + (int64_t)search * s.out_search + (int64_t)run * s.out_run + at;
         const uint64_t left = s.run_bytes - at;
         if (left >= 16) {
-            move<Words4, kBeams>(in, out, s.in_beam, s.out_beam, parents, beams, n, in_place);
+            move<Words4, kBeams, kStream>(in, out, s.in_beam, s.out_beam, parents, beams, n, in_place);
             continue;
         }
-        // the end of a run: other threads' pieces may be written already, so it keeps to its own
         uint32_t o = 0;
         if (left & 8) move<uint64_t, kBeams>(in, out, s.in_beam, s.out_beam, parents, beams, n, in_place), o += 8;
         if (left & 4) move<uint32_t, kBeams>(in + o, out + o, s.in_beam, s.out_beam, parents, beams, n, in_place), o += 4;
@@ -611,6 +619,11 @@ hipError_t launch_beam_select(const spiky_lm_beams_args &a, void *workspace, hip
 
 hipError_t launch_reorder(const spiky_lm_state *states, uint64_t count, const void *parents, bool parents_i64,
                           uint64_t searches, uint64_t beams, uint64_t n, hipStream_t st) {
+    // Results past twice the last cache do not stay there for their reader: stored past it, 1.1 GB to 4
+    // beams take 449 us against 504.
+    uint64_t bytes = 0;
+    for (uint64_t i = 0; i < count; i++) bytes += states[i].runs * states[i].run_bytes * n * searches;
+    const bool stream = bytes >= 2 * kLastCache;
     for (uint64_t at = 0; at < count; at += kMostStates) {
         const uint64_t here = min(count - at, (uint64_t)kMostStates);
         States group = {};
@@ -630,8 +643,10 @@ hipError_t launch_reorder(const spiky_lm_state *states, uint64_t count, const vo
                                                             first);
                 return hipGetLastError();
             };
-            const hipError_t e = n <= 4 ? go(k_reorder<4>) : n <= 8 ? go(k_reorder<8>) : n <= 16 ? go(k_reorder<16>)
-                                 : n <= 32 ? go(k_reorder<32>) : go(k_reorder<64>);
+            const hipError_t e = n <= 4 ? stream ? go(k_reorder<4, true>) : go(k_reorder<4, false>)
+                                 : n <= 8 ? stream ? go(k_reorder<8, true>) : go(k_reorder<8, false>)
+                                 : n <= 16 ? go(k_reorder<16, false>) : n <= 32 ? go(k_reorder<32, false>)
+                                 : go(k_reorder<64, false>);
             if (e != hipSuccess) return e;
         }
     }

@@ -189,7 +189,6 @@ __global__ __launch_bounds__(kSortWaves * 64) void k_embed_sort(const Tok *__res
 // tokens' gradient, ten times the rest.
 constexpr uint32_t kChunk = 32;
 constexpr uint64_t kManyGroups = 64 * kCUs;
-constexpr uint64_t kLastCache = 256u << 20;  // bytes; what is written past it does not stay there for its reader
 
 // The sum over positions [from, to) of the columns at d_out; `from < to`.
 template <int N, typename T>

@@ -16,6 +16,7 @@ namespace spiky {
 namespace lm {
 
 constexpr uint32_t kCUs = 256;
+constexpr uint64_t kLastCache = 256u << 20;  // bytes
 
 // ---- elements --------------------------------------------------------------
 struct bf16 {
