@@ -84,16 +84,15 @@ __device__ __forceinline__ uint32_t narrow(int64_t token) {
 }
 __device__ __forceinline__ uint32_t narrow(int32_t token) { return (uint32_t)token; }
 
-template <typename Tok>
-__global__ __launch_bounds__(kSortWaves * 64) void k_embed_sort(const Tok *__restrict__ tokens, uint32_t n,
-                                                                uint32_t vocab, uint32_t range,
-                                                                uint32_t *__restrict__ start,
-                                                                uint32_t *__restrict__ order) {
-    extern __shared__ uint32_t counts[];  // [kSortWaves][range]
-    __shared__ uint32_t lists[kSortWaves][kList], below_of[kSortWaves], sum_of[kSortWaves];
+// A workgroup's part: its tokens' positions to `order`, which takes the ones of this range from
+// *from_below on.  In the end counts [kSortWaves - 1][o] is where those of token base + o end.
+template <typename Tok, typename Start>
+__device__ __forceinline__ void sort_range(const Tok *tokens, uint32_t n, uint32_t base, uint32_t size, uint32_t range,
+                                           uint32_t *counts, uint32_t (*lists)[kList], uint32_t *order, bool from_below,
+                                           Start start) {
+    __shared__ uint32_t below_of[kSortWaves], sum_of[kSortWaves];
     const uint32_t wave = threadIdx.x / 64, lane = threadIdx.x & 63;
     const uint64_t lower = ((uint64_t)1 << lane) - 1;
-    const uint32_t base = blockIdx.x * range, size = min(range, vocab - base);
     for (uint32_t i = threadIdx.x; i < kSortWaves * range; i += kSortWaves * 64) counts[i] = 0;
     __syncthreads();
     const uint32_t share = (n / (kSortWaves * 64) + 1) * 64;
@@ -121,7 +120,7 @@ __global__ __launch_bounds__(kSortWaves * 64) void k_embed_sort(const Tok *__res
         const uint64_t own = __ballot(o < size);
         if (own == 0) return;
         // many lanes with one token, as where a batch is padded with it, count as one: 32768 times one
-        // token take KK us against 43
+        // token take 25 us against 43
         uint32_t counted = ~0u;
         if (__popcll(own) >= 16) {
             counted = __builtin_amdgcn_readlane(o, __builtin_ctzll(own));
@@ -149,10 +148,9 @@ __global__ __launch_bounds__(kSortWaves * 64) void k_embed_sort(const Tok *__res
     if (lane == 63) sum_of[wave] = upto;
     __syncthreads();
     uint32_t at = upto - total;
-    for (uint32_t w = 0; w < kSortWaves; w++) at += below_of[w] + (w < wave ? sum_of[w] : 0);
+    for (uint32_t w = 0; w < kSortWaves; w++) at += (from_below ? below_of[w] : 0) + (w < wave ? sum_of[w] : 0);
     if (threadIdx.x < size) {
-        start[base + threadIdx.x] = at;
-        if (base + threadIdx.x == vocab - 1) start[vocab] = at + total;
+        start(threadIdx.x, at, total);
         for (int w = 0; w < kSortWaves; w++) {
             const uint32_t c = counts[w * range + threadIdx.x];
             counts[w * range + threadIdx.x] = at;
@@ -181,6 +179,20 @@ __global__ __launch_bounds__(kSortWaves * 64) void k_embed_sort(const Tok *__res
     } else {
         each([&](uint32_t first, uint32_t id) { place(first + lane, id - base < size ? id - base : ~0u); });
     }
+}
+
+template <typename Tok>
+__global__ __launch_bounds__(kSortWaves * 64) void k_embed_sort(const Tok *__restrict__ tokens, uint32_t n,
+                                                                uint32_t vocab, uint32_t range,
+                                                                uint32_t *__restrict__ start,
+                                                                uint32_t *__restrict__ order) {
+    extern __shared__ uint32_t counts[];  // [kSortWaves][range]
+    __shared__ uint32_t lists[kSortWaves][kList];
+    const uint32_t base = blockIdx.x * range, size = min(range, vocab - base);
+    sort_range(tokens, n, base, size, range, counts, lists, order, true, [&](uint32_t o, uint32_t at, uint32_t total) {
+        start[base + o] = at;
+        if (base + o == vocab - 1) start[vocab] = at + total;
+    });
 }
 
 // Positions of a token that are added up one after the other: tokens with more ("frequent") go in
@@ -348,6 +360,97 @@ __global__ __launch_bounds__(kThreads) void k_embed_join(const Tok *__restrict__
     }
 }
 
+// Both in one launch, for few positions: a workgroup takes `range` tokens and a slab of `lanes` pieces of
+// their rows, sorts for itself, and adds up.  Its groups of `lanes` threads take a token each, and all
+// of them one that has more than kTogether positions, a share each.  The three launches take 21 us
+// for 8192 positions of 256 columns in a table of 256 rows, this one 17; 26 and 22 for 512 of 1024 in
+// one of 50000.
+constexpr uint32_t kSmall = 8192, kTogether = 16;
+
+template <typename Tok, typename T, typename W>
+__global__ __launch_bounds__(kSortWaves * 64) void k_embed_small(const Tok *__restrict__ tokens,
+                                                                 const T *__restrict__ d_out, int64_t stride,
+                                                                 W *__restrict__ d_weight, uint32_t n, uint32_t vocab,
+                                                                 uint64_t cols, uint32_t range, uint32_t lanes,
+                                                                 float scale) {
+    constexpr int N = piece<W, T>();
+    constexpr uint32_t kAll = kSortWaves * 64;
+    extern __shared__ uint32_t counts[];  // [kSortWaves][range], then the order [n]
+    __shared__ union {
+        uint32_t lists[kSortWaves][kList];
+        float partial[N][kAll];
+    } shared;
+    __shared__ uint32_t together[kSmall / kTogether], n_together;
+    static_assert(sizeof(shared) <= 32768, "two workgroups to a CU");
+    uint32_t *order = counts + kSortWaves * range;
+    const uint32_t base = blockIdx.x * range, size = min(range, vocab - base);
+    if (threadIdx.x == 0) n_together = 0;
+    // the first barrier lies between this and the calls
+    sort_range(tokens, n, base, size, range, counts, shared.lists, order, false, [&](uint32_t o, uint32_t, uint32_t total) {
+        if (total > kTogether) together[atomicAdd(&n_together, 1u)] = o;
+    });
+    __syncthreads();
+    const uint32_t *ends = counts + (kSortWaves - 1) * range;
+    const uint32_t group = threadIdx.x / lanes, groups = kAll / lanes;
+    Place<N> place;
+    place.set(cols, ((uint64_t)blockIdx.y * lanes + (threadIdx.x & (lanes - 1))) * N);
+    d_out += place.col;
+    d_weight += (uint64_t)base * cols + place.col;
+    float sum[N];
+    for (uint32_t h = 0; h < n_together; h++) {
+        const uint32_t o = together[h], from = o ? ends[o - 1] : 0, to = ends[o];
+        const uint32_t share = (to - from + groups - 1) / groups, begin = from + group * share;
+        if (begin < to && place.n > 0) {
+            sum_rows(sum, d_out, stride, order, begin, min(begin + share, to), place.n);
+        } else {
+#pragma unroll
+            for (int k = 0; k < N; k++) sum[k] = 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < N; k++) shared.partial[k][threadIdx.x] = sum[k];
+        __syncthreads();
+        for (uint32_t half = kAll / 2; half >= lanes; half /= 2) {
+            if (threadIdx.x < half)
+#pragma unroll
+                for (int k = 0; k < N; k++) shared.partial[k][threadIdx.x] += shared.partial[k][threadIdx.x + half];
+            __syncthreads();
+        }
+        if (group == 0 && place.n > 0) {
+#pragma unroll
+            for (int k = 0; k < N; k++) sum[k] = shared.partial[k][threadIdx.x] * scale;
+            store(d_weight + o * cols, sum, place.n);
+        }
+        __syncthreads();
+    }
+    if (place.n == 0) return;
+    for (uint32_t o = group; o < size; o += groups) {
+        const uint32_t from = o ? ends[o - 1] : 0, to = ends[o];
+        if (to - from > kTogether) continue;
+        if (from < to) {
+            sum_rows(sum, d_out, stride, order, from, to, place.n);
+        } else {
+#pragma unroll
+            for (int k = 0; k < N; k++) sum[k] = 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < N; k++) sum[k] *= scale;
+        store(d_weight + o * cols, sum, place.n);
+    }
+}
+
+// Few enough: every slab's workgroups read all positions, and one workgroup of a table's 256 writes
+// all zeros of its tokens in the slab.  With two slabs 8001 positions of 1001 columns take 26 us either
+// way, with four 8192 of 1024 take 47 against 26.
+template <typename W, typename T>
+bool is_small(const spiky_lm_embed_args &a, uint32_t &lanes, uint64_t &slabs) {
+    constexpr uint64_t N = piece<W, T>();
+    const uint64_t pieces = (a.cols + N - 1) / N;
+    lanes = 1;
+    while (lanes < pieces && lanes < 64) lanes *= 2;
+    slabs = (pieces + lanes - 1) / lanes;
+    return slabs <= 2 && a.n * slabs <= kSmall;
+}
+
 // The workspace: starts, order, and the chunks' sums.
 uint64_t order_at(const spiky_lm_embed_args &a) { return (a.vocab + 1) * 4; }
 uint64_t partial_at(const spiky_lm_embed_args &a) { return order_at(a) + a.n * 4; }
@@ -355,10 +458,13 @@ uint64_t chunks_of(const spiky_lm_embed_args &a) {
     return a.n > kChunk ? (a.n + kChunk - 1) / kChunk : 0;  // no token is frequent among so few
 }
 
+uint32_t range_of(const spiky_lm_embed_args &a) {
+    return (uint32_t)min(max((a.vocab + kCUs - 1) / kCUs, (uint64_t)1), (uint64_t)kMostRange);
+}
+
 template <typename Tok>
 hipError_t sort(const spiky_lm_embed_args &a, uint32_t *start, uint32_t *order, hipStream_t st) {
-    const uint32_t vocab = (uint32_t)a.vocab;
-    const uint32_t range = min(max((vocab + kCUs - 1) / kCUs, 1u), (uint32_t)kMostRange);
+    const uint32_t vocab = (uint32_t)a.vocab, range = range_of(a);
     k_embed_sort<Tok><<<dim3((vocab + range - 1) / range), dim3(kSortWaves * 64), kSortWaves * range * 4, st>>>(
         static_cast<const Tok *>(a.tokens), (uint32_t)a.n, vocab, range, start, order);
     return hipGetLastError();
@@ -418,15 +524,29 @@ hipError_t launch_embed(const spiky_lm_embed_args &a, void *out, hipStream_t st)
 
 uint64_t embed_workspace(const spiky_lm_embed_args &a) { return partial_at(a) + chunks_of(a) * 2 * a.cols * 4; }
 
-hipError_t launch_embed_backward(const spiky_lm_embed_args &a, const void *d_out, int64_t d_out_stride, void *d_weight,
-                                 void *workspace, hipStream_t st) {
+template <typename Tok, typename W, typename T>
+hipError_t gradient(const spiky_lm_embed_args &a, const void *d_out, int64_t stride, void *d_weight, void *workspace,
+                    hipStream_t st) {
+    uint32_t lanes;
+    uint64_t slabs;
+    if (is_small<W, T>(a, lanes, slabs)) {
+        const uint32_t vocab = (uint32_t)a.vocab, range = range_of(a), lds = (kSortWaves * range + (uint32_t)a.n) * 4;
+        k_embed_small<Tok, T, W><<<dim3((vocab + range - 1) / range, (uint32_t)slabs), dim3(kSortWaves * 64), lds, st>>>(
+            static_cast<const Tok *>(a.tokens), static_cast<const T *>(d_out), stride, static_cast<W *>(d_weight),
+            (uint32_t)a.n, vocab, a.cols, range, lanes, (float)a.scale);
+        return hipGetLastError();
+    }
     uint32_t *start = static_cast<uint32_t *>(workspace);
     uint32_t *order = reinterpret_cast<uint32_t *>(static_cast<char *>(workspace) + order_at(a));
-    const hipError_t e = a.tokens_i64 ? sort<int64_t>(a, start, order, st) : sort<int32_t>(a, start, order, st);
-    if (e != hipSuccess) return e;
+    const hipError_t e = sort<Tok>(a, start, order, st);
+    return e != hipSuccess ? e : sums<Tok, W, T>(a, d_out, stride, d_weight, workspace, st);
+}
+
+hipError_t launch_embed_backward(const spiky_lm_embed_args &a, const void *d_out, int64_t d_out_stride, void *d_weight,
+                                 void *workspace, hipStream_t st) {
     return by_types(a.weight_dtype, a.out_dtype, [&](auto w, auto t) {
-        return a.tokens_i64 ? sums<int64_t, decltype(w), decltype(t)>(a, d_out, d_out_stride, d_weight, workspace, st)
-                            : sums<int32_t, decltype(w), decltype(t)>(a, d_out, d_out_stride, d_weight, workspace, st);
+        return a.tokens_i64 ? gradient<int64_t, decltype(w), decltype(t)>(a, d_out, d_out_stride, d_weight, workspace, st)
+                            : gradient<int32_t, decltype(w), decltype(t)>(a, d_out, d_out_stride, d_weight, workspace, st);
     });
 }
 
