@@ -39,7 +39,7 @@ int spiky_lm_embed(const spiky_lm_embed_args *args, void *out, void *stream);
 /* d_weight[v] = scale * the sum of d_out[i] over tokens[i] == v, in 32 bits and in an
  * order that the tokens alone decide, rounded once; zeros for other rows.  Writes all
  * of d_weight [vocab][cols].  d_out: [n][cols], rows d_out_stride elements apart.
- * Host: the workspace's bytes, 4 bytes aligned. */
+ * Host: the workspace's bytes, 16 bytes aligned. */
 uint64_t spiky_lm_embed_workspace(const spiky_lm_embed_args *args);
 int spiky_lm_embed_backward(const spiky_lm_embed_args *args, const void *d_out, int64_t d_out_stride, void *d_weight,
                             void *workspace, uint64_t workspace_bytes, void *stream);

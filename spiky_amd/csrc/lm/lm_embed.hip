@@ -69,11 +69,16 @@ hipError_t lookup(const spiky_lm_embed_args &a, void *out, hipStream_t st) {
 
 // ---- gradient ------------------------------------------------------------------
 // The tokens' positions, sorted by token and for each token in ascending order, and where each
-// token's begin: start [vocab + 1], order [start[vocab]].  One launch without any exchange between
+// token's begin: start [vocab + 1], order [start[vocab]]; and for every chunk of `chunk` sorted positions
+// the run of one token that its first position is in.  One launch without any exchange between
 // workgroups: a workgroup owns `range` consecutive tokens of the vocabulary, reads all n, lists its
 // own for each wave's share of the positions, counts these and the ones below its range, adds up,
 // and places its own.  A wave with more of its own than its list holds reads its share again.
 // Tokens outside the vocabulary are in no range.
+struct Run {
+    uint32_t from, to, token, unused;
+};
+
 constexpr int kSortWaves = 16, kMostRange = 1024;
 constexpr uint32_t kList = 512;                        // of a wave
 constexpr uint32_t kListShare = 0xffffffffu / kMostRange;  // positions of a share that a list's words can tell apart
@@ -183,95 +188,103 @@ __device__ __forceinline__ void sort_range(const Tok *tokens, uint32_t n, uint32
 
 template <typename Tok>
 __global__ __launch_bounds__(kSortWaves * 64) void k_embed_sort(const Tok *__restrict__ tokens, uint32_t n,
-                                                                uint32_t vocab, uint32_t range,
+                                                                uint32_t vocab, uint32_t range, uint32_t chunk,
                                                                 uint32_t *__restrict__ start,
-                                                                uint32_t *__restrict__ order) {
+                                                                uint32_t *__restrict__ order, Run *__restrict__ runs) {
     extern __shared__ uint32_t counts[];  // [kSortWaves][range]
     __shared__ uint32_t lists[kSortWaves][kList];
     const uint32_t base = blockIdx.x * range, size = min(range, vocab - base);
     sort_range(tokens, n, base, size, range, counts, lists, order, true, [&](uint32_t o, uint32_t at, uint32_t total) {
         start[base + o] = at;
         if (base + o == vocab - 1) start[vocab] = at + total;
+        for (uint32_t c = (at + chunk - 1) / chunk; c * chunk < at + total; c++) runs[c] = {at, at + total, base + o, 0};
     });
 }
 
 // Positions of a token that are added up one after the other: tokens with more ("frequent") go in
 // chunks of this many sorted positions, whose sums a launch of its own adds up.  A text's most
 // frequent token stands at every tenth position or so: as one row's sum it took 1.9 ms of 32768
-// tokens' gradient, ten times the rest.
-constexpr uint32_t kChunk = 32;
+// tokens' gradient, ten times the rest.  Fewer, down to kLeastChunk, where chunks would not fill the chip.
+constexpr uint32_t kMostChunk = 32, kLeastChunk = 8;
 constexpr uint64_t kManyGroups = 64 * kCUs;
 
-// The sum over positions [from, to) of the columns at d_out; `from < to`.
+// The sum over positions [from, to) of the n columns at d_out; `from < to`, n > 0.  No load of a whole
+// piece hangs on a condition, so as many rows as registers hold are in flight.
 template <int N, typename T>
 __device__ __forceinline__ void sum_rows(float (&sum)[N], const T *d_out, int64_t stride, const uint32_t *order,
                                          uint32_t from, uint32_t to, int n) {
-    constexpr uint32_t kAhead = 32 / (N * sizeof(T) / 4);  // rows in flight, in 32 registers
+    constexpr uint32_t kAhead = 32 / (N * sizeof(T) / 4);
 #pragma unroll
     for (int k = 0; k < N; k++) sum[k] = 0.f;
-    uint32_t at[kAhead];
+    if (n < N) {  // rows narrower than a piece
+        for (uint32_t i = from; i < to; i++) {
+            float v[N];
+            load(v, d_out + (int64_t)order[i] * stride, n);
+#pragma unroll
+            for (int k = 0; k < N; k++) sum[k] += v[k];
+        }
+        return;
+    }
+    uint32_t at[kAhead], i = from;
 #pragma unroll
     for (uint32_t j = 0; j < kAhead; j++) at[j] = order[min(from + j, to - 1)];
-    for (uint32_t i = from; i < to; i += kAhead) {
-        Raw<T, N> raw[kAhead];
+    Raw<T, N> raw[kAhead];
+    for (; i + kAhead <= to; i += kAhead) {
 #pragma unroll
-        for (uint32_t j = 0; j < kAhead; j++) {
-            raw[j].clear();
-            if (i + j < to) raw[j].load(d_out + (int64_t)at[j] * stride, n);
-        }
+        for (uint32_t j = 0; j < kAhead; j++)
+            __builtin_memcpy(raw[j].w, d_out + (int64_t)at[j] * stride, sizeof(raw[j].w));
 #pragma unroll
         for (uint32_t j = 0; j < kAhead; j++) at[j] = order[min(i + kAhead + j, to - 1)];
 #pragma unroll
-        for (uint32_t j = 0; j < kAhead; j++) {
-            if (i + j >= to) break;
+        for (uint32_t j = 0; j < kAhead; j++)
 #pragma unroll
             for (int k = 0; k < N; k++) sum[k] += raw[j][k];
-        }
+    }
+    // the last few, which for most tokens are one or two and all
+#pragma unroll
+    for (uint32_t j = 0; j < kAhead; j++)
+        if (i + j < to) __builtin_memcpy(raw[j].w, d_out + (int64_t)at[j] * stride, sizeof(raw[j].w));
+#pragma unroll
+    for (uint32_t j = 0; j < kAhead; j++) {
+        if (i + j >= to) break;
+#pragma unroll
+        for (int k = 0; k < N; k++) sum[k] += raw[j][k];
     }
 }
 
-struct Run {
-    uint32_t from, to;
-    bool frequent;
-};
-
-// The run of one token that position i of the sorted ones belongs to.
-template <typename Tok>
-__device__ __forceinline__ Run run_at(const Tok *tokens, const uint32_t *start, const uint32_t *order, uint32_t i) {
-    const uint64_t token = (uint64_t)tokens[order[i]];
-    const Run r = {start[token], start[token + 1], false};
-    return {r.from, r.to, r.to - r.from > kChunk};
-}
-
-// The first `chunks` workgroups of x take chunk blockIdx.x of the sorted positions: the runs of its
-// first and its last one are the only frequent ones that it can hold a part of, since these are
-// longer; their sums go to partial [2 * chunk] and [2 * chunk + 1].  The others take
-// kRows rows a thread of the table's gradient, of tokens that are not frequent.  `lanes` threads, a power of two, take the
-// pieces of a row.
-template <typename Tok, typename T, typename W, uint32_t kRows, bool kStream>
-__global__ __launch_bounds__(kThreads) void k_embed_sum(const Tok *__restrict__ tokens, const T *__restrict__ d_out,
-                                                        int64_t stride, const uint32_t *__restrict__ start,
-                                                        const uint32_t *__restrict__ order, W *__restrict__ d_weight,
-                                                        float *__restrict__ partial, uint32_t vocab, uint64_t cols,
-                                                        uint32_t chunks, uint32_t chunk_groups, uint32_t lanes,
-                                                        float scale) {
+// The first `chunk_groups` workgroups of x take chunks of the sorted positions, `lanes` threads, a
+// power of two, each: frequent runs are longer than a chunk, so the only ones that a chunk holds a
+// part of are the one of its first position and the one of the next chunk's.  Their sums go to partial
+// [2 * chunk] and [2 * chunk + 1].  The others take kRows rows a thread of the table's gradient, of
+// tokens that are not frequent.
+template <typename T, typename W, uint32_t kRows, bool kStream>
+__global__ __launch_bounds__(kThreads) void k_embed_sum(const T *__restrict__ d_out, int64_t stride,
+                                                        const uint32_t *__restrict__ start,
+                                                        const uint32_t *__restrict__ order,
+                                                        const Run *__restrict__ runs, W *__restrict__ d_weight,
+                                                        float *__restrict__ partial, uint64_t pitch, uint32_t vocab,
+                                                        uint64_t cols,
+                                                        uint32_t size, uint32_t chunks, uint32_t chunk_groups,
+                                                        uint32_t lanes, float scale) {
     constexpr int N = piece<W, T>();
     Place<N> place;
     place.set(cols, ((uint64_t)blockIdx.y * lanes + (threadIdx.x & (lanes - 1))) * N);
     const uint32_t rows = kThreads / lanes, own = threadIdx.x / lanes;
     float sum[N];
     if (blockIdx.x < chunk_groups) {
-        const uint32_t chunk = blockIdx.x * rows + own, n = start[vocab], begin = chunk * kChunk;
-        if (chunk >= chunks || begin >= n || place.n == 0) return;
-        const uint32_t end = min(begin + kChunk, n);
-        const Run first = run_at(tokens, start, order, begin), last = run_at(tokens, start, order, end - 1);
-        if (first.frequent) {
+        const uint32_t chunk = blockIdx.x * rows + own, begin = chunk * size;
+        if (chunk >= chunks || place.n == 0) return;
+        const uint32_t n = start[vocab];
+        const Run first = runs[chunk], next = runs[min(chunk + 1, chunks - 1)];  // not written past n
+        if (begin >= n) return;
+        const uint32_t end = min(begin + size, n);
+        if (first.to - first.from > size) {
             sum_rows(sum, d_out + place.col, stride, order, begin, min(end, first.to), place.n);
-            store(partial + (uint64_t)chunk * 2 * cols + place.col, sum, place.n);
+            store(partial + (uint64_t)chunk * 2 * pitch + place.col, sum, place.n);
         }
-        if (last.frequent && last.from != first.from) {
-            sum_rows(sum, d_out + place.col, stride, order, last.from, end, place.n);
-            store(partial + ((uint64_t)chunk * 2 + 1) * cols + place.col, sum, place.n);
+        if (begin + size < n && next.from > begin && next.from < end && next.to - next.from > size) {
+            sum_rows(sum, d_out + place.col, stride, order, next.from, end, place.n);
+            store(partial + ((uint64_t)chunk * 2 + 1) * pitch + place.col, sum, place.n);
         }
         return;
     }
@@ -286,7 +299,7 @@ __global__ __launch_bounds__(kThreads) void k_embed_sum(const Tok *__restrict__ 
     if (place.n == 0) return;
 #pragma unroll
     for (uint32_t r = 0; r < kRows; r++) {
-        if (to[r] - from[r] > kChunk) continue;
+        if (to[r] - from[r] > size) continue;
         if (from[r] < to[r]) {
             sum_rows(sum, d_out + place.col, stride, order, from[r], to[r], place.n);
         } else {
@@ -303,50 +316,46 @@ __global__ __launch_bounds__(kThreads) void k_embed_sum(const Tok *__restrict__ 
     }
 }
 
-// The rows of frequent tokens, from their chunks' sums: workgroup x adds up the runs that begin in
-// kJoined chunks from x * kJoined on and go on into the next one, 64 lanes a group of columns, wave w the
-// sums number w, w + 4, ... of a run.
-constexpr uint32_t kJoined = 8;
-
-template <typename Tok, typename W>
-__global__ __launch_bounds__(kThreads) void k_embed_join(const Tok *__restrict__ tokens,
-                                                         const uint32_t *__restrict__ start,
-                                                         const uint32_t *__restrict__ order, W *__restrict__ d_weight,
-                                                         const float *__restrict__ partial, uint32_t vocab,
-                                                         uint64_t cols, float scale) {
+// The rows of frequent tokens, from their chunks' sums: workgroup x adds up the runs whose first whole
+// chunk is one of `joined` from x * joined on, 64 lanes a group of columns, wave w the sums number w,
+// w + 4, ... of a run.
+template <typename W>
+__global__ __launch_bounds__(kThreads) void k_embed_join(const uint32_t *__restrict__ start,
+                                                         const Run *__restrict__ runs, W *__restrict__ d_weight,
+                                                         const float *__restrict__ partial, uint64_t pitch, uint32_t vocab,
+                                                         uint64_t cols, uint32_t size, uint32_t chunks,
+                                                         uint32_t joined, float scale) {
     constexpr int N = 4, kAhead = 8;
     constexpr uint32_t kWaves = kThreads / 64;
     __shared__ float sums[kWaves - 1][N][64];
     const uint32_t n = start[vocab], wave = threadIdx.x / 64, lane = threadIdx.x & 63;
-    const uint32_t chunk0 = blockIdx.x * kJoined;
     // a lane a chunk, the same in all waves
-    Run mine = {0, 0, false};
-    if (lane < kJoined && (chunk0 + lane) * kChunk < n) {
-        mine = run_at(tokens, start, order, min((chunk0 + lane + 1) * kChunk, n) - 1);
-        mine.frequent = mine.frequent && mine.from >= (chunk0 + lane) * kChunk;
-    }
+    const uint32_t mine = min(blockIdx.x * joined + lane, chunks - 1);
+    const Run run = runs[mine];
+    const bool begins = lane < joined && blockIdx.x * joined + lane < chunks && mine * size < n &&
+                        run.to - run.from > size && run.from + size > mine * size;
     Place<N> place;
     place.set(cols, ((uint64_t)blockIdx.y * 64 + lane) * N);
-    for (uint64_t found = __ballot(mine.frequent); found; found &= found - 1) {
-        const uint32_t l = __builtin_ctzll(found), chunk = chunk0 + l;
-        const uint32_t from = __builtin_amdgcn_readlane(mine.from, l), to = __builtin_amdgcn_readlane(mine.to, l);
-        const uint32_t parts = (to - 1) / kChunk - chunk + 1;
-        // a run that begins inside its first chunk is that one's last
-        const uint32_t skew = from > chunk * kChunk ? 1 : 0;
-        const float *p = partial + (uint64_t)chunk * 2 * cols + place.col;
+    for (uint64_t found = __ballot(begins); found; found &= found - 1) {
+        const uint32_t l = __builtin_ctzll(found);
+        const uint32_t from = __builtin_amdgcn_readlane(run.from, l), to = __builtin_amdgcn_readlane(run.to, l);
+        const uint32_t token = __builtin_amdgcn_readlane(run.token, l);
+        const uint32_t chunk = from / size, parts = (to - 1) / size - chunk + 1;
+        // a run that begins inside a chunk is that one's second
+        const uint32_t skew = from > chunk * size ? 1 : 0;
+        const float *p = partial + (uint64_t)chunk * 2 * pitch + place.col;
         float sum[N] = {};
         for (uint32_t i = wave; i < parts; i += kWaves * kAhead) {
             Raw<float, N> raw[kAhead];
 #pragma unroll
             for (uint32_t j = 0; j < kAhead; j++) {
-                const uint32_t k = i + j * kWaves;
-                raw[j].clear();
-                if (k < parts) raw[j].load(p + ((uint64_t)k * 2 + (k == 0 ? skew : 0)) * cols, place.n);
+                const uint32_t k = min(i + j * kWaves, parts - 1);
+                __builtin_memcpy(raw[j].w, p + ((uint64_t)k * 2 + (k == 0 ? skew : 0)) * pitch, sizeof(raw[j].w));
             }
 #pragma unroll
             for (uint32_t j = 0; j < kAhead; j++)
 #pragma unroll
-                for (int k = 0; k < N; k++) sum[k] += raw[j][k];
+                for (int k = 0; k < N; k++) sum[k] += i + j * kWaves < parts ? raw[j][k] : 0.f;
         }
         __syncthreads();  // the sums of the run before are read
         if (wave > 0)
@@ -356,7 +365,7 @@ __global__ __launch_bounds__(kThreads) void k_embed_join(const Tok *__restrict__
         for (uint32_t w = 0; w < kWaves - 1; w++)
             for (int k = 0; k < N; k++) sum[k] += sums[w][k][lane];
         for (int k = 0; k < N; k++) sum[k] *= scale;
-        store(d_weight + (uint64_t)tokens[order[from]] * cols + place.col, sum, place.n);
+        store(d_weight + (uint64_t)token * cols + place.col, sum, place.n);
     }
 }
 
@@ -366,6 +375,7 @@ __global__ __launch_bounds__(kThreads) void k_embed_join(const Tok *__restrict__
 // for 8192 positions of 256 columns in a table of 256 rows, this one 17; 26 and 22 for 512 of 1024 in
 // one of 50000.
 constexpr uint32_t kSmall = 8192, kTogether = 16;
+constexpr uint64_t kSmallBytes = 4 << 20;
 
 template <typename Tok, typename T, typename W>
 __global__ __launch_bounds__(kSortWaves * 64) void k_embed_small(const Tok *__restrict__ tokens,
@@ -438,9 +448,10 @@ __global__ __launch_bounds__(kSortWaves * 64) void k_embed_small(const Tok *__re
     }
 }
 
-// Few enough: every slab's workgroups read all positions, and one workgroup of a table's 256 writes
+// Few enough: one workgroup adds up a frequent token's rows, and every slab's workgroups read all positions, and one workgroup of a table's 256 writes
 // all zeros of its tokens in the slab.  With two slabs 8001 positions of 1001 columns take 26 us either
 // way, with four 8192 of 1024 take 47 against 26.
+// 8192 of 256 fp32 columns that no cache holds take 29 us against 26.
 template <typename W, typename T>
 bool is_small(const spiky_lm_embed_args &a, uint32_t &lanes, uint64_t &slabs) {
     constexpr uint64_t N = piece<W, T>();
@@ -448,59 +459,61 @@ bool is_small(const spiky_lm_embed_args &a, uint32_t &lanes, uint64_t &slabs) {
     lanes = 1;
     while (lanes < pieces && lanes < 64) lanes *= 2;
     slabs = (pieces + lanes - 1) / lanes;
-    return slabs <= 2 && a.n * slabs <= kSmall;
+    return slabs <= 2 && a.n * slabs <= kSmall && a.n * a.cols * sizeof(T) <= kSmallBytes;
 }
 
-// The workspace: starts, order, and the chunks' sums.
-uint64_t order_at(const spiky_lm_embed_args &a) { return (a.vocab + 1) * 4; }
-uint64_t partial_at(const spiky_lm_embed_args &a) { return order_at(a) + a.n * 4; }
-uint64_t chunks_of(const spiky_lm_embed_args &a) {
-    return a.n > kChunk ? (a.n + kChunk - 1) / kChunk : 0;  // no token is frequent among so few
+// Positions of a chunk, a power of two, and chunks: two workgroups of columns by four to a CU, or
+// chunks of the fewest positions.
+uint64_t chunk_of(const spiky_lm_embed_args &a) {
+    uint64_t chunk = kMostChunk;
+    while (chunk > kLeastChunk && a.n / chunk * ((a.cols + 3) / 4) < kCUs / 2 * kThreads) chunk /= 2;
+    return chunk;
 }
+uint64_t chunks_of(const spiky_lm_embed_args &a) { return (a.n + chunk_of(a) - 1) / chunk_of(a); }
+
+// The workspace: runs, starts, order, and the chunks' sums.
+uint64_t start_at(const spiky_lm_embed_args &a) { return chunks_of(a) * sizeof(Run); }
+uint64_t order_at(const spiky_lm_embed_args &a) { return start_at(a) + (a.vocab + 1) * 4; }
+uint64_t partial_at(const spiky_lm_embed_args &a) { return order_at(a) + a.n * 4; }
+uint64_t pitch_of(const spiky_lm_embed_args &a) { return max(a.cols, (uint64_t)4); }  // of a chunk's sums: a piece at least
 
 uint32_t range_of(const spiky_lm_embed_args &a) {
     return (uint32_t)min(max((a.vocab + kCUs - 1) / kCUs, (uint64_t)1), (uint64_t)kMostRange);
 }
 
-template <typename Tok>
-hipError_t sort(const spiky_lm_embed_args &a, uint32_t *start, uint32_t *order, hipStream_t st) {
-    const uint32_t vocab = (uint32_t)a.vocab, range = range_of(a);
-    k_embed_sort<Tok><<<dim3((vocab + range - 1) / range), dim3(kSortWaves * 64), kSortWaves * range * 4, st>>>(
-        static_cast<const Tok *>(a.tokens), (uint32_t)a.n, vocab, range, start, order);
-    return hipGetLastError();
-}
-
-template <typename Tok, typename W, typename T>
-hipError_t sums(const spiky_lm_embed_args &a, const void *d_out_, int64_t stride, void *d_weight_, void *workspace,
-                hipStream_t st) {
+template <typename W, typename T>
+hipError_t sums(const spiky_lm_embed_args &a, const void *d_out_, int64_t stride, void *d_weight_, const Run *runs,
+                const uint32_t *start, const uint32_t *order, float *partial, hipStream_t st) {
     constexpr uint64_t N = piece<W, T>();
-    const uint32_t *start = static_cast<const uint32_t *>(workspace);
-    const uint32_t *order = reinterpret_cast<const uint32_t *>(static_cast<char *>(workspace) + order_at(a));
-    float *partial = reinterpret_cast<float *>(static_cast<char *>(workspace) + partial_at(a));
-    const Tok *tokens = static_cast<const Tok *>(a.tokens);
     const T *d_out = static_cast<const T *>(d_out_);
     W *d_weight = static_cast<W *>(d_weight_);
     const uint64_t pieces = (a.cols + N - 1) / N;
     uint32_t lanes = 1;
     while (lanes < pieces && lanes < kThreads) lanes *= 2;
-    const uint32_t rows = kThreads / lanes, chunks = (uint32_t)chunks_of(a), groups = (chunks + rows - 1) / rows;
+    const uint32_t rows = kThreads / lanes, chunk = (uint32_t)chunk_of(a), chunks = (uint32_t)chunks_of(a);
+    const uint32_t groups = a.n > chunk ? (chunks + rows - 1) / rows : 0;  // no token is frequent among fewer
     const uint64_t slabs = (pieces + lanes - 1) / lanes;
     auto go = [&](auto kernel, uint64_t each) {
         const uint64_t all = groups + (a.vocab + rows * each - 1) / (rows * each);
         if (all * kThreads > 0xffffffffull) return hipErrorInvalidValue;
         kernel<<<dim3((uint32_t)all, (uint32_t)slabs), dim3(kThreads), 0, st>>>(
-            tokens, d_out, stride, start, order, d_weight, partial, (uint32_t)a.vocab, a.cols, chunks, groups, lanes,
+            d_out, stride, start, order, runs, d_weight, partial, pitch_of(a), (uint32_t)a.vocab, a.cols, chunk, chunks, groups, lanes,
             (float)a.scale);
         return hipGetLastError();
     };
-    // several rows to a thread where there are enough: most have no token, and only their zeros to write
+    // Several rows to a thread where there are enough: most have no token, and only their zeros to write.
+    // 1, 4, 8 and 16 rows take 424, 325, 332 and 373 us of 32768 tokens' 4096 bf16 columns and 152000
+    // rows.  There results go past the last cache, which would not hold them for their reader: 306 us.
+    // 32000 rows of 2048 fp32 columns, which it holds, take 78 stored as usual and 112 past it.
     const bool many = a.vocab / rows * slabs >= kManyGroups;
     const bool stream = a.vocab * a.cols * sizeof(W) >= kLastCache * 2;
-    const hipError_t e = many ? stream ? go(k_embed_sum<Tok, T, W, 4, true>, 4) : go(k_embed_sum<Tok, T, W, 4, false>, 4)
-                              : go(k_embed_sum<Tok, T, W, 1, false>, 1);
-    if (e != hipSuccess || chunks == 0) return e;
-    k_embed_join<Tok, W><<<dim3((chunks + kJoined - 1) / kJoined, (uint32_t)((a.cols + 255) / 256)), dim3(kThreads), 0, st>>>(
-        tokens, start, order, d_weight, partial, (uint32_t)a.vocab, a.cols, (float)a.scale);
+    const hipError_t e = many ? stream ? go(k_embed_sum<T, W, 4, true>, 4) : go(k_embed_sum<T, W, 4, false>, 4)
+                              : go(k_embed_sum<T, W, 1, false>, 1);
+    if (e != hipSuccess || groups == 0) return e;
+    // most chunks begin no run: where there are many, a workgroup looks at several
+    const uint32_t col_groups = (uint32_t)((a.cols + 255) / 256), joined = (uint64_t)chunks * col_groups > 4 * kCUs ? 8 : 1;
+    k_embed_join<W><<<dim3((chunks + joined - 1) / joined, col_groups), dim3(kThreads), 0, st>>>(
+        start, runs, d_weight, partial, pitch_of(a), (uint32_t)a.vocab, a.cols, chunk, chunks, joined, (float)a.scale);
     return hipGetLastError();
 }
 
@@ -522,7 +535,7 @@ hipError_t launch_embed(const spiky_lm_embed_args &a, void *out, hipStream_t st)
     });
 }
 
-uint64_t embed_workspace(const spiky_lm_embed_args &a) { return partial_at(a) + chunks_of(a) * 2 * a.cols * 4; }
+uint64_t embed_workspace(const spiky_lm_embed_args &a) { return partial_at(a) + chunks_of(a) * 2 * pitch_of(a) * 4; }
 
 template <typename Tok, typename W, typename T>
 hipError_t gradient(const spiky_lm_embed_args &a, const void *d_out, int64_t stride, void *d_weight, void *workspace,
@@ -536,10 +549,15 @@ hipError_t gradient(const spiky_lm_embed_args &a, const void *d_out, int64_t str
             (uint32_t)a.n, vocab, a.cols, range, lanes, (float)a.scale);
         return hipGetLastError();
     }
-    uint32_t *start = static_cast<uint32_t *>(workspace);
-    uint32_t *order = reinterpret_cast<uint32_t *>(static_cast<char *>(workspace) + order_at(a));
-    const hipError_t e = sort<Tok>(a, start, order, st);
-    return e != hipSuccess ? e : sums<Tok, W, T>(a, d_out, stride, d_weight, workspace, st);
+    char *w = static_cast<char *>(workspace);
+    Run *runs = reinterpret_cast<Run *>(w);
+    uint32_t *start = reinterpret_cast<uint32_t *>(w + start_at(a)), *order = reinterpret_cast<uint32_t *>(w + order_at(a));
+    const uint32_t vocab = (uint32_t)a.vocab, range = range_of(a);
+    k_embed_sort<Tok><<<dim3((vocab + range - 1) / range), dim3(kSortWaves * 64), kSortWaves * range * 4, st>>>(
+        static_cast<const Tok *>(a.tokens), (uint32_t)a.n, vocab, range, (uint32_t)chunk_of(a), start, order, runs);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    return sums<W, T>(a, d_out, stride, d_weight, runs, start, order, reinterpret_cast<float *>(w + partial_at(a)), st);
 }
 
 hipError_t launch_embed_backward(const spiky_lm_embed_args &a, const void *d_out, int64_t d_out_stride, void *d_weight,
