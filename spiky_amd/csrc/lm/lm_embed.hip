@@ -204,7 +204,7 @@ __global__ __launch_bounds__(kSortWaves * 64) void k_embed_sort(const Tok *__res
 // Positions of a token that are added up one after the other: tokens with more ("frequent") go in
 // chunks of this many sorted positions, whose sums a launch of its own adds up.  A text's most
 // frequent token stands at every tenth position or so: as one row's sum it took 1.9 ms of 32768
-// tokens' gradient, ten times the rest.  Fewer, down to kLeastChunk, where chunks would not fill the chip.
+// tokens' gradient, ten times the rest.  Fewer positions, down to kLeastChunk, where chunks would not fill the chip.
 constexpr uint32_t kMostChunk = 32, kLeastChunk = 8;
 constexpr uint64_t kManyGroups = 64 * kCUs;
 
@@ -371,11 +371,10 @@ __global__ __launch_bounds__(kThreads) void k_embed_join(const uint32_t *__restr
 
 // Both in one launch, for few positions: a workgroup takes `range` tokens and a slab of `lanes` pieces of
 // their rows, sorts for itself, and adds up.  Its groups of `lanes` threads take a token each, and all
-// of them one that has more than kTogether positions, a share each.  The three launches take 21 us
-// for 8192 positions of 256 columns in a table of 256 rows, this one 17; 26 and 22 for 512 of 1024 in
-// one of 50000.
+// of them one that has more than kTogether positions, a share each.  64 positions of 256 columns in a
+// table of 256 rows take 5 us, in three launches 14.
 constexpr uint32_t kSmall = 8192, kTogether = 16;
-constexpr uint64_t kSmallBytes = 4 << 20;
+constexpr uint64_t kSmallBytes = 2 << 20;
 
 template <typename Tok, typename T, typename W>
 __global__ __launch_bounds__(kSortWaves * 64) void k_embed_small(const Tok *__restrict__ tokens,
@@ -448,10 +447,11 @@ __global__ __launch_bounds__(kSortWaves * 64) void k_embed_small(const Tok *__re
     }
 }
 
-// Few enough: one workgroup adds up a frequent token's rows, and every slab's workgroups read all positions, and one workgroup of a table's 256 writes
-// all zeros of its tokens in the slab.  With two slabs 8001 positions of 1001 columns take 26 us either
-// way, with four 8192 of 1024 take 47 against 26.
-// 8192 of 256 fp32 columns that no cache holds take 29 us against 26.
+// Few enough: here one workgroup adds up a frequent token's rows, and every slab's workgroups read all
+// positions.  Where no cache holds the gradient, one launch and three take 27 and 31 us for 512
+// positions of 1024 bf16 columns (1 MB) in a table of 50000 rows, 26 and 32 for 8192 of 64 fp32 (2 MB)
+// in one of 152000, 35 and 33 for 2048 of 1024 bf16 (4 MB), 29 and 22 for 8192 of 256 fp32 (8 MB) in
+// one of 256.
 template <typename W, typename T>
 bool is_small(const spiky_lm_embed_args &a, uint32_t &lanes, uint64_t &slabs) {
     constexpr uint64_t N = piece<W, T>();
@@ -462,8 +462,9 @@ bool is_small(const spiky_lm_embed_args &a, uint32_t &lanes, uint64_t &slabs) {
     return slabs <= 2 && a.n * slabs <= kSmall && a.n * a.cols * sizeof(T) <= kSmallBytes;
 }
 
-// Positions of a chunk, a power of two, and chunks: two workgroups of columns by four to a CU, or
-// chunks of the fewest positions.
+// Positions of a chunk, a power of two, and chunks: half a workgroup of pieces of four columns to a CU,
+// or chunks of the fewest positions.  8192 positions of 256 columns, one in nine the same token, take
+// 22.3 us with 16 positions to a chunk, 24.6 with 8 and 23.4 with 32, which is as good from 1001 columns on.
 uint64_t chunk_of(const spiky_lm_embed_args &a) {
     uint64_t chunk = kMostChunk;
     while (chunk > kLeastChunk && a.n / chunk * ((a.cols + 3) / 4) < kCUs / 2 * kThreads) chunk /= 2;

@@ -246,3 +246,25 @@ def test_zeros_of_both_signs_are_equal(cuda_device):
         x[:, :, 100:] = -1.0
         got = run(cuda_device, x, torch.tensor([[-0.0, 0.0]]), 5)
         assert got[2].tolist() == [[0, 1, 2, 3, 4]] and got[1].tolist() == [[0] * 5]
+
+
+@pytest.mark.parametrize("dtype", [F, B])
+def test_sorted_logits(cuda_device, dtype):
+    """The first candidates side by side, at either end, in many slices."""
+    for vocab in (3000, 8200, 70000):
+        x = torch.linspace(-30.0, 5.0, vocab).to(dtype).expand(2, 2, vocab).contiguous()
+        scores = torch.tensor([[-1.0, -2.5], [-0.25, -0.25]])
+        for n in (1, 7, 64):
+            run(cuda_device, x, scores, n)
+            run(cuda_device, x.flip(2).contiguous(), scores, n)
+
+
+@pytest.mark.parametrize("beams,n", [(3, 64), (16, 64), (64, 3), (7, 5)])
+def test_many_equal_ranks(cuda_device, beams, n):
+    """More candidates of one rank than the join lists."""
+    for vocab in (40, 9000, 40000):
+        x = torch.zeros(2, beams, vocab, dtype=B)
+        x[1, :, ::3] = 1.0
+        scores = torch.zeros(2, beams)
+        run(cuda_device, x, scores, n)
+        run(cuda_device, x, scores, n, lengths=torch.full((2, beams), 3), length_penalty=0.5)

@@ -249,3 +249,23 @@ def test_derivatives_that_there_are_none_of(cuda_device):
             embed_tokens(tokens, dual)
     with pytest.raises(RuntimeError, match="cannot be traced"):
         torch.jit.trace(lambda x: embed_tokens(tokens, x), w.detach())
+
+
+@pytest.mark.parametrize("n,vocab,cols,weight,out", [
+    (8192, 300, 64, F, F), (8193, 300, 64, F, F), (8192, 20, 65, F, F), (4096, 900, 128, F, F), (4096, 900, 129, F, F),
+    (2048, 3000, 512, B, B), (2048, 3000, 513, B, B), (2049, 3000, 512, B, B), (4095, 40, 500, H, H)])
+def test_sizes_at_which_another_way_is_taken(cuda_device, n, vocab, cols, weight, out):
+    """One launch or three, one slab of columns or two."""
+    gen = torch.Generator().manual_seed(5)
+    both(cuda_device, text(gen, vocab, n).to(cuda_device), vocab, cols, weight, out, 0.3)
+
+
+@pytest.mark.parametrize("cols", [24, 320, 1000])
+def test_runs_at_the_ends_of_chunks(cuda_device, cols):
+    """Chunks of 8, 16 and 32 sorted positions: runs that are as long, one longer, begin with one or inside."""
+    for first in (0, 1, 7, 8, 16, 31, 32):
+        counts = [first, 8, 9, 7, 16, 17, 15, 32, 33, 31, 64, 65, 63, 1, 0, 0, 2, 1000, 24, 25, 0, 3000, 96, 5200]
+        tokens = torch.repeat_interleave(torch.arange(len(counts)), torch.tensor(counts))
+        tokens = tokens[torch.randperm(len(tokens), generator=torch.Generator().manual_seed(first))]
+        both(cuda_device, tokens.to(cuda_device), len(counts), cols, F, B)
+        both(cuda_device, torch.cat([tokens, torch.full((77,), -1)]).to(cuda_device), len(counts) + 3, cols, F, B)
