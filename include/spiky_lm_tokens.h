@@ -30,7 +30,7 @@ typedef struct {
     const void *tokens;        /* [n] */
     const void *weight;        /* [vocab][cols], rows weight_stride elements apart (not read by the gradient) */
     int64_t weight_stride;
-    double scale;              /* as a float */
+    double scale;              /* as a float, finite */
 } spiky_lm_embed_args;
 
 /* out [n][cols] */

@@ -84,6 +84,7 @@ void check(const spiky_lm_embed_args *a) {
             "the table and the result must have one type, or one of them fp32");
     require(a->n < 0x80000000ull && a->vocab < 0x80000000ull && a->cols <= 0x800000ull,
             "too many tokens, rows or columns");
+    require(std::isfinite((float)a->scale), "the scale must be finite in 32 bits");
 }
 
 void check(const spiky_lm_beams_args *a) {

@@ -1,6 +1,7 @@
 // lm_tokens_torch.cpp -- the operators of include/spiky_lm_tokens.h on torch tensors.
 // Host code only; all device work goes through the C ABI of libspiky_lut.so.
 #include <algorithm>
+#include <cmath>
 #include <vector>
 
 #include "lm_torch.h"
@@ -178,6 +179,7 @@ PyObject *embed_tokens(PyObject *, PyObject *const *args, Py_ssize_t n) {
     const Tensor given = device_tensor(args[Tokens], "tokens", weight.device());
     is_index(given, "tokens");
     const double scale = number(args[Scale]);
+    TORCH_CHECK_VALUE(std::isfinite((float)scale), "scale must be finite in 32 bits, got ", scale);
     ScalarType dtype = weight.scalar_type();
     if (args[Dtype] != Py_None) {
         TORCH_CHECK(THPDtype_Check(args[Dtype]), "dtype must be a torch.dtype");
@@ -334,6 +336,7 @@ PyObject *reorder_states(PyObject *, PyObject *const *args, Py_ssize_t n) {
             }
         }
         const bool empty = in[i].numel() == 0 || out[i].numel() == 0;
+        if (in[i].numel() == 0 && out[i].numel() > 0) out[i].zero_();  // of no beams, every parent is outside
         states[i] = {reinterpret_cast<const void *>(a.at), reinterpret_cast<void *>(b.at), empty ? 0 : a.runs,
                      a.run_bytes, a.search, a.beam, a.run, b.search, b.beam, b.run};
     }

@@ -10,7 +10,7 @@ def embed_tokens(tokens, weight, scale=1.0, dtype=None):
 
     tokens: int32 or int64 on a HIP device, any shape.  weight: [V, E], float32, bfloat16 or float16,
     rows at any distance.  The result has the weight's type, or `dtype`: float32, or any of the three
-    beside a float32 weight.  scale: a number, used in 32 bits; each product is rounded to 32 bits and
+    beside a float32 weight.  scale: a number, finite in 32 bits; each product is rounded to 32 bits and
     then to the result's type.
 
     The gradient of the weight is dense: scale times the sum of the output's gradient over a token's

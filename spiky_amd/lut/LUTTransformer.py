@@ -287,6 +287,8 @@ class LUTTransformer(nn.Module):
         search is left with no continuation, or with logits of NaN or infinity."""
         B, L = tokens.shape
         K, S, device = beams, self.context_size, tokens.device
+        if not 1 <= K <= 64:
+            raise ValueError(f"beams must be 1 to 64, got {K}")
         prompt = torch.full((B,), L, dtype=torch.int64, device=device) if lengths is None else \
             lengths.to(device=device, dtype=torch.int64)
         if L == 0 or int(prompt.min()) < 1 or int(prompt.max()) > L:

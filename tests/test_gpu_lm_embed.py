@@ -225,6 +225,8 @@ REFUSED = [
     (lambda t: embed_tokens(t["i"], t["w"], dtype=torch.float64), ValueError, "dtype must be"),
     (lambda t: embed_tokens(t["i"], t["w"], dtype="half"), RuntimeError, "torch.dtype"),
     (lambda t: embed_tokens(t["i"], t["w"], "large"), TypeError, "real number"),
+    (lambda t: embed_tokens(t["i"], t["w"], math.nan), ValueError, "must be finite"),
+    (lambda t: embed_tokens(t["i"], t["w"], -1e39), ValueError, "must be finite"),
 ]
 
 
@@ -269,3 +271,34 @@ def test_runs_at_the_ends_of_chunks(cuda_device, cols):
         tokens = tokens[torch.randperm(len(tokens), generator=torch.Generator().manual_seed(first))]
         both(cuda_device, tokens.to(cuda_device), len(counts), cols, F, B)
         both(cuda_device, torch.cat([tokens, torch.full((77,), -1)]).to(cuda_device), len(counts) + 3, cols, F, B)
+
+
+def test_a_capture_beside_an_eager_graph_of_the_same_leaf_is_refused(cuda_device):
+    """The eager graph's leaf belongs to the default stream; without it the capture is made."""
+    w = torch.randn(64, 16, device=cuda_device, requires_grad=True)
+    tokens, dy = torch.randint(0, 64, (9,), device=cuda_device), torch.randn(9, 16, device=cuda_device)
+    eager = embed_tokens(tokens, w)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="belongs to the default stream"):
+        with torch.cuda.graph(graph):
+            torch.autograd.grad(embed_tokens(tokens, w), w, dy)
+    del eager
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        (dw,) = torch.autograd.grad(embed_tokens(tokens, w), w, dy)
+    graph.replay()
+    torch.cuda.synchronize()
+    close(dw, *plain.embed_gradient(tokens, dy, 64, 1.0))
+
+
+def test_one_leaf_looked_up_twice(cuda_device):
+    """Its gradients add up."""
+    w = torch.randn(30, 40, device=cuda_device, requires_grad=True)
+    first, second = torch.randint(0, 30, (2, 50), device=cuda_device)
+    a, b = torch.randn(2, 50, 40, device=cuda_device)
+    ((embed_tokens(first, w) * a).sum() + (embed_tokens(second, w, 2.0) * b).sum()).backward()
+    sums, errors = plain.embed_gradient(first, a, 30, 1.0)
+    more, others = plain.embed_gradient(second, b, 30, 2.0)
+    # the sum of both is rounded once more
+    close(w.grad, sums + more, errors + others + (sums.abs() + more.abs()) * 2 * plain.STEP32)

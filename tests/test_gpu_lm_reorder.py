@@ -119,6 +119,16 @@ def test_parents_outside_are_zeros(cuda_device):
         assert torch.equal(y, want)
 
 
+def test_no_beams_and_no_positions(cuda_device):
+    x = torch.ones(2, 0, 5, device=cuda_device)
+    assert torch.equal(reorder_states(x, torch.zeros(2, 3, dtype=torch.int64, device=cuda_device)), torch.zeros(2, 3, 5, device=cuda_device))
+    none = torch.zeros(2, 0, dtype=torch.int64, device=cuda_device)
+    assert reorder_states(x, none).shape == (2, 0, 5) and reorder_states(x, none, out=x) is x
+    assert reorder_states(torch.ones(2, 4, 5, device=cuda_device), none).shape == (2, 0, 5)
+    assert reorder_states(torch.ones(2, 4, 0, device=cuda_device), none + 1).shape == (2, 0, 0)
+    assert reorder_states(torch.ones(0, 4, 3, device=cuda_device), torch.zeros(0, 4, dtype=torch.int32, device=cuda_device)).shape == (0, 4, 3)
+
+
 def test_offsets_past_32_bits(cuda_device):
     x = torch.zeros(2, 3, (1 << 30) + 77, dtype=torch.uint8, device=cuda_device)
     x[0, 1, -1], x[1, 0, -3], x[1, 2, 5] = 11, 12, 13

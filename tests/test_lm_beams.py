@@ -137,6 +137,9 @@ def test_refusals(model):
     for lengths in (torch.tensor([0, 1]), torch.tensor([1, 2])):
         with pytest.raises(ValueError, match="a prompt has 1 to L tokens"):
             model.generate_beams(prompt, 2, 2, lengths=lengths)
+    for beams in (0, -1, 65):
+        with pytest.raises(ValueError, match="1 to 64"):
+            model.generate_beams(prompt, 0, beams)
     with pytest.raises(ValueError, match="no continuation to choose"):
         model.generate_beams(prompt, 2, 2, mask=torch.zeros(VOCAB, dtype=torch.bool))
     model.table.data[4, 1] = math.nan

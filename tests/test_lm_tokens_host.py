@@ -53,6 +53,8 @@ def embed_args(**kw):
     (dict(cols=(1 << 26) + 1), "too many"),
     (dict(tokens=None), "null pointer"),
     (dict(weight=None), "null pointer"),
+    (dict(scale=float("inf")), "must be finite"),
+    (dict(scale=1e39), "must be finite"),
 ])
 def test_embed_entry_refuses(change, message):
     refuse(_native.lib().spiky_lm_embed(embed_args(**change), 16, None), message)
