@@ -23,31 +23,39 @@ __global__ __launch_bounds__(kThreads) void k_embed(const Tok *__restrict__ toke
     const uint64_t first = (uint64_t)blockIdx.x * (kThreads * kPieces);
     const uint64_t row0 = first < 0x100000000ull ? row_pieces.divide((uint32_t)first) : first / row_pieces.d;
     const uint32_t piece0 = (uint32_t)(first - row0 * row_pieces.d);
+    // first all tokens, then all pieces, then the results: no load waits for another piece's
+    uint64_t row[kPieces], token[kPieces];
+    Place<N> place[kPieces];
+    Raw<W, N> raw[kPieces];
 #pragma unroll
     for (int i = 0; i < kPieces; i++) {
         const uint64_t at = (uint64_t)piece0 + i * kThreads + threadIdx.x;
         // a long row ends at most once in the workgroup's pieces, a short one's numbers fit 32 bits
         const uint32_t down = row_pieces.d >= kThreads * kPieces ? at >= row_pieces.d
                                                                  : row_pieces.divide((uint32_t)at);
-        const uint64_t row = row0 + down;
-        if (row >= n) break;
-        Place<N> place;
-        place.set(cols, (at - (uint64_t)down * row_pieces.d) * N);
-        const int64_t token = tokens[row];
+        row[i] = row0 + down;
+        place[i].set(cols, (at - (uint64_t)down * row_pieces.d) * N);
+        token[i] = (uint64_t)(int64_t)tokens[min(row[i], n - 1)];
+    }
+#pragma unroll
+    for (int i = 0; i < kPieces; i++) {
+        const W *from = weight + (int64_t)(token[i] < vocab ? token[i] : 0) * stride + place[i].col;
+        if (cols >= N && vocab > 0)
+            __builtin_memcpy(raw[i].w, from, sizeof(raw[i].w));
+        else
+            raw[i].clear(), raw[i].load(from, vocab > 0 ? place[i].n : 0);
+    }
+#pragma unroll
+    for (int i = 0; i < kPieces; i++) {
+        if (row[i] >= n) break;
         float v[N];
-        if ((uint64_t)token < vocab) {
-            load(v, weight + token * stride + place.col, place.n);
 #pragma unroll
-            for (int k = 0; k < N; k++) {
-                v[k] *= scale;
-                // the product rounds to 32 bits and then to T, for every T alike
-                if (sizeof(T) == 2) asm("" : "+v"(v[k]));
-            }
-        } else {
-#pragma unroll
-            for (int k = 0; k < N; k++) v[k] = 0.f;
+        for (int k = 0; k < N; k++) {
+            v[k] = token[i] < vocab ? raw[i][k] * scale : 0.f;
+            // the product rounds to 32 bits and then to T, for every T alike
+            if (sizeof(T) == 2) asm("" : "+v"(v[k]));
         }
-        store(out + row * cols + place.col, v, place.n);
+        store(out + row[i] * cols + place[i].col, v, place[i].n);
     }
 }
 
@@ -57,14 +65,15 @@ hipError_t lookup(const spiky_lm_embed_args &a, void *out, hipStream_t st) {
     const uint64_t row_pieces = (a.cols + N - 1) / N, pieces = a.n * row_pieces;
     const Divider by((uint32_t)row_pieces);
     auto go = [&](auto kernel, uint64_t each) {
-        const uint64_t groups = (pieces + each - 1) / each;
+        const uint64_t groups = (pieces + kThreads * each - 1) / (kThreads * each);
         if (groups * kThreads > 0xffffffffull) return hipErrorInvalidValue;
         kernel<<<dim3((uint32_t)groups), dim3(kThreads), 0, st>>>(
             static_cast<const Tok *>(a.tokens), static_cast<const W *>(a.weight), a.weight_stride,
             static_cast<T *>(out), a.n, a.vocab, a.cols, by, (float)a.scale);
         return hipGetLastError();
     };
-    return go(k_embed<Tok, W, T, 4>, kThreads * 4);
+    // a piece a thread where more would leave CUs idle
+    return pieces < 8 * kCUs * kThreads ? go(k_embed<Tok, W, T, 1>, 1) : go(k_embed<Tok, W, T, 4>, 4);
 }
 
 // ---- gradient ------------------------------------------------------------------
@@ -263,9 +272,8 @@ __global__ __launch_bounds__(kThreads) void k_embed_sum(const T *__restrict__ d_
                                                         const uint32_t *__restrict__ order,
                                                         const Run *__restrict__ runs, W *__restrict__ d_weight,
                                                         float *__restrict__ partial, uint64_t pitch, uint32_t vocab,
-                                                        uint64_t cols,
-                                                        uint32_t size, uint32_t chunks, uint32_t chunk_groups,
-                                                        uint32_t lanes, float scale) {
+                                                        uint64_t cols, uint32_t size, uint32_t chunks,
+                                                        uint32_t chunk_groups, uint32_t lanes, float scale) {
     constexpr int N = piece<W, T>();
     Place<N> place;
     place.set(cols, ((uint64_t)blockIdx.y * lanes + (threadIdx.x & (lanes - 1))) * N);
@@ -498,8 +506,8 @@ hipError_t sums(const spiky_lm_embed_args &a, const void *d_out_, int64_t stride
         const uint64_t all = groups + (a.vocab + rows * each - 1) / (rows * each);
         if (all * kThreads > 0xffffffffull) return hipErrorInvalidValue;
         kernel<<<dim3((uint32_t)all, (uint32_t)slabs), dim3(kThreads), 0, st>>>(
-            d_out, stride, start, order, runs, d_weight, partial, pitch_of(a), (uint32_t)a.vocab, a.cols, chunk, chunks, groups, lanes,
-            (float)a.scale);
+            d_out, stride, start, order, runs, d_weight, partial, pitch_of(a), (uint32_t)a.vocab, a.cols, chunk, chunks,
+            groups, lanes, (float)a.scale);
         return hipGetLastError();
     };
     // Several rows to a thread where there are enough: most have no token, and only their zeros to write.
