@@ -48,10 +48,10 @@ int spiky_lm_embed_backward(const spiky_lm_embed_args *args, const void *d_out, 
  * Beam k of search b has a score, the sum of its tokens' log-probabilities.  Each of
  * its tokens v is a candidate of score
  *   s = scores[b][k] + logits[b][k][v] - log(sum over u of exp(logits[b][k][u]))
- * in 64 bits, but where s is -infinity.  A finished beam has one candidate, token `pad`
- * with the beam's own score.  The n candidates of largest s / length^length_penalty go
- * on, in this order; length is lengths[b][k], plus 1 where the beam is not finished,
- * and at least 1.  Of equal ones, the lower beam comes first, then the larger logit, then
+ * in 64 bits, over exponentials and sums of a slice's in 32, but where s is -infinity.  A
+ * finished beam has one candidate, token `pad` with the beam's own score.  The n candidates of
+ * largest s / length^length_penalty go on, in this order; length is lengths[b][k], plus 1 where
+ * the beam is not finished, and at least 1.  Of equal ones, the lower beam comes first, then the larger logit, then
  * the lower token.  Where there are fewer than n, the others are (-infinity, beam 0, pad).
  * A beam that is not finished and whose score or one of whose logits is NaN or
  * +infinity has candidates of score NaN, in the order of their tokens; NaN ranks as +infinity. */

@@ -22,7 +22,8 @@ def beam_select(logits, scores, n=None, *, finished=None, pad=0, lengths=None, l
     logits: [B, K, V], float32, bfloat16 or float16 on a HIP device, the vocabulary contiguous, rows at
     any distance.  scores: float32 [B, K].  n: K without.  finished: bool [B, K].  lengths: int32 or
     int64 [B, K].  K and n are at most 64, the penalty -8 to 8.  Scores are float32, parents and tokens
-    int64; the order is that of the scores in 64 bits.  There is no gradient."""
+    int64; the order is that of the scores in 64 bits, over exponentials and sums of them in 32.  There
+    is no gradient."""
     return _native.lm().beam_select(logits, scores, n, finished, pad, lengths, length_penalty)
 
 
