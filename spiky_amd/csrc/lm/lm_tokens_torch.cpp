@@ -136,22 +136,49 @@ bool once_each(const Side &s, int64_t searches, int64_t beams) {
     return true;
 }
 
-// Sides that share no byte: one ends before the other, or all strides of both are multiples of one
-// number within which they take different parts, as the keys and values of one cache may.
+// Whether two sides share a byte: `d` bytes from a's first to b's first, and for each its steps from the largest
+// on and its run's bytes.  Steps that both have are taken together, as only the difference of the indexes counts; else
+// the larger step goes index by index, `left` of them in all: past that, they are taken to share one.
+struct Steps {
+    const std::pair<int64_t, int64_t> *first, *last;
+    int64_t bytes;
+
+    int64_t span() const {
+        int64_t span = bytes;
+        for (auto s = first; s != last; s++) span += s->first * (s->second - 1);
+        return span;
+    }
+    Steps inner() const { return {first + 1, last, bytes}; }
+};
+
+bool meet(int64_t d, const Steps &a, const Steps &b, int &left) {
+    if (d >= a.span() || -d >= b.span()) return false;
+    if (a.first == a.last && b.first == b.last) return true;
+    const int64_t of_a = a.first == a.last ? 0 : a.first->first, of_b = b.first == b.last ? 0 : b.first->first;
+    const Steps in_a = of_a >= of_b ? a.inner() : a, in_b = of_b >= of_a ? b.inner() : b;
+    const int64_t step = std::max(of_a, of_b);
+    // the indexes of b minus a's for which the inner parts' spans meet: -in_b.span() < d + i * step < in_a.span()
+    const auto below = [&](int64_t x) { return x >= 0 ? x / step : -((-x + step - 1) / step); };
+    const int64_t from = std::max(of_a >= of_b ? 1 - a.first->second : 0, below(-in_b.span() - d) + 1);
+    const int64_t to = std::min(of_b >= of_a ? b.first->second - 1 : 0, -below(d - in_a.span()) - 1);
+    for (int64_t i = from; i <= to; i++)
+        if (left-- <= 0 || meet(d + i * step, in_a, in_b, left)) return true;
+    return false;
+}
+
+// Sides that share no byte, as the keys and values of one cache.
 bool apart(const Side &a, const Side &b, int64_t searches, int64_t beams_a, int64_t beams_b) {
     if (end_of(a, searches, beams_a) <= b.at || end_of(b, searches, beams_b) <= a.at) return true;
-    int64_t unit = 0;
-    for (const auto &steps : {steps_of(a, searches, beams_a), steps_of(b, searches, beams_b)})
-        for (const auto &step : steps) {
-            int64_t x = unit, y = step.first;
-            while (y) std::swap(x %= y, y);
-            unit = x;
-        }
-    if (unit == 0) return false;
-    const uint64_t part = (uint64_t)((b.at - a.at) % (uint64_t)unit);
-    // b.at - a.at wraps where b lies before a
-    const uint64_t shift = b.at >= a.at ? part : (uint64_t)(unit - (int64_t)((a.at - b.at) % (uint64_t)unit)) % unit;
-    return a.run_bytes <= shift && shift + b.run_bytes <= (uint64_t)unit;
+    const auto down = [&](const Side &s, int64_t beams) {
+        auto steps = steps_of(s, searches, beams);
+        while (!steps.empty() && steps.front().first == 0) steps.erase(steps.begin());  // an expanded dimension
+        std::reverse(steps.begin(), steps.end());
+        return steps;
+    };
+    const auto of_a = down(a, beams_a), of_b = down(b, beams_b);
+    int left = 1 << 14;
+    return !meet((int64_t)(b.at - a.at), {of_a.data(), of_a.data() + of_a.size(), (int64_t)a.run_bytes},
+                 {of_b.data(), of_b.data() + of_b.size(), (int64_t)b.run_bytes}, left);
 }
 
 // The tensors of a list, a tuple or one tensor.
