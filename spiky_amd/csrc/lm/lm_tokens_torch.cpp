@@ -356,10 +356,12 @@ PyObject *reorder_states(PyObject *, PyObject *const *args, Py_ssize_t n) {
                 longer.run = (int64_t)shorter.run_bytes;
                 longer.runs = shorter.runs;
                 longer.run_bytes = shorter.run_bytes;
-            } else {
-                TORCH_CHECK_VALUE(!to, "out and its state have runs that do not fit each other");
+            } else {  // of which in place there are none
                 in[i] = in[i].contiguous();
                 side_of(in[i], a);
+                a.run = (int64_t)b.run_bytes;
+                a.runs = b.runs;
+                a.run_bytes = b.run_bytes;
             }
         }
         const bool empty = in[i].numel() == 0 || out[i].numel() == 0;

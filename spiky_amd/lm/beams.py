@@ -35,5 +35,6 @@ def reorder_states(states, parents, out=None):
     tensors of the results' shapes that share no memory with the states, or `states` themselves, which
     are then reordered in place (n = K, at most 64; beams that stay where they are cost nothing).  A
     cache of which some positions are in use is passed as a view of these, without a copy where the
-    dimensions behind [B, K] are contiguous but for one.  There is no gradient."""
+    dimensions behind [B, K] are contiguous but for one, as they have to be of `out`.  There is no
+    gradient."""
     return _native.lm().reorder_states(states, parents, out)

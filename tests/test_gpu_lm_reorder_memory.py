@@ -87,3 +87,15 @@ def test_any_two_layouts(cuda_device):
             want.as_strided(*p).copy_(chosen(base.as_strided(*p), parents))
         assert torch.equal(there.cpu(), want), (turn, places)
     assert 60 <= sum(found) <= 240
+
+
+@pytest.mark.parametrize("flip", [False, True])
+def test_runs_that_do_not_nest(cuda_device, flip):
+    """Positions in use of a cache into rows with a gap behind each, and the other way."""
+    parents = torch.tensor([[0, 0, 1], [2, 1, 1]], device=cuda_device)
+    cache, rows = torch.randn(2, 3, 5, 40, 9, device=cuda_device), torch.randn(2, 3, 5, 16, 12, device=cuda_device)
+    x, out = (rows[..., :9], cache[:, :, :, :16]) if flip else (cache[:, :, :, :16], rows[..., :9])
+    kept, before, want = (cache if flip else rows).clone(), x.clone(), chosen(x, parents)
+    (kept[:, :, :, :16] if flip else kept[..., :9]).copy_(want)
+    assert reorder_states([x], parents, out=[out])[0] is out
+    assert torch.equal(cache if flip else rows, kept) and torch.equal(x, before)
