@@ -254,7 +254,7 @@ PyObject *beam_select(PyObject *, PyObject *const *args, Py_ssize_t n) {
     const Tensor scores = by_beam(args[Scores], "scores", shape, device);
     TORCH_CHECK(scores.scalar_type() == at::kFloat, "tensor scores must be float32, got ", scores.scalar_type());
     int64_t count = beams;
-    if (args[N] != Py_None) count = (int64_t)bits64(args[N]);
+    if (args[N] != Py_None) count = whole(args[N], "n");
     TORCH_CHECK_VALUE(beams >= 1 && beams <= 64 && count >= 1 && count <= 64, "beams and n must be 1 to 64, got ",
                       beams, " and ", count);
     const Tensor finished = by_beam(args[Finished], "finished", shape, device);
@@ -266,7 +266,7 @@ PyObject *beam_select(PyObject *, PyObject *const *args, Py_ssize_t n) {
     TORCH_CHECK_VALUE(a.length_penalty == 0.0 || lengths.defined(), "a length_penalty needs lengths");
     TORCH_CHECK_VALUE(a.length_penalty >= -8.0 && a.length_penalty <= 8.0, "length_penalty must be -8 to 8, got ",
                       a.length_penalty);
-    a.pad = (int64_t)bits64(args[Pad]);
+    a.pad = whole(args[Pad], "pad");
     a.searches = searches;
     a.beams = beams;
     a.vocab = vocab;

@@ -100,6 +100,16 @@ inline uint64_t bits64(PyObject *o) {
     return v;
 }
 
+// A whole number of 64 bits with its sign.
+inline int64_t whole(PyObject *o, const char *name) {
+    THPObjectPtr index(PyNumber_Index(o));
+    if (!index) throw python_error();
+    int past = 0;
+    const int64_t v = PyLong_AsLongLongAndOverflow(index.get(), &past);
+    TORCH_CHECK_VALUE(!past, name, " must fit 64 bits");
+    return v;
+}
+
 inline double probability(PyObject *o) {
     const double p = number(o);
     TORCH_CHECK_VALUE(p >= 0.0 && p <= 1.0, "dropout probability must be between 0 and 1, got ", p);

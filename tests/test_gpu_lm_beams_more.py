@@ -1,0 +1,22 @@
+"""beam_select on the GPU: numbers past 64 bits."""
+import pytest
+import torch
+
+from spiky_amd import beam_select
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("how", [dict(n=(1 << 64) + 2), dict(n=-(1 << 64) + 2), dict(pad=1 << 63), dict(pad=-(1 << 63) - 1),
+                                 dict(pad=(1 << 64) + 3)])
+def test_whole_numbers_past_64_bits_are_refused(cuda_device, how):
+    x, scores = torch.zeros(2, 3, 9, device=cuda_device), torch.zeros(2, 3, device=cuda_device)
+    with pytest.raises(ValueError, match="must fit 64 bits"):
+        beam_select(x, scores, **how)
+
+
+@pytest.mark.parametrize("pad", [-1, (1 << 63) - 1, -(1 << 63)])
+def test_pads_of_64_bits(cuda_device, pad):
+    x, scores = torch.zeros(1, 1, 2, device=cuda_device), torch.zeros(1, 1, device=cuda_device)
+    got = beam_select(x, scores, 3, finished=torch.ones(1, 1, dtype=torch.bool, device=cuda_device), pad=pad)
+    assert got[2].tolist() == [[pad] * 3]
