@@ -240,6 +240,8 @@ PyObject *beam_select(PyObject *, PyObject *const *args, Py_ssize_t n) {
     TORCH_CHECK_TYPE(n == 7, "beam_select takes 7 arguments");
     check_trace();
     enum { Logits, Scores, N, Finished, Pad, Lengths, LengthPenalty };
+    check_tangent(args[Logits], "logits");
+    check_tangent(args[Scores], "scores");
     at::AutoGradMode off(false);
     Tensor logits = device_tensor(args[Logits], "logits");
     spiky_lm_beams_args a = {};
@@ -295,6 +297,16 @@ PyObject *reorder_states(PyObject *, PyObject *const *args, Py_ssize_t n) {
     TORCH_CHECK_TYPE(n == 3, "reorder_states takes 3 arguments");
     check_trace();
     enum { States, Parents, Out };
+    bool one = false, one_out = false;
+    const std::vector<PyObject *> given = each_of(args[States], one);
+    std::vector<PyObject *> results;
+    const bool to = args[Out] != Py_None;
+    if (to) {
+        results = each_of(args[Out], one_out);
+        TORCH_CHECK_VALUE(results.size() == given.size() && one == one_out, "out must be as many tensors as states");
+    }
+    for (PyObject *o : given) check_tangent(o, "states");
+    for (PyObject *o : results) check_tangent(o, "out");
     at::AutoGradMode off(false);
     Tensor parents = device_tensor(args[Parents], "parents");
     const bool i64 = is_index(parents, "parents");
@@ -304,14 +316,6 @@ PyObject *reorder_states(PyObject *, PyObject *const *args, Py_ssize_t n) {
     TORCH_CHECK_VALUE(count <= 4096, "parents must be of at most 4096 beams, got ", count);
     OnDevice on(device);
     parents = parents.contiguous();
-    bool one = false, one_out = false;
-    const std::vector<PyObject *> given = each_of(args[States], one);
-    std::vector<PyObject *> results;
-    const bool to = args[Out] != Py_None;
-    if (to) {
-        results = each_of(args[Out], one_out);
-        TORCH_CHECK_VALUE(results.size() == given.size() && one == one_out, "out must be as many tensors as states");
-    }
     std::vector<Tensor> in(given.size()), out(given.size());
     std::vector<Side> from(given.size()), into(given.size());
     std::vector<spiky_lm_state> states(given.size());
