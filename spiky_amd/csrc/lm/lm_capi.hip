@@ -234,9 +234,13 @@ int spiky_lm_reorder(const spiky_lm_state *states, uint64_t count, const void *p
         require(states || count == 0, "null pointer");
         require(searches < 0x80000000ull && beams < 0x80000000ull && n <= 4096, "too many searches or beams");
         for (uint64_t i = 0; i < count; i++) {
-            check(states[i]);
-            require(states[i].in != states[i].out || states[i].runs == 0 || (n == beams && n <= 64),
-                    "in place, n must be the number of beams, at most 64");
+            const spiky_lm_state &s = states[i];
+            check(s);
+            if (s.in != s.out || s.runs == 0) continue;
+            require(n == beams && n <= 64, "in place, n must be the number of beams, at most 64");
+            require((searches <= 1 || s.in_search == s.out_search) && (beams <= 1 || s.in_beam == s.out_beam) &&
+                        (s.runs == 1 || s.in_run == s.out_run),
+                    "in place, both strides must be the same");
         }
         if (searches == 0 || n == 0) return;
         require(parents != nullptr, "null pointer");
