@@ -302,6 +302,7 @@ struct Beam {
 };
 
 constexpr int kJoinThreads = 512, kJoinWaves = kJoinThreads / 64;
+constexpr uint32_t kSearchesX = 1u << 20;  // of a grid's x, whose threads have to stay below 2^32
 
 // The natural logarithm of a positive normal number: of its mantissa m in [0.7, 1.5), 2 artanh z with
 // z = (m - 1) / (m + 1), |z| < 0.2, as its series up to z^21 / 21.  The library's functions of
@@ -339,7 +340,8 @@ __global__ __launch_bounds__(kJoinThreads) void k_beam_join(const spiky_lm_beams
     __shared__ Candidate list[kMost], wave_best[2][kJoinWaves];
     __shared__ uint32_t ranks[kMost];
     __shared__ uint32_t group_top[64], open_list[kMost], threshold, open, listed;
-    const uint32_t search = blockIdx.x, row0 = search * (uint32_t)a.beams;  // searches * beams < 2^24
+    const uint32_t search = blockIdx.x + blockIdx.y * kSearchesX, row0 = search * (uint32_t)a.beams;  // searches * beams < 2^24
+    if (search >= a.searches) return;
     const uint32_t wave = threadIdx.x / 64, lane = threadIdx.x & 63;
     const uint32_t lists = (uint32_t)a.beams * parts.slices;
     const float *logits = parts.logits + (uint64_t)row0 * parts.slices * parts.n;
@@ -613,7 +615,8 @@ hipError_t launch_beam_select(const spiky_lm_beams_args &a, void *workspace, hip
         k_beam_slices<f16><<<grid, dim3(kThreads), 0, st>>>(a, parts);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    k_beam_join<<<dim3((uint32_t)a.searches), dim3(kJoinThreads), 0, st>>>(a, parts);
+    const dim3 searches((uint32_t)min(a.searches, (uint64_t)kSearchesX), (uint32_t)((a.searches + kSearchesX - 1) / kSearchesX));
+    k_beam_join<<<searches, dim3(kJoinThreads), 0, st>>>(a, parts);
     return hipGetLastError();
 }
 

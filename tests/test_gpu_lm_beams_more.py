@@ -1,4 +1,4 @@
-"""beam_select on the GPU: numbers past 64 bits."""
+"""beam_select on the GPU: numbers past 64 bits, more searches than one side of a grid."""
 import pytest
 import torch
 
@@ -20,3 +20,16 @@ def test_pads_of_64_bits(cuda_device, pad):
     x, scores = torch.zeros(1, 1, 2, device=cuda_device), torch.zeros(1, 1, device=cuda_device)
     got = beam_select(x, scores, 3, finished=torch.ones(1, 1, dtype=torch.bool, device=cuda_device), pad=pad)
     assert got[2].tolist() == [[pad] * 3]
+
+
+@pytest.mark.parametrize("searches", [(1 << 20) + 1, (1 << 23) + 5])
+def test_many_searches(cuda_device, searches):
+    """More searches than one side of a grid takes."""
+    gen = torch.Generator(cuda_device).manual_seed(3)
+    x = torch.randn(searches, 1, 3, generator=gen, device=cuda_device)
+    scores = -torch.rand(searches, 1, generator=gen, device=cuda_device)
+    got = beam_select(x, scores, 2)
+    s, tokens = torch.sort((torch.log_softmax(x.double(), -1) + scores.double()[..., None])[:, 0], descending=True, stable=True)
+    assert torch.equal(got[2], tokens[:, :2]) and not bool(got[1].any())
+    # three exponentials and their sum, each off by a few half steps, then the score's own rounding
+    assert float((got[0].double() - s[:, :2]).abs().max()) <= (48 + 3 * 2 + 16) * 2.0 ** -24
