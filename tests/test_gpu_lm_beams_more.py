@@ -1,8 +1,9 @@
-"""beam_select on the GPU: numbers past 64 bits, more searches than one side of a grid."""
+"""beam_select on the GPU: numbers past 64 bits, more searches than one side of a grid, values with an offset."""
 import pytest
 import torch
 
 from spiky_amd import beam_select
+import lm_tokens_plain as plain
 
 pytestmark = pytest.mark.gpu
 
@@ -33,3 +34,19 @@ def test_many_searches(cuda_device, searches):
     assert torch.equal(got[2], tokens[:, :2]) and not bool(got[1].any())
     # three exponentials and their sum, each off by a few half steps, then the score's own rounding
     assert float((got[0].double() - s[:, :2]).abs().max()) <= (48 + 3 * 2 + 16) * 2.0 ** -24
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("offset", [0.0, -2.0, 1000.0, -60000.0])
+def test_values_with_an_offset(cuda_device, dtype, offset):
+    """Scores of a long search, and logits that are all large: the choice is by differences."""
+    gen = torch.Generator().manual_seed(8)
+    x = (torch.randn(2, 5, 20003, generator=gen) * 4 + offset).to(dtype)
+    for at in (0.0, -1.5e3, -3e4, 1e7):
+        scores = at - 3 * torch.rand(2, 5, generator=gen)
+        finished, lengths = torch.rand(2, 5, generator=gen) < 0.3, torch.randint(1, 2000, (2, 5), generator=gen)
+        for n, alpha in ((16, 0.0), (64, 0.0), (16, 0.7)):
+            how = dict(finished=finished, lengths=lengths, length_penalty=alpha)
+            got = beam_select(x.to(cuda_device), scores.to(cuda_device), n, **{
+                k: v.to(cuda_device) if isinstance(v, torch.Tensor) else v for k, v in how.items()})
+            plain.check_select(got, x, scores, n, **how)
