@@ -319,7 +319,7 @@ __global__ __launch_bounds__(kThreads) void k_embed_sum(const T *__restrict__ d_
 #pragma unroll
         for (int k = 0; k < N; k++) sum[k] *= scale;
         W *to_row = d_weight + (row0 + r * rows) * cols + place.col;
-        if (kStream)
+        if constexpr (kStream)
             stream_out(to_row, sum, place.n);
         else
             store(to_row, sum, place.n);
@@ -514,12 +514,18 @@ hipError_t sums(const spiky_lm_embed_args &a, const void *d_out_, int64_t stride
     };
     // Several rows to a thread where there are enough: most have no token, and only their zeros to write.
     // 1, 4, 8 and 16 rows take 424, 325, 332 and 373 us of 32768 tokens' 4096 bf16 columns and 152000
-    // rows.  There results go past the last cache, which would not hold them for their reader: 306 us.
-    // 32000 rows of 2048 fp32 columns, which it holds, take 78 stored as usual and 112 past it.
+    // rows.  A table that the last cache would not hold for its reader is stored past it, where a thread's
+    // piece is one store: 16384 tokens' 600 MB of 4096 columns in fp32 take 161 and, stored as usual, 195 us,
+    // in bf16 123 and 167; 2.4 GB 466 and 528, 442 and 475.  fp32 rows of 16-bit results are two
+    // stores a piece, and go as usual: 185 us for 283, 488 for 1090.  Of smaller tables it hangs on the tokens:
+    // 256 MB in fp32 take 111 and 126 us with 16384 of them, 55 and 41 with 256.
     const bool many = a.vocab / rows * slabs >= kManyGroups;
-    const bool stream = a.vocab * a.cols * sizeof(W) >= kLastCache * 2;
-    const hipError_t e = many ? stream ? go(k_embed_sum<T, W, 4, true>, 4) : go(k_embed_sum<T, W, 4, false>, 4)
-                              : go(k_embed_sum<T, W, 1, false>, 1);
+    const hipError_t e = [&] {
+        if (!many) return go(k_embed_sum<T, W, 1, false>, 1);
+        if constexpr (N * sizeof(W) == 16)
+            if (a.vocab * a.cols * sizeof(W) >= kLastCache * 2) return go(k_embed_sum<T, W, 4, true>, 4);
+        return go(k_embed_sum<T, W, 4, false>, 4);
+    }();
     if (e != hipSuccess || groups == 0) return e;
     // most chunks begin no run: where there are many, a workgroup looks at several
     const uint32_t col_groups = (uint32_t)((a.cols + 255) / 256), joined = (uint64_t)chunks * col_groups > 4 * kCUs ? 8 : 1;

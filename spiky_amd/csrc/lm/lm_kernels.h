@@ -140,24 +140,21 @@ __device__ __forceinline__ void store(T *p, const float (&v)[N], int n) {
 }
 
 // The same past the caches' ordinary replacement, so that what other workgroups read again stays in L2.
+// One store a thread: nothing puts the parts of a line together that several store one after the other.
 template <typename T, int N>
 __device__ __forceinline__ void stream_out(T *p, const float (&v)[N], int n) {
-    static_assert(N * sizeof(T) % 16 == 0, "16-byte pieces");
+    static_assert(N * sizeof(T) == 16, "16-byte pieces");
     if (n < N) {
         store(p, v, n);
         return;
     }
     typedef uint32_t Piece __attribute__((ext_vector_type(4), aligned(2)));
-    constexpr int kEach = 16 / sizeof(T);
     T t[N];
 #pragma unroll
     for (int i = 0; i < N; i++) t[i] = from_f32<T>(v[i]);
-#pragma unroll
-    for (int i = 0; i < N; i += kEach) {
-        Piece q;
-        __builtin_memcpy(&q, t + i, sizeof(q));
-        __builtin_nontemporal_store(q, reinterpret_cast<Piece *>(p + i));
-    }
+    Piece q;
+    __builtin_memcpy(&q, t, sizeof(q));
+    __builtin_nontemporal_store(q, reinterpret_cast<Piece *>(p));
 }
 
 // A thread's piece of N columns of every row.  The last piece of a row that N does
