@@ -99,3 +99,19 @@ def test_runs_that_do_not_nest(cuda_device, flip):
     (kept[:, :, :, :16] if flip else kept[..., :9]).copy_(want)
     assert reorder_states([x], parents, out=[out])[0] is out
     assert torch.equal(cache if flip else rows, kept) and torch.equal(x, before)
+
+
+@pytest.mark.parametrize("beams,n", [(4, 4), (8, 8), (16, 16), (31, 31), (64, 64), (64, 100), (7, 130)])
+def test_results_past_the_last_cache(cuda_device, beams, n):
+    """More than 512 MiB of results, runs that end inside 16 bytes, some beams that stay and parents that there are none of."""
+    width = ((600 << 20) // (2 * n * 3) & ~15) + 13
+    gen = torch.Generator(cuda_device).manual_seed(n)
+    x = torch.randint(0, 256, (2, beams, 3, width), generator=gen, device=cuda_device, dtype=torch.uint8)
+    parents = torch.randint(0, beams, (2, n), generator=gen, device=cuda_device)
+    parents[0, :min(beams, n) // 2] = torch.arange(min(beams, n) // 2, device=cuda_device)
+    parents[1, n - 1] = -1
+    want = torch.where((parents >= 0)[:, :, None, None], chosen(x, parents.clamp_min(0)), 0)
+    assert torch.equal(reorder_states(x, parents), want)
+    if n == beams:
+        reorder_states(x, parents, out=x)
+        assert torch.equal(x, want)
