@@ -58,22 +58,24 @@ __device__ __forceinline__ uint64_t ordered(double x) {
     return u ^ ((uint64_t)((int64_t)u >> 63) | (uint64_t)1 << 63);
 }
 
-// A distance from the largest of all, as a number that is the larger the nearer: without a sign, so bit 31 is
-// set.  Its steps grow with the distances that are asked about, and not with an offset that all values have: by
-// 7 or 8 bits of the values' own mantissas, 64 searches of 8 beams of 152000, n = 16, took 38 us with scores near
-// -20 and 103 near -1500, where a thousand candidates reach, and fp32 logits near 1000 80 for 61.
-__device__ __forceinline__ uint32_t nearness(float distance) { return ~__float_as_uint(distance); }
+// Half of how far x lies below the top: finite for all but -infinity, which is no candidate.
+__device__ __forceinline__ float below(float top, float x) { return fmaf(x, -0.5f, 0.5f * top); }
 
-// The largest number of kSteps bits behind bit 31 that at least n of the wave's 64 reach.
-constexpr int kSteps = 15;  // of a float, the exponent and 7
-__device__ __forceinline__ uint32_t reached_by(uint32_t near, uint32_t n) {
+// The least distance from the top, to kSteps bits, that at least n of the wave's 64 values are within; the largest
+// finite one where fewer are above -infinity.  Steps grow with the distance that is asked about, and not with
+// an offset that all values have: by 7 or 8 bits of the values' own mantissas, 64 searches of 8 beams of 152000,
+// n = 16, took 38 us with scores near -20 and 103 near -1500, where a thousand candidates reach, and fp32 logits
+// near 1000 80 for 61.
+constexpr int kSteps = 15;  // of a float without its sign, the exponent and 7
+__device__ __forceinline__ float reach_of(float distance, uint32_t n) {
+    const uint32_t near = ~__float_as_uint(distance);
     uint32_t found = 1u << 31;
 #pragma unroll
     for (int i = 30; i > 30 - kSteps; i--) {
         const uint32_t more = found | 1u << i;
         if (__popcll(__ballot(near >= more)) >= n) found = more;
     }
-    return found;
+    return __uint_as_float(min(~found, 0x7f7fffffu));
 }
 
 // The lane's value combined with those of its row of 16 lanes and of the rows before: lane 63 has all.
@@ -164,7 +166,7 @@ template <typename T>
 __global__ __launch_bounds__(kThreads) void k_beam_slices(const spiky_lm_beams_args a, const Parts parts) {
     constexpr int N = 16 / sizeof(T);
     constexpr uint32_t kUnit = kPieces * N;
-    __shared__ float group_top[64], wave_sum[kWaves], farthest;
+    __shared__ float group_top[64], wave_sum[kWaves], reach;
     __shared__ uint64_t list[kMostListed];
     __shared__ uint32_t units[kThreads], n_units, listed;
     const uint32_t row = blockIdx.y + blockIdx.z * 32768, beams = (uint32_t)a.beams;  // searches * beams < 2^24
@@ -205,11 +207,9 @@ __global__ __launch_bounds__(kThreads) void k_beam_slices(const spiky_lm_beams_a
     __syncthreads();
     const float of_group = group_top[lane];
     top = wave_max(of_group);
-    // halves, whose difference is finite for all but -infinity, which is no candidate
-    auto below_top = [&](float x) { return fmaf(x, -0.5f, 0.5f * top); };
     if (wave == 0) {
-        const uint32_t t = reached_by(nearness(below_top(of_group)), parts.n);
-        if (lane == 0) farthest = __uint_as_float(min(~t, 0x7f7fffffu));
+        const float t = reach_of(below(top, of_group), parts.n);
+        if (lane == 0) reach = t;
     }
     float sum = 0.f;
     if (fabsf(top) <= 1e6f) {  // relative to 2^power, and in the end to exp(top)
@@ -232,8 +232,8 @@ __global__ __launch_bounds__(kThreads) void k_beam_slices(const spiky_lm_beams_a
         parts.stats[at] = make_float2(top, sum);
     }
     // NaN reaches nothing: it makes its beam's candidates known without a list
-    const float most = farthest;
-    if (below_top(here) <= most) units[atomicAdd(&n_units, 1u)] = threadIdx.x;
+    const float most = reach;
+    if (below(top, here) <= most) units[atomicAdd(&n_units, 1u)] = threadIdx.x;
     __syncthreads();
     // a unit's logits are read again, a few by each thread
     constexpr uint32_t kAhead = 4;
@@ -249,7 +249,7 @@ __global__ __launch_bounds__(kThreads) void k_beam_slices(const spiky_lm_beams_a
         }
 #pragma unroll
         for (uint32_t j = 0; j < kAhead; j++) {
-            if (i + j * kThreads >= all || col[j] >= vocab || !(below_top(to_f32(y[j])) <= most)) continue;
+            if (i + j * kThreads >= all || col[j] >= vocab || !(below(top, to_f32(y[j])) <= most)) continue;
             const uint32_t k = atomicAdd(&listed, 1u);
             if (k < kMostListed) list[k] = (uint64_t)ordered(to_f32(y[j])) << 32 | (uint32_t)~col[j];
         }
@@ -347,8 +347,8 @@ __global__ __launch_bounds__(kJoinThreads) void k_beam_join(const spiky_lm_beams
     __shared__ Beam beams[kMostBeams];
     __shared__ Candidate list[kMost], wave_best[2][kJoinWaves];
     __shared__ uint32_t ranks[kMost];
-    __shared__ uint32_t group_top[64], open_list[kMost], threshold, open, listed;
-    __shared__ double wave_rank[kJoinWaves];
+    __shared__ uint32_t group_top[64], open_list[kMost], open, listed;
+    __shared__ float2 top_and_reach;
     const uint32_t search = blockIdx.x + blockIdx.y * kSearchesX, row0 = search * (uint32_t)a.beams;  // searches * beams < 2^24
     if (search >= a.searches) return;
     const uint32_t wave = threadIdx.x / 64, lane = threadIdx.x & 63;
@@ -362,12 +362,6 @@ __global__ __launch_bounds__(kJoinThreads) void k_beam_join(const spiky_lm_beams
     const uint32_t first_at = head_at(min(threadIdx.x, lists * heads - 1));
     const float first_logit = logits[first_at];  // of no use where the list's beam is not alive
     const uint32_t first_token = tokens[first_at];
-    // NaN ranks as +infinity
-    auto rank_of = [](const Beam &b, double score) {
-        const double rank = b.length == 1.0 ? score : score / b.length;
-        return rank != rank ? INFINITY : rank;
-    };
-    double best = -INFINITY;  // of the wave's beams
     for (uint32_t k = wave; k < a.beams; k += kJoinWaves) {
         const uint32_t row = row0 + k;
         const float score = a.scores[row];
@@ -403,17 +397,13 @@ __global__ __launch_bounds__(kJoinThreads) void k_beam_join(const spiky_lm_beams
         b.log_sum = log_of(sum);
         b.length = grown == 1.0 ? 1.0 : exp_of(a.length_penalty * log_of(grown));
         if (lane == 0) beams[k] = b;
-        // as of a candidate with the largest logit
-        if (b.kind != kNothing) best = fmax(best, rank_of(b, b.kind == kFinished ? b.score : b.unknown ? NAN : -b.log_sum + b.score));
     }
-    if (lane == 0) wave_rank[wave] = best;
     if (threadIdx.x == 0) listed = open = 0;
-    if (threadIdx.x < 64) group_top[threadIdx.x] = 0;
+    if (threadIdx.x < 64) group_top[threadIdx.x] = ordered(-INFINITY);
     __syncthreads();
-    for (int w = 0; w < kJoinWaves; w++) best = fmax(best, wave_rank[w]);
     const Candidate none = {0, ~(uint64_t)0, ~0u, -INFINITY};
-    // Candidate `o` of list `l`, or none, from its logit and token; and how near its rank is to the best, 0 for none.
-    auto made = [&](uint32_t l, uint32_t o, float logit, uint32_t token, uint32_t &near) {
+    // Candidate `o` of list `l`, or none, from its logit and token; and its rank in 32 bits, finite, or -infinity for none.
+    auto made = [&](uint32_t l, uint32_t o, float logit, uint32_t token, float &coarse) {
         const uint32_t k = parts.by_slices.divide(l);
         const Beam &b = beams[k];
         const bool only = l == k * parts.slices;  // what finished and unknown beams have is in their first list
@@ -425,41 +415,42 @@ __global__ __launch_bounds__(kJoinThreads) void k_beam_join(const spiky_lm_beams
             token = b.kind == kFinished ? 0 : o;
             logit = 0.f;
         }
-        const double rank = rank_of(b, score);
-        near = there ? nearness(rank == best ? 0.f : (float)(best - rank)) : 0;
+        double rank = b.length == 1.0 ? score : score / b.length;
+        rank = rank != rank ? INFINITY : rank;
+        coarse = there ? fminf(fmaxf((float)rank, -__FLT_MAX__), __FLT_MAX__) : -INFINITY;
         if (!there) return none;
         return Candidate{ordered(rank), (uint64_t)k << 32 | (uint32_t)~ordered(logit), token, (float)score};
     };
     // The candidate at `at` of the search's part of the workspace, at most 64 * 2^19 * 64 = 2^31 long.
-    auto candidate = [&](uint32_t at, uint32_t &near) {
+    auto candidate = [&](uint32_t at, float &coarse) {
         const uint32_t l = parts.by_n.divide(at);
-        return made(l, at - l * parts.n, logits[at], tokens[at], near);
+        return made(l, at - l * parts.n, logits[at], tokens[at], coarse);
     };
     // The heads are in 64 groups; n or more of these hold one.
     for (uint32_t i = threadIdx.x; i < lists * heads; i += kJoinThreads) {
         const uint32_t at = head_at(i), l = parts.by_n.divide(at);
-        uint32_t near;
+        float coarse;
         if (i == threadIdx.x)
-            made(l, at - l * parts.n, first_logit, first_token, near);
+            made(l, at - l * parts.n, first_logit, first_token, coarse);
         else
-            candidate(at, near);
-        atomicMax(&group_top[i & 63], near);
+            candidate(at, coarse);
+        atomicMax(&group_top[i & 63], ordered(coarse));
     }
     __syncthreads();
     if (wave == 0) {
-        const uint32_t t = reached_by(group_top[lane], parts.n);
-        if (lane == 0) threshold = t;
+        const float x = from_ordered(group_top[lane]), top = wave_max(x), t = reach_of(below(top, x), parts.n);
+        if (lane == 0) top_and_reach = make_float2(top, t);
     }
     __syncthreads();
     // the lists whose first candidate reaches the threshold, and of these the candidates that do
-    const uint32_t least = threshold;
+    const float top = top_and_reach.x, most = top_and_reach.y;
     for (uint32_t l = threadIdx.x; l < lists; l += kJoinThreads) {
-        uint32_t near;
+        float coarse;
         if (l == threadIdx.x && heads == 1)
-            made(l, 0, first_logit, first_token, near);
+            made(l, 0, first_logit, first_token, coarse);
         else
-            candidate(l * parts.n, near);
-        if (near < least) continue;
+            candidate(l * parts.n, coarse);
+        if (!(below(top, coarse) <= most)) continue;
         const uint32_t k = atomicAdd(&open, 1u);
         if (k < kMost) open_list[k] = l;
     }
@@ -467,9 +458,9 @@ __global__ __launch_bounds__(kJoinThreads) void k_beam_join(const spiky_lm_beams
     const bool every = open > kMost;
     for (uint32_t i = threadIdx.x; i < (every ? lists : open) * parts.n; i += kJoinThreads) {
         const uint32_t l = parts.by_n.divide(i);
-        uint32_t near;
-        const Candidate c = candidate(every ? i : open_list[l] * parts.n + (i - l * parts.n), near);
-        if (near < least) continue;
+        float coarse;
+        const Candidate c = candidate(every ? i : open_list[l] * parts.n + (i - l * parts.n), coarse);
+        if (!(below(top, coarse) <= most)) continue;
         const uint32_t k = atomicAdd(&listed, 1u);
         if (k < kMost) {
             list[k] = c;
@@ -509,8 +500,8 @@ __global__ __launch_bounds__(kJoinThreads) void k_beam_join(const spiky_lm_beams
         Candidate best = none;
 #pragma unroll 1
         for (uint32_t i = threadIdx.x; i < lists * parts.n; i += kJoinThreads) {
-            uint32_t near;
-            const Candidate c = candidate(i, near);
+            float coarse;
+            const Candidate c = candidate(i, coarse);
             if (c.first && last.before(c) && c.before(best)) best = c;
         }
 #pragma unroll 1
