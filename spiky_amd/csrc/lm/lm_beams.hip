@@ -641,9 +641,10 @@ hipError_t launch_beam_select(const spiky_lm_beams_args &a, void *workspace, hip
 hipError_t launch_reorder(const spiky_lm_state *states, uint64_t count, const void *parents, bool parents_i64,
                           uint64_t searches, uint64_t beams, uint64_t n, hipStream_t st) {
     // Results past twice the last cache do not stay there for their reader.  Stored past it, bf16 states of 4, 8,
-    // 16, 32 and 64 beams, 1.8 GB of results, take 433, 445, 486, 462 and 454 us against 468, 467, 495, 478 and
+    // 16, 32 and 64 beams, 1.6 GB of results, take 433, 445, 486, 462 and 454 us against 468, 467, 495, 478 and
     // 491, and in place, where beams that stay are not moved, 344, 421, 473, 427 and 480 against 367, 446, 485,
-    // 446 and 519; 600 MB 149, 151, 147, 146 and 146 against 166, 168, 166, 167 and 174.
+    // 446 and 519.  The call by itself gains as much at 0.5 GB (147 for 167); at 175 MB, which a reader finds in
+    // the cache, it takes 42 to 47 for 47 to 54, and in place 35 to 52 either way.
     uint64_t bytes = 0;
     for (uint64_t i = 0; i < count; i++) bytes += states[i].runs * states[i].run_bytes * n * searches;
     const bool stream = bytes >= 2 * kLastCache;
