@@ -2,6 +2,7 @@
 // Host code only; all device work goes through the C ABI of libspiky_lut.so.
 #include <algorithm>
 #include <cmath>
+#include <numeric>
 #include <vector>
 
 #include "lm_torch.h"
@@ -166,7 +167,8 @@ bool meet(int64_t d, const Steps &a, const Steps &b, int &left) {
     return false;
 }
 
-// Sides that share no byte, as the keys and values of one cache.
+// Sides that share no byte, as the keys and values of one cache: one ends before the other, or all strides of both
+// are multiples of one number within which they take different parts, or no two of their runs meet.
 bool apart(const Side &a, const Side &b, int64_t searches, int64_t beams_a, int64_t beams_b) {
     if (end_of(a, searches, beams_a) <= b.at || end_of(b, searches, beams_b) <= a.at) return true;
     const auto down = [&](const Side &s, int64_t beams) {
@@ -176,8 +178,16 @@ bool apart(const Side &a, const Side &b, int64_t searches, int64_t beams_a, int6
         return steps;
     };
     const auto of_a = down(a, beams_a), of_b = down(b, beams_b);
+    const int64_t distance = (int64_t)(b.at - a.at);
+    int64_t unit = 0;
+    for (const auto &steps : {of_a, of_b})
+        for (const auto &step : steps) unit = std::gcd(unit, step.first);
+    if (unit > 0) {
+        const uint64_t shift = (uint64_t)((distance % unit + unit) % unit);
+        if (a.run_bytes <= shift && shift + b.run_bytes <= (uint64_t)unit) return true;
+    }
     int left = 1 << 14;
-    return !meet((int64_t)(b.at - a.at), {of_a.data(), of_a.data() + of_a.size(), (int64_t)a.run_bytes},
+    return !meet(distance, {of_a.data(), of_a.data() + of_a.size(), (int64_t)a.run_bytes},
                  {of_b.data(), of_b.data() + of_b.size(), (int64_t)b.run_bytes}, left);
 }
 

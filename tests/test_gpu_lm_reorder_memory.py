@@ -115,3 +115,15 @@ def test_results_past_the_last_cache(cuda_device, beams, n):
     if n == beams:
         reorder_states(x, parents, out=x)
         assert torch.equal(x, want)
+
+
+def test_every_other_value_in_two_groupings(cuda_device):
+    """One state's values lie 2 apart, the other's 4, between them: told apart without going through all."""
+    base = torch.randint(0, 256, (2, 3, 1 << 18, 2), device=cuda_device, dtype=torch.uint8)
+    states = [base[..., 0], base.view(2, 3, 1 << 17, 4)[..., 1]]
+    parents = torch.tensor([[0, 0, 1], [2, 1, 1]], device=cuda_device)
+    want = base.clone()
+    want[..., 0] = chosen(states[0], parents)
+    want.view(2, 3, 1 << 17, 4)[..., 1] = chosen(states[1], parents)
+    reorder_states(states, parents, out=states)
+    assert torch.equal(base, want)
