@@ -2,6 +2,7 @@
 // Host code only; all device work goes through the C ABI of libspiky_lut.so.
 #include <algorithm>
 #include <cmath>
+#include <functional>
 #include <numeric>
 #include <vector>
 
@@ -113,28 +114,40 @@ bool side_of(const Tensor &t, Side &s) {
     return true;
 }
 
-// The first byte past a side.
-uintptr_t end_of(const Side &s, int64_t searches, int64_t beams) {
-    return s.at + (searches - 1) * s.search + (beams - 1) * s.beam + (s.runs - 1) * s.run + s.run_bytes;
-}
+// A side's bytes: the steps of its dimensions of more than one index, from the largest on, and their numbers of indexes.
+struct Bytes {
+    uintptr_t at = 0, end = 0;  // the first byte, and the first past it
+    int64_t run = 0;
+    std::pair<int64_t, int64_t> steps[3];
+    int n = 0;
+    int64_t unit = 0;       // all steps are multiples of it
+    bool expanded = false;  // a dimension's indexes are all at one place
 
-// The strides of dimensions of more than one index, and their numbers of indexes.
-std::vector<std::pair<int64_t, int64_t>> steps_of(const Side &s, int64_t searches, int64_t beams) {
-    std::vector<std::pair<int64_t, int64_t>> steps;
-    for (const auto &[step, n] : {std::pair<int64_t, int64_t>{s.search, searches}, {s.beam, beams}, {s.run, s.runs}})
-        if (n > 1) steps.push_back({step, n});
-    std::sort(steps.begin(), steps.end());
-    return steps;
-}
-
-// No byte of a side is in it twice: each stride reaches past what the smaller ones span.
-bool once_each(const Side &s, int64_t searches, int64_t beams) {
-    int64_t span = s.run_bytes;
-    for (const auto &[step, n] : steps_of(s, searches, beams)) {
-        if (step < span) return false;
-        span = step * (n - 1) + span;
+    Bytes(const Side &s, int64_t searches, int64_t beams) : at(s.at), run((int64_t)s.run_bytes) {
+        for (const auto &[step, many] :
+             {std::pair<int64_t, int64_t>{s.search, searches}, {s.beam, beams}, {s.run, (int64_t)s.runs}}) {
+            if (many <= 1) continue;
+            if (step == 0) {
+                expanded = true;
+                continue;
+            }
+            steps[n++] = {step, many};
+            unit = std::gcd(unit, step);
+        }
+        std::sort(steps, steps + n, std::greater<>());
+        end = at + s.run_bytes;
+        for (int i = 0; i < n; i++) end += steps[i].first * (steps[i].second - 1);
     }
-    return true;
+};
+
+// No byte is there twice: each stride reaches past what the smaller ones span.
+bool once_each(const Bytes &b) {
+    int64_t span = b.run;
+    for (int i = b.n - 1; i >= 0; i--) {
+        if (b.steps[i].first < span) return false;
+        span += b.steps[i].first * (b.steps[i].second - 1);
+    }
+    return !b.expanded;
 }
 
 // Whether two sides share a byte: `d` bytes from a's first to b's first, and for each its steps from the largest
@@ -169,26 +182,15 @@ bool meet(int64_t d, const Steps &a, const Steps &b, int &left) {
 
 // Sides that share no byte, as the keys and values of one cache: one ends before the other, or all strides of both
 // are multiples of one number within which they take different parts, or no two of their runs meet.
-bool apart(const Side &a, const Side &b, int64_t searches, int64_t beams_a, int64_t beams_b) {
-    if (end_of(a, searches, beams_a) <= b.at || end_of(b, searches, beams_b) <= a.at) return true;
-    const auto down = [&](const Side &s, int64_t beams) {
-        auto steps = steps_of(s, searches, beams);
-        while (!steps.empty() && steps.front().first == 0) steps.erase(steps.begin());  // an expanded dimension
-        std::reverse(steps.begin(), steps.end());
-        return steps;
-    };
-    const auto of_a = down(a, beams_a), of_b = down(b, beams_b);
-    const int64_t distance = (int64_t)(b.at - a.at);
-    int64_t unit = 0;
-    for (const auto &steps : {of_a, of_b})
-        for (const auto &step : steps) unit = std::gcd(unit, step.first);
+bool apart(const Bytes &a, const Bytes &b) {
+    if (a.end <= b.at || b.end <= a.at) return true;
+    const int64_t distance = (int64_t)(b.at - a.at), unit = std::gcd(a.unit, b.unit);
     if (unit > 0) {
-        const uint64_t shift = (uint64_t)((distance % unit + unit) % unit);
-        if (a.run_bytes <= shift && shift + b.run_bytes <= (uint64_t)unit) return true;
+        const int64_t shift = (distance % unit + unit) % unit;
+        if (a.run <= shift && shift + b.run <= unit) return true;
     }
     int left = 1 << 14;
-    return !meet(distance, {of_a.data(), of_a.data() + of_a.size(), (int64_t)a.run_bytes},
-                 {of_b.data(), of_b.data() + of_b.size(), (int64_t)b.run_bytes}, left);
+    return !meet(distance, {a.steps, a.steps + a.n, a.run}, {b.steps, b.steps + b.n, b.run}, left);
 }
 
 // The tensors of a list, a tuple or one tensor.
@@ -387,21 +389,27 @@ PyObject *reorder_states(PyObject *, PyObject *const *args, Py_ssize_t n) {
         Side by;
         by.at = reinterpret_cast<uintptr_t>(parents.data_ptr());
         by.run_bytes = parents.numel() * parents.element_size();
+        const Bytes of_parents(by, 1, 1);
+        std::vector<Bytes> source, target;
+        std::vector<bool> in_place(given.size());
+        for (size_t i = 0; i < given.size(); i++) {
+            const Side &a = from[i], &b = into[i];
+            source.emplace_back(a, searches, beams);
+            target.emplace_back(b, searches, count);
+            in_place[i] = a.at == b.at && a.search == b.search && a.beam == b.beam && a.run == b.run && a.runs == b.runs;
+        }
         for (size_t i = 0; i < given.size(); i++) {
             if (out[i].numel() == 0) continue;
-            TORCH_CHECK_VALUE(once_each(into[i], searches, count), "the beams of out must not overlap");
-            TORCH_CHECK_VALUE(end_of(into[i], searches, count) <= by.at || end_of(by, 1, 1) <= into[i].at,
-                              "out must not overlap parents");
+            const Bytes &b = target[i];
+            TORCH_CHECK_VALUE(once_each(b), "the beams of out must not overlap");
+            TORCH_CHECK_VALUE(b.end <= of_parents.at || of_parents.end <= b.at, "out must not overlap parents");
+            TORCH_CHECK_VALUE(!in_place[i] || in[i].numel() == 0 || (count == beams && count <= 64),
+                              "in place, parents must be [B, K] of at most 64 beams");
             for (size_t j = 0; j < given.size(); j++) {
-                if (in[j].numel() == 0) continue;
-                const Side &a = from[j], &b = into[i];
-                const bool same = i == j && a.at == b.at && a.search == b.search && a.beam == b.beam && a.run == b.run &&
-                                  a.runs == b.runs;
-                if (same)
-                    TORCH_CHECK_VALUE(count == beams && count <= 64, "in place, parents must be [B, K] of at most 64 beams");
-                TORCH_CHECK_VALUE(same || apart(a, b, searches, beams, count),
+                // a state in place of its result is looked at as that
+                TORCH_CHECK_VALUE(in[j].numel() == 0 || in_place[j] || apart(source[j], b),
                                   "out must be its state, or share no memory with any");
-                TORCH_CHECK_VALUE(i == j || out[j].numel() == 0 || apart(into[j], b, searches, count, count),
+                TORCH_CHECK_VALUE(j >= i || out[j].numel() == 0 || apart(target[j], b),
                                   "the tensors of out must share no memory");
             }
         }
